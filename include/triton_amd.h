@@ -27,8 +27,9 @@
 extern "C" {
 #endif
 
-/* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates */
-#define TAMD_VERSION 2
+/* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
+ * 3: tamd_moe_layer */
+#define TAMD_VERSION 3
 
 /* error codes (negative) */
 #define TAMD_E_INVALID (-1)     /* bad shape / stride / pointer / enum */
@@ -382,6 +383,51 @@ int tamd_reduce_ex(const tamd_reduce_args *args, void *stream);
  */
 int tamd_swiglu(const void *a, int dtype, int64_t M, int64_t N_out, int64_t a_stride_m, void *out,
                 int64_t out_stride_m, float alpha, float limit, int has_limit, void *stream);
+
+/*
+ * A whole mixture-of-experts layer for a few tokens, in two launches (no counterpart in the reference, which chains topk,
+ * metadata, two products and a reduction):
+ *
+ *   y[t] = sum_j g[t,j] * (h[t,j] W_down[e] + b_down[e]),   h[t,j] = swiglu(x[t] W_up[e] + b_up[e]),   e = pick j of token t
+ *
+ * picks and g as tamd_topk_forward with softmax gives them (ties: lower column; g stays float32), swiglu over the column pairs
+ * (2i, 2i+1) as in tamd_matmul, but a NaN passes the clamps.  x, y F16 or BF16 (one type), logits and biases F32 / F16 / BF16, weights MXFP4 contiguous
+ * along K or in 4 KB blocks, scales strided or pre-shuffled, each product its own.  h is held in the workspace with twice the
+ * bits of x's type; sums and the activation are float32; y is rounded once.
+ * Limits: n_tokens <= 64, n_experts <= 512, 1 <= n_picks <= min(n_experts, 16), n_tokens * n_picks <= 512 (TAMD_E_TOO_LARGE);
+ * hidden and inter multiples of 32; x rows and strided weight columns start on 16-byte boundaries (TAMD_E_ALIGNMENT).
+ * workspace: tamd_moe_layer_workspace(n_tokens, n_picks, inter) bytes on a 16-byte boundary, any contents; calls that may
+ * run at the same time need one each.
+ */
+typedef struct tamd_moe_weights {
+  const void *w;           /* up [E, hidden, 2*inter], down [E, inter, hidden] */
+  int64_t w_stride_e, w_stride_n;          /* bytes; blocks: only the first is read */
+  const uint8_t *scale;
+  int64_t scale_stride_e, scale_stride_n;  /* bytes; pre-shuffled: only the first is read */
+  const void *bias;                        /* [E, columns] or NULL */
+  int64_t bias_stride_e;
+  int bias_dtype;
+  int w_layout;            /* TAMD_W_* */
+  int scale_layout;        /* TAMD_SCALE_* */
+} tamd_moe_weights;
+typedef struct tamd_moe_layer_args {
+  const void *x;
+  int64_t x_stride_m;
+  const void *logits;
+  int64_t logits_stride;
+  void *y;
+  int64_t y_stride_m;
+  void *workspace;
+  tamd_moe_weights up, down;
+  int x_dtype, logits_dtype;
+  int n_tokens, n_experts, n_picks, hidden, inter;
+  float act_alpha, act_limit;
+  int act_has_limit;
+} tamd_moe_layer_args;
+
+int64_t tamd_moe_layer_workspace(int n_tokens, int n_picks, int inter);
+/* args_size: sizeof(tamd_moe_layer_args) as the caller was compiled; other sizes are refused */
+int tamd_moe_layer(const tamd_moe_layer_args *args, size_t args_size, void *stream);
 
 #ifdef __cplusplus
 }

@@ -102,6 +102,30 @@ class ReduceArgs(C.Structure):
 
 PP_NONE, PP_SWIGLU, PP_PLUS_A_PAIRSUM = 0, 1, 2
 
+
+class MoeWeights(C.Structure):
+    """Mirror of `tamd_moe_weights`."""
+    _fields_ = [
+        ("w", C.c_void_p), ("w_stride_e", C.c_int64), ("w_stride_n", C.c_int64),
+        ("scale", C.c_void_p), ("scale_stride_e", C.c_int64), ("scale_stride_n", C.c_int64),
+        ("bias", C.c_void_p), ("bias_stride_e", C.c_int64),
+        ("bias_dtype", C.c_int), ("w_layout", C.c_int), ("scale_layout", C.c_int),
+    ]
+
+
+class MoeLayerArgs(C.Structure):
+    """Mirror of `tamd_moe_layer_args`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride_m", C.c_int64), ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+        ("y", C.c_void_p), ("y_stride_m", C.c_int64), ("workspace", C.c_void_p),
+        ("up", MoeWeights), ("down", MoeWeights),
+        ("x_dtype", C.c_int), ("logits_dtype", C.c_int),
+        ("n_tokens", C.c_int), ("n_experts", C.c_int), ("n_picks", C.c_int), ("hidden", C.c_int), ("inter", C.c_int),
+        ("act_alpha", C.c_float), ("act_limit", C.c_float), ("act_has_limit", C.c_int),
+    ]
+
+
+
 _I64, _INT, _PTR, _F = C.c_int64, C.c_int, C.c_void_p, C.c_float
 _SIGNATURES = {
     "tamd_version": ([], C.c_int),
@@ -132,6 +156,8 @@ _SIGNATURES = {
                      _PTR, _INT, _I64, _I64, _PTR], C.c_int),
     "tamd_reduce_ex": ([C.POINTER(ReduceArgs), _PTR], C.c_int),
     "tamd_swiglu": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
+    "tamd_moe_layer_workspace": ([_INT, _INT, _INT], C.c_int64),
+    "tamd_moe_layer": ([C.POINTER(MoeLayerArgs), C.c_size_t, _PTR], C.c_int),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -133,6 +133,43 @@ TAMD_DEVICE int wave_incl_scan(int v) {
   return v;
 }
 
+// Order-preserving map of a logit's bits.  -0.0 counts as +0.0, so that both zeros tie, as they do under the reference's
+// stable argsort of -x (topk_details/_topk_forward.py:15-30; the sum with +0.0 takes the sign).
+TAMD_DEVICE uint32_t ordered_bits(float x) {
+  const uint32_t u = f32_to_bits(x + 0.0f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+// Its inverse (a -0.0 logit comes back as +0.0).
+TAMD_DEVICE float logit_of(uint32_t u) { return bits_to_f32(u ^ (~(uint32_t)((int32_t)u >> 31) | 0x80000000u)); }
+
+// Reductions over aligned groups of L lanes; every lane gets the result.  Step O (1, 2, 4, ...) of the butterfly combines a lane with
+// one of the other aligned block of O lanes.  All lanes of a block of O hold the same value by then, so for O = 4 and 8 the
+// partner may be the mirrored lane, which, like the swaps inside a quad, the data-parallel move does in the register
+// file; for 16 and 32 rows of lanes change places, and the two registers that hold the halves then are combined.
+template <int O>
+TAMD_DEVICE void butterfly(uint32_t v, uint32_t &a, uint32_t &b) {
+  a = v;
+  if constexpr (O == 1) b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);        // quad_perm [1,0,3,2]
+  else if constexpr (O == 2) b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);   // quad_perm [2,3,0,1]
+  else if constexpr (O == 4) b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true);  // row_half_mirror
+  else if constexpr (O == 8) b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true);  // row_mirror
+  else if constexpr (O == 16) { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); a = r[0]; b = r[1]; }
+  else { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); a = r[0]; b = r[1]; }
+}
+template <int L, int O = 1, typename OP>
+TAMD_DEVICE uint32_t group_reduce(uint32_t v, OP op) {
+  if constexpr (O >= L) {
+    return v;
+  } else {
+    uint32_t a, b;
+    butterfly<O>(v, a, b);
+    return group_reduce<L, O * 2>(op(a, b), op);
+  }
+}
+template <int L>
+TAMD_DEVICE uint32_t group_max_u32(uint32_t v) {
+  return group_reduce<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
 inline int dtype_size(int dt) {
   switch (dt) {
     case TAMD_F32: return 4;
