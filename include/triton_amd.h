@@ -28,7 +28,7 @@ extern "C" {
 #endif
 
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
- * 3: tamd_moe_layer */
+ * 3: tamd_moe_layer, tamd_matvec */
 #define TAMD_VERSION 3
 
 /* error codes (negative) */
@@ -428,6 +428,35 @@ typedef struct tamd_moe_layer_args {
 int64_t tamd_moe_layer_workspace(int n_tokens, int n_picks, int inter);
 /* args_size: sizeof(tamd_moe_layer_args) as the caller was compiled; other sizes are refused */
 int tamd_moe_layer(const tamd_moe_layer_args *args, size_t args_size, void *stream);
+
+/*
+ * A few rows times a matrix of 4-bit weights with a scale and possibly a zero point per group (no counterpart in the reference):
+ *
+ *   y[m, n] = sum_k x[m, k] * (q[k, n] - z[k / group, n]) * s[k / group, n] + bias[n]        q, z in 0..15, z = 8 if zeros is NULL
+ *
+ * x [M, K] F16 or BF16, s F16 or BF16, bias and y F32 / F16 / BF16; sums are float32, y is rounded once.  group 32, 64 or 128,
+ * K a multiple of it.  With S = ceil(N / 16) strips of 16 columns and B = ceil(K / 128):
+ *   codes   uint8 [S, B, 4 h, 16 c, 4 t, 4]: dword t of lane (h, c) holds K 128 b + 32 t + 8 h .. + 8 of column 16 s + c, the code of the
+ *           chunk's K 2 i in bits 4 i .. and that of K 2 i + 1 in bits 16 + 4 i ..;
+ *   scales  [S, B, 16 c, 128 / group],  zeros  uint8, laid out like the scales.
+ * What pads columns and K may hold anything but NaN and infinite scales; x rows start on 16-byte boundaries, codes, scales and
+ * zeros too.  Made for up to 64 rows; every further 64 read the weights again.
+ */
+typedef struct tamd_matvec_args {
+  const void *x;
+  int64_t x_stride_m;
+  const uint8_t *codes;
+  const void *scales;
+  const uint8_t *zeros;
+  const void *bias;
+  void *y;
+  int64_t y_stride_m;
+  int x_dtype, scale_dtype, bias_dtype, y_dtype;
+  int M, N, K, group;
+} tamd_matvec_args;
+
+/* args_size: sizeof(tamd_matvec_args) as the caller was compiled; other sizes are refused */
+int tamd_matvec(const tamd_matvec_args *args, size_t args_size, void *stream);
 
 #ifdef __cplusplus
 }

@@ -126,6 +126,16 @@ class MoeLayerArgs(C.Structure):
 
 
 
+class MatvecArgs(C.Structure):
+    """Mirror of `tamd_matvec_args`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride_m", C.c_int64), ("codes", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p),
+        ("bias", C.c_void_p), ("y", C.c_void_p), ("y_stride_m", C.c_int64),
+        ("x_dtype", C.c_int), ("scale_dtype", C.c_int), ("bias_dtype", C.c_int), ("y_dtype", C.c_int),
+        ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("group", C.c_int),
+    ]
+
+
 _I64, _INT, _PTR, _F = C.c_int64, C.c_int, C.c_void_p, C.c_float
 _SIGNATURES = {
     "tamd_version": ([], C.c_int),
@@ -158,6 +168,7 @@ _SIGNATURES = {
     "tamd_swiglu": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
     "tamd_moe_layer_workspace": ([_INT, _INT, _INT], C.c_int64),
     "tamd_moe_layer": ([C.POINTER(MoeLayerArgs), C.c_size_t, _PTR], C.c_int),
+    "tamd_matvec": ([C.POINTER(MatvecArgs), C.c_size_t, _PTR], C.c_int),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -54,6 +54,8 @@ struct Buffer {
   template <int NT = 0>
   TAMD_DEVICE u32x4_t load16(uint32_t off, uint32_t uniform = 0) const { return __builtin_amdgcn_raw_buffer_load_b128(r, off, uniform, NT); }
   TAMD_DEVICE u32x2_t load8(uint32_t off, uint32_t uniform = 0) const { return __builtin_amdgcn_raw_buffer_load_b64(r, off, uniform, 0); }
+  TAMD_DEVICE uint32_t load4(uint32_t off, uint32_t uniform = 0) const { return __builtin_amdgcn_raw_buffer_load_b32(r, off, uniform, 0); }
+  TAMD_DEVICE uint32_t load2(uint32_t off, uint32_t uniform = 0) const { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, uniform, 0); }
   TAMD_DEVICE uint32_t load1(uint32_t off, uint32_t uniform = 0) const { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, off, uniform, 0); }
 };
 
