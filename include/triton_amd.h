@@ -28,7 +28,7 @@ extern "C" {
 #endif
 
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
- * 3: tamd_moe_layer, tamd_matvec */
+ * 3: tamd_moe_layer, tamd_matvec, tamd_sample */
 #define TAMD_VERSION 3
 
 /* error codes (negative) */
@@ -457,6 +457,39 @@ typedef struct tamd_matvec_args {
 
 /* args_size: sizeof(tamd_matvec_args) as the caller was compiled; other sizes are refused */
 int tamd_matvec(const tamd_matvec_args *args, size_t args_size, void *stream);
+
+/*
+ * One token per row of logits [R, V] (F32 / F16 / BF16), by a given uniform number u of [0, 1) (no counterpart in the reference).
+ * Order of a row: by logit, the largest first, equal ones by index (as in tamd_topk_forward); w = exp((x - max) / temperature).  Kept is
+ *   the first top_k (top_k <= 0: all), of these the shortest prefix with a sum of w of at least top_p times theirs (top_p >= 1: all),
+ *   of these what has w >= min_p; the first always.
+ * The token is the first kept one, in that order, whose running sum of w exceeds u times the sum of all kept.  Sums are exact to
+ * 2^-37 of the row's and do not depend on how the work is cut.
+ * temperature <= 0 or NaN: the first of the order.  NaN logits count as -inf; a row of nothing but -inf gives -1; with +inf logits these
+ * share the mass alike.  u is clamped to [0, 1), min_p to at most 1; a NaN top_p or min_p keeps all, a NaN u is 0.
+ * temperature, top_k, top_p, min_p: per row if the pointer is given, else the value for all.  Limits: V <= 2^20, R <= 2^20.
+ * workspace: tamd_sample_workspace(R, V) bytes on a 16-byte boundary, any contents; calls that may run at the same time need one each.
+ */
+typedef struct tamd_sample_args {
+  const void *logits;
+  int64_t logits_stride;
+  const float *u;
+  const float *temperature;
+  const int32_t *top_k;
+  const float *top_p;
+  const float *min_p;
+  int32_t *tokens;
+  void *workspace;
+  int logits_dtype;
+  int R, V;
+  float temperature_value;
+  int top_k_value;
+  float top_p_value, min_p_value;
+} tamd_sample_args;
+
+int64_t tamd_sample_workspace(int R, int V);
+/* args_size: sizeof(tamd_sample_args) as the caller was compiled; other sizes are refused */
+int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream);
 
 #ifdef __cplusplus
 }

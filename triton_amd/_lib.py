@@ -136,6 +136,16 @@ class MatvecArgs(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    """Mirror of `tamd_sample_args`."""
+    _fields_ = [
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("tokens", C.c_void_p), ("workspace", C.c_void_p),
+        ("logits_dtype", C.c_int), ("R", C.c_int), ("V", C.c_int),
+        ("temperature_value", C.c_float), ("top_k_value", C.c_int), ("top_p_value", C.c_float), ("min_p_value", C.c_float),
+    ]
+
+
 _I64, _INT, _PTR, _F = C.c_int64, C.c_int, C.c_void_p, C.c_float
 _SIGNATURES = {
     "tamd_version": ([], C.c_int),
@@ -168,6 +178,8 @@ _SIGNATURES = {
     "tamd_swiglu": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
     "tamd_moe_layer_workspace": ([_INT, _INT, _INT], C.c_int64),
     "tamd_moe_layer": ([C.POINTER(MoeLayerArgs), C.c_size_t, _PTR], C.c_int),
+    "tamd_sample_workspace": ([_INT, _INT], C.c_int64),
+    "tamd_sample": ([C.POINTER(SampleArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_matvec": ([C.POINTER(MatvecArgs), C.c_size_t, _PTR], C.c_int),
 }
 
