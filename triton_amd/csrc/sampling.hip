@@ -4,17 +4,30 @@
 // a prefix of that order, and the token is the first of it whose running sum of w exceeds u times the sum of all kept: nothing
 // has to be sorted, every question is "where does the running count or sum reach this".
 //
-// w is taken in 64 bits and held as a whole number of units of 2^-(62 - log2 V): sums of whole numbers do not depend on their order, so
-// the same row gives the same token however the work is cut, and they are off by less than 2^-37 of the row's mass.
+// w is taken in 64 bits and held as a whole number of units of 2^-fraction, 2^fraction * V < 2^62: sums of whole numbers do not depend on
+// their order, so the same row gives the same token however the work is cut, and they are off by less than 2^-37 of the row's mass.
+// What rounds to zero is not there at all: it cannot be drawn, and adds nothing to what top-k keeps.
+//
+// Three launches over (chunk of a row, row):
+//   extremes   the largest logit with its index, and the smallest;
+//   histogram  count and mass of the logits in 2048 bins of equal width between the two (or down to where w is zero);
+//   pick       every workgroup finds in the histogram the few bins in which the ends of top-k, top-p and min-p and the token can
+//              lie, and collects its chunk's logits of those; the row's last workgroup sorts them (a few hundred of the whole
+//              vocabulary) and answers the questions exactly.
+// Rows of up to 4096 logits are sorted as they are, in one launch.  A row that has more than 4096 logits in those bins -- many
+// equal or nearly equal ones -- is searched by the bits of its keys (search_row): slower, but right for any row.
 #include "common.h"
 
 namespace tamd {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
+constexpr int kBins = 2048, kMost = 4096;   // candidates that are sorted
+constexpr int kChunk = 8192, kMaxChunks = 64;
+constexpr int kRowsAtOnce = 4096;           // of one round of launches (the workspace holds as many)
 
 struct RowSettings {
-  double t;
+  double t;          // temperature
   double top_p, min_p, u;
   int top_k;         // 0: all
   bool greedy;
@@ -43,12 +56,50 @@ TAMD_DEVICE uint32_t key_at(const void *logits, int64_t i) {
 }
 constexpr uint32_t kNothing = 0x007FFFFFu;   // key of -inf
 
-// Weight of a logit in a row whose largest is `top` (> -inf): with infinite ones, all of these alike and nothing else.
-TAMD_DEVICE double weight_of(uint32_t key, double top, double t) {
-  const double v = logit_of(key);
-  if (v == top) return 1.0;
-  return key <= kNothing || top == __builtin_inf() ? 0.0 : exp((v - top) / t);
+// 2^(-j / 256) by the threads of a workgroup.
+TAMD_DEVICE void make_powers(double *powers) {
+  if (threadIdx.x < 256) powers[threadIdx.x] = exp2((double)threadIdx.x * -0.00390625);
 }
+
+// Weights of a row whose largest logit is `top` (> -inf).  y = log2(1 / w).
+struct RowScale {
+  double top, to_y, to_bin;
+  int fraction;
+  uint32_t top_key;
+  bool infinite;     // with infinite logits these weigh alike and nothing else does
+  const double *powers;
+  TAMD_DEVICE RowScale(uint32_t top_key_, uint32_t least_key, double t, int V, const double *powers_)
+      : top(logit_of(top_key_)), to_y(1.4426950408889634 / t), fraction(62 - (32 - __builtin_clz((uint32_t)V))), top_key(top_key_),
+        infinite(logit_of(top_key_) == __builtin_inff()), powers(powers_) {
+    const double most = y_of(least_key), range = most < fraction ? most : fraction;
+    to_bin = range > 0.0 ? kBins / range : 0.0;
+  }
+  TAMD_DEVICE double y_of(uint32_t key) const {
+    if (key == top_key) return 0.0;
+    return key <= kNothing || infinite ? 1e9 : (top - logit_of(key)) * to_y;
+  }
+  TAMD_DEVICE bool counts(double y) const { return y < fraction; }
+  TAMD_DEVICE int bin_of(double y) const {
+    const double b = y * to_bin;
+    return b >= kBins - 1 ? kBins - 1 : (int)b;
+  }
+  // 2^(fraction - y), y cut into a whole number, a multiple of 1/256 (the table) and a rest below it (the series of 2^-r: five terms
+  // are off by 2^-52): a third of the instructions of exp(), which took longer than reading the logits
+  TAMD_DEVICE uint64_t units_of(double y) const {
+    if (!counts(y)) return 0;
+    // (fused by hand: the histogram and the candidates have to agree to the last unit in every kernel)
+    const int n = (int)y;
+    const double f = y - n;
+    const int j = (int)(f * 256.0);
+    const double r = __builtin_fma(j, -0.00390625, f) * 0.6931471805599453;
+    double p = __builtin_fma(r, 1.0 / 24.0, -1.0 / 6.0);
+    p = __builtin_fma(r, p, 0.5);
+    p = __builtin_fma(r, p, -1.0);
+    p = __builtin_fma(r, p, 1.0);
+    return (uint64_t)(powers[j] * p * (double)(1ull << fraction)) >> n;
+  }
+  TAMD_DEVICE uint64_t units(uint32_t key) const { return units_of(y_of(key)); }
+};
 
 struct Found {
   uint32_t key;      // of the element
@@ -69,95 +120,122 @@ TAMD_DEVICE T block_sum(T v, T *tmp) {
   return s;
 }
 
-// The element of a whole row at which the running count (by_mass: mass) reaches `target` >= 1, three bits of its key at a time.
+// Inclusive scan over the workgroup of one value per thread; `tmp` has a place per wave.
+template <typename T>
+TAMD_DEVICE T block_scan(T v, T *tmp) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const T x = __shfl_up(v, o);
+    v += lane >= o ? x : 0;
+  }
+  if (lane == kWave - 1) tmp[wave] = v;
+  sync_threads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v += w < wave ? tmp[w] : 0;
+  sync_threads();
+  return v;
+}
+
+// What one thread finds and the others wait for.
+struct Shared {
+  uint64_t tmp[kWaves];
+  uint64_t sum;
+  uint64_t found_mass, found_count;
+  int digit;
+  int at[2];
+  int token;
+  bool last;
+};
+
+// The element of a whole row at which the running count (by_mass: mass) reaches `target` >= 1, eleven bits of its key at a time: a
+// histogram of the next bits of the keys that share the bits so far.  hist: room for kBins 12-byte entries.
 template <int DT>
-TAMD_DEVICE Found find_in_row(const void *logits, int64_t row, int V, double top, double t, double unit, bool by_mass, uint64_t target, uint64_t *tmp) {
+TAMD_DEVICE Found find_in_row(const void *logits, int64_t row, int V, const RowScale &scale, bool by_mass, uint64_t target, uint64_t *hist, Shared &sh) {
+  const int tid = threadIdx.x;
+  uint64_t *mass = hist;
+  uint32_t *count = (uint32_t *)(hist + kBins);
   Found f{0, 0, 0};
-  for (int shift = 30; shift >= 0; shift -= 3) {
-    const int bits = shift == 30 ? 2 : 3;
-    uint32_t count[8] = {};
-    uint64_t mass[8] = {};
-    for (int i = threadIdx.x; i < V; i += kThreads) {
+#pragma clang loop unroll(disable)
+  for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift == 10 ? 0 : -1) {
+    const int bits = shift ? 11 : 10;
+    for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
+    sync_threads();
+    for (int i = tid; i < V; i += kThreads) {
       const uint32_t key = key_at<DT>(logits, row + i);
-      if (shift + bits < 32 && key >> (shift + bits) != f.key >> (shift + bits)) continue;
+      if (shift < 21 && key >> (shift + bits) != f.key >> (shift + bits)) continue;
       const uint32_t d = key >> shift & ((1u << bits) - 1u);
-      const uint64_t w = (uint64_t)(weight_of(key, top, t) * unit + 0.5);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) count[j] += d == j, mass[j] += d == j ? w : 0;
+      atomicAdd((unsigned long long *)&mass[d], (unsigned long long)scale.units(key));
+      atomicAdd(&count[d], 1u);
     }
-    int at = 0;
-    bool found = false;
-#pragma unroll
-    for (int j = 7; j >= 0; --j) {
-      const uint64_t n = block_sum<uint64_t>(count[j], tmp), m = block_sum<uint64_t>(mass[j], tmp);
-      const uint64_t upto = by_mass ? f.mass + m : f.count + n;
-      if (!found && (upto >= target || j == 0)) found = true, at = j;
-      else if (!found) f.count += n, f.mass += m;
-    }
-    f.key |= (uint32_t)at << shift;
+    sync_threads();
+    // from the largest digit down: thread t has the digits kBins - 1 - 2 t and the one below
+    const int d = kBins - 1 - 2 * tid;
+    const uint64_t m0 = mass[d], m1 = mass[d - 1], n0 = count[d], n1 = count[d - 1];
+    const uint64_t ms = block_scan<uint64_t>(m0 + m1, sh.tmp) - m0 - m1 + f.mass, ns = block_scan<uint64_t>(n0 + n1, sh.tmp) - n0 - n1 + (uint64_t)f.count;
+    const uint64_t c0 = by_mass ? ms : ns, c1 = c0 + (by_mass ? m0 : n0), c2 = c1 + (by_mass ? m1 : n1);
+    if (c0 < target && target <= c1) sh.digit = d, sh.found_mass = ms, sh.found_count = ns;
+    if (c1 < target && target <= c2) sh.digit = d - 1, sh.found_mass = ms + m0, sh.found_count = ns + n0;
+    sync_threads();
+    f.key |= (uint32_t)sh.digit << shift, f.mass = sh.found_mass, f.count = (int64_t)sh.found_count;
+    sync_threads();
   }
   return f;
 }
 
+// Where the kept prefix ends, from the row's sums: with `least` units or more.
+TAMD_DEVICE uint64_t least_units(const RowSettings &s, const RowScale &scale) {
+  return s.min_p > 0.0 ? (uint64_t)ceil(s.min_p * (double)(1ull << scale.fraction)) : 1;
+}
+TAMD_DEVICE uint64_t top_p_target(double top_p, uint64_t sum) {   // the prefix ends where the sum reaches it
+  const double want = ceil(top_p * (double)sum);
+  return want >= 1.0 ? (want < (double)sum ? (uint64_t)want : sum) : 1;
+}
+TAMD_DEVICE uint64_t token_target(double u, uint64_t sum) {       // the token is where the sum reaches it
+  const uint64_t at = (uint64_t)(u * (double)sum) + 1;
+  return at < sum ? at : sum;
+}
+
+// The token of a row whose largest logit is known, by the bits of the keys.
 template <int DT>
-TAMD_DEVICE int sample_row(const tamd_sample_args &a, int r, uint64_t *tmp) {
+TAMD_DEVICE int search_row(const tamd_sample_args &a, int r, const RowSettings &s, const RowScale &scale, uint64_t *hist, Shared &sh) {
   const int tid = threadIdx.x, V = a.V;
+  uint64_t *tmp = sh.tmp;
   const int64_t row = r * a.logits_stride;
-  const RowSettings s = settings_of(a, r);
-  // the first of the largest
-  uint64_t best = 0;
-  for (int i = tid; i < V; i += kThreads) {
-    const uint64_t v = (uint64_t)key_at<DT>(a.logits, row + i) << 32 | (0xFFFFFFFFu - (uint32_t)i);
-    best = v > best ? v : best;
-  }
-#pragma unroll
-  for (int o = 1; o < kWave; o *= 2) {
-    const uint64_t v = __shfl_xor(best, o);
-    best = v > best ? v : best;
-  }
-  if (tid % kWave == 0) tmp[tid / kWave] = best;
-  sync_threads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) best = tmp[w] > best ? tmp[w] : best;
-  sync_threads();
-  const uint32_t top_key = (uint32_t)(best >> 32);
-  if (top_key <= kNothing) return -1;
-  if (s.greedy) return (int)(0xFFFFFFFFu - (uint32_t)best);
-  const double top = logit_of(top_key), t = s.t, unit = (double)(1ull << (62 - (32 - __builtin_clz((uint32_t)V))));
-  const auto fixed = [&](uint32_t key) { return (uint64_t)(weight_of(key, top, t) * unit + 0.5); };
-  // the kept prefix: what has a larger key than `last`, and `ties` elements of it
-  uint32_t last = 0;
-  int64_t ties = V;
-  uint64_t sum;
-  if (s.top_k) {
-    const Found f = find_in_row<DT>(a.logits, row, V, top, t, unit, false, (uint64_t)s.top_k, tmp);
-    last = f.key, ties = s.top_k - f.count;
-    sum = f.mass + (uint64_t)ties * fixed(last);
-  } else {
-    uint64_t mine = 0;
-    for (int i = tid; i < V; i += kThreads) mine += fixed(key_at<DT>(a.logits, row + i));
-    sum = block_sum<uint64_t>(mine, tmp);
-  }
-  if (s.top_p < 1.0) {
-    const double want = ceil(s.top_p * (double)sum);
-    const uint64_t target = want >= 1.0 ? (want < (double)sum ? (uint64_t)want : sum) : 1;
-    const Found f = find_in_row<DT>(a.logits, row, V, top, t, unit, true, target, tmp);
-    const uint64_t w = fixed(f.key);
-    const int64_t n = w ? (int64_t)((target - f.mass + w - 1) / w) : 1;
-    if (f.key > last || (f.key == last && n < ties)) last = f.key, ties = n, sum = f.mass + (uint64_t)n * w;
-  }
-  if (s.min_p > 0.0 && weight_of(last, top, t) < s.min_p) {
+  const auto sum_of = [&](uint32_t above, uint64_t least) {   // of larger keys with at least that many units
     uint64_t mine = 0;
     for (int i = tid; i < V; i += kThreads) {
       const uint32_t key = key_at<DT>(a.logits, row + i);
-      if (key > last && (key == top_key || weight_of(key, top, t) >= s.min_p)) mine += fixed(key);
+      const uint64_t w = key > above ? scale.units(key) : 0;
+      mine += w >= least ? w : 0;
     }
-    sum = block_sum<uint64_t>(mine, tmp);
+    return block_sum<uint64_t>(mine, tmp);
+  };
+  // the kept prefix: what has a larger key than `last`, and `ties` elements of it
+  uint32_t last = kNothing + 1;
+  int64_t ties = V;
+  uint64_t sum = s.top_k ? 0 : sum_of(kNothing, 0), target = 0;
+  Found f{0, 0, 0};
+  // where top-k ends, where top-p ends, the token
+#pragma clang loop unroll(disable)
+  for (int ask = s.top_k ? 0 : s.top_p < 1.0 ? 1 : 2; ask < 3; ask = ask == 0 && s.top_p < 1.0 ? 1 : ask == 2 ? 3 : 2) {
+    if (ask == 2) {
+      const uint64_t least = least_units(s, scale);
+      if (s.min_p > 0.0 && scale.units(last) < least) sum = sum_of(last, least);
+    }
+    target = ask == 0 ? (uint64_t)s.top_k : ask == 1 ? top_p_target(s.top_p, sum) : token_target(s.u, sum);
+    f = find_in_row<DT>(a.logits, row, V, scale, ask != 0, target, hist, sh);
+    const uint64_t w = scale.units(f.key);
+    if (ask == 0) {
+      last = f.key, ties = s.top_k - f.count;
+      sum = f.mass + (uint64_t)ties * w;
+    } else if (ask == 1) {
+      const int64_t n = w ? (int64_t)((target - f.mass + w - 1) / w) : 1;
+      if (f.key > last || (f.key == last && n < ties)) last = f.key, ties = n, sum = f.mass + (uint64_t)n * w;
+    }
   }
-  const uint64_t at = (uint64_t)(s.u * (double)sum) + 1, target = at < sum ? at : sum;
-  const Found f = find_in_row<DT>(a.logits, row, V, top, t, unit, true, target, tmp);
   // which of the equal ones
-  int64_t skip = (int64_t)((target - f.mass - 1) / fixed(f.key));
+  int64_t skip = (int64_t)((target - f.mass - 1) / scale.units(f.key));
   for (int i0 = 0; i0 < V; i0 += kThreads) {
     const int i = i0 + tid;
     const uint64_t mask = __ballot(i < V && key_at<DT>(a.logits, row + (i < V ? i : 0)) == f.key);
@@ -182,11 +260,374 @@ TAMD_DEVICE int sample_row(const tamd_sample_args &a, int r, uint64_t *tmp) {
   return -1;   // (not reached)
 }
 
+// A chunk's logits as keys, four at a time per thread whatever the row's alignment.
+template <int DT, typename F>
+TAMD_DEVICE void for_chunk(const tamd_sample_args &a, int64_t row, int begin, int end, F use) {
+  for (int i0 = begin + 4 * (int)threadIdx.x; i0 < end; i0 += 4 * kThreads) {
+    if (i0 + 4 <= end) {
+      float v[4];
+      if constexpr (DT == TAMD_F32) {
+        __builtin_memcpy(v, (const float *)a.logits + row + i0, 16);
+      } else {
+        uint16_t b[4];
+        __builtin_memcpy(b, (const uint16_t *)a.logits + row + i0, 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = DT == TAMD_BF16 ? bf16_bits_to_f32(b[j]) : f16_bits_to_f32(b[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) use(i0 + j, ordered_bits(v[j] != v[j] ? -__builtin_inff() : v[j]));
+    } else {
+      for (int i = i0; i < end; ++i) use(i, key_at<DT>(a.logits, row + i));
+    }
+  }
+}
+
+// Element of the order as one number: the larger, the earlier.
+TAMD_DEVICE uint64_t element_of(uint32_t key, int i) { return (uint64_t)key << 32 | (0xFFFFFFFFu - (uint32_t)i); }
+TAMD_DEVICE uint32_t key_of(uint64_t e) { return (uint32_t)(e >> 32); }
+TAMD_DEVICE int index_of(uint64_t e) { return (int)(0xFFFFFFFFu - (uint32_t)e); }
+
+struct Workspace {
+  uint64_t *first;        // [rows, chunks] largest element
+  uint32_t *least;        // [rows, chunks] smallest key above -inf (0xFFFFFFFF: none)
+  uint64_t *mass;         // [rows, bins]
+  uint32_t *count;        // [rows, bins]
+  uint32_t *collected;    // [rows] candidates
+  uint32_t *ticket;       // [rows] workgroups that are done
+  uint64_t *candidates;   // [rows, kMost]
+};
+constexpr int64_t kRowBytes = kMaxChunks * 12 + kBins * 12 + 8 + kMost * 8;
+
+inline Workspace workspace_of(void *p, int rows) {
+  uint8_t *at = (uint8_t *)p;
+  const auto take = [&](int64_t bytes) { uint8_t *q = at; at += bytes * rows; return q; };
+  Workspace w;
+  w.candidates = (uint64_t *)take(kMost * 8), w.mass = (uint64_t *)take(kBins * 8), w.first = (uint64_t *)take(kMaxChunks * 8);
+  w.count = (uint32_t *)take(kBins * 4), w.least = (uint32_t *)take(kMaxChunks * 4), w.collected = (uint32_t *)take(4), w.ticket = (uint32_t *)take(4);
+  return w;
+}
+
 template <int DT>
-__global__ __launch_bounds__(kThreads, 4) void sample_kernel(tamd_sample_args a) {
-  __shared__ uint64_t tmp[kWaves];
-  const int token = sample_row<DT>(a, blockIdx.x, tmp);
-  if (threadIdx.x == 0) a.tokens[blockIdx.x] = token;
+__global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, Workspace ws, int chunk) {
+  __shared__ uint64_t s_first[kWaves];
+  __shared__ uint32_t s_least[kWaves];
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
+  for (int b = c * kThreads + tid; b < kBins; b += gridDim.x * kThreads) ws.mass[(int64_t)r * kBins + b] = 0, ws.count[(int64_t)r * kBins + b] = 0;
+  if (c == 0 && tid == 0) ws.collected[r] = 0, ws.ticket[r] = 0;
+  uint64_t first = 0;
+  uint32_t least = 0xFFFFFFFFu;
+  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, uint32_t key) {
+    const uint64_t e = element_of(key, i);
+    first = e > first ? e : first;
+    least = key > kNothing && key < least ? key : least;
+  });
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const uint64_t e = __shfl_xor(first, o);
+    const uint32_t l = __shfl_xor(least, o);
+    first = e > first ? e : first;
+    least = l < least ? l : least;
+  }
+  if (tid % kWave == 0) s_first[tid / kWave] = first, s_least[tid / kWave] = least;
+  sync_threads();
+  if (tid == 0) {
+    for (int w = 0; w < kWaves; ++w) {
+      first = s_first[w] > first ? s_first[w] : first;
+      least = s_least[w] < least ? s_least[w] : least;
+    }
+    ws.first[r * kMaxChunks + c] = first, ws.least[r * kMaxChunks + c] = least;
+  }
+}
+
+// A row's extremes from its chunks', by every thread.
+TAMD_DEVICE void row_extremes(const Workspace &ws, int r, int chunks, uint64_t &first, uint32_t &least) {
+  const int lane = threadIdx.x % kWave;
+  first = lane < chunks ? ws.first[r * kMaxChunks + lane] : 0;
+  least = lane < chunks ? ws.least[r * kMaxChunks + lane] : 0xFFFFFFFFu;
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) {
+    const uint64_t e = __shfl_xor(first, o);
+    const uint32_t l = __shfl_xor(least, o);
+    first = e > first ? e : first;
+    least = l < least ? l : least;
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a, Workspace ws, int chunk) {
+  __shared__ uint64_t mass[kBins];
+  __shared__ uint32_t count[kBins];
+  __shared__ double powers[256];
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
+  uint64_t first;
+  uint32_t least;
+  row_extremes(ws, r, gridDim.x, first, least);
+  const RowSettings s = settings_of(a, r);
+  if (s.greedy || key_of(first) <= kNothing) return;
+  make_powers(powers);
+  for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
+  const RowScale scale(key_of(first), least, s.t, a.V, powers);
+  sync_threads();
+  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int, uint32_t key) {
+    const double y = scale.y_of(key);
+    if (scale.counts(y)) {
+      const int b = scale.bin_of(y);
+      atomicAdd((unsigned long long *)&mass[b], (unsigned long long)scale.units_of(y));
+      atomicAdd(&count[b], 1u);
+    }
+  });
+  sync_threads();
+  for (int b = tid; b < kBins; b += kThreads)
+    if (count[b]) {
+      atomicAdd((unsigned long long *)&ws.mass[(int64_t)r * kBins + b], (unsigned long long)mass[b]);
+      atomicAdd(&ws.count[(int64_t)r * kBins + b], count[b]);
+    }
+}
+
+// n elements in `list` (room for the next power of two), largest first afterwards.
+TAMD_DEVICE void sort_elements(uint64_t *list, int n) {
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) list[i] = 0;
+  sync_threads();
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      for (int p = threadIdx.x; p < size / 2; p += kThreads) {
+        const int i = 2 * j * (p / j) + p % j;
+        const uint64_t x = list[i], y = list[i + j];
+        if ((x < y) == ((i & k) == 0)) list[i] = y, list[i + j] = x;
+      }
+      sync_threads();
+    }
+}
+
+// The token, from n <= kMost sorted candidates.  before_mass / before_rank: what lies in front of a bin (null: the candidates are the
+// whole row); min_lo, min_hi: the bins in which min-p ends, min_mass: what lies in front of them.
+TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const uint64_t *list, int n, uint64_t *before_mass, uint32_t *before_rank, uint64_t total_mass,
+                           uint32_t total_count, int min_lo, int min_hi, uint64_t min_mass, Shared &sh) {
+  constexpr int PER = kMost / kThreads;
+  const int tid = threadIdx.x;
+  uint64_t units[PER], before[PER], run = 0, enough = 0;
+  uint32_t rank[PER];
+  int bin[PER];
+  const uint64_t least = least_units(s, scale);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * tid + j;
+    const double y = i < n ? scale.y_of(key_of(list[i])) : 1e9;
+    units[j] = scale.units_of(y);
+    bin[j] = i < n && scale.counts(y) ? scale.bin_of(y) : -1;
+    before[j] = run;
+    run += units[j];
+    enough += bin[j] >= min_lo && bin[j] <= min_hi && units[j] >= least ? units[j] : 0;
+  }
+  const uint64_t start = block_scan<uint64_t>(run, sh.tmp) - run;
+  if (before_mass) {   // the first candidate of a bin turns what lies in front of the bin into what its candidates' running sums lack
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = PER * tid + j;
+      if (bin[j] >= 0 && (i == 0 || scale.bin_of(scale.y_of(key_of(list[i - 1]))) != bin[j])) {
+        before_mass[bin[j]] -= start + before[j];
+        before_rank[bin[j]] -= (uint32_t)i;
+      }
+    }
+  }
+  if (tid == 0) sh.sum = total_mass, sh.token = -1;
+  sync_threads();
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const bool adds = before_mass && bin[j] >= 0;
+    before[j] += start + (adds ? before_mass[bin[j]] : 0);
+    rank[j] = (uint32_t)(PER * tid + j) + (adds ? before_rank[bin[j]] : 0u);
+  }
+  if (s.top_k && (uint32_t)s.top_k < total_count) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (bin[j] >= 0 && rank[j] == (uint32_t)s.top_k - 1) sh.sum = before[j] + units[j];
+    sync_threads();
+  }
+  if (s.top_p < 1.0) {
+    const uint64_t target = top_p_target(s.top_p, sh.sum);
+    sync_threads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (bin[j] >= 0 && before[j] < target && target <= before[j] + units[j]) sh.sum = before[j] + units[j];
+    sync_threads();
+  }
+  uint64_t sum = sh.sum;
+  if (s.min_p > 0.0) {
+    const uint64_t has = min_mass + block_sum<uint64_t>(enough, sh.tmp);
+    sum = has < sum ? has : sum;
+  }
+  const uint64_t target = token_target(s.u, sum);
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (bin[j] >= 0 && before[j] < target && target <= before[j] + units[j]) sh.token = index_of(list[PER * tid + j]);
+  sync_threads();
+  return sh.token;
+}
+
+// The bin in which the running count or sum reaches `target`, from the prefix sums in front of the bins; every thread gets it.
+template <typename T>
+TAMD_DEVICE int bin_reaching(const T *before, T target, int &slot) {
+  target = target < 1 ? 1 : target > before[kBins] ? before[kBins] : target;
+#pragma unroll
+  for (int j = 0; j < kBins / kThreads; ++j) {
+    const int b = threadIdx.x * (kBins / kThreads) + j;
+    if (before[b] < target && target <= before[b + 1]) slot = b;
+  }
+  sync_threads();
+  const int found = slot;
+  sync_threads();
+  return found;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void pick_kernel(tamd_sample_args a, Workspace ws, int chunk) {
+  __shared__ uint64_t before_mass[kBins + 1];
+  __shared__ uint64_t list[kMost];
+  __shared__ uint32_t before_rank[kBins + 1];
+  __shared__ double powers[256];
+  __shared__ Shared sh;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
+  uint64_t first;
+  uint32_t least;
+  row_extremes(ws, r, gridDim.x, first, least);
+  const RowSettings s = settings_of(a, r);
+  if (s.greedy || key_of(first) <= kNothing) {
+    if (c == 0 && tid == 0) a.tokens[r] = key_of(first) <= kNothing ? -1 : index_of(first);
+    return;
+  }
+  make_powers(powers);
+  const RowScale scale(key_of(first), least, s.t, a.V, powers);
+  // ---- what lies in front of every bin
+  static_assert(kBins == 2 * kThreads);
+  const int64_t h = (int64_t)r * kBins + 2 * tid;
+  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1];
+  const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1];
+  const uint64_t upto = block_scan<uint64_t>(m0 + m1, sh.tmp);
+  const uint64_t upto_n = block_scan<uint64_t>(n0 + n1, sh.tmp);
+  before_mass[2 * tid] = upto - m0 - m1, before_mass[2 * tid + 1] = upto - m1;
+  before_rank[2 * tid] = (uint32_t)upto_n - n0 - n1, before_rank[2 * tid + 1] = (uint32_t)upto_n - n1;
+  if (tid == kThreads - 1) before_mass[kBins] = upto, before_rank[kBins] = (uint32_t)upto_n;
+  sync_threads();
+  const uint64_t total = before_mass[kBins];
+  const uint32_t total_n = before_rank[kBins];
+  // ---- the bins of the candidates: lo and hi enclose the sum of what is kept
+  int from[4] = {kBins, kBins, kBins, kBins}, to[4] = {-1, -1, -1, -1};
+  uint64_t lo = total, hi = total;
+  if (s.top_k && (uint32_t)s.top_k < total_n) {
+    from[0] = to[0] = bin_reaching<uint32_t>(before_rank, (uint32_t)s.top_k, sh.at[0]);
+    lo = before_mass[from[0]], hi = before_mass[to[0] + 1];
+  }
+  if (s.top_p < 1.0) {
+    from[1] = bin_reaching<uint64_t>(before_mass, top_p_target(s.top_p, lo), sh.at[0]);
+    to[1] = bin_reaching<uint64_t>(before_mass, top_p_target(s.top_p, hi), sh.at[1]);
+    lo = before_mass[from[1]];
+    hi = before_mass[to[1] + 1] < hi ? before_mass[to[1] + 1] : hi;
+  }
+  uint64_t min_mass = 0;
+  if (s.min_p > 0.0) {
+    const double y = -log2(s.min_p);
+    const int b = scale.counts(y) ? scale.bin_of(y) : kBins - 1;
+    from[2] = b > 0 ? b - 1 : 0, to[2] = b < kBins - 1 ? b + 1 : kBins - 1;
+    min_mass = before_mass[from[2]];
+    lo = min_mass < lo ? min_mass : lo;
+    hi = before_mass[to[2] + 1] < hi ? before_mass[to[2] + 1] : hi;
+  }
+  from[3] = bin_reaching<uint64_t>(before_mass, token_target(s.u, lo), sh.at[0]);
+  to[3] = bin_reaching<uint64_t>(before_mass, token_target(s.u, hi), sh.at[1]);
+  const auto wanted = [&](int b) {
+    bool is = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) is |= b >= from[j] && b <= to[j];
+    return is;
+  };
+  const uint64_t n_all = block_sum<uint64_t>((wanted(2 * tid) ? n0 : 0u) + (wanted(2 * tid + 1) ? n1 : 0u), sh.tmp);
+  if (n_all > kMost) {
+    if (c == 0) {
+      const int token = search_row<DT>(a, r, s, scale, list, sh);
+      if (tid == 0) a.tokens[r] = token;
+    }
+    return;
+  }
+  // ---- collect them; the row's last workgroup goes on
+  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, uint32_t key) {
+    const double y = scale.y_of(key);
+    if (scale.counts(y) && wanted(scale.bin_of(y))) {
+      const uint32_t at = atomicAdd(&ws.collected[r], 1u);
+      if (at < kMost) ws.candidates[(int64_t)r * kMost + at] = element_of(key, i);
+    }
+  });
+  __threadfence();
+  sync_threads();
+  if (tid == 0) sh.last = atomicAdd(&ws.ticket[r], 1u) + 1 == gridDim.x;
+  sync_threads();
+  if (!sh.last) return;
+  __threadfence();
+  const int n = (int)n_all;
+  for (int i = tid; i < n; i += kThreads) list[i] = __hip_atomic_load(&ws.candidates[(int64_t)r * kMost + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  sort_elements(list, n);
+  const int token = pick_among(s, scale, list, n, before_mass, before_rank, total, total_n, from[2], to[2], min_mass, sh);
+  if (tid == 0) a.tokens[r] = token;
+}
+
+// Rows of up to kMost logits: all of them are candidates.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void short_row_kernel(tamd_sample_args a) {
+  __shared__ uint64_t list[kMost];
+  __shared__ double powers[256];
+  __shared__ Shared sh;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const RowSettings s = settings_of(a, r);
+  make_powers(powers);
+  for (int i = tid; i < a.V; i += kThreads) list[i] = element_of(key_at<DT>(a.logits, r * a.logits_stride + i), i);
+  sort_elements(list, a.V);
+  const uint32_t top = key_of(list[0]);
+  int token = -1;
+  if (top > kNothing) {
+    if (s.greedy) {
+      token = index_of(list[0]);
+    } else {
+      const RowScale scale(top, top, s.t, a.V, powers);   // (one bin)
+      uint64_t mine = 0;
+      for (int i = tid; i < a.V; i += kThreads) mine += scale.units(key_of(list[i]));
+      const uint64_t total = block_sum<uint64_t>(mine, sh.tmp);
+      token = pick_among(s, scale, list, a.V, nullptr, nullptr, total, (uint32_t)a.V, 0, kBins, 0, sh);
+    }
+  }
+  if (tid == 0) a.tokens[r] = token;
+}
+
+template <int DT>
+int launch_sample(const tamd_sample_args &args, hipStream_t st) {
+  if (args.V <= kMost) {
+    short_row_kernel<DT><<<args.R, kThreads, 0, st>>>(args);
+    return launch_status();
+  }
+  int cus = 0;
+  if (int rc = cu_count(cus)) return rc;
+  for (int r = 0; r < args.R; r += kRowsAtOnce) {
+    tamd_sample_args a = args;
+    a.R = args.R - r < kRowsAtOnce ? args.R - r : kRowsAtOnce;
+    a.logits = (const uint8_t *)a.logits + r * a.logits_stride * dtype_size(a.logits_dtype);
+    a.u += r, a.tokens += r;
+    if (a.temperature) a.temperature += r;
+    if (a.top_k) a.top_k += r;
+    if (a.top_p) a.top_p += r;
+    if (a.min_p) a.min_p += r;
+    // chunks of 8192, longer ones where these are more than two workgroups per CU (each scans the row's histogram) or more than a wave reads
+    int chunk = kChunk;
+    while ((int64_t)((a.V + chunk - 1) / chunk) * a.R > 2 * cus && chunk < 8 * kChunk) chunk *= 2;
+    while ((a.V + chunk - 1) / chunk > kMaxChunks) chunk *= 2;
+    const Workspace ws = workspace_of(a.workspace, a.R);
+    const dim3 grid((unsigned)((a.V + chunk - 1) / chunk), (unsigned)a.R);
+    extremes_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
+    histogram_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
+    pick_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
+    if (int rc = launch_status()) return rc;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -194,7 +635,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_kernel(tamd_sample_args a)
 
 using namespace tamd;
 
-extern "C" int64_t tamd_sample_workspace(int R, int V) { return R < 0 || V < 0 ? TAMD_E_INVALID : 16; }
+extern "C" int64_t tamd_sample_workspace(int R, int V) {
+  if (R < 0 || V < 0) return TAMD_E_INVALID;
+  return V <= kMost ? 16 : (R < kRowsAtOnce ? R : kRowsAtOnce) * kRowBytes + 16;
+}
 
 extern "C" int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream) {
   if (!args || args_size != sizeof(tamd_sample_args)) return TAMD_E_INVALID;
@@ -204,9 +648,7 @@ extern "C" int tamd_sample(const tamd_sample_args *args, size_t args_size, void 
   if (a.V > (1 << 20) || a.R > (1 << 20)) return TAMD_E_TOO_LARGE;
   if (a.R == 0) return 0;
   if (!a.logits || !a.u || !a.tokens || !a.workspace || a.logits_stride < 0) return TAMD_E_INVALID;
+  if ((uintptr_t)a.workspace % 16 != 0) return TAMD_E_ALIGNMENT;
   hipStream_t st = (hipStream_t)stream;
-  if (a.logits_dtype == TAMD_F32) sample_kernel<TAMD_F32><<<a.R, kThreads, 0, st>>>(a);
-  else if (a.logits_dtype == TAMD_BF16) sample_kernel<TAMD_BF16><<<a.R, kThreads, 0, st>>>(a);
-  else sample_kernel<TAMD_F16><<<a.R, kThreads, 0, st>>>(a);
-  return launch_status();
+  return a.logits_dtype == TAMD_F32 ? launch_sample<TAMD_F32>(a, st) : a.logits_dtype == TAMD_BF16 ? launch_sample<TAMD_BF16>(a, st) : launch_sample<TAMD_F16>(a, st);
 }
