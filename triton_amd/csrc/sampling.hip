@@ -8,12 +8,12 @@
 // their order, so the same row gives the same token however the work is cut, and they are off by less than 2^-37 of the row's mass.
 // What rounds to zero is not there at all: it cannot be drawn, and adds nothing to what top-k keeps.
 //
-// Three launches over (chunk of a row, row):
+// Four launches, three of them over (chunk of a row, row):
 //   extremes   the largest logit with its index, and the smallest;
-//   histogram  count and mass of the logits in 2048 bins of equal width between the two (or down to where w is zero);
-//   pick       every workgroup finds in the histogram the few bins in which the ends of top-k, top-p and min-p and the token can
-//              lie, and collects its chunk's logits of those; the row's last workgroup sorts them (a few hundred of the whole
-//              vocabulary) and answers the questions exactly.
+//   histogram  mass (and for top-k count) of the logits in 2048 bins of equal width between the two, or down to where w is zero;
+//   collect    every workgroup finds in the histogram the few bins in which the ends of top-k, top-p and min-p and the token can
+//              lie, and gathers its chunk's logits of those, a few hundred of the whole vocabulary;
+//   finish     a workgroup per row sorts them and answers the questions exactly.
 // Rows of up to 4096 logits are sorted as they are, in one launch.  A row that has more than 4096 logits in those bins -- many
 // equal or nearly equal ones -- is searched by the bits of its keys (search_row): slower, but right for any row.
 #include "common.h"
@@ -56,49 +56,56 @@ TAMD_DEVICE uint32_t key_at(const void *logits, int64_t i) {
 }
 constexpr uint32_t kNothing = 0x007FFFFFu;   // key of -inf
 
-// 2^(-j / 256) by the threads of a workgroup.
-TAMD_DEVICE void make_powers(double *powers) {
-  if (threadIdx.x < 256) powers[threadIdx.x] = exp2((double)threadIdx.x * -0.00390625);
+// Bits of a weight of one: a row's weights together stay below 2^62, one below 2^51 (units_of).
+TAMD_DEVICE int fraction_bits(int V) {
+  const int b = 62 - (32 - __builtin_clz((uint32_t)V));
+  return b < 51 ? b : 51;
+}
+
+// 2^(fraction - j / 256) by the threads of a workgroup.
+TAMD_DEVICE void make_powers(double *powers, int V) {
+  if (threadIdx.x < 256) powers[threadIdx.x] = exp2(fraction_bits(V) - (double)threadIdx.x * 0.00390625);
 }
 
 // Weights of a row whose largest logit is `top` (> -inf).  y = log2(1 / w).
 struct RowScale {
   double top, to_y, to_bin;
   int fraction;
-  uint32_t top_key;
   bool infinite;     // with infinite logits these weigh alike and nothing else does
   const double *powers;
-  TAMD_DEVICE RowScale(uint32_t top_key_, uint32_t least_key, double t, int V, const double *powers_)
-      : top(logit_of(top_key_)), to_y(1.4426950408889634 / t), fraction(62 - (32 - __builtin_clz((uint32_t)V))), top_key(top_key_),
-        infinite(logit_of(top_key_) == __builtin_inff()), powers(powers_) {
-    const double most = y_of(least_key), range = most < fraction ? most : fraction;
+  TAMD_DEVICE RowScale(uint32_t top_key, uint32_t least_key, double t, int V, const double *powers_)
+      : top(logit_of(top_key)), to_y(1.4426950408889634 / t), fraction(fraction_bits(V)), infinite(logit_of(top_key) == __builtin_inff()), powers(powers_) {
+    const double most = y_of(logit_of(least_key)), range = most < fraction ? most : fraction;
     to_bin = range > 0.0 ? kBins / range : 0.0;
   }
-  TAMD_DEVICE double y_of(uint32_t key) const {
-    if (key == top_key) return 0.0;
-    return key <= kNothing || infinite ? 1e9 : (top - logit_of(key)) * to_y;
+  // (of -inf: infinite, or NaN at an infinite temperature; neither counts)
+  TAMD_DEVICE double y_of(float v) const {
+    if (infinite) return v == __builtin_inff() ? 0.0 : 1e9;
+    return (top - (double)v) * to_y;
   }
   TAMD_DEVICE bool counts(double y) const { return y < fraction; }
   TAMD_DEVICE int bin_of(double y) const {
     const double b = y * to_bin;
     return b >= kBins - 1 ? kBins - 1 : (int)b;
   }
-  // 2^(fraction - y), y cut into a whole number, a multiple of 1/256 (the table) and a rest below it (the series of 2^-r: five terms
-  // are off by 2^-52): a third of the instructions of exp(), which took longer than reading the logits
+  // 2^(fraction - y) of a y that counts, in units.  y in units of 2^-40 (the low bits of y + 1.5 * 2^12) is a whole number, eight bits for
+  // the table and the rest r for the series of 2^-r, whose first four terms leave 2.3e-12 of w; adding 2^52 makes a whole number
+  // of the product.  (With exp() and conversions this took longer than reading the logits.  Fused by hand: the histogram and
+  // the candidates have to agree to the last unit in every kernel.)
   TAMD_DEVICE uint64_t units_of(double y) const {
-    if (!counts(y)) return 0;
-    // (fused by hand: the histogram and the candidates have to agree to the last unit in every kernel)
-    const int n = (int)y;
-    const double f = y - n;
-    const int j = (int)(f * 256.0);
-    const double r = __builtin_fma(j, -0.00390625, f) * 0.6931471805599453;
-    double p = __builtin_fma(r, 1.0 / 24.0, -1.0 / 6.0);
-    p = __builtin_fma(r, p, 0.5);
+    const uint64_t fixed = __builtin_bit_cast(uint64_t, y + 6144.0) & 0xFFFFFFFFFFFFull;   // 6144 = 1.5 * 2^12: the lowest bit is 2^-40
+    const uint32_t whole = (uint32_t)(fixed >> 40) & 0x7FFu;
+    const double r = (double)(uint32_t)fixed * (0.6931471805599453 * 0x1p-40);
+    double p = __builtin_fma(r, -1.0 / 6.0, 0.5);
     p = __builtin_fma(r, p, -1.0);
     p = __builtin_fma(r, p, 1.0);
-    return (uint64_t)(powers[j] * p * (double)(1ull << fraction)) >> n;
+    const double x = __builtin_fma(powers[(uint32_t)(fixed >> 32) & 0xFFu], p, 0x1p52);
+    return (__builtin_bit_cast(uint64_t, x) & 0xFFFFFFFFFFFFFull) >> whole;
   }
-  TAMD_DEVICE uint64_t units(uint32_t key) const { return units_of(y_of(key)); }
+  TAMD_DEVICE uint64_t units(uint32_t key) const {
+    const double y = y_of(logit_of(key));
+    return counts(y) ? units_of(y) : 0;
+  }
 };
 
 struct Found {
@@ -146,7 +153,6 @@ struct Shared {
   int at[2];
   int token;
   uint32_t n, base;
-  bool last;
 };
 
 // The element of a whole row at which the running count (by_mass: mass) reaches `target` >= 1, eleven bits of its key at a time: a
@@ -261,7 +267,7 @@ TAMD_DEVICE int search_row(const tamd_sample_args &a, int r, const RowSettings &
   return -1;   // (not reached)
 }
 
-// A chunk's logits as keys, four at a time per thread whatever the row's alignment.
+// A chunk's logits, NaN as -inf, four at a time per thread whatever the row's alignment.
 template <int DT, typename F>
 TAMD_DEVICE void for_chunk(const tamd_sample_args &a, int64_t row, int begin, int end, F use) {
   for (int i0 = begin + 4 * (int)threadIdx.x; i0 < end; i0 += 4 * kThreads) {
@@ -276,9 +282,12 @@ TAMD_DEVICE void for_chunk(const tamd_sample_args &a, int64_t row, int begin, in
         for (int j = 0; j < 4; ++j) v[j] = DT == TAMD_BF16 ? bf16_bits_to_f32(b[j]) : f16_bits_to_f32(b[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) use(i0 + j, ordered_bits(v[j] != v[j] ? -__builtin_inff() : v[j]));
+      for (int j = 0; j < 4; ++j) use(i0 + j, v[j] != v[j] ? -__builtin_inff() : v[j]);
     } else {
-      for (int i = i0; i < end; ++i) use(i, key_at<DT>(a.logits, row + i));
+      for (int i = i0; i < end; ++i) {
+        const float v = load_as_f32<DT>(a.logits, row + i);
+        use(i, v != v ? -__builtin_inff() : v);
+      }
     }
   }
 }
@@ -294,17 +303,16 @@ struct Workspace {
   uint64_t *mass;         // [rows, bins]
   uint32_t *count;        // [rows, bins]
   uint32_t *collected;    // [rows] candidates
-  uint32_t *ticket;       // [rows] workgroups that are done
   uint64_t *candidates;   // [rows, kMost]
 };
-constexpr int64_t kRowBytes = kMaxChunks * 12 + kBins * 12 + 8 + kMost * 8;
+constexpr int64_t kRowBytes = kMaxChunks * 12 + kBins * 12 + 4 + kMost * 8;
 
 inline Workspace workspace_of(void *p, int rows) {
   uint8_t *at = (uint8_t *)p;
   const auto take = [&](int64_t bytes) { uint8_t *q = at; at += bytes * rows; return q; };
   Workspace w;
   w.candidates = (uint64_t *)take(kMost * 8), w.mass = (uint64_t *)take(kBins * 8), w.first = (uint64_t *)take(kMaxChunks * 8);
-  w.count = (uint32_t *)take(kBins * 4), w.least = (uint32_t *)take(kMaxChunks * 4), w.collected = (uint32_t *)take(4), w.ticket = (uint32_t *)take(4);
+  w.count = (uint32_t *)take(kBins * 4), w.least = (uint32_t *)take(kMaxChunks * 4), w.collected = (uint32_t *)take(4);
   return w;
 }
 
@@ -314,10 +322,11 @@ __global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, 
   __shared__ uint32_t s_least[kWaves];
   const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
   for (int b = c * kThreads + tid; b < kBins; b += gridDim.x * kThreads) ws.mass[(int64_t)r * kBins + b] = 0, ws.count[(int64_t)r * kBins + b] = 0;
-  if (c == 0 && tid == 0) ws.collected[r] = 0, ws.ticket[r] = 0;
+  if (c == 0 && tid == 0) ws.collected[r] = 0;
   uint64_t first = 0;
   uint32_t least = 0xFFFFFFFFu;
-  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, uint32_t key) {
+  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, float v) {
+    const uint32_t key = ordered_bits(v);
     const uint64_t e = element_of(key, i);
     first = e > first ? e : first;
     least = key > kNothing && key < least ? key : least;
@@ -365,23 +374,23 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
   row_extremes(ws, r, gridDim.x, first, least);
   const RowSettings s = settings_of(a, r);
   if (s.greedy || key_of(first) <= kNothing) return;
-  make_powers(powers);
+  make_powers(powers, a.V);
   for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
   const RowScale scale(key_of(first), least, s.t, a.V, powers);
   sync_threads();
-  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int, uint32_t key) {
-    const double y = scale.y_of(key);
+  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int, float v) {
+    const double y = scale.y_of(v);
     if (scale.counts(y)) {
       const int b = scale.bin_of(y);
       atomicAdd((unsigned long long *)&mass[b], (unsigned long long)scale.units_of(y));
-      atomicAdd(&count[b], 1u);
+      if (s.top_k) atomicAdd(&count[b], 1u);   // (nothing else asks for counts)
     }
   });
   sync_threads();
   for (int b = tid; b < kBins; b += kThreads)
-    if (count[b]) {
+    if (mass[b]) {
       atomicAdd((unsigned long long *)&ws.mass[(int64_t)r * kBins + b], (unsigned long long)mass[b]);
-      atomicAdd(&ws.count[(int64_t)r * kBins + b], count[b]);
+      if (s.top_k) atomicAdd(&ws.count[(int64_t)r * kBins + b], count[b]);
     }
 }
 
@@ -415,9 +424,9 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int i = PER * tid + j;
-    const double y = i < n ? scale.y_of(key_of(list[i])) : 1e9;
-    units[j] = scale.units_of(y);
-    bin[j] = i < n && scale.counts(y) ? scale.bin_of(y) : -1;
+    const double y = i < n ? scale.y_of(logit_of(key_of(list[i]))) : 1e9;
+    units[j] = scale.counts(y) ? scale.units_of(y) : 0;
+    bin[j] = scale.counts(y) ? scale.bin_of(y) : -1;
     before[j] = run;
     run += units[j];
     enough += bin[j] >= min_lo && bin[j] <= min_hi && units[j] >= least ? units[j] : 0;
@@ -427,9 +436,9 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int i = PER * tid + j;
-      if (bin[j] >= 0 && (i == 0 || scale.bin_of(scale.y_of(key_of(list[i - 1]))) != bin[j])) {
+      if (bin[j] >= 0 && (i == 0 || scale.bin_of(scale.y_of(logit_of(key_of(list[i - 1])))) != bin[j])) {
         before_mass[bin[j]] -= start + before[j];
-        before_rank[bin[j]] -= (uint32_t)i;
+        if (s.top_k) before_rank[bin[j]] -= (uint32_t)i;
       }
     }
   }
@@ -439,7 +448,7 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
   for (int j = 0; j < PER; ++j) {
     const bool adds = before_mass && bin[j] >= 0;
     before[j] += start + (adds ? before_mass[bin[j]] : 0);
-    rank[j] = (uint32_t)(PER * tid + j) + (adds ? before_rank[bin[j]] : 0u);
+    rank[j] = (uint32_t)(PER * tid + j) + (adds && s.top_k ? before_rank[bin[j]] : 0u);
   }
   if (s.top_k && (uint32_t)s.top_k < total_count) {
 #pragma unroll
@@ -483,107 +492,123 @@ TAMD_DEVICE int bin_reaching(const T *before, T target, int &slot) {
   return found;
 }
 
+// What lies in front of every bin of a row's histogram, and the bins in which the ends of what is kept and the token can lie:
+// lo and hi enclose the sum of what is kept.  Every thread of the workgroup comes along.
+struct BinSums {
+  uint64_t mass[kBins + 1];
+  uint32_t rank[kBins + 1];
+};
+struct Wanted {
+  int from[4] = {kBins, kBins, kBins, kBins}, to[4] = {-1, -1, -1, -1};
+  uint64_t min_mass = 0;   // in front of the bins in which min-p ends
+  TAMD_DEVICE bool has(int b) const {
+    bool is = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) is |= b >= from[j] && b <= to[j];
+    return is;
+  }
+};
+TAMD_DEVICE Wanted wanted_bins(const Workspace &ws, int r, const RowSettings &s, const RowScale &scale, BinSums &before, Shared &sh) {
+  static_assert(kBins == 2 * kThreads);
+  const int tid = threadIdx.x;
+  const int64_t h = (int64_t)r * kBins + 2 * tid;
+  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1], upto = block_scan<uint64_t>(m0 + m1, sh.tmp);
+  before.mass[2 * tid] = upto - m0 - m1, before.mass[2 * tid + 1] = upto - m1;
+  if (tid == kThreads - 1) before.mass[kBins] = upto;
+  if (s.top_k) {
+    const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1], n = (uint32_t)block_scan<uint64_t>(n0 + n1, sh.tmp);
+    before.rank[2 * tid] = n - n0 - n1, before.rank[2 * tid + 1] = n - n1;
+    if (tid == kThreads - 1) before.rank[kBins] = n;
+  }
+  sync_threads();
+  Wanted w;
+  uint64_t lo = before.mass[kBins], hi = lo;
+  if (s.top_k && (uint32_t)s.top_k < before.rank[kBins]) {
+    w.from[0] = w.to[0] = bin_reaching<uint32_t>(before.rank, (uint32_t)s.top_k, sh.at[0]);
+    lo = before.mass[w.from[0]], hi = before.mass[w.to[0] + 1];
+  }
+  if (s.top_p < 1.0) {
+    w.from[1] = bin_reaching<uint64_t>(before.mass, top_p_target(s.top_p, lo), sh.at[0]);
+    w.to[1] = bin_reaching<uint64_t>(before.mass, top_p_target(s.top_p, hi), sh.at[1]);
+    lo = before.mass[w.from[1]];
+    hi = before.mass[w.to[1] + 1] < hi ? before.mass[w.to[1] + 1] : hi;
+  }
+  if (s.min_p > 0.0) {
+    const double y = -log2(s.min_p);
+    const int b = scale.counts(y) ? scale.bin_of(y) : kBins - 1;
+    w.from[2] = b > 0 ? b - 1 : 0, w.to[2] = b < kBins - 1 ? b + 1 : kBins - 1;
+    w.min_mass = before.mass[w.from[2]];
+    lo = w.min_mass < lo ? w.min_mass : lo;
+    hi = before.mass[w.to[2] + 1] < hi ? before.mass[w.to[2] + 1] : hi;
+  }
+  w.from[3] = bin_reaching<uint64_t>(before.mass, token_target(s.u, lo), sh.at[0]);
+  w.to[3] = bin_reaching<uint64_t>(before.mass, token_target(s.u, hi), sh.at[1]);
+  return w;
+}
+
+// A chunk's candidates, gathered in LDS first: an atomic on the row's counter takes a trip to memory, and they take turns (one per
+// candidate: 282 us for 64 rows of 131072).  More than kMost are only counted.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void pick_kernel(tamd_sample_args a, Workspace ws, int chunk) {
-  __shared__ uint64_t before_mass[kBins + 1];
+__global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, Workspace ws, int chunk) {
+  __shared__ BinSums before;
   __shared__ uint64_t list[kMost];
-  __shared__ uint32_t before_rank[kBins + 1];
-  __shared__ double powers[256];
   __shared__ Shared sh;
   const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
   uint64_t first;
   uint32_t least;
   row_extremes(ws, r, gridDim.x, first, least);
   const RowSettings s = settings_of(a, r);
-  if (s.greedy || key_of(first) <= kNothing) {
-    if (c == 0 && tid == 0) a.tokens[r] = key_of(first) <= kNothing ? -1 : index_of(first);
-    return;
-  }
-  make_powers(powers);
-  const RowScale scale(key_of(first), least, s.t, a.V, powers);
-  // ---- what lies in front of every bin
-  static_assert(kBins == 2 * kThreads);
-  const int64_t h = (int64_t)r * kBins + 2 * tid;
-  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1];
-  const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1];
-  const uint64_t upto = block_scan<uint64_t>(m0 + m1, sh.tmp);
-  const uint64_t upto_n = block_scan<uint64_t>(n0 + n1, sh.tmp);
-  before_mass[2 * tid] = upto - m0 - m1, before_mass[2 * tid + 1] = upto - m1;
-  before_rank[2 * tid] = (uint32_t)upto_n - n0 - n1, before_rank[2 * tid + 1] = (uint32_t)upto_n - n1;
-  if (tid == kThreads - 1) before_mass[kBins] = upto, before_rank[kBins] = (uint32_t)upto_n;
-  sync_threads();
-  const uint64_t total = before_mass[kBins];
-  const uint32_t total_n = before_rank[kBins];
-  // ---- the bins of the candidates: lo and hi enclose the sum of what is kept
-  int from[4] = {kBins, kBins, kBins, kBins}, to[4] = {-1, -1, -1, -1};
-  uint64_t lo = total, hi = total;
-  if (s.top_k && (uint32_t)s.top_k < total_n) {
-    from[0] = to[0] = bin_reaching<uint32_t>(before_rank, (uint32_t)s.top_k, sh.at[0]);
-    lo = before_mass[from[0]], hi = before_mass[to[0] + 1];
-  }
-  if (s.top_p < 1.0) {
-    from[1] = bin_reaching<uint64_t>(before_mass, top_p_target(s.top_p, lo), sh.at[0]);
-    to[1] = bin_reaching<uint64_t>(before_mass, top_p_target(s.top_p, hi), sh.at[1]);
-    lo = before_mass[from[1]];
-    hi = before_mass[to[1] + 1] < hi ? before_mass[to[1] + 1] : hi;
-  }
-  uint64_t min_mass = 0;
-  if (s.min_p > 0.0) {
-    const double y = -log2(s.min_p);
-    const int b = scale.counts(y) ? scale.bin_of(y) : kBins - 1;
-    from[2] = b > 0 ? b - 1 : 0, to[2] = b < kBins - 1 ? b + 1 : kBins - 1;
-    min_mass = before_mass[from[2]];
-    lo = min_mass < lo ? min_mass : lo;
-    hi = before_mass[to[2] + 1] < hi ? before_mass[to[2] + 1] : hi;
-  }
-  from[3] = bin_reaching<uint64_t>(before_mass, token_target(s.u, lo), sh.at[0]);
-  to[3] = bin_reaching<uint64_t>(before_mass, token_target(s.u, hi), sh.at[1]);
-  const auto wanted = [&](int b) {
-    bool is = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) is |= b >= from[j] && b <= to[j];
-    return is;
-  };
-  const uint64_t n_all = block_sum<uint64_t>((wanted(2 * tid) ? n0 : 0u) + (wanted(2 * tid + 1) ? n1 : 0u), sh.tmp);
-  if (n_all > kMost) {
-    if (c == 0) {
-      const int token = search_row<DT>(a, r, s, scale, list, sh);
-      if (tid == 0) a.tokens[r] = token;
-    }
-    return;
-  }
-  // ---- collect them, in LDS first (an atomic on the row's counter takes a trip to memory, and they take turns: with one per candidate
-  // the launch took 282 us for 64 rows of 131072); the row's last workgroup goes on
+  if (s.greedy || key_of(first) <= kNothing) return;
+  const RowScale scale(key_of(first), least, s.t, a.V, nullptr);
   if (tid == 0) sh.n = 0;
-  sync_threads();
-  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, uint32_t key) {
-    const double y = scale.y_of(key);
-    if (scale.counts(y) && wanted(scale.bin_of(y))) {
+  const Wanted wanted = wanted_bins(ws, r, s, scale, before, sh);
+  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, float v) {
+    const double y = scale.y_of(v);
+    if (scale.counts(y) && wanted.has(scale.bin_of(y))) {
       const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < kMost) list[at] = element_of(key, i);
+      if (at < kMost) list[at] = element_of(ordered_bits(v), i);
     }
   });
   sync_threads();
-  const uint32_t mine = sh.n < kMost ? sh.n : kMost;
-  if (tid == 0) sh.base = mine ? atomicAdd(&ws.collected[r], mine) : 0;
+  const uint32_t n = sh.n, stored = n < kMost ? n : kMost;
+  if (n == 0) return;
+  if (tid == 0) sh.base = atomicAdd(&ws.collected[r], n);
   sync_threads();
-  for (uint32_t i = tid; i < mine; i += kThreads)
-    if (sh.base + i < kMost)
-      __hip_atomic_store(&ws.candidates[(int64_t)r * kMost + sh.base + i], list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // One thread releases for all, behind a barrier that waits for their stores: a fence of every wave writes the XCD's L2 back
-  // sixteen times per workgroup.
-  sync_threads();
-  if (tid == 0) {
-    __threadfence();
-    sh.last = atomicAdd(&ws.ticket[r], 1u) + 1 == gridDim.x;
-    __threadfence();
+  for (uint32_t i = tid; i < stored; i += kThreads)
+    if (sh.base + i < kMost) ws.candidates[(int64_t)r * kMost + sh.base + i] = list[i];
+}
+
+// The token of a row.  (A launch of its own: as the last workgroup of the row in the launch before, found by a ticket, it cost a
+// write-back of the L2 per workgroup, 61 us for 64 rows of 131072 instead of TODO.)
+template <int DT>
+__global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Workspace ws, int chunks) {
+  __shared__ BinSums before;
+  __shared__ uint64_t list[kMost];
+  __shared__ double powers[256];
+  __shared__ Shared sh;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  uint64_t first;
+  uint32_t least;
+  row_extremes(ws, r, chunks, first, least);
+  const RowSettings s = settings_of(a, r);
+  int token = -1;
+  if (key_of(first) > kNothing && s.greedy) {
+    token = index_of(first);
+  } else if (key_of(first) > kNothing) {
+    make_powers(powers, a.V);
+    const RowScale scale(key_of(first), least, s.t, a.V, powers);
+    const int n = (int)(ws.collected[r] < kMost + 1 ? ws.collected[r] : kMost + 1);
+    for (int i = tid; i < n && i < kMost; i += kThreads) list[i] = ws.candidates[(int64_t)r * kMost + i];
+    if (n > kMost) {
+      sync_threads();
+      token = search_row<DT>(a, r, s, scale, list, sh);
+    } else {
+      const Wanted wanted = wanted_bins(ws, r, s, scale, before, sh);
+      sort_elements(list, n);
+      token = pick_among(s, scale, list, n, before.mass, before.rank, before.mass[kBins], s.top_k ? before.rank[kBins] : 0u, wanted.from[2], wanted.to[2],
+                         wanted.min_mass, sh);
+    }
   }
-  sync_threads();
-  if (!sh.last) return;
-  const int n = (int)n_all;
-  for (int i = tid; i < n; i += kThreads) list[i] = __hip_atomic_load(&ws.candidates[(int64_t)r * kMost + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  sort_elements(list, n);
-  const int token = pick_among(s, scale, list, n, before_mass, before_rank, total, total_n, from[2], to[2], min_mass, sh);
   if (tid == 0) a.tokens[r] = token;
 }
 
@@ -595,7 +620,7 @@ __global__ __launch_bounds__(kThreads) void short_row_kernel(tamd_sample_args a)
   __shared__ Shared sh;
   const int r = blockIdx.x, tid = threadIdx.x;
   const RowSettings s = settings_of(a, r);
-  make_powers(powers);
+  make_powers(powers, a.V);
   for (int i = tid; i < a.V; i += kThreads) list[i] = element_of(key_at<DT>(a.logits, r * a.logits_stride + i), i);
   sort_elements(list, a.V);
   const uint32_t top = key_of(list[0]);
@@ -639,7 +664,8 @@ int launch_sample(const tamd_sample_args &args, hipStream_t st) {
     const dim3 grid((unsigned)((a.V + chunk - 1) / chunk), (unsigned)a.R);
     extremes_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
     histogram_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
-    pick_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
+    collect_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
+    finish_kernel<DT><<<a.R, kThreads, 0, st>>>(a, ws, (int)grid.x);
     if (int rc = launch_status()) return rc;
   }
   return 0;
