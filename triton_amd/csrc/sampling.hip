@@ -8,11 +8,12 @@
 // their order, so the same row gives the same token however the work is cut, and they are off by less than 2^-37 of the row's mass.
 // What rounds to zero is not there at all: it cannot be drawn, and adds nothing to what top-k keeps.
 //
-// Four launches, three of them over (chunk of a row, row):
+// Five launches, three of them over (chunk of a row, row):
 //   extremes   the largest logit with its index, and the smallest;
 //   histogram  mass (and for top-k count) of the logits in 2048 bins of equal width between the two, or down to where w is zero;
-//   collect    every workgroup finds in the histogram the few bins in which the ends of top-k, top-p and min-p and the token can
-//              lie, and gathers its chunk's logits of those, a few hundred of the whole vocabulary;
+//   bounds     a workgroup per row finds in the histogram the few bins in which the ends of top-k, top-p and min-p and the token
+//              can lie;
+//   collect    gathers the logits of those, a few hundred of the whole vocabulary;
 //   finish     a workgroup per row sorts them and answers the questions exactly.
 // Rows of up to 4096 logits are sorted as they are, in one launch.  A row that has more than 4096 logits in those bins -- many
 // equal or nearly equal ones -- is searched by the bits of its keys (search_row): slower, but right for any row.
@@ -73,6 +74,8 @@ struct RowScale {
   int fraction;
   bool infinite;     // with infinite logits these weigh alike and nothing else does
   const double *powers;
+  TAMD_DEVICE RowScale(double top_, double to_y_, double to_bin_, int V, const double *powers_)
+      : top(top_), to_y(to_y_), to_bin(to_bin_), fraction(fraction_bits(V)), infinite(top_ == __builtin_inf()), powers(powers_) {}
   TAMD_DEVICE RowScale(uint32_t top_key, uint32_t least_key, double t, int V, const double *powers_)
       : top(logit_of(top_key)), to_y(1.4426950408889634 / t), fraction(fraction_bits(V)), infinite(logit_of(top_key) == __builtin_inff()), powers(powers_) {
     const double most = y_of(logit_of(least_key)), range = most < fraction ? most : fraction;
@@ -267,30 +270,52 @@ TAMD_DEVICE int search_row(const tamd_sample_args &a, int r, const RowSettings &
   return -1;   // (not reached)
 }
 
-// A chunk's logits, NaN as -inf, four at a time per thread whatever the row's alignment.
-template <int DT, typename F>
-TAMD_DEVICE void for_chunk(const tamd_sample_args &a, int64_t row, int begin, int end, F use) {
-  for (int i0 = begin + 4 * (int)threadIdx.x; i0 < end; i0 += 4 * kThreads) {
-    if (i0 + 4 <= end) {
-      float v[4];
-      if constexpr (DT == TAMD_F32) {
-        __builtin_memcpy(v, (const float *)a.logits + row + i0, 16);
+// A chunk's logits, NaN as -inf, eight per thread at a time in two vectors whatever the row's alignment; what is past the end is
+// -inf.  The next eight are requested before the last are used, the first eight as soon as this is made: each launch has a
+// trip to memory or two in front of its first use, and with one vector in flight the largest logit of 64 rows of 131072 took 9.6 us.
+template <int DT>
+struct Chunk {
+  static constexpr int kStep = 8 * kThreads;
+  const tamd_sample_args &a;
+  int64_t row;
+  int at, end;
+  float v[8];
+  TAMD_DEVICE Chunk(const tamd_sample_args &a_, int r, int c, int chunk)
+      : a(a_), row(r * a_.logits_stride), at(c * chunk), end(at + chunk < a_.V ? at + chunk : a_.V) { request(); }
+  TAMD_DEVICE void request() {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int i = at + 4 * (q * kThreads + (int)threadIdx.x);
+      float *to = v + 4 * q;
+      if (i + 4 <= end) {
+        if constexpr (DT == TAMD_F32) {
+          __builtin_memcpy(to, (const float *)a.logits + row + i, 16);
+        } else {
+          uint16_t b[4];
+          __builtin_memcpy(b, (const uint16_t *)a.logits + row + i, 8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[j] = DT == TAMD_BF16 ? bf16_bits_to_f32(b[j]) : f16_bits_to_f32(b[j]);
+        }
       } else {
-        uint16_t b[4];
-        __builtin_memcpy(b, (const uint16_t *)a.logits + row + i0, 8);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = DT == TAMD_BF16 ? bf16_bits_to_f32(b[j]) : f16_bits_to_f32(b[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) use(i0 + j, v[j] != v[j] ? -__builtin_inff() : v[j]);
-    } else {
-      for (int i = i0; i < end; ++i) {
-        const float v = load_as_f32<DT>(a.logits, row + i);
-        use(i, v != v ? -__builtin_inff() : v);
+        for (int j = 0; j < 4; ++j) to[j] = i + j < end ? load_as_f32<DT>(a.logits, row + i + j) : -__builtin_inff();
       }
     }
   }
-}
+  template <typename F>
+  TAMD_DEVICE void each(F use) {
+    while (at < end) {
+      float now[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now[j] = v[j];
+      const int from = at + 4 * (int)threadIdx.x;
+      at += kStep;
+      if (at < end) request();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) use(from + (j / 4) * 4 * kThreads + j % 4, now[j] != now[j] ? -__builtin_inff() : now[j]);
+    }
+  }
+};
 
 // Element of the order as one number: the larger, the earlier.
 TAMD_DEVICE uint64_t element_of(uint32_t key, int i) { return (uint64_t)key << 32 | (0xFFFFFFFFu - (uint32_t)i); }
@@ -304,14 +329,15 @@ struct Workspace {
   uint32_t *count;        // [rows, bins]
   uint32_t *collected;    // [rows] candidates
   uint64_t *candidates;   // [rows, kMost]
+  void *bounds;           // [rows] Bounds
 };
-constexpr int64_t kRowBytes = kMaxChunks * 12 + kBins * 12 + 4 + kMost * 8;
+constexpr int64_t kRowBytes = kMaxChunks * 12 + kBins * 12 + 4 + kMost * 8 + 96;
 
 inline Workspace workspace_of(void *p, int rows) {
   uint8_t *at = (uint8_t *)p;
   const auto take = [&](int64_t bytes) { uint8_t *q = at; at += bytes * rows; return q; };
   Workspace w;
-  w.candidates = (uint64_t *)take(kMost * 8), w.mass = (uint64_t *)take(kBins * 8), w.first = (uint64_t *)take(kMaxChunks * 8);
+  w.candidates = (uint64_t *)take(kMost * 8), w.bounds = take(96), w.mass = (uint64_t *)take(kBins * 8), w.first = (uint64_t *)take(kMaxChunks * 8);
   w.count = (uint32_t *)take(kBins * 4), w.least = (uint32_t *)take(kMaxChunks * 4), w.collected = (uint32_t *)take(4);
   return w;
 }
@@ -320,12 +346,13 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, Workspace ws, int chunk) {
   __shared__ uint64_t s_first[kWaves];
   __shared__ uint32_t s_least[kWaves];
-  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  Chunk<DT> logits(a, r, c, chunk);
   for (int b = c * kThreads + tid; b < kBins; b += gridDim.x * kThreads) ws.mass[(int64_t)r * kBins + b] = 0, ws.count[(int64_t)r * kBins + b] = 0;
   if (c == 0 && tid == 0) ws.collected[r] = 0;
   uint64_t first = 0;
   uint32_t least = 0xFFFFFFFFu;
-  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, float v) {
+  logits.each([&](int i, float v) {
     const uint32_t key = ordered_bits(v);
     const uint64_t e = element_of(key, i);
     first = e > first ? e : first;
@@ -368,7 +395,8 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
   __shared__ uint64_t mass[kBins];
   __shared__ uint32_t count[kBins];
   __shared__ double powers[256];
-  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  Chunk<DT> logits(a, r, c, chunk);
   uint64_t first;
   uint32_t least;
   row_extremes(ws, r, gridDim.x, first, least);
@@ -378,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
   for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
   const RowScale scale(key_of(first), least, s.t, a.V, powers);
   sync_threads();
-  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int, float v) {
+  logits.each([&](int, float v) {
     const double y = scale.y_of(v);
     if (scale.counts(y)) {
       const int b = scale.bin_of(y);
@@ -394,15 +422,32 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
     }
 }
 
-// n elements in `list` (room for the next power of two), largest first afterwards.
-TAMD_DEVICE void sort_elements(uint64_t *list, int n) {
+// n <= kMost elements of `list` (room for the next power of two), largest first afterwards.  Up to 1024 by counting the larger ones of
+// each, all threads sharing the comparisons (a few hundred: one barrier or two instead of 45), else in steps of the bitonic network.
+TAMD_DEVICE void sort_elements(uint64_t *list, int n, uint32_t *rank) {
+  const int tid = threadIdx.x;
+  if (n <= kThreads) {
+    int wide = kWave;
+    while (wide < n) wide *= 2;
+    const int i = tid % wide, part = tid / wide, parts = kThreads / wide;
+    rank[tid] = 0;
+    sync_threads();
+    const uint64_t e = i < n ? list[i] : 0;
+    uint32_t larger = 0;
+    for (int j = n * part / parts; j < n * (part + 1) / parts; ++j) larger += list[j] > e;
+    if (i < n && larger) atomicAdd(&rank[i], larger);
+    sync_threads();
+    if (tid < n) list[rank[tid]] = e;   // (wide >= n: thread tid holds element tid; all are different)
+    sync_threads();
+    return;
+  }
   int size = 2;
   while (size < n) size *= 2;
-  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) list[i] = 0;
+  for (int i = n + tid; i < size; i += kThreads) list[i] = 0;
   sync_threads();
   for (int k = 2; k <= size; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
-      for (int p = threadIdx.x; p < size / 2; p += kThreads) {
+      for (int p = tid; p < size / 2; p += kThreads) {
         const int i = 2 * j * (p / j) + p % j;
         const uint64_t x = list[i], y = list[i + j];
         if ((x < y) == ((i & k) == 0)) list[i] = y, list[i + j] = x;
@@ -411,10 +456,10 @@ TAMD_DEVICE void sort_elements(uint64_t *list, int n) {
     }
 }
 
-// The token, from n <= kMost sorted candidates.  before_mass / before_rank: what lies in front of a bin (null: the candidates are the
+// The token, from n <= kMost sorted candidates.  before_mass / before_rank: what lies in front of every bin (null: the candidates are the
 // whole row); min_lo, min_hi: the bins in which min-p ends, min_mass: what lies in front of them.
-TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const uint64_t *list, int n, uint64_t *before_mass, uint32_t *before_rank, uint64_t total_mass,
-                           uint32_t total_count, int min_lo, int min_hi, uint64_t min_mass, Shared &sh) {
+TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const uint64_t *list, int n, const uint64_t *before_mass, const uint32_t *before_rank,
+                           uint64_t total_mass, uint32_t total_count, int min_lo, int min_hi, uint64_t min_mass, uint64_t *bin_mass, uint32_t *bin_rank, Shared &sh) {
   constexpr int PER = kMost / kThreads;
   const int tid = threadIdx.x;
   uint64_t units[PER], before[PER], run = 0, enough = 0;
@@ -432,13 +477,13 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
     enough += bin[j] >= min_lo && bin[j] <= min_hi && units[j] >= least ? units[j] : 0;
   }
   const uint64_t start = block_scan<uint64_t>(run, sh.tmp) - run;
-  if (before_mass) {   // the first candidate of a bin turns what lies in front of the bin into what its candidates' running sums lack
+  if (before_mass) {   // the first candidate of a bin leaves what the running sums of the bin's candidates lack
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int i = PER * tid + j;
       if (bin[j] >= 0 && (i == 0 || scale.bin_of(scale.y_of(logit_of(key_of(list[i - 1])))) != bin[j])) {
-        before_mass[bin[j]] -= start + before[j];
-        if (s.top_k) before_rank[bin[j]] -= (uint32_t)i;
+        bin_mass[bin[j]] = before_mass[bin[j]] - (start + before[j]);
+        if (s.top_k) bin_rank[bin[j]] = before_rank[bin[j]] - (uint32_t)i;
       }
     }
   }
@@ -447,8 +492,8 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const bool adds = before_mass && bin[j] >= 0;
-    before[j] += start + (adds ? before_mass[bin[j]] : 0);
-    rank[j] = (uint32_t)(PER * tid + j) + (adds && s.top_k ? before_rank[bin[j]] : 0u);
+    before[j] += start + (adds ? bin_mass[bin[j]] : 0);
+    rank[j] = (uint32_t)(PER * tid + j) + (adds && s.top_k ? bin_rank[bin[j]] : 0u);
   }
   if (s.top_k && (uint32_t)s.top_k < total_count) {
 #pragma unroll
@@ -492,81 +537,100 @@ TAMD_DEVICE int bin_reaching(const T *before, T target, int &slot) {
   return found;
 }
 
-// What lies in front of every bin of a row's histogram, and the bins in which the ends of what is kept and the token can lie:
-// lo and hi enclose the sum of what is kept.  Every thread of the workgroup comes along.
-struct BinSums {
-  uint64_t mass[kBins + 1];
-  uint32_t rank[kBins + 1];
+// What the last two launches are told about a row.
+struct Bounds {
+  int from[4], to[4];      // bins of the candidates: the ends of top-k, top-p and min-p, and the token
+  uint64_t mass, min_mass; // of the row; in front of the bins in which min-p ends
+  double top, to_y, to_bin;
+  uint32_t count;
+  int done;                // the token is known
 };
-struct Wanted {
-  int from[4] = {kBins, kBins, kBins, kBins}, to[4] = {-1, -1, -1, -1};
-  uint64_t min_mass = 0;   // in front of the bins in which min-p ends
-  TAMD_DEVICE bool has(int b) const {
-    bool is = false;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) is |= b >= from[j] && b <= to[j];
-    return is;
-  }
-};
-TAMD_DEVICE Wanted wanted_bins(const Workspace &ws, int r, const RowSettings &s, const RowScale &scale, BinSums &before, Shared &sh) {
+static_assert(sizeof(Bounds) <= 96);
+
+// The bins in which the ends of what is kept and the token can lie: lo and hi enclose the sum of what is kept.  The row's histogram
+// becomes what lies in front of every bin.  (In a launch of its own: done by every workgroup of the next two, as at first, these took
+// 40 us for 64 rows of 131072; the three now take 33, for one row 18 instead of 21.)
+__global__ __launch_bounds__(kThreads) void bounds_kernel(tamd_sample_args a, Workspace ws, int chunks) {
+  __shared__ uint64_t mass[kBins + 1];
+  __shared__ uint32_t rank[kBins + 1];
+  __shared__ Shared sh;
   static_assert(kBins == 2 * kThreads);
-  const int tid = threadIdx.x;
+  const int r = blockIdx.x, tid = threadIdx.x;
   const int64_t h = (int64_t)r * kBins + 2 * tid;
-  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1], upto = block_scan<uint64_t>(m0 + m1, sh.tmp);
-  before.mass[2 * tid] = upto - m0 - m1, before.mass[2 * tid + 1] = upto - m1;
-  if (tid == kThreads - 1) before.mass[kBins] = upto;
+  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1];
+  const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1];
+  uint64_t first;
+  uint32_t least;
+  row_extremes(ws, r, chunks, first, least);
+  const RowSettings s = settings_of(a, r);
+  Bounds *out = (Bounds *)ws.bounds + r;
+  if (s.greedy || key_of(first) <= kNothing) {
+    if (tid == 0) out->done = 1, a.tokens[r] = key_of(first) <= kNothing ? -1 : index_of(first);
+    return;
+  }
+  const RowScale scale(key_of(first), least, s.t, a.V, nullptr);
+  const uint64_t upto = block_scan<uint64_t>(m0 + m1, sh.tmp);
+  ws.mass[h] = mass[2 * tid] = upto - m0 - m1, ws.mass[h + 1] = mass[2 * tid + 1] = upto - m1;
+  if (tid == kThreads - 1) mass[kBins] = upto;
   if (s.top_k) {
-    const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1], n = (uint32_t)block_scan<uint64_t>(n0 + n1, sh.tmp);
-    before.rank[2 * tid] = n - n0 - n1, before.rank[2 * tid + 1] = n - n1;
-    if (tid == kThreads - 1) before.rank[kBins] = n;
+    const uint32_t n = block_scan<uint32_t>(n0 + n1, (uint32_t *)sh.tmp);
+    ws.count[h] = rank[2 * tid] = n - n0 - n1, ws.count[h + 1] = rank[2 * tid + 1] = n - n1;
+    if (tid == kThreads - 1) rank[kBins] = n;
   }
   sync_threads();
-  Wanted w;
-  uint64_t lo = before.mass[kBins], hi = lo;
-  if (s.top_k && (uint32_t)s.top_k < before.rank[kBins]) {
-    w.from[0] = w.to[0] = bin_reaching<uint32_t>(before.rank, (uint32_t)s.top_k, sh.at[0]);
-    lo = before.mass[w.from[0]], hi = before.mass[w.to[0] + 1];
+  Bounds b;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b.from[j] = kBins, b.to[j] = -1;
+  b.mass = mass[kBins], b.count = s.top_k ? rank[kBins] : 0u, b.min_mass = 0, b.done = 0;
+  b.top = scale.top, b.to_y = scale.to_y, b.to_bin = scale.to_bin;
+  uint64_t lo = b.mass, hi = lo;
+  if (s.top_k && (uint32_t)s.top_k < b.count) {
+    b.from[0] = b.to[0] = bin_reaching<uint32_t>(rank, (uint32_t)s.top_k, sh.at[0]);
+    lo = mass[b.from[0]], hi = mass[b.to[0] + 1];
   }
   if (s.top_p < 1.0) {
-    w.from[1] = bin_reaching<uint64_t>(before.mass, top_p_target(s.top_p, lo), sh.at[0]);
-    w.to[1] = bin_reaching<uint64_t>(before.mass, top_p_target(s.top_p, hi), sh.at[1]);
-    lo = before.mass[w.from[1]];
-    hi = before.mass[w.to[1] + 1] < hi ? before.mass[w.to[1] + 1] : hi;
+    b.from[1] = bin_reaching<uint64_t>(mass, top_p_target(s.top_p, lo), sh.at[0]);
+    b.to[1] = lo == hi ? b.from[1] : bin_reaching<uint64_t>(mass, top_p_target(s.top_p, hi), sh.at[1]);
+    lo = mass[b.from[1]];
+    hi = mass[b.to[1] + 1] < hi ? mass[b.to[1] + 1] : hi;
   }
   if (s.min_p > 0.0) {
     const double y = -log2(s.min_p);
-    const int b = scale.counts(y) ? scale.bin_of(y) : kBins - 1;
-    w.from[2] = b > 0 ? b - 1 : 0, w.to[2] = b < kBins - 1 ? b + 1 : kBins - 1;
-    w.min_mass = before.mass[w.from[2]];
-    lo = w.min_mass < lo ? w.min_mass : lo;
-    hi = before.mass[w.to[2] + 1] < hi ? before.mass[w.to[2] + 1] : hi;
+    const int at = scale.counts(y) ? scale.bin_of(y) : kBins - 1;
+    b.from[2] = at > 0 ? at - 1 : 0, b.to[2] = at < kBins - 1 ? at + 1 : kBins - 1;
+    b.min_mass = mass[b.from[2]];
+    lo = b.min_mass < lo ? b.min_mass : lo;
+    hi = mass[b.to[2] + 1] < hi ? mass[b.to[2] + 1] : hi;
   }
-  w.from[3] = bin_reaching<uint64_t>(before.mass, token_target(s.u, lo), sh.at[0]);
-  w.to[3] = bin_reaching<uint64_t>(before.mass, token_target(s.u, hi), sh.at[1]);
-  return w;
+  b.from[3] = bin_reaching<uint64_t>(mass, token_target(s.u, lo), sh.at[0]);
+  b.to[3] = lo == hi ? b.from[3] : bin_reaching<uint64_t>(mass, token_target(s.u, hi), sh.at[1]);
+  if (tid == 0) *out = b;
 }
 
 // A chunk's candidates, gathered in LDS first: an atomic on the row's counter takes a trip to memory, and they take turns (one per
 // candidate: 282 us for 64 rows of 131072).  More than kMost are only counted.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, Workspace ws, int chunk) {
-  __shared__ BinSums before;
   __shared__ uint64_t list[kMost];
   __shared__ Shared sh;
-  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, begin = c * chunk, end = begin + chunk < a.V ? begin + chunk : a.V;
-  uint64_t first;
-  uint32_t least;
-  row_extremes(ws, r, gridDim.x, first, least);
-  const RowSettings s = settings_of(a, r);
-  if (s.greedy || key_of(first) <= kNothing) return;
-  const RowScale scale(key_of(first), least, s.t, a.V, nullptr);
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  Chunk<DT> logits(a, r, c, chunk);
+  const Bounds b = ((const Bounds *)ws.bounds)[r];
+  if (b.done) return;
+  const RowScale scale(b.top, b.to_y, b.to_bin, a.V, nullptr);
   if (tid == 0) sh.n = 0;
-  const Wanted wanted = wanted_bins(ws, r, s, scale, before, sh);
-  for_chunk<DT>(a, r * a.logits_stride, begin, end, [&](int i, float v) {
+  sync_threads();
+  logits.each([&](int i, float v) {
     const double y = scale.y_of(v);
-    if (scale.counts(y) && wanted.has(scale.bin_of(y))) {
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < kMost) list[at] = element_of(ordered_bits(v), i);
+    if (scale.counts(y)) {
+      const int bin = scale.bin_of(y);
+      bool is = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) is |= bin >= b.from[j] && bin <= b.to[j];
+      if (is) {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < kMost) list[at] = element_of(ordered_bits(v), i);
+      }
     }
   });
   sync_threads();
@@ -578,36 +642,31 @@ __global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, W
     if (sh.base + i < kMost) ws.candidates[(int64_t)r * kMost + sh.base + i] = list[i];
 }
 
-// The token of a row.  (A launch of its own: as the last workgroup of the row in the launch before, found by a ticket, it cost a
-// write-back of the L2 per workgroup, 61 us for 64 rows of 131072 instead of TODO.)
+// The token of a row.  (As the last workgroup of the row in the launch before, found by a ticket, this cost a write-back of the L2 per
+// workgroup: 61 us for the two together, 64 rows of 131072.)
 template <int DT>
-__global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Workspace ws, int chunks) {
-  __shared__ BinSums before;
+__global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Workspace ws) {
   __shared__ uint64_t list[kMost];
+  __shared__ uint64_t bin_mass[kBins];
+  __shared__ uint32_t bin_rank[kBins];
   __shared__ double powers[256];
   __shared__ Shared sh;
   const int r = blockIdx.x, tid = threadIdx.x;
-  uint64_t first;
-  uint32_t least;
-  row_extremes(ws, r, chunks, first, least);
+  const Bounds b = ((const Bounds *)ws.bounds)[r];
+  if (b.done) return;
+  const uint32_t collected = ws.collected[r];
   const RowSettings s = settings_of(a, r);
-  int token = -1;
-  if (key_of(first) > kNothing && s.greedy) {
-    token = index_of(first);
-  } else if (key_of(first) > kNothing) {
-    make_powers(powers, a.V);
-    const RowScale scale(key_of(first), least, s.t, a.V, powers);
-    const int n = (int)(ws.collected[r] < kMost + 1 ? ws.collected[r] : kMost + 1);
-    for (int i = tid; i < n && i < kMost; i += kThreads) list[i] = ws.candidates[(int64_t)r * kMost + i];
-    if (n > kMost) {
-      sync_threads();
-      token = search_row<DT>(a, r, s, scale, list, sh);
-    } else {
-      const Wanted wanted = wanted_bins(ws, r, s, scale, before, sh);
-      sort_elements(list, n);
-      token = pick_among(s, scale, list, n, before.mass, before.rank, before.mass[kBins], s.top_k ? before.rank[kBins] : 0u, wanted.from[2], wanted.to[2],
-                         wanted.min_mass, sh);
-    }
+  make_powers(powers, a.V);
+  const RowScale scale(b.top, b.to_y, b.to_bin, a.V, powers);
+  int token;
+  if (collected > kMost) {
+    sync_threads();
+    token = search_row<DT>(a, r, s, scale, list, sh);
+  } else {
+    const int n = (int)collected;
+    for (int i = tid; i < n; i += kThreads) list[i] = ws.candidates[(int64_t)r * kMost + i];
+    sort_elements(list, n, bin_rank);
+    token = pick_among(s, scale, list, n, ws.mass + (int64_t)r * kBins, ws.count + (int64_t)r * kBins, b.mass, b.count, b.from[2], b.to[2], b.min_mass, bin_mass, bin_rank, sh);
   }
   if (tid == 0) a.tokens[r] = token;
 }
@@ -616,13 +675,14 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Wo
 template <int DT>
 __global__ __launch_bounds__(kThreads) void short_row_kernel(tamd_sample_args a) {
   __shared__ uint64_t list[kMost];
+  __shared__ uint32_t rank[kThreads];
   __shared__ double powers[256];
   __shared__ Shared sh;
   const int r = blockIdx.x, tid = threadIdx.x;
   const RowSettings s = settings_of(a, r);
   make_powers(powers, a.V);
   for (int i = tid; i < a.V; i += kThreads) list[i] = element_of(key_at<DT>(a.logits, r * a.logits_stride + i), i);
-  sort_elements(list, a.V);
+  sort_elements(list, a.V, rank);
   const uint32_t top = key_of(list[0]);
   int token = -1;
   if (top > kNothing) {
@@ -633,7 +693,7 @@ __global__ __launch_bounds__(kThreads) void short_row_kernel(tamd_sample_args a)
       uint64_t mine = 0;
       for (int i = tid; i < a.V; i += kThreads) mine += scale.units(key_of(list[i]));
       const uint64_t total = block_sum<uint64_t>(mine, sh.tmp);
-      token = pick_among(s, scale, list, a.V, nullptr, nullptr, total, (uint32_t)a.V, 0, kBins, 0, sh);
+      token = pick_among(s, scale, list, a.V, nullptr, nullptr, total, (uint32_t)a.V, 0, kBins, 0, nullptr, nullptr, sh);
     }
   }
   if (tid == 0) a.tokens[r] = token;
@@ -662,10 +722,12 @@ int launch_sample(const tamd_sample_args &args, hipStream_t st) {
     while ((a.V + chunk - 1) / chunk > kMaxChunks) chunk *= 2;
     const Workspace ws = workspace_of(a.workspace, a.R);
     const dim3 grid((unsigned)((a.V + chunk - 1) / chunk), (unsigned)a.R);
+    chunk = ((a.V + (int)grid.x - 1) / (int)grid.x + 255) / 256 * 256;   // all of them alike (grid.x of these are V or more)
     extremes_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
     histogram_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
+    bounds_kernel<<<a.R, kThreads, 0, st>>>(a, ws, (int)grid.x);
     collect_kernel<DT><<<grid, kThreads, 0, st>>>(a, ws, chunk);
-    finish_kernel<DT><<<a.R, kThreads, 0, st>>>(a, ws, (int)grid.x);
+    finish_kernel<DT><<<a.R, kThreads, 0, st>>>(a, ws);
     if (int rc = launch_status()) return rc;
   }
   return 0;
