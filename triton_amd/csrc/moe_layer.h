@@ -35,11 +35,11 @@ constexpr uint32_t kMoeOob = 0x7FFFFFF0u;   // past the end of every buffer: suc
 struct MoeTables {
   int32_t n_active;
   int32_t pad[3];
-  uint64_t mask[kMoeExperts];       // of the picked experts in ascending order: their tokens
-  uint16_t expert[kMoeExperts];
+  uint16_t expert[kMoeExperts];     // the picked ones in ascending order
   uint16_t start[kMoeExperts];      // first row of the expert's tokens in h
   float gate[kMoeSlots];            // [T, k]
   uint16_t pick[kMoeSlots];
+  uint8_t token[kMoeSlots];         // of a row of h
 };
 constexpr int64_t kMoeTableBytes = (sizeof(MoeTables) + 255) / 256 * 256;
 
@@ -77,33 +77,35 @@ struct ExpertWeights {
         sc(p.scale + e * p.scale_stride_e, SHUFFLED ? (int64_t)(N / 32) * ((K + 255) / 256) * 256 : (int64_t)(N - 1) * p.scale_stride_n + K / 32),
         groups((uint32_t)K / 32u), n_kb((uint32_t)(K + 127) / 128u), col_bytes((uint32_t)p.w_stride_n), sc_col((uint32_t)p.scale_stride_n) {}
 
-  // 32 codes of column 32 * strip + 2 c + f, K 128 kb + 32 h ..; zeros past K
-  TAMD_DEVICE u32x4_t codes(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h) const {
+  // 32 codes of column 32 * strip + 2 c + f, K 128 kb + 32 h ..; zeros past K and where `there` is false.  (No branches around loads:
+  // behind one the compiler no longer knows how many requests are outstanding and waits for all of them.)
+  TAMD_DEVICE u32x4_t codes(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, bool there) const {
     if constexpr (BLOCKS) {
-      const uint32_t slot = h ^ ((c >> 2) & 3u) ^ (2u * f);
-      return w.template load16<2>((c + 32u * f + 16u * (strip & 1u)) * 64u + slot * 16u, ((strip >> 1) * n_kb + kb) * 4096u);
+      const uint32_t slot = h ^ ((c >> 2) & 3u) ^ (2u * f), off = (c + 32u * f + 16u * (strip & 1u)) * 64u + slot * 16u;
+      return w.template load16<2>(there ? off : kMoeOob, there ? ((strip >> 1) * n_kb + kb) * 4096u : 0u);
     } else {
-      return w.template load16<2>(4u * kb + h < groups ? (32u * strip + 2u * c + f) * col_bytes + 64u * kb + 16u * h : kMoeOob);
+      return w.template load16<2>(there && 4u * kb + h < groups ? (32u * strip + 2u * c + f) * col_bytes + 64u * kb + 16u * h : kMoeOob);
     }
   }
   // their scale, as a dword whose byte `scale_shift` is it
-  TAMD_DEVICE void scales2(uint32_t strip, uint32_t kb, uint32_t c, uint32_t h, uint32_t &s0, uint32_t &s1) const {
+  TAMD_DEVICE void scales2(uint32_t strip, uint32_t kb, uint32_t c, uint32_t h, bool there, uint32_t &s0, uint32_t &s1) const {
     if constexpr (SHUFFLED) {
-      const u32x2_t v = sc.load8(64u * h + 4u * ((2u * c) & 15u), (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u);
+      const uint32_t off = 64u * h + 4u * ((2u * c) & 15u);
+      const u32x2_t v = sc.load8(there ? off : kMoeOob, there ? (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u : 0u);
       s0 = v.x, s1 = v.y;
     } else {
       const uint32_t g = 4u * kb + h, at = (32u * strip + 2u * c) * sc_col + g;
-      s0 = sc.load1(g < groups ? at : kMoeOob);
-      s1 = sc.load1(g < groups ? at + sc_col : kMoeOob);
+      s0 = sc.load1(there && g < groups ? at : kMoeOob);
+      s1 = sc.load1(there && g < groups ? at + sc_col : kMoeOob);
     }
   }
-  TAMD_DEVICE uint32_t scale1(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h) const {
+  TAMD_DEVICE uint32_t scale1(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, bool there) const {
     if constexpr (SHUFFLED) {
-      const uint32_t n = 2u * c + f;
-      return sc.load1(64u * h + 4u * (n & 15u) + 2u * (kb & 1u) + (n >> 4), (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u);
+      const uint32_t n = 2u * c + f, off = 64u * h + 4u * (n & 15u) + 2u * (kb & 1u) + (n >> 4);
+      return sc.load1(there ? off : kMoeOob, there ? (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u : 0u);
     } else {
       const uint32_t g = 4u * kb + h;
-      return sc.load1(g < groups ? (32u * strip + 2u * c + f) * sc_col + g : kMoeOob);
+      return sc.load1(there && g < groups ? (32u * strip + 2u * c + f) * sc_col + g : kMoeOob);
     }
   }
   // the scale as the conversion takes it: a float32 of which only the exponent counts
@@ -119,44 +121,39 @@ struct MoeRouting {
   uint16_t expert[kMoeExperts], start[kMoeExperts], first[kMoeExperts];
   uint16_t pick[kMoeSlots];
   float gate[kMoeSlots], row_gate[kMoeSlots];
+  uint8_t row_token[kMoeSlots];
   int32_t wave_sum[8];
   int32_t n_active;
 };
 
-// Picks of all tokens, by a workgroup of 512 threads.  A wave takes a row at a time, its logits in the lanes' registers; ties go to the
-// lower column, order and softmax are those of tamd_topk_forward, the gate weights stay float32.
-TAMD_DEVICE void moe_route(const tamd_moe_layer_args &a, MoeRouting &r) {
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+// Picks of a wave's tokens, a row's logits EPL per lane; ties go to the lower column, order and softmax are those of
+// tamd_topk_forward, the gate weights stay float32.
+template <int EPL>
+TAMD_DEVICE void moe_pick(const tamd_moe_layer_args &a, MoeRouting &r, int wave, int lane) {
   const int E = a.n_experts, k = a.n_picks;
-  r.by_expert[tid] = 0;
-  sync_threads();
   for (int t = wave; t < a.n_tokens; t += 8) {
-    uint32_t key[8];
+    uint32_t key[EPL];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < EPL; ++j) {   // (key 0 stands for no column: the lowest NaN shares the second lowest key)
       const int col = j * kWave + lane;
-      key[j] = 0;
-      if (j * kWave < E) {   // (key 0 stands for no column: the lowest NaN shares the second lowest key)
-        const float v = load_any_f32(a.logits, a.logits_dtype, t * a.logits_stride + (col < E ? col : E - 1));
-        const uint32_t u = ordered_bits(v);
-        key[j] = col < E ? (u > 1u ? u : 1u) : 0u;
-      }
+      const uint32_t u = ordered_bits(load_any_f32(a.logits, a.logits_dtype, t * a.logits_stride + (col < E ? col : E - 1)));
+      key[j] = col < E ? (u > 1u ? u : 1u) : 0u;
     }
     uint32_t top = 0, mine = 0;
     int my_col = 0;
     for (int p = 0; p < k; ++p) {
       uint32_t m = key[0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) m = key[j] > m ? key[j] : m;
+      for (int j = 1; j < EPL; ++j) m = key[j] > m ? key[j] : m;
       m = group_max_u32<kWave>(m);
       int col = 0;
 #pragma unroll
-      for (int j = 7; j >= 0; --j) {
+      for (int j = EPL - 1; j >= 0; --j) {
         const uint64_t at = __ballot(key[j] == m);
         if (at) col = j * kWave + __builtin_ctzll(at);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < EPL; ++j)
         if (j * kWave + lane == col) key[j] = 0;
       if (p == 0) top = m;
       if (lane == p) mine = m, my_col = col;
@@ -169,6 +166,17 @@ TAMD_DEVICE void moe_route(const tamd_moe_layer_args &a, MoeRouting &r) {
       atomicOr((unsigned long long *)&r.by_expert[my_col], 1ull << t);
     }
   }
+}
+
+// Routing of all tokens, by a workgroup of 512 threads, a wave per row.
+TAMD_DEVICE void moe_route(const tamd_moe_layer_args &a, MoeRouting &r) {
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int E = a.n_experts, k = a.n_picks;
+  r.by_expert[tid] = 0;
+  sync_threads();
+  if (E <= kWave) moe_pick<1>(a, r, wave, lane);
+  else if (E <= 2 * kWave) moe_pick<2>(a, r, wave, lane);
+  else moe_pick<8>(a, r, wave, lane);
   sync_threads();
   // the picked experts in ascending order, and where their rows begin: one scan of both counts
   const uint64_t m = r.by_expert[tid];
@@ -189,7 +197,9 @@ TAMD_DEVICE void moe_route(const tamd_moe_layer_args &a, MoeRouting &r) {
   sync_threads();
   if (tid < a.n_tokens * k) {
     const int e = r.pick[tid], t = tid / k;
-    r.row_gate[r.first[e] + __popcll(r.by_expert[e] & ((1ull << t) - 1ull))] = r.gate[tid];
+    const int row = r.first[e] + __popcll(r.by_expert[e] & ((1ull << t) - 1ull));
+    r.row_gate[row] = r.gate[tid];
+    r.row_token[row] = (uint8_t)t;
   }
   sync_threads();
 }
@@ -203,12 +213,16 @@ TAMD_DEVICE float swiglu_keeping_nan(const tamd_moe_layer_args &a, float g, floa
   return swiglu_fast(g, l, a.act_alpha, 0.f, false);
 }
 
-// NB blocks of 128 K per wave at a time.
-template <int XDT, bool BLOCKS, bool SHUFFLED, int NB>
-__global__ __launch_bounds__(512, NB >= 3 ? 2 : 4) void moe_up_kernel(tamd_moe_layer_args a) {
+// A workgroup per CU takes a contiguous part of the units (picked expert, strip of 32 columns): consecutive strips of an expert, whose
+// rows of x then stay in registers.  Its eight waves split K, NB blocks of 128 each; the weights of two units are in flight
+// (48 KB per CU with NB = 3), their partial sums meet in LDS, a barrier per unit.  A stage is a unit, 16 of its rows and 8 * NB
+// blocks of K; with ROUNDS there may be several of a unit (long K, more than 16 tokens) and x travels with the weights.
+// As a loop without requests ahead, two workgroups per CU, 16 tokens of 128 experts of 2880 x 5760 took 154 us instead of TODO.
+template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, bool ROUNDS>
+__global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
   __shared__ MoeRouting r;
-  __shared__ f32x4_t red[8][2][kWave];
+  __shared__ f32x4_t red[2][8][2][kWave];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const uint32_t c = lane & 15, h = lane >> 4;
   const int K = a.hidden, I = a.inter;
@@ -218,178 +232,288 @@ __global__ __launch_bounds__(512, NB >= 3 ? 2 : 4) void moe_up_kernel(tamd_moe_l
   uint16_t *planes = (uint16_t *)((uint8_t *)a.workspace + kMoeTableBytes);
   if (blockIdx.x == 0) {
     if (tid == 0) tab->n_active = n_active;
-    if (tid < n_active) tab->mask[tid] = r.mask[tid], tab->expert[tid] = r.expert[tid], tab->start[tid] = r.start[tid];
-    if (tid < a.n_tokens * a.n_picks) tab->gate[tid] = r.gate[tid], tab->pick[tid] = r.pick[tid];
+    if (tid < n_active) tab->expert[tid] = r.expert[tid], tab->start[tid] = r.start[tid];
+    if (tid < a.n_tokens * a.n_picks) tab->gate[tid] = r.gate[tid], tab->pick[tid] = r.pick[tid], tab->token[tid] = r.row_token[tid];
   }
-  const uint32_t strips = (uint32_t)I / 16u, n_kb = (uint32_t)(K + 127) / 128u;
+  const uint32_t strips = (uint32_t)I / 16u, n_kb = (uint32_t)(K + 127) / 128u, units = (uint32_t)n_active * strips;
+  const uint32_t unit0 = (uint32_t)((uint64_t)units * blockIdx.x / gridDim.x), unit1 = (uint32_t)((uint64_t)units * (blockIdx.x + 1) / gridDim.x);
+  if (unit0 == unit1) return;
   const Buffer x(a.x, (int64_t)(a.n_tokens - 1) * a.x_stride_m * 2 + 2 * K);
-  for (uint32_t u = blockIdx.x; u < (uint32_t)n_active * strips; u += gridDim.x) {
-    const uint32_t at = u / strips, strip = u % strips;
-    const int e = __builtin_amdgcn_readfirstlane((int)r.expert[at]);
-    const uint64_t mask = uniform64(r.mask[at]);
-    const int rows = __popcll(mask), start = __builtin_amdgcn_readfirstlane((int)r.start[at]);
-    const ExpertWeights<BLOCKS, SHUFFLED> w(a.up, e, K, 2 * I);
-    // lane m: the m-th token of the expert (each token's lane sends itself there)
-    const int rank = __popcll(mask & ((1ull << lane) - 1ull));
-    const int token_at = __builtin_amdgcn_ds_permute(4 * ((mask >> lane & 1) ? rank : 63 - (lane - rank)), lane);
-    for (int m0 = 0; m0 < rows; m0 += 16) {
-      const int token = __builtin_amdgcn_ds_bpermute(4 * (m0 + (int)c), token_at);
-      const uint32_t x_row = m0 + (int)c < rows ? (uint32_t)(token * a.x_stride_m * 2) + 64u * h : kMoeOob;
-      f32x4_t acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
-      for (uint32_t k0 = 0; k0 < n_kb; k0 += 8 * NB) {
-        const uint32_t kb0 = k0 + (uint32_t)wave * NB;
-        u32x4_t q0[NB], q1[NB], xr[NB][4];
-        uint32_t s0[NB], s1[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          if (kb0 + i < n_kb) {
-            q0[i] = w.codes(strip, 0, kb0 + i, c, h);
-            q1[i] = w.codes(strip, 1, kb0 + i, c, h);
-            w.scales2(strip, kb0 + i, c, h, s0[i], s1[i]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) xr[i][j] = x.load16(4u * (kb0 + i) + h < w.groups ? x_row + 256u * (kb0 + i) + 16u * j : kMoeOob);
-          }
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          if (kb0 + i < n_kb) {
-            const float f0 = w.factor2(s0[i], kb0 + i, c), f1 = w.factor2(s1[i], kb0 + i, c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              acc0 = Mma16<XDT>::mma(as_frag<XDT>(xr[i][j]), M::expand(q0[i][j], f0), acc0);
-              acc1 = Mma16<XDT>::mma(as_frag<XDT>(xr[i][j]), M::expand(q1[i][j], f1), acc1);
-            }
-          }
-      }
-      red[wave][0][lane] = acc0;
-      red[wave][1][lane] = acc1;
-      sync_threads();
-      // row m of the tile, pair c of the strip: element (4 h + i) of lanes (c, h)
-      const int m = tid >> 4, pair = tid & 15;
-      if (m < 16 && m0 + m < rows) {
-        const int from = (m >> 2) * 16 + pair;
-        float g = 0.f, l = 0.f;
-#pragma unroll
-        for (int v = 0; v < 8; ++v) g += ((const float *)&red[v][0][from])[m & 3], l += ((const float *)&red[v][1][from])[m & 3];
-        if (a.up.bias) {
-          const int64_t b = e * a.up.bias_stride_e + 32 * (int64_t)strip + 2 * pair;
-          g += load_any_f32(a.up.bias, a.up.bias_dtype, b);
-          l += load_any_f32(a.up.bias, a.up.bias_dtype, b + 1);
-        }
-        const int row = start + m0 + m;
-        const float v = r.row_gate[row] * swiglu_keeping_nan(a, g, l);
-        const uint32_t hi = XDT == TAMD_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
-        const float rest = v - (XDT == TAMD_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi));
-        const float lo = rest - rest == 0.f ? rest : 0.f;   // (infinities leave nothing)
-        uint16_t *p = planes + (int64_t)row * 2 * I + 16 * strip + pair;
-        p[0] = (uint16_t)hi;
-        p[I] = (uint16_t)(XDT == TAMD_BF16 ? f32_to_bf16_bits(lo) : f32_to_f16_bits(lo));
-      }
-      sync_threads();
+  const int total_rows = a.n_tokens * a.n_picks;
+  const auto first_row = [&](uint32_t at) { return (int)r.start[at]; };
+  const auto end_row = [&](uint32_t at) { return (int)at + 1 < n_active ? (int)r.start[at + 1] : total_rows; };
+
+  struct Cursor {
+    uint32_t unit, at, strip, k0;
+    int m0;
+  };
+  const auto advance = [&](Cursor &p) {
+    if constexpr (ROUNDS) {
+      p.k0 += 8 * NB;
+      if (p.k0 < n_kb) return;
+      p.k0 = 0;
+      p.m0 += 16;
+      if (p.m0 < __builtin_amdgcn_readfirstlane(end_row(p.at) - first_row(p.at))) return;
+      p.m0 = 0;
     }
+    ++p.unit;
+    if (++p.strip == strips) p.strip = 0, ++p.at;
+  };
+  struct Stage {
+    u32x4_t q0[NB], q1[NB], x[ROUNDS ? NB : 1][4];
+    uint32_t s0[NB], s1[NB];
+  };
+  const auto request_x = [&](u32x4_t (&to)[ROUNDS ? NB : 1][4], int i, const Cursor &p, uint32_t x_row, bool there) {
+    const uint32_t kb = p.k0 + (uint32_t)wave * NB + i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[i][j] = x.load16(there && 4u * kb + h < (uint32_t)K / 32u ? x_row + 256u * kb + 16u * j : kMoeOob);
+  };
+  const auto x_row_of = [&](const Cursor &p) {   // row c of the tile: the byte offset of its token's x
+    const int row = __builtin_amdgcn_readfirstlane(first_row(p.at)) + p.m0 + (int)c;
+    return row < __builtin_amdgcn_readfirstlane(end_row(p.at)) ? (uint32_t)r.row_token[row] * (uint32_t)(2 * a.x_stride_m) + 64u * h : kMoeOob;
+  };
+  const auto request = [&](Stage &s, Cursor &p) {
+    const bool live = p.unit < unit1;
+    const uint32_t at = live ? p.at : 0u;
+    const ExpertWeights<BLOCKS, SHUFFLED> w(a.up, __builtin_amdgcn_readfirstlane((int)r.expert[at]), K, 2 * I);
+    uint32_t x_row = 0;
+    if constexpr (ROUNDS) x_row = x_row_of(Cursor{p.unit, at, p.strip, p.k0, p.m0});
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const uint32_t kb = p.k0 + (uint32_t)wave * NB + i;
+      const bool there = live && kb < n_kb;
+      s.q0[i] = w.codes(p.strip, 0, kb, c, h, there);
+      s.q1[i] = w.codes(p.strip, 1, kb, c, h, there);
+      w.scales2(p.strip, kb, c, h, there, s.s0[i], s.s1[i]);
+      if constexpr (ROUNDS) request_x(s.x, i, p, x_row, there);
+    }
+    if (live) advance(p);
+  };
+
+  Cursor ask, now;
+  ask.unit = unit0, ask.at = unit0 / strips, ask.strip = unit0 % strips, ask.k0 = 0, ask.m0 = 0;
+  now = ask;
+  u32x4_t xr[ROUNDS ? 1 : NB][4];
+  uint32_t x_at = 0xFFFFFFFFu;
+  f32x4_t acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
+  uint32_t turn = 0;
+  const auto load_x = [&]() {
+    if constexpr (!ROUNDS) {
+      const uint32_t x_row = x_row_of(now);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t kb = (uint32_t)wave * NB + i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xr[i][j] = x.load16(4u * kb + h < (uint32_t)K / 32u ? x_row + 256u * kb + 16u * j : kMoeOob);
+      }
+      x_at = now.at;
+    }
+  };
+  const auto multiply = [&](const Stage &s) {
+    if constexpr (!ROUNDS)
+      if (x_at != now.at) load_x();
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const uint32_t kb = now.k0 + (uint32_t)wave * NB + i;
+      const float f0 = ExpertWeights<BLOCKS, SHUFFLED>::factor2(s.s0[i], kb, c), f1 = ExpertWeights<BLOCKS, SHUFFLED>::factor2(s.s1[i], kb, c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x4_t xv;
+        if constexpr (ROUNDS) xv = s.x[i][j];
+        else xv = xr[i][j];
+        acc0 = Mma16<XDT>::mma(as_frag<XDT>(xv), M::expand(s.q0[i][j], f0), acc0);
+        acc1 = Mma16<XDT>::mma(as_frag<XDT>(xv), M::expand(s.q1[i][j], f1), acc1);
+      }
+    }
+    const Cursor done = now;
+    advance(now);
+    if (ROUNDS && now.k0 != 0) return;   // (more of this unit's K)
+    red[turn][wave][0][lane] = acc0;
+    red[turn][wave][1][lane] = acc1;
+    acc0 = acc1 = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    sync_threads();
+    // row m of the tile, pair of the strip: element m % 4 of lanes (pair, m / 4)
+    const int m = tid >> 4, pair = tid & 15, row = first_row(done.at) + done.m0 + m;
+    if (m < 16 && row < end_row(done.at)) {
+      const int from = (m >> 2) * 16 + pair;
+      float g = 0.f, l = 0.f;
+#pragma unroll
+      for (int v = 0; v < 8; ++v) g += ((const float *)&red[turn][v][0][from])[m & 3], l += ((const float *)&red[turn][v][1][from])[m & 3];
+      if (a.up.bias) {
+        const int64_t b = (int)r.expert[done.at] * a.up.bias_stride_e + 32 * (int64_t)done.strip + 2 * pair;
+        g += load_any_f32(a.up.bias, a.up.bias_dtype, b);
+        l += load_any_f32(a.up.bias, a.up.bias_dtype, b + 1);
+      }
+      const float v = r.row_gate[row] * swiglu_keeping_nan(a, g, l);
+      const uint32_t hi = XDT == TAMD_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+      const float rest = v - (XDT == TAMD_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi));
+      const float lo = rest - rest == 0.f ? rest : 0.f;   // (infinities leave nothing)
+      uint16_t *p = planes + (int64_t)row * 2 * I + 16 * done.strip + pair;
+      p[0] = (uint16_t)hi;
+      p[I] = (uint16_t)(XDT == TAMD_BF16 ? f32_to_bf16_bits(lo) : f32_to_f16_bits(lo));
+    }
+    turn ^= 1;   // (the next stage's sums go to the other half: one barrier between two uses of either)
+  };
+
+  load_x();
+  Stage s0, s1;
+  request(s0, ask);
+  request(s1, ask);
+  for (;;) {
+    multiply(s0);
+    if (now.unit == unit1) break;
+    request(s0, ask);
+    multiply(s1);
+    if (now.unit == unit1) break;
+    request(s1, ask);
   }
 }
 
-// MT tiles of 16 rows, which are eight tokens with two planes each.  W waves, U blocks of 128 K requested together.
-template <int XDT, bool BLOCKS, bool SHUFFLED, int MT, int U, int W>
-__global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_args a) {
+struct MoeDownLds {
+  float gate[kMoeSlots];
+  uint16_t expert[kMoeExperts], start[kMoeExperts + 8], pick[kMoeSlots];
+  uint8_t token[kMoeSlots];
+};
+static_assert(sizeof(MoeDownLds) % 16 == 0);
+
+// A workgroup owns 16 columns of y, its sixteen waves equal parts of the list of items (picked expert, 128 K).  A wave has the weights
+// of 2 U items in flight, across experts.  Rows of a tile are the two planes of up to eight of the expert's tokens, MT tiles at a
+// time; at an expert's end a wave adds its tokens' sums to its own copy of the output in LDS, where the copies are added
+// up at last: no atomics, and NaN or infinite weights stay with the tokens that picked them.
+template <int XDT, bool BLOCKS, bool SHUFFLED, int MT, int U>
+__global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
-  __shared__ uint64_t s_mask[kMoeExperts];
-  __shared__ uint16_t s_expert[kMoeExperts], s_start[kMoeExperts], s_pick[kMoeSlots];
-  __shared__ float s_gate[kMoeSlots];
-  __shared__ f32x4_t red[W][kWave];
+  constexpr int W = 16;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  MoeDownLds &s = *(MoeDownLds *)lds;
+  float *sums = (float *)(lds + sizeof(MoeDownLds));   // [W, n_tokens, 16]
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const uint32_t c = lane & 15, h = lane >> 4;
-  const int K = a.inter, N = a.hidden;
+  const int K = a.inter, N = a.hidden, T = a.n_tokens;
   const MoeTables *tab = (const MoeTables *)a.workspace;
-  const int slots = a.n_tokens * a.n_picks;
-  if (tid < slots) {   // (no more experts than slots, no more slots than threads)
-    s_mask[tid] = tab->mask[tid], s_expert[tid] = tab->expert[tid], s_start[tid] = tab->start[tid];
-    s_gate[tid] = tab->gate[tid], s_pick[tid] = tab->pick[tid];
-  }
+  const int slots = T * a.n_picks;
   const uint32_t n_active = (uint32_t)__builtin_amdgcn_readfirstlane(tab->n_active);
+  if (tid < slots) {   // (no more experts than slots)
+    s.expert[tid] = tab->expert[tid], s.start[tid] = (uint32_t)tid < n_active ? tab->start[tid] : (uint16_t)slots;
+    s.gate[tid] = tab->gate[tid], s.pick[tid] = tab->pick[tid], s.token[tid] = tab->token[tid];
+  }
+  if (tid == 0) s.start[slots] = (uint16_t)slots;
+  for (int i = tid; i < W * T * 16; i += 1024) sums[i] = 0.f;
   sync_threads();
   const Buffer planes((const uint8_t *)a.workspace + kMoeTableBytes, (int64_t)slots * 4 * K);
   const uint32_t strip = blockIdx.x >> 1, f = blockIdx.x & 1u, n_kb = (uint32_t)(K + 127) / 128u, total = n_active * n_kb;
-  uint32_t item = (uint32_t)((uint64_t)total * (uint32_t)wave / (uint32_t)W);
-  const uint32_t end = (uint32_t)((uint64_t)total * (uint32_t)(wave + 1) / (uint32_t)W);
-  f32x4_t sum[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) sum[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  while (item < end) {
-    const uint32_t at = item / n_kb;
-    uint32_t kb = item - at * n_kb;
-    const uint32_t kb_end = n_kb - kb < end - item ? n_kb : kb + (end - item);
-    item += kb_end - kb;
-    const uint64_t mask = uniform64(s_mask[at]);
-    const ExpertWeights<BLOCKS, SHUFFLED> w(a.down, __builtin_amdgcn_readfirstlane((int)s_expert[at]), K, N);
-    const uint32_t start = s_start[at];
-    // row 2 i + p of tile t is plane p of token 8 t + i, if that token picked the expert
-    uint32_t row[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int token = 8 * t + (int)(c >> 1);
-      const uint32_t at_row = start + (uint32_t)__popcll(mask & ((1ull << token) - 1ull));
-      row[t] = (mask >> token & 1) ? (at_row * 2u + (c & 1u)) * (uint32_t)(2 * K) + 64u * h : kMoeOob;
+  const uint32_t begin = (uint32_t)((uint64_t)total * (uint32_t)wave / W), end = (uint32_t)((uint64_t)total * (uint32_t)(wave + 1) / W);
+
+  struct Cursor {
+    uint32_t item, at, kb;
+    TAMD_DEVICE void next(uint32_t n_kb_) {
+      ++item;
+      if (++kb == n_kb_) kb = 0, ++at;
     }
+  };
+  struct Batch {
+    u32x4_t q[U];
+    uint32_t s[U];
+  };
+  const auto request = [&](Batch &b, Cursor &p) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const bool there = p.item < end;
+      const ExpertWeights<BLOCKS, SHUFFLED> w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[there ? p.at : 0u]), K, N);
+      b.q[i] = w.codes(strip, f, p.kb, c, h, there);
+      b.s[i] = w.scale1(strip, f, p.kb, c, h, there);
+      if (there) p.next(n_kb);
+    }
+  };
+  // row c of tile t of the rows from `row` on
+  const auto request_x = [&](u32x4_t (&to)[4], uint32_t row, uint32_t rows, int t, uint32_t kb, bool there) {
+    const bool mine = there && 16u * t + c < 2u * rows && 4u * kb + h < (uint32_t)K / 32u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = planes.load16(mine ? (2u * row + 16u * t + c) * (uint32_t)(2 * K) + 256u * kb + 64u * h + 16u * j : kMoeOob);
+  };
+  const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
+    row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
+    rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at + 1]) - row;
+  };
+
+  if (begin < end) {
+    Cursor ask{begin, begin / n_kb, begin % n_kb}, ask_x = ask, now = ask;
     f32x4_t acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (; kb < kb_end; kb += U) {
-      u32x4_t q[U];
-      uint32_t s[U];
+    u32x4_t xr[2][4];   // first tile's rows of the next two items
+    const auto ask_rows = [&](u32x4_t (&to)[4]) {
+      const bool there = ask_x.item < end;
+      uint32_t row, rows;
+      rows_at(there ? ask_x.at : 0u, row, rows);
+      request_x(to, row, rows, 0, ask_x.kb, there);
+      if (there) ask_x.next(n_kb);
+    };
+    const auto multiply = [&](const Batch &b, int i) {
+      uint32_t row, rows;
+      rows_at(now.at, row, rows);
+      const float factor = bits_to_f32(b.s[i] << 23);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const auto w = M::expand(b.q[i][j], factor);
+        acc[0] = Mma16<XDT>::mma(as_frag<XDT>(xr[i & 1][j]), w, acc[0]);
+      }
+      if constexpr (MT > 1) {
+#pragma unroll
+        for (int t = 1; t < MT; ++t)
+          if (8u * t < rows) {
+            u32x4_t xt[4];
+            request_x(xt, row, rows, t, now.kb, true);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[t] = Mma16<XDT>::mma(as_frag<XDT>(xt[j]), M::expand(b.q[i][j], factor), acc[t]);
+          }
+      }
+      now.next(n_kb);
+      if (now.kb == 0 || now.item == end) {   // the expert's end: elements 2 p and 2 p + 1 of lane (c, h) are the planes of row 8 t + 2 h + p
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const uint32_t of = 8u * t + 2u * h + p;
+            if (of < rows) sums[(wave * T + s.token[row + of]) * 16 + (int)c] += acc[t][2 * p] + acc[t][2 * p + 1];
+          }
+          acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+      }
+      ask_rows(xr[i & 1]);
+    };
+    static_assert(U % 2 == 0);
+    Batch b0, b1;
+    request(b0, ask);
+    ask_rows(xr[0]);
+    ask_rows(xr[1]);
+    request(b1, ask);
+    while (true) {
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if (kb + i < kb_end) {
-          q[i] = w.codes(strip, f, kb + i, c, h);
-          s[i] = w.scale1(strip, f, kb + i, c, h);
-        }
+        if (now.item < end) multiply(b0, i);
+      if (now.item == end) break;
+      request(b0, ask);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (MT > 1 && !((uint32_t)(mask >> (8 * t)) & 0xFFu)) continue;
-        u32x4_t xr[U][4];
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-          if (kb + i < kb_end) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) xr[i][j] = planes.load16(4u * (kb + i) + h < w.groups ? row[t] + 256u * (kb + i) + 16u * j : kMoeOob);
-          }
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-          if (kb + i < kb_end) {
-            const float factor = bits_to_f32(s[i] << 23);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[t] = Mma16<XDT>::mma(as_frag<XDT>(xr[i][j]), M::expand(q[i][j], factor), acc[t]);
-          }
-      }
+      for (int i = 0; i < U; ++i)
+        if (now.item < end) multiply(b1, i);
+      if (now.item == end) break;
+      request(b1, ask);
     }
-    // only the rows of the expert's own tokens: its NaN or infinite weights are no other token's
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (mask >> (8 * t + 2 * h + (i >> 1)) & 1) sum[t][i] += acc[t][i];
   }
+  sync_threads();
+  for (int i = tid; i < T * 16; i += 1024) {
+    const int token = i >> 4;
+    float v = 0.f;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    red[wave][lane] = sum[t];
-    sync_threads();
-    const int i = tid >> 4, col = tid & 15, token = 8 * t + i;   // token i of the tile: elements 2 (i % 2) and the next of lanes (col, i / 2)
-    if (i < 8 && token < a.n_tokens) {
-      float v = 0.f;
-#pragma unroll
-      for (int s = 0; s < W; ++s) {
-        const float *p = (const float *)&red[s][(i >> 1) * 16 + col] + 2 * (i & 1);
-        v += p[0] + p[1];
+    for (int w = 0; w < W; ++w) v += sums[w * T * 16 + i];
+    const int64_t n = 32 * (int64_t)strip + 2 * (i & 15) + f;
+    if (a.down.bias)
+      for (int j = 0; j < a.n_picks; ++j) {
+        const int slot = token * a.n_picks + j;
+        v = __builtin_fmaf(s.gate[slot], load_any_f32(a.down.bias, a.down.bias_dtype, s.pick[slot] * a.down.bias_stride_e + n), v);
       }
-      const int64_t n = 32 * (int64_t)strip + 2 * col + f;
-      if (a.down.bias)
-        for (int j = 0; j < a.n_picks; ++j) {
-          const int slot = token * a.n_picks + j;
-          v = __builtin_fmaf(s_gate[slot], load_any_f32(a.down.bias, a.down.bias_dtype, s_pick[slot] * a.down.bias_stride_e + n), v);
-        }
-      store_any(a.y, XDT, token * a.y_stride_m + n, v);
-    }
-    sync_threads();
+    store_any(a.y, XDT, token * a.y_stride_m + n, v);
   }
 }
 
@@ -397,7 +521,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_
 inline int moe_up_nb(int hidden) {
   const int n_kb = (hidden + 127) / 128;
   int best = 1, least = 1 << 30;
-  for (int nb = 4; nb >= 1; --nb) {
+  for (int nb = 3; nb >= 1; --nb) {
     const int cost = (n_kb + 8 * nb - 1) / (8 * nb) * nb;
     if (cost < least) least = cost, best = nb;
   }
@@ -409,12 +533,20 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
   int cus = 0;
   if (int rc = cu_count(cus)) return rc;
   const int64_t slots = (int64_t)a.n_tokens * a.n_picks, most = (slots < a.n_experts ? slots : a.n_experts) * (a.inter / 16);
-  const dim3 grid((unsigned)(most < 2 * cus ? most : 2 * cus));
-  switch (moe_up_nb(a.hidden)) {
-    case 1: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 1><<<grid, 512, 0, st>>>(a); break;
-    case 2: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 2><<<grid, 512, 0, st>>>(a); break;
-    case 3: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 3><<<grid, 512, 0, st>>>(a); break;
-    default: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 4><<<grid, 512, 0, st>>>(a); break;
+  const dim3 grid((unsigned)(most < cus ? most : cus));
+  const int nb = moe_up_nb(a.hidden);
+  if (a.n_tokens > 16 || 8 * nb < (a.hidden + 127) / 128) {
+    switch (nb) {
+      case 1: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 1, true><<<grid, 512, 0, st>>>(a); break;
+      case 2: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 2, true><<<grid, 512, 0, st>>>(a); break;
+      default: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 3, true><<<grid, 512, 0, st>>>(a); break;
+    }
+  } else {
+    switch (nb) {
+      case 1: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 1, false><<<grid, 512, 0, st>>>(a); break;
+      case 2: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 2, false><<<grid, 512, 0, st>>>(a); break;
+      default: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 3, false><<<grid, 512, 0, st>>>(a); break;
+    }
   }
   return launch_status();
 }
@@ -422,10 +554,10 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
 template <int XDT, bool BLOCKS, bool SHUFFLED>
 int launch_moe_down(const tamd_moe_layer_args &a, hipStream_t st) {
   const dim3 grid((unsigned)(a.hidden / 16));
-  if (a.n_tokens <= 8) moe_down_kernel<XDT, BLOCKS, SHUFFLED, 1, 3, 16><<<grid, 1024, 0, st>>>(a);
-  else if (a.n_tokens <= 16) moe_down_kernel<XDT, BLOCKS, SHUFFLED, 2, 2, 16><<<grid, 1024, 0, st>>>(a);
-  else if (a.n_tokens <= 32) moe_down_kernel<XDT, BLOCKS, SHUFFLED, 4, 4, 8><<<grid, 512, 0, st>>>(a);
-  else moe_down_kernel<XDT, BLOCKS, SHUFFLED, 8, 2, 8><<<grid, 512, 0, st>>>(a);
+  const size_t lds = sizeof(MoeDownLds) + (size_t)a.n_tokens * 16 * 16 * 4;
+  const auto kernel = a.n_tokens <= 8 ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, 1, 4> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, 8, 2>;
+  if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
+  kernel<<<grid, 1024, lds, st>>>(a);
   return launch_status();
 }
 
