@@ -404,7 +404,7 @@ typedef struct tamd_moe_weights {
   int64_t w_stride_e, w_stride_n;          /* bytes; blocks: only the first is read */
   const uint8_t *scale;
   int64_t scale_stride_e, scale_stride_n;  /* bytes; pre-shuffled: only the first is read */
-  const void *bias;                        /* [E, columns] or NULL */
+  const void *bias;                        /* [E, columns] or NULL; 16-bit ones on 4-byte boundaries */
   int64_t bias_stride_e;
   int bias_dtype;
   int w_layout;            /* TAMD_W_* */

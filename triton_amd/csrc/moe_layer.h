@@ -66,6 +66,14 @@ TAMD_DEVICE uint64_t uniform64(uint64_t v) {
 template <int XDT>
 TAMD_DEVICE typename Mma<XDT>::frag_t as_frag(u32x4_t v) { return __builtin_bit_cast(typename Mma<XDT>::frag_t, v); }
 
+// What is added to an offset: nothing, or what takes it past the end.  Hidden from the compiler, which otherwise branches around the
+// loads; behind a branch it no longer knows how many requests are outstanding and waits for all of them.
+TAMD_DEVICE uint32_t dead_unless(bool there) {
+  uint32_t d = there ? 0u : kMoeOob;
+  asm volatile("" : "+s"(d));
+  return d;
+}
+
 // One expert's weights of one product as the lanes of a wave read them.  BLOCKS / SHUFFLED: values in 4 KB blocks, scales in the
 // CDNA4 pre-shuffle; else both contiguous along K, column by column.
 template <bool BLOCKS, bool SHUFFLED>
@@ -77,35 +85,34 @@ struct ExpertWeights {
         sc(p.scale + e * p.scale_stride_e, SHUFFLED ? (int64_t)(N / 32) * ((K + 255) / 256) * 256 : (int64_t)(N - 1) * p.scale_stride_n + K / 32),
         groups((uint32_t)K / 32u), n_kb((uint32_t)(K + 127) / 128u), col_bytes((uint32_t)p.w_stride_n), sc_col((uint32_t)p.scale_stride_n) {}
 
-  // 32 codes of column 32 * strip + 2 c + f, K 128 kb + 32 h ..; zeros past K and where `there` is false.  (No branches around loads:
-  // behind one the compiler no longer knows how many requests are outstanding and waits for all of them.)
-  TAMD_DEVICE u32x4_t codes(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, bool there) const {
+  // 32 codes of column 32 * strip + 2 c + f, K 128 kb + 32 h ..; zeros past K.  `dead` is added to every offset: kMoeOob for what is not there
+  // (see dead_unless).
+  TAMD_DEVICE u32x4_t codes(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, uint32_t dead) const {
     if constexpr (BLOCKS) {
-      const uint32_t slot = h ^ ((c >> 2) & 3u) ^ (2u * f), off = (c + 32u * f + 16u * (strip & 1u)) * 64u + slot * 16u;
-      return w.template load16<2>(there ? off : kMoeOob, there ? ((strip >> 1) * n_kb + kb) * 4096u : 0u);
+      const uint32_t slot = h ^ ((c >> 2) & 3u) ^ (2u * f);
+      return w.template load16<2>(dead + (c + 32u * f + 16u * (strip & 1u)) * 64u + slot * 16u, ((strip >> 1) * n_kb + kb) * 4096u);
     } else {
-      return w.template load16<2>(there && 4u * kb + h < groups ? (32u * strip + 2u * c + f) * col_bytes + 64u * kb + 16u * h : kMoeOob);
+      return w.template load16<2>(4u * kb + h < groups ? dead + (32u * strip + 2u * c + f) * col_bytes + 64u * kb + 16u * h : kMoeOob);
     }
   }
-  // their scale, as a dword whose byte `scale_shift` is it
-  TAMD_DEVICE void scales2(uint32_t strip, uint32_t kb, uint32_t c, uint32_t h, bool there, uint32_t &s0, uint32_t &s1) const {
+  // the scales of columns 2 c and 2 c + 1 of a strip, each as a dword that `factor2` takes it from
+  TAMD_DEVICE void scales2(uint32_t strip, uint32_t kb, uint32_t c, uint32_t h, uint32_t dead, uint32_t &s0, uint32_t &s1) const {
     if constexpr (SHUFFLED) {
-      const uint32_t off = 64u * h + 4u * ((2u * c) & 15u);
-      const u32x2_t v = sc.load8(there ? off : kMoeOob, there ? (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u : 0u);
+      const u32x2_t v = sc.load8(dead + 64u * h + 4u * ((2u * c) & 15u), (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u);
       s0 = v.x, s1 = v.y;
     } else {
-      const uint32_t g = 4u * kb + h, at = (32u * strip + 2u * c) * sc_col + g;
-      s0 = sc.load1(there && g < groups ? at : kMoeOob);
-      s1 = sc.load1(there && g < groups ? at + sc_col : kMoeOob);
+      const uint32_t g = 4u * kb + h, at = dead + (32u * strip + 2u * c) * sc_col + g;
+      s0 = sc.load1(g < groups ? at : kMoeOob);
+      s1 = sc.load1(g < groups ? at + sc_col : kMoeOob);
     }
   }
-  TAMD_DEVICE uint32_t scale1(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, bool there) const {
+  TAMD_DEVICE uint32_t scale1(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, uint32_t dead) const {
     if constexpr (SHUFFLED) {
-      const uint32_t n = 2u * c + f, off = 64u * h + 4u * (n & 15u) + 2u * (kb & 1u) + (n >> 4);
-      return sc.load1(there ? off : kMoeOob, there ? (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u : 0u);
+      const uint32_t n = 2u * c + f;
+      return sc.load1(dead + 64u * h + 4u * (n & 15u) + 2u * (kb & 1u) + (n >> 4), (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u);
     } else {
       const uint32_t g = 4u * kb + h;
-      return sc.load1(there && g < groups ? (32u * strip + 2u * c + f) * sc_col + g : kMoeOob);
+      return sc.load1(g < groups ? dead + (32u * strip + 2u * c + f) * sc_col + g : kMoeOob);
     }
   }
   // the scale as the conversion takes it: a float32 of which only the exponent counts
@@ -262,11 +269,14 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
   struct Stage {
     u32x4_t q0[NB], q1[NB], x[ROUNDS ? NB : 1][4];
     uint32_t s0[NB], s1[NB];
+    u32x2_t bias;   // of the pair tid % 16 of the strip: two float32, or two 16-bit numbers in the first dword
   };
-  const auto request_x = [&](u32x4_t (&to)[ROUNDS ? NB : 1][4], int i, const Cursor &p, uint32_t x_row, bool there) {
+  const bool bias_f32 = a.up.bias_dtype == TAMD_F32;
+  const int bias_bytes = a.up.bias ? (bias_f32 ? 4 : 2) : 0;
+  const auto request_x = [&](u32x4_t (&to)[ROUNDS ? NB : 1][4], int i, const Cursor &p, uint32_t x_row, uint32_t dead) {
     const uint32_t kb = p.k0 + (uint32_t)wave * NB + i;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) to[i][j] = x.load16(there && 4u * kb + h < (uint32_t)K / 32u ? x_row + 256u * kb + 16u * j : kMoeOob);
+    for (int j = 0; j < 4; ++j) to[i][j] = x.load16(4u * kb + h < (uint32_t)K / 32u ? dead + x_row + 256u * kb + 16u * j : kMoeOob);
   };
   const auto x_row_of = [&](const Cursor &p) {   // row c of the tile: the byte offset of its token's x
     const int row = __builtin_amdgcn_readfirstlane(first_row(p.at)) + p.m0 + (int)c;
@@ -275,17 +285,26 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
   const auto request = [&](Stage &s, Cursor &p) {
     const bool live = p.unit < unit1;
     const uint32_t at = live ? p.at : 0u;
-    const ExpertWeights<BLOCKS, SHUFFLED> w(a.up, __builtin_amdgcn_readfirstlane((int)r.expert[at]), K, 2 * I);
+    const int e = __builtin_amdgcn_readfirstlane((int)r.expert[at]);
+    const ExpertWeights<BLOCKS, SHUFFLED> w(a.up, e, K, 2 * I);
     uint32_t x_row = 0;
     if constexpr (ROUNDS) x_row = x_row_of(Cursor{p.unit, at, p.strip, p.k0, p.m0});
+    const Buffer bias((const uint8_t *)a.up.bias + e * a.up.bias_stride_e * bias_bytes, 2 * (int64_t)I * bias_bytes);
+    s.bias = bias.load8((16u * p.strip + (uint32_t)(tid & 15)) * 2u * (uint32_t)bias_bytes);
+    __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const uint32_t kb = p.k0 + (uint32_t)wave * NB + i;
-      const bool there = live && kb < n_kb;
-      s.q0[i] = w.codes(p.strip, 0, kb, c, h, there);
-      s.q1[i] = w.codes(p.strip, 1, kb, c, h, there);
-      w.scales2(p.strip, kb, c, h, there, s.s0[i], s.s1[i]);
-      if constexpr (ROUNDS) request_x(s.x, i, p, x_row, there);
+      const uint32_t kb = p.k0 + (uint32_t)wave * NB + i, dead = dead_unless(live && kb < n_kb);
+      s.q0[i] = w.codes(p.strip, 0, kb, c, h, dead);
+      __builtin_amdgcn_sched_barrier(0);
+      s.q1[i] = w.codes(p.strip, 1, kb, c, h, dead);
+      __builtin_amdgcn_sched_barrier(0);
+      w.scales2(p.strip, kb, c, h, dead, s.s0[i], s.s1[i]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (ROUNDS) {
+        request_x(s.x, i, p, x_row, dead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (live) advance(p);
   };
@@ -306,12 +325,18 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) xr[i][j] = x.load16(4u * kb + h < (uint32_t)K / 32u ? x_row + 256u * kb + 16u * j : kMoeOob);
       }
+      // awaited here: behind the branch the compiler would have to await everything in every stage
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(xr[i][j]));
       x_at = now.at;
     }
   };
   const auto multiply = [&](const Stage &s) {
+    const bool live = now.unit < unit1;
     if constexpr (!ROUNDS)
-      if (x_at != now.at) load_x();
+      if (live && x_at != now.at) load_x();
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const uint32_t kb = now.k0 + (uint32_t)wave * NB + i;
@@ -326,24 +351,22 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
       }
     }
     const Cursor done = now;
-    advance(now);
+    if (live) advance(now);
     if (ROUNDS && now.k0 != 0) return;   // (more of this unit's K)
     red[turn][wave][0][lane] = acc0;
     red[turn][wave][1][lane] = acc1;
     acc0 = acc1 = f32x4_t{0.f, 0.f, 0.f, 0.f};
     sync_threads();
     // row m of the tile, pair of the strip: element m % 4 of lanes (pair, m / 4)
-    const int m = tid >> 4, pair = tid & 15, row = first_row(done.at) + done.m0 + m;
-    if (m < 16 && row < end_row(done.at)) {
+    const uint32_t done_at = live ? done.at : 0u;
+    const int m = tid >> 4, pair = tid & 15, row = first_row(done_at) + done.m0 + m;
+    if (live && m < 16 && row < end_row(done_at)) {
       const int from = (m >> 2) * 16 + pair;
       float g = 0.f, l = 0.f;
 #pragma unroll
       for (int v = 0; v < 8; ++v) g += ((const float *)&red[turn][v][0][from])[m & 3], l += ((const float *)&red[turn][v][1][from])[m & 3];
-      if (a.up.bias) {
-        const int64_t b = (int)r.expert[done.at] * a.up.bias_stride_e + 32 * (int64_t)done.strip + 2 * pair;
-        g += load_any_f32(a.up.bias, a.up.bias_dtype, b);
-        l += load_any_f32(a.up.bias, a.up.bias_dtype, b + 1);
-      }
+      g += bias_f32 ? bits_to_f32(s.bias.x) : a.up.bias_dtype == TAMD_BF16 ? bf16_bits_to_f32(s.bias.x & 0xFFFFu) : f16_bits_to_f32(s.bias.x & 0xFFFFu);
+      l += bias_f32 ? bits_to_f32(s.bias.y) : a.up.bias_dtype == TAMD_BF16 ? bf16_bits_to_f32(s.bias.x >> 16) : f16_bits_to_f32(s.bias.x >> 16);
       const float v = r.row_gate[row] * swiglu_keeping_nan(a, g, l);
       const uint32_t hi = XDT == TAMD_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
       const float rest = v - (XDT == TAMD_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi));
@@ -359,12 +382,10 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
   Stage s0, s1;
   request(s0, ask);
   request(s1, ask);
-  for (;;) {
+  while (now.unit < unit1) {
     multiply(s0);
-    if (now.unit == unit1) break;
     request(s0, ask);
-    multiply(s1);
-    if (now.unit == unit1) break;
+    multiply(s1);   // (possibly of nothing: with a way out in between the compiler would await all requests of a round)
     request(s1, ask);
   }
 }
@@ -419,17 +440,22 @@ __global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const bool there = p.item < end;
+      const uint32_t dead = dead_unless(there);
       const ExpertWeights<BLOCKS, SHUFFLED> w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[there ? p.at : 0u]), K, N);
-      b.q[i] = w.codes(strip, f, p.kb, c, h, there);
-      b.s[i] = w.scale1(strip, f, p.kb, c, h, there);
+      b.q[i] = w.codes(strip, f, p.kb, c, h, dead);
+      __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
+      b.s[i] = w.scale1(strip, f, p.kb, c, h, dead);
+      __builtin_amdgcn_sched_barrier(0);
       if (there) p.next(n_kb);
     }
   };
   // row c of tile t of the rows from `row` on
-  const auto request_x = [&](u32x4_t (&to)[4], uint32_t row, uint32_t rows, int t, uint32_t kb, bool there) {
-    const bool mine = there && 16u * t + c < 2u * rows && 4u * kb + h < (uint32_t)K / 32u;
+  const auto request_x = [&](u32x4_t (&to)[4], uint32_t row, uint32_t rows, int t, uint32_t kb) {
+    uint32_t off = 16u * t + c < 2u * rows && 4u * kb + h < (uint32_t)K / 32u ? (2u * row + 16u * t + c) * (uint32_t)(2 * K) + 256u * kb + 64u * h : kMoeOob;
+    asm volatile("" : "+v"(off));   // (as in dead_unless)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) to[j] = planes.load16(mine ? (2u * row + 16u * t + c) * (uint32_t)(2 * K) + 256u * kb + 64u * h + 16u * j : kMoeOob);
+    for (int j = 0; j < 4; ++j) to[j] = planes.load16(off + 16u * j);
+    __builtin_amdgcn_sched_barrier(0);
   };
   const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
     row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
@@ -446,30 +472,30 @@ __global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a
       const bool there = ask_x.item < end;
       uint32_t row, rows;
       rows_at(there ? ask_x.at : 0u, row, rows);
-      request_x(to, row, rows, 0, ask_x.kb, there);
+      request_x(to, row, there ? rows : 0u, 0, ask_x.kb);
       if (there) ask_x.next(n_kb);
     };
+    // (items past the end multiply zeros: no branch around what requests)
     const auto multiply = [&](const Batch &b, int i) {
       uint32_t row, rows;
-      rows_at(now.at, row, rows);
+      const bool there = now.item < end;
+      rows_at(there ? now.at : 0u, row, rows);
+      rows = there ? rows : 0u;
       const float factor = bits_to_f32(b.s[i] << 23);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const auto w = M::expand(b.q[i][j], factor);
-        acc[0] = Mma16<XDT>::mma(as_frag<XDT>(xr[i & 1][j]), w, acc[0]);
-      }
+      for (int j = 0; j < 4; ++j) acc[0] = Mma16<XDT>::mma(as_frag<XDT>(xr[i & 1][j]), M::expand(b.q[i][j], factor), acc[0]);
       if constexpr (MT > 1) {
 #pragma unroll
         for (int t = 1; t < MT; ++t)
           if (8u * t < rows) {
             u32x4_t xt[4];
-            request_x(xt, row, rows, t, now.kb, true);
+            request_x(xt, row, rows, t, now.kb);
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[t] = Mma16<XDT>::mma(as_frag<XDT>(xt[j]), M::expand(b.q[i][j], factor), acc[t]);
           }
       }
-      now.next(n_kb);
-      if (now.kb == 0 || now.item == end) {   // the expert's end: elements 2 p and 2 p + 1 of lane (c, h) are the planes of row 8 t + 2 h + p
+      if (there) now.next(n_kb);
+      if (there && (now.kb == 0 || now.item == end)) {   // the expert's end: elements 2 p and 2 p + 1 of lane (c, h) are the planes of row 8 t + 2 h + p
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
@@ -488,16 +514,12 @@ __global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a
     ask_rows(xr[0]);
     ask_rows(xr[1]);
     request(b1, ask);
-    while (true) {
+    while (now.item < end) {
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (now.item < end) multiply(b0, i);
-      if (now.item == end) break;
+      for (int i = 0; i < U; ++i) multiply(b0, i);
       request(b0, ask);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (now.item < end) multiply(b1, i);
-      if (now.item == end) break;
+      for (int i = 0; i < U; ++i) multiply(b1, i);
       request(b1, ask);
     }
   }

@@ -13,6 +13,7 @@ int check_moe_weights(const tamd_moe_weights &p, int64_t K, int64_t N) {
   if (p.w_stride_e < 0 || p.scale_stride_e < 0 || (!blocks && p.w_stride_n < 0) || (!shuffled && p.scale_stride_n < 0)) return TAMD_E_INVALID;
   if (!aligned(p.w, 16) || p.w_stride_e % 16 != 0 || (!blocks && p.w_stride_n % 16 != 0)) return TAMD_E_ALIGNMENT;
   if (shuffled && (!aligned(p.scale, 16) || p.scale_stride_e % 16 != 0)) return TAMD_E_ALIGNMENT;
+  if (p.bias && (!aligned(p.bias, 4) || (p.bias_dtype != TAMD_F32 && p.bias_stride_e % 2 != 0))) return TAMD_E_ALIGNMENT;   // pairs of 16-bit numbers
   // one expert is addressed with 32 bits
   const int64_t most = kMoeOob, w_bytes = blocks ? (N + 63) / 64 * ((K + 127) / 128) * 4096 : K / 2;
   if (w_bytes >= most || (!blocks && p.w_stride_n >= (most - w_bytes) / N)) return TAMD_E_UNSUPPORTED;

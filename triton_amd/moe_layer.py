@@ -72,7 +72,10 @@ def _weights(into, w, pc, bias, E, K, N, device, n):
             f"bias{n}: a tensor of shape {(E, N)} with unit stride along its last axis, on the device of x"
         if bias.dtype not in _BIAS_TYPES:
             raise NotImplementedError(f"bias{n}: dtype {bias.dtype} is not built")
+        if bias.data_ptr() % 4 or bias.stride(0) % 2:
+            bias = bias.clone(memory_format=torch.contiguous_format)
         into.bias, into.bias_stride_e, into.bias_dtype = bias.data_ptr(), bias.stride(0), _lib.dtype_code(bias.dtype)
+        return bias   # (alive until the launch)
 
 
 def moe_layer(x: torch.Tensor, logits: torch.Tensor, n_expts_act: int, w1, bias1: Optional[torch.Tensor], w2,
@@ -111,8 +114,8 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, n_expts_act: int, w1, bias1
     if H % 32 or inter % 32 or not H or not inter:
         raise ValueError(f"hidden ({H}) and inter ({inter}) must be multiples of 32")
     a = _lib.MoeLayerArgs()
-    _weights(a.up, w1, precision_config1, bias1, E, H, two_inter, x.device, 1)
-    _weights(a.down, w2, precision_config2, bias2, E, inter, H, x.device, 2)
+    held = [_weights(a.up, w1, precision_config1, bias1, E, H, two_inter, x.device, 1),
+            _weights(a.down, w2, precision_config2, bias2, E, inter, H, x.device, 2)]  # noqa: F841
     if out is None:
         out = torch.empty((T, H), dtype=x.dtype, device=x.device)
     else:
