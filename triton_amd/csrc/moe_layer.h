@@ -106,14 +106,17 @@ struct ExpertWeights {
       s1 = sc.load1(g < groups ? at + sc_col : kMoeOob);
     }
   }
-  TAMD_DEVICE uint32_t scale1(uint32_t strip, uint32_t f, uint32_t kb, uint32_t c, uint32_t h, uint32_t dead) const {
-    if constexpr (SHUFFLED) {
-      const uint32_t n = 2u * c + f;
-      return sc.load1(dead + 64u * h + 4u * (n & 15u) + 2u * (kb & 1u) + (n >> 4), (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u);
-    } else {
-      const uint32_t g = 4u * kb + h;
-      return sc.load1(g < groups ? dead + (32u * strip + 2u * c + f) * sc_col + g : kMoeOob);
-    }
+  // the same of one column (f) in parts: what depends on the lane, and the scalar offset of a block; nothing is masked
+  TAMD_DEVICE uint32_t code_offset(uint32_t strip, uint32_t f, uint32_t c, uint32_t h) const {
+    return BLOCKS ? (c + 32u * f + 16u * (strip & 1u)) * 64u + (h ^ ((c >> 2) & 3u) ^ (2u * f)) * 16u : (32u * strip + 2u * c + f) * col_bytes + 16u * h;
+  }
+  TAMD_DEVICE uint32_t code_block(uint32_t strip, uint32_t kb) const { return BLOCKS ? ((strip >> 1) * n_kb + kb) * 4096u : 64u * kb; }
+  TAMD_DEVICE uint32_t scale_offset(uint32_t strip, uint32_t f, uint32_t c, uint32_t h) const {
+    const uint32_t n = 2u * c + f;
+    return SHUFFLED ? 64u * h + 4u * (n & 15u) + (n >> 4) : (32u * strip + n) * sc_col + h;
+  }
+  TAMD_DEVICE uint32_t scale_block(uint32_t strip, uint32_t kb) const {
+    return SHUFFLED ? (strip * ((groups + 7u) / 8u) + (kb >> 1)) * 256u + 2u * (kb & 1u) : 4u * kb;
   }
   // the scale as the conversion takes it: a float32 of which only the exponent counts
   TAMD_DEVICE static float factor2(uint32_t word, uint32_t kb, uint32_t c) {
@@ -397,14 +400,13 @@ struct MoeDownLds {
 };
 static_assert(sizeof(MoeDownLds) % 16 == 0);
 
-// A workgroup owns 16 columns of y, its sixteen waves equal parts of the list of items (picked expert, 128 K).  A wave has the weights
+// A workgroup owns 16 columns of y, its W waves equal parts of the list of items (picked expert, 128 K).  A wave has the weights
 // of 2 U items in flight, across experts.  Rows of a tile are the two planes of up to eight of the expert's tokens, MT tiles at a
 // time; at an expert's end a wave adds its tokens' sums to its own copy of the output in LDS, where the copies are added
 // up at last: no atomics, and NaN or infinite weights stay with the tokens that picked them.
-template <int XDT, bool BLOCKS, bool SHUFFLED, int MT, int U>
-__global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a) {
+template <int XDT, bool BLOCKS, bool SHUFFLED, int MT, int U, int W>
+__global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
-  constexpr int W = 16;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   MoeDownLds &s = *(MoeDownLds *)lds;
   float *sums = (float *)(lds + sizeof(MoeDownLds));   // [W, n_tokens, 16]
@@ -419,83 +421,108 @@ __global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a
     s.gate[tid] = tab->gate[tid], s.pick[tid] = tab->pick[tid], s.token[tid] = tab->token[tid];
   }
   if (tid == 0) s.start[slots] = (uint16_t)slots;
-  for (int i = tid; i < W * T * 16; i += 1024) sums[i] = 0.f;
+  for (int i = tid; i < W * T * 16; i += 64 * W) sums[i] = 0.f;
   sync_threads();
+  // the biases of this thread's outputs by their gate weights, eight picks requested at a time
+  const auto bias_of = [&](int i) {
+    float v = 0.f;
+    const int token = i >> 4;
+    const int64_t n = 32 * (int64_t)(blockIdx.x >> 1) + 2 * (i & 15) + (blockIdx.x & 1);
+    for (int j0 = 0; j0 < a.n_picks; j0 += 8) {
+      float b[8], g[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int pick = j0 + j < a.n_picks ? j0 + j : a.n_picks - 1, slot = token * a.n_picks + pick;
+        g[j] = j0 + j < a.n_picks ? s.gate[slot] : 0.f;
+        b[j] = load_any_f32(a.down.bias, a.down.bias_dtype, s.pick[slot] * a.down.bias_stride_e + n);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = j0 + j < a.n_picks ? __builtin_fmaf(g[j], b[j], v) : v;
+    }
+    return v;
+  };
+  float from_bias[2] = {0.f, 0.f};   // (64 tokens x 16 columns: two outputs per thread at most)
+  if (a.down.bias) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+      if (tid + m * 64 * W < T * 16) from_bias[m] = bias_of(tid + m * 64 * W);
+  }
   const Buffer planes((const uint8_t *)a.workspace + kMoeTableBytes, (int64_t)slots * 4 * K);
   const uint32_t strip = blockIdx.x >> 1, f = blockIdx.x & 1u, n_kb = (uint32_t)(K + 127) / 128u, total = n_active * n_kb;
   const uint32_t begin = (uint32_t)((uint64_t)total * (uint32_t)wave / W), end = (uint32_t)((uint64_t)total * (uint32_t)(wave + 1) / W);
 
-  struct Cursor {
-    uint32_t item, at, kb;
-    TAMD_DEVICE void next(uint32_t n_kb_) {
-      ++item;
-      if (++kb == n_kb_) kb = 0, ++at;
-    }
-  };
-  struct Batch {
-    u32x4_t q[U];
-    uint32_t s[U];
-  };
-  const auto request = [&](Batch &b, Cursor &p) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const bool there = p.item < end;
-      const uint32_t dead = dead_unless(there);
-      const ExpertWeights<BLOCKS, SHUFFLED> w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[there ? p.at : 0u]), K, N);
-      b.q[i] = w.codes(strip, f, p.kb, c, h, dead);
-      __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
-      b.s[i] = w.scale1(strip, f, p.kb, c, h, dead);
-      __builtin_amdgcn_sched_barrier(0);
-      if (there) p.next(n_kb);
-    }
-  };
-  // row c of tile t of the rows from `row` on
-  const auto request_x = [&](u32x4_t (&to)[4], uint32_t row, uint32_t rows, int t, uint32_t kb) {
-    uint32_t off = 16u * t + c < 2u * rows && 4u * kb + h < (uint32_t)K / 32u ? (2u * row + 16u * t + c) * (uint32_t)(2 * K) + 256u * kb + 64u * h : kMoeOob;
-    asm volatile("" : "+v"(off));   // (as in dead_unless)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) to[j] = planes.load16(off + 16u * j);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
-    row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
-    rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at + 1]) - row;
-  };
-
   if (begin < end) {
-    Cursor ask{begin, begin / n_kb, begin % n_kb}, ask_x = ask, now = ask;
+    struct Batch {
+      u32x4_t q[U], x[U][4];
+      uint32_t s[U];
+    };
+    typedef ExpertWeights<BLOCKS, SHUFFLED> Weights;
+    const uint32_t groups = (uint32_t)K / 32u, tail = groups - 4u * (n_kb - 1u);   // groups of the last block
+    const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
+      row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
+      rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at + 1]) - row;
+    };
+    // row c of tile t of an expert's rows of h
+    const auto x_offset = [&](uint32_t row, uint32_t rows, int t) {
+      return 16u * t + c < 2u * rows ? (2u * row + 16u * t + c) * (uint32_t)(2 * K) + 64u * h : kMoeOob;
+    };
+    const auto request_x = [&](u32x4_t (&to)[4], uint32_t off, uint32_t kb) {
+      uint32_t last = (uint32_t)__builtin_amdgcn_readfirstlane(kb + 1u == n_kb ? -1 : 0);
+      asm volatile("" : "+s"(last));   // (as in dead_unless)
+      const uint32_t beyond = h >= tail && off != kMoeOob ? kMoeOob : 0u;
+      off += beyond & last;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[j] = planes.load16(off + 16u * j, 256u * kb);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // ---- requests: constant offsets of the lane, the block in the scalar offset.  Weights past K in a last block are multiplied by
+    // zeros of h; what is past the last item comes from empty buffers.
+    uint32_t ask = begin, ask_at = begin / n_kb, ask_kb = begin % n_kb, row, rows;
+    rows_at(ask_at, row, rows);
+    uint32_t x_off = x_offset(row, rows, 0);
+    Weights w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[ask_at]), K, N);
+    const uint32_t code_off = w.code_offset(strip, f, c, h), scale_off = w.scale_offset(strip, f, c, h);
+    const auto request = [&](Batch &b) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        request_x(b.x[i], x_off, ask_kb);
+        b.q[i] = w.w.template load16<2>(code_off, w.code_block(strip, ask_kb));
+        __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
+        b.s[i] = w.sc.load1(scale_off, w.scale_block(strip, ask_kb));
+        __builtin_amdgcn_sched_barrier(0);
+        ++ask_kb, ++ask;
+        if (ask_kb == n_kb || ask >= end) {
+          ask_kb = 0, ++ask_at;
+          const uint32_t next = ask < end ? ask_at : 0u;
+          uint32_t row_x, rows_x;
+          rows_at(next, row_x, rows_x);
+          x_off = x_offset(row_x, ask < end ? rows_x : 0u, 0);
+          w = Weights(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[next]), K, N);
+          if (ask >= end) w.w = w.sc = Buffer(a.down.w, 0);
+        }
+      }
+    };
+    // ---- products
+    uint32_t item = begin, at = ask_at, kb = ask_kb;
     f32x4_t acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    u32x4_t xr[2][4];   // first tile's rows of the next two items
-    const auto ask_rows = [&](u32x4_t (&to)[4]) {
-      const bool there = ask_x.item < end;
-      uint32_t row, rows;
-      rows_at(there ? ask_x.at : 0u, row, rows);
-      request_x(to, row, there ? rows : 0u, 0, ask_x.kb);
-      if (there) ask_x.next(n_kb);
-    };
-    // (items past the end multiply zeros: no branch around what requests)
-    const auto multiply = [&](const Batch &b, int i) {
-      uint32_t row, rows;
-      const bool there = now.item < end;
-      rows_at(there ? now.at : 0u, row, rows);
-      rows = there ? rows : 0u;
-      const float factor = bits_to_f32(b.s[i] << 23);
+    const auto multiply = [&](const Batch &b, int i) {   // (an item past the end: zeros)
+      const float factor = bits_to_f32((SHUFFLED || 4u * kb + h < groups ? b.s[i] : 127u) << 23);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[0] = Mma16<XDT>::mma(as_frag<XDT>(xr[i & 1][j]), M::expand(b.q[i][j], factor), acc[0]);
+      for (int j = 0; j < 4; ++j) acc[0] = Mma16<XDT>::mma(as_frag<XDT>(b.x[i][j]), M::expand(b.q[i][j], factor), acc[0]);
       if constexpr (MT > 1) {
 #pragma unroll
         for (int t = 1; t < MT; ++t)
           if (8u * t < rows) {
             u32x4_t xt[4];
-            request_x(xt, row, rows, t, now.kb);
+            request_x(xt, x_offset(row, rows, t), kb);
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[t] = Mma16<XDT>::mma(as_frag<XDT>(xt[j]), M::expand(b.q[i][j], factor), acc[t]);
           }
       }
-      if (there) now.next(n_kb);
-      if (there && (now.kb == 0 || now.item == end)) {   // the expert's end: elements 2 p and 2 p + 1 of lane (c, h) are the planes of row 8 t + 2 h + p
+      ++kb, ++item;
+      if (kb == n_kb || item == end) {   // the expert's end: elements 2 p and 2 p + 1 of lane (c, h) are the planes of row 8 t + 2 h + p
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
@@ -505,37 +532,34 @@ __global__ __launch_bounds__(1024, 4) void moe_down_kernel(tamd_moe_layer_args a
           }
           acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
+        kb = 0, ++at;
+        if (item < end) rows_at(at, row, rows);
+        else rows = 0;
       }
-      ask_rows(xr[i & 1]);
     };
-    static_assert(U % 2 == 0);
     Batch b0, b1;
-    request(b0, ask);
-    ask_rows(xr[0]);
-    ask_rows(xr[1]);
-    request(b1, ask);
-    while (now.item < end) {
+    request(b0);
+    request(b1);
+    while (item < end) {
 #pragma unroll
       for (int i = 0; i < U; ++i) multiply(b0, i);
-      request(b0, ask);
+      request(b0);
 #pragma unroll
       for (int i = 0; i < U; ++i) multiply(b1, i);
-      request(b1, ask);
+      request(b1);
     }
   }
   sync_threads();
-  for (int i = tid; i < T * 16; i += 1024) {
-    const int token = i >> 4;
-    float v = 0.f;
+  static_assert(kMoeTokens * 16 <= 2 * 64 * W);
 #pragma unroll
-    for (int w = 0; w < W; ++w) v += sums[w * T * 16 + i];
-    const int64_t n = 32 * (int64_t)strip + 2 * (i & 15) + f;
-    if (a.down.bias)
-      for (int j = 0; j < a.n_picks; ++j) {
-        const int slot = token * a.n_picks + j;
-        v = __builtin_fmaf(s.gate[slot], load_any_f32(a.down.bias, a.down.bias_dtype, s.pick[slot] * a.down.bias_stride_e + n), v);
-      }
-    store_any(a.y, XDT, token * a.y_stride_m + n, v);
+  for (int m = 0; m < 2; ++m) {
+    const int i = tid + m * 64 * W;
+    if (i < T * 16) {
+      float v = from_bias[m];
+#pragma unroll
+      for (int w = 0; w < W; ++w) v += sums[w * T * 16 + i];
+      store_any(a.y, XDT, (i >> 4) * a.y_stride_m + 32 * (int64_t)strip + 2 * (i & 15) + f, v);
+    }
   }
 }
 
@@ -576,10 +600,10 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
 template <int XDT, bool BLOCKS, bool SHUFFLED>
 int launch_moe_down(const tamd_moe_layer_args &a, hipStream_t st) {
   const dim3 grid((unsigned)(a.hidden / 16));
-  const size_t lds = sizeof(MoeDownLds) + (size_t)a.n_tokens * 16 * 16 * 4;
-  const auto kernel = a.n_tokens <= 8 ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, 1, 4> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, 8, 2>;
-  if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
-  kernel<<<grid, 1024, lds, st>>>(a);
+  constexpr int W = 8;
+  const size_t lds = sizeof(MoeDownLds) + (size_t)a.n_tokens * W * 16 * 4;
+  const auto kernel = a.n_tokens <= 8 ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, 1, 4, W> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, 8, 3, W>;
+  kernel<<<grid, 64 * W, lds, st>>>(a);
   return launch_status();
 }
 
