@@ -226,7 +226,7 @@ TAMD_DEVICE float swiglu_keeping_nan(const tamd_moe_layer_args &a, float g, floa
 // A workgroup per CU takes a contiguous part of the units (picked expert, strip of 32 columns): consecutive strips of an expert, whose
 // rows of x then stay in registers.  Its eight waves split K, NB blocks of 128 each; the weights of two units are in flight
 // (48 KB per CU with NB = 3), their partial sums meet in LDS, a barrier per unit.  A stage is a unit, 16 of its rows and 8 * NB
-// blocks of K; with ROUNDS there may be several of a unit (long K, more than 16 tokens) and x travels with the weights.
+// blocks of K; with ROUNDS (long K, many rows per expert) a unit may have several of K and x travels with the weights.
 // As a loop without requests ahead, two workgroups per CU, 16 tokens of 128 experts of 2880 x 5760 took 154 us instead of TODO.
 template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, bool ROUNDS>
 __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
@@ -257,6 +257,7 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
     uint32_t unit, at, strip, k0;
     int m0;
   };
+  // With ROUNDS a unit's stages follow each other; else all strips of an expert come before its next 16 rows: x stays.
   const auto advance = [&](Cursor &p) {
     if constexpr (ROUNDS) {
       p.k0 += 8 * NB;
@@ -266,8 +267,13 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
       if (p.m0 < __builtin_amdgcn_readfirstlane(end_row(p.at) - first_row(p.at))) return;
       p.m0 = 0;
     }
-    ++p.unit;
-    if (++p.strip == strips) p.strip = 0, ++p.at;
+    ++p.unit, ++p.strip;
+    if (!ROUNDS && (p.strip == strips || p.unit == unit1) && p.m0 + 16 < __builtin_amdgcn_readfirstlane(end_row(p.at) - first_row(p.at))) {
+      const uint32_t first = p.at * strips > unit0 ? p.at * strips : unit0;
+      p.m0 += 16, p.strip -= p.unit - first, p.unit = first;
+    } else if (p.strip == strips) {
+      p.strip = 0, p.m0 = 0, ++p.at;
+    }
   };
   struct Stage {
     u32x4_t q0[NB], q1[NB], x[ROUNDS ? NB : 1][4];
@@ -317,6 +323,7 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
   now = ask;
   u32x4_t xr[ROUNDS ? 1 : NB][4];
   uint32_t x_at = 0xFFFFFFFFu;
+  int x_m0 = 0;
   f32x4_t acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = acc0;
   uint32_t turn = 0;
   const auto load_x = [&]() {
@@ -333,13 +340,13 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
       for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(xr[i][j]));
-      x_at = now.at;
+      x_at = now.at, x_m0 = now.m0;
     }
   };
   const auto multiply = [&](const Stage &s) {
     const bool live = now.unit < unit1;
     if constexpr (!ROUNDS)
-      if (live && x_at != now.at) load_x();
+      if (live && (x_at != now.at || x_m0 != now.m0)) load_x();
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const uint32_t kb = now.k0 + (uint32_t)wave * NB + i;
@@ -399,18 +406,28 @@ struct MoeDownLds {
   uint8_t token[kMoeSlots];
 };
 static_assert(sizeof(MoeDownLds) % 16 == 0);
+template <int NB, int RC>
+constexpr int kMoeDownPitch = 256 * NB + 16;   // bytes of a row of h in a wave's buffer (rows 16 bytes apart on the banks)
 
-// A workgroup owns 16 columns of y, its W waves equal parts of the list of items (picked expert, 128 K).  A wave has the weights
-// of 2 U items in flight, across experts.  Rows of a tile are the two planes of up to eight of the expert's tokens, MT tiles at a
-// time; at an expert's end a wave adds its tokens' sums to its own copy of the output in LDS, where the copies are added
-// up at last: no atomics, and NaN or infinite weights stay with the tokens that picked them.
-template <int XDT, bool BLOCKS, bool SHUFFLED, int MT, int U, int W>
-__global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_args a) {
+// A workgroup owns 16 columns of y; its eight waves split K, NB blocks of 128 each, and walk over the picked experts with the weights of
+// D experts in flight.  A row of a tile is a plane of one of the expert's tokens, RC tokens at a time; when these are multiplied
+// a wave adds the tokens' sums to its own copy of the output in LDS, where the copies are added up at last: no atomics, and
+// NaN or infinite weights stay with the tokens that picked them.
+//
+// h comes as a few dense requests and goes through LDS, a buffer per wave, to where the MFMAs want it: requested in their layout
+// it takes four requests per block, most lanes of which bring nothing, and a request costs the CU about 20 cycles whatever it
+// brings (16 tokens of 128 experts of 2880 x 2880: 90 us, 50 without these requests, TODO now).
+template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D>
+__global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
+  typedef ExpertWeights<BLOCKS, SHUFFLED> Weights;
+  constexpr int W = 8, PITCH = kMoeDownPitch<NB, RC>, XR = NB * RC / 2 > 0 ? (NB * RC + 1) / 2 : 1;   // dense requests of 2 RC rows
+  constexpr int NS = SHUFFLED ? NB / 2 + 1 : NB;   // scale requests: a dword of the pre-shuffle serves blocks 2 i and 2 i + 1
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   MoeDownLds &s = *(MoeDownLds *)lds;
-  float *sums = (float *)(lds + sizeof(MoeDownLds));   // [W, n_tokens, 16]
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  uint8_t *const rows_lds = lds + sizeof(MoeDownLds) + wave * (2 * RC * PITCH);
+  float *const sums = (float *)(lds + sizeof(MoeDownLds) + W * (2 * RC * PITCH));   // [W, n_tokens, 16]
   const uint32_t c = lane & 15, h = lane >> 4;
   const int K = a.inter, N = a.hidden, T = a.n_tokens;
   const MoeTables *tab = (const MoeTables *)a.workspace;
@@ -423,17 +440,130 @@ __global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_
   if (tid == 0) s.start[slots] = (uint16_t)slots;
   for (int i = tid; i < W * T * 16; i += 64 * W) sums[i] = 0.f;
   sync_threads();
-  // the biases of this thread's outputs by their gate weights, eight picks requested at a time
+  const Buffer planes((const uint8_t *)a.workspace + kMoeTableBytes, (int64_t)slots * 4 * K);
+  const uint32_t strip = blockIdx.x >> 1, f = blockIdx.x & 1u, n_kb = (uint32_t)(K + 127) / 128u, groups = (uint32_t)K / 32u;
+
+  // ---- a stage is an expert and up to 8 NB blocks of K, cut evenly: the wave's are kb0 .. kb0 + n - 1
+  struct Cursor {
+    uint32_t at, k0, kb0, n;
+  };
+  const auto part = [&](Cursor &p) {
+    const uint32_t here = n_kb - p.k0 < 8u * NB ? n_kb - p.k0 : 8u * NB, from = here * (uint32_t)wave / W;
+    p.kb0 = p.k0 + from, p.n = here * (uint32_t)(wave + 1) / W - from;
+  };
+  const auto advance = [&](Cursor &p) {
+    p.k0 += 8 * NB;
+    if (p.k0 >= n_kb) p.k0 = 0, ++p.at;
+    if (8 * NB < n_kb) part(p);
+  };
+  const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
+    row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
+    rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at + 1]) - row;
+  };
+  struct Stage {
+    u32x4_t q[NB], x[XR];
+    uint32_t s[NS];
+  };
+  // 16-byte chunk i * 64 + lane of the rows: row by row, 16 NB chunks each; zeros past K and past the rows
+  const auto request_x = [&](u32x4_t (&to)[XR], uint32_t row, uint32_t rows, uint32_t kb0, uint32_t dead) {
+#pragma unroll
+    for (int i = 0; i < XR; ++i) {
+      const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), at = chunk % (16u * NB), k = 128u * kb0 + 8u * at;
+      uint32_t off = of < 2u * rows && of < 2u * RC && k < (uint32_t)K ? (2u * row + of) * (uint32_t)(2 * K) + 2u * k : kMoeOob;
+      asm volatile("" : "+v"(off));   // (as in dead_unless)
+      to[i] = planes.load16(off + (off == kMoeOob ? 0u : dead));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  Cursor ask{0, 0, 0, 0}, now;
+  part(ask);
+  now = ask;
+  const uint32_t code_off = Weights(a.down, 0, K, N).code_offset(strip, f, c, h), scale_off = Weights(a.down, 0, K, N).scale_offset(strip, f, c, h);
+  const auto request = [&](Stage &st) {
+    const bool live = ask.at < n_active;
+    const uint32_t at = live ? ask.at : 0u;
+    const Weights w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[at]), K, N);
+    uint32_t row, rows;
+    rows_at(at, row, rows);
+    request_x(st.x, row, rows, ask.kb0, dead_unless(live));
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {   // (one order wherever this is expanded: the waits are counted from it)
+      const uint32_t kb = ask.kb0 + i, dead = dead_unless(live && i < (int)ask.n);
+      if constexpr (BLOCKS) st.q[i] = w.w.template load16<2>(code_off + dead, w.code_block(strip, kb));
+      else st.q[i] = w.w.template load16<2>(4u * kb + h < groups ? code_off + dead : kMoeOob, w.code_block(strip, kb));
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (!SHUFFLED) {
+        st.s[i] = w.sc.load1(4u * kb + h < groups ? scale_off + dead : kMoeOob, w.scale_block(strip, kb));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if constexpr (SHUFFLED) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {   // blocks 2 (kb0 / 2 + i) and the next
+        const uint32_t pair = (ask.kb0 >> 1) + i;
+        st.s[i] = w.sc.load4((scale_off & ~3u) + dead_unless(live && 2u * pair < n_kb), w.scale_block(strip, 2u * pair));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (live) advance(ask);
+  };
+  const auto multiply = [&](const Stage &st) {
+    const bool live = now.at < n_active;
+    uint32_t row, rows;
+    rows_at(live ? now.at : 0u, row, rows);
+    for (uint32_t t0 = 0; t0 < (live ? rows : 0u); t0 += RC) {
+      const auto put = [&](const u32x4_t (&x)[XR]) {
+#pragma unroll
+        for (int i = 0; i < XR; ++i) {
+          const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), at = chunk % (16u * NB);
+          if (XR * kWave == 2 * RC * 16 * NB || of < 2u * RC) *(u32x4_t *)(rows_lds + of * PITCH + 16u * at) = x[i];
+        }
+      };
+      if (t0 == 0) {
+        put(st.x);
+      } else {   // more tokens than are requested ahead (awaited here, not behind the branch: the writes do that)
+        u32x4_t x[XR];
+        request_x(x, row + t0, rows - t0, now.kb0, 0);
+        put(x);
+      }
+      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t kb = now.kb0 + i;
+        uint32_t scale;
+        if constexpr (SHUFFLED) {
+          const uint32_t word0 = st.s[i / 2], word1 = st.s[i & 1 ? (i / 2 + 1 < NS ? i / 2 + 1 : i / 2) : i / 2];
+          scale = (now.kb0 & 1u ? word1 : word0) >> (8u * (((2u * c + f) >> 4) + 2u * (kb & 1u))) & 0xFFu;
+        } else {
+          scale = st.s[i];
+        }
+        const float factor = bits_to_f32(scale << 23);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {   // (rows past the buffer's repeat: no one reads their sums)
+          const u32x4_t xv = *(const u32x4_t *)(rows_lds + (c & (2u * RC - 1u)) * PITCH + 256u * i + 64u * h + 16u * j);
+          acc = Mma16<XDT>::mma(as_frag<XDT>(xv), M::expand(st.q[i][j], factor), acc);
+        }
+      }
+      // elements 2 p and 2 p + 1 of lane (c, h) are the planes of token 2 h + p of the tile
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t of = 2u * h + p;
+        if (of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * p] + acc[2 * p + 1];
+      }
+    }
+    if (live) advance(now);
+  };
+
+  // ---- the biases of this thread's outputs by their gate weights, eight picks requested at a time
   const auto bias_of = [&](int i) {
     float v = 0.f;
-    const int token = i >> 4;
-    const int64_t n = 32 * (int64_t)(blockIdx.x >> 1) + 2 * (i & 15) + (blockIdx.x & 1);
+    const int64_t n = 32 * (int64_t)strip + 2 * (i & 15) + f;
     for (int j0 = 0; j0 < a.n_picks; j0 += 8) {
       float b[8], g[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int pick = j0 + j < a.n_picks ? j0 + j : a.n_picks - 1, slot = token * a.n_picks + pick;
-        g[j] = j0 + j < a.n_picks ? s.gate[slot] : 0.f;
+        const int slot = (i >> 4) * a.n_picks + (j0 + j < a.n_picks ? j0 + j : a.n_picks - 1);
+        g[j] = s.gate[slot];
         b[j] = load_any_f32(a.down.bias, a.down.bias_dtype, s.pick[slot] * a.down.bias_stride_e + n);
       }
 #pragma unroll
@@ -441,116 +571,25 @@ __global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_
     }
     return v;
   };
-  float from_bias[2] = {0.f, 0.f};   // (64 tokens x 16 columns: two outputs per thread at most)
+  static_assert(kMoeTokens * 16 <= 2 * 64 * W);   // two outputs per thread at most
+  float from_bias[2] = {0.f, 0.f};
   if (a.down.bias) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
       if (tid + m * 64 * W < T * 16) from_bias[m] = bias_of(tid + m * 64 * W);
   }
-  const Buffer planes((const uint8_t *)a.workspace + kMoeTableBytes, (int64_t)slots * 4 * K);
-  const uint32_t strip = blockIdx.x >> 1, f = blockIdx.x & 1u, n_kb = (uint32_t)(K + 127) / 128u, total = n_active * n_kb;
-  const uint32_t begin = (uint32_t)((uint64_t)total * (uint32_t)wave / W), end = (uint32_t)((uint64_t)total * (uint32_t)(wave + 1) / W);
 
-  if (begin < end) {
-    struct Batch {
-      u32x4_t q[U], x[U][4];
-      uint32_t s[U];
-    };
-    typedef ExpertWeights<BLOCKS, SHUFFLED> Weights;
-    const uint32_t groups = (uint32_t)K / 32u, tail = groups - 4u * (n_kb - 1u);   // groups of the last block
-    const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
-      row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
-      rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at + 1]) - row;
-    };
-    // row c of tile t of an expert's rows of h
-    const auto x_offset = [&](uint32_t row, uint32_t rows, int t) {
-      return 16u * t + c < 2u * rows ? (2u * row + 16u * t + c) * (uint32_t)(2 * K) + 64u * h : kMoeOob;
-    };
-    const auto request_x = [&](u32x4_t (&to)[4], uint32_t off, uint32_t kb) {
-      uint32_t last = (uint32_t)__builtin_amdgcn_readfirstlane(kb + 1u == n_kb ? -1 : 0);
-      asm volatile("" : "+s"(last));   // (as in dead_unless)
-      const uint32_t beyond = h >= tail && off != kMoeOob ? kMoeOob : 0u;
-      off += beyond & last;
+  Stage st[D];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to[j] = planes.load16(off + 16u * j, 256u * kb);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    // ---- requests: constant offsets of the lane, the block in the scalar offset.  Weights past K in a last block are multiplied by
-    // zeros of h; what is past the last item comes from empty buffers.
-    uint32_t ask = begin, ask_at = begin / n_kb, ask_kb = begin % n_kb, row, rows;
-    rows_at(ask_at, row, rows);
-    uint32_t x_off = x_offset(row, rows, 0);
-    Weights w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[ask_at]), K, N);
-    const uint32_t code_off = w.code_offset(strip, f, c, h), scale_off = w.scale_offset(strip, f, c, h);
-    const auto request = [&](Batch &b) {
+  for (int d = 0; d < D; ++d) request(st[d]);
+  while (now.at < n_active) {
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        request_x(b.x[i], x_off, ask_kb);
-        b.q[i] = w.w.template load16<2>(code_off, w.code_block(strip, ask_kb));
-        __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
-        b.s[i] = w.sc.load1(scale_off, w.scale_block(strip, ask_kb));
-        __builtin_amdgcn_sched_barrier(0);
-        ++ask_kb, ++ask;
-        if (ask_kb == n_kb || ask >= end) {
-          ask_kb = 0, ++ask_at;
-          const uint32_t next = ask < end ? ask_at : 0u;
-          uint32_t row_x, rows_x;
-          rows_at(next, row_x, rows_x);
-          x_off = x_offset(row_x, ask < end ? rows_x : 0u, 0);
-          w = Weights(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[next]), K, N);
-          if (ask >= end) w.w = w.sc = Buffer(a.down.w, 0);
-        }
-      }
-    };
-    // ---- products
-    uint32_t item = begin, at = ask_at, kb = ask_kb;
-    f32x4_t acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const auto multiply = [&](const Batch &b, int i) {   // (an item past the end: zeros)
-      const float factor = bits_to_f32((SHUFFLED || 4u * kb + h < groups ? b.s[i] : 127u) << 23);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[0] = Mma16<XDT>::mma(as_frag<XDT>(b.x[i][j]), M::expand(b.q[i][j], factor), acc[0]);
-      if constexpr (MT > 1) {
-#pragma unroll
-        for (int t = 1; t < MT; ++t)
-          if (8u * t < rows) {
-            u32x4_t xt[4];
-            request_x(xt, x_offset(row, rows, t), kb);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[t] = Mma16<XDT>::mma(as_frag<XDT>(xt[j]), M::expand(b.q[i][j], factor), acc[t]);
-          }
-      }
-      ++kb, ++item;
-      if (kb == n_kb || item == end) {   // the expert's end: elements 2 p and 2 p + 1 of lane (c, h) are the planes of row 8 t + 2 h + p
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const uint32_t of = 8u * t + 2u * h + p;
-            if (of < rows) sums[(wave * T + s.token[row + of]) * 16 + (int)c] += acc[t][2 * p] + acc[t][2 * p + 1];
-          }
-          acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        }
-        kb = 0, ++at;
-        if (item < end) rows_at(at, row, rows);
-        else rows = 0;
-      }
-    };
-    Batch b0, b1;
-    request(b0);
-    request(b1);
-    while (item < end) {
-#pragma unroll
-      for (int i = 0; i < U; ++i) multiply(b0, i);
-      request(b0);
-#pragma unroll
-      for (int i = 0; i < U; ++i) multiply(b1, i);
-      request(b1);
+    for (int d = 0; d < D; ++d) {
+      multiply(st[d]);
+      request(st[d]);
     }
   }
   sync_threads();
-  static_assert(kMoeTokens * 16 <= 2 * 64 * W);
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     const int i = tid + m * 64 * W;
@@ -563,9 +602,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void moe_down_kernel(tamd_moe_layer_
   }
 }
 
-// NB of the up projection: rounds of 8 NB blocks; the fewest blocks' time, then the fewest rounds.
-inline int moe_up_nb(int hidden) {
-  const int n_kb = (hidden + 127) / 128;
+// Blocks of 128 K per wave: rounds of 8 NB blocks; the fewest blocks' time, then the fewest rounds.
+inline int moe_nb(int K) {
+  const int n_kb = (K + 127) / 128;
   int best = 1, least = 1 << 30;
   for (int nb = 3; nb >= 1; --nb) {
     const int cost = (n_kb + 8 * nb - 1) / (8 * nb) * nb;
@@ -580,8 +619,8 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
   if (int rc = cu_count(cus)) return rc;
   const int64_t slots = (int64_t)a.n_tokens * a.n_picks, most = (slots < a.n_experts ? slots : a.n_experts) * (a.inter / 16);
   const dim3 grid((unsigned)(most < cus ? most : cus));
-  const int nb = moe_up_nb(a.hidden);
-  if (a.n_tokens > 16 || 8 * nb < (a.hidden + 127) / 128) {
+  const int nb = moe_nb(a.hidden);
+  if ((int64_t)a.n_tokens * a.n_picks > 8 * (int64_t)a.n_experts || 8 * nb < (a.hidden + 127) / 128) {
     switch (nb) {
       case 1: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 1, true><<<grid, 512, 0, st>>>(a); break;
       case 2: moe_up_kernel<XDT, BLOCKS, SHUFFLED, 2, true><<<grid, 512, 0, st>>>(a); break;
@@ -597,14 +636,32 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
   return launch_status();
 }
 
+template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D>
+int launch_moe_down_of(const tamd_moe_layer_args &a, hipStream_t st) {
+  const auto kernel = moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D>;
+  const size_t lds = sizeof(MoeDownLds) + 8 * 2 * RC * kMoeDownPitch<NB, RC> + (size_t)a.n_tokens * 8 * 16 * 4;
+  if (lds > 64 * 1024)
+    if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
+  kernel<<<dim3((unsigned)(a.hidden / 16)), 512, lds, st>>>(a);
+  return launch_status();
+}
+
+// Tokens of an expert that are requested ahead: two where more are rare, four, or eight.
+template <int XDT, bool BLOCKS, bool SHUFFLED, int NB>
+int launch_moe_down_nb(const tamd_moe_layer_args &a, hipStream_t st) {
+  const float rows = (float)(a.n_tokens * a.n_picks) / (float)a.n_experts;
+  if (a.n_tokens <= 2 || rows <= 0.75f) return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB, 2, 4>(a, st);
+  if (a.n_tokens <= 4 || rows <= 2.5f) return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB, 4, 3>(a, st);
+  return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB < 3 ? NB : 2, 8, 2>(a, st);   // (eight tokens of three blocks do not fit the registers)
+}
+
 template <int XDT, bool BLOCKS, bool SHUFFLED>
 int launch_moe_down(const tamd_moe_layer_args &a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.hidden / 16));
-  constexpr int W = 8;
-  const size_t lds = sizeof(MoeDownLds) + (size_t)a.n_tokens * W * 16 * 4;
-  const auto kernel = a.n_tokens <= 8 ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, 1, 4, W> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, 8, 3, W>;
-  kernel<<<grid, 64 * W, lds, st>>>(a);
-  return launch_status();
+  switch (moe_nb(a.inter)) {
+    case 1: return launch_moe_down_nb<XDT, BLOCKS, SHUFFLED, 1>(a, st);
+    case 2: return launch_moe_down_nb<XDT, BLOCKS, SHUFFLED, 2>(a, st);
+    default: return launch_moe_down_nb<XDT, BLOCKS, SHUFFLED, 3>(a, st);
+  }
 }
 
 template <int XDT>
