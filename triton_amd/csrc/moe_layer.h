@@ -511,20 +511,11 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
     const bool live = now.at < n_active;
     uint32_t row, rows;
     rows_at(live ? now.at : 0u, row, rows);
-    for (uint32_t t0 = 0; t0 < (live ? rows : 0u); t0 += RC) {
-      const auto put = [&](const u32x4_t (&x)[XR]) {
+    const auto tile = [&](const u32x4_t (&x)[XR], uint32_t t0) {
 #pragma unroll
-        for (int i = 0; i < XR; ++i) {
-          const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), at = chunk % (16u * NB);
-          if (XR * kWave == 2 * RC * 16 * NB || of < 2u * RC) *(u32x4_t *)(rows_lds + of * PITCH + 16u * at) = x[i];
-        }
-      };
-      if (t0 == 0) {
-        put(st.x);
-      } else {   // more tokens than are requested ahead (awaited here, not behind the branch: the writes do that)
-        u32x4_t x[XR];
-        request_x(x, row + t0, rows - t0, now.kb0, 0);
-        put(x);
+      for (int i = 0; i < XR; ++i) {
+        const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), at = chunk % (16u * NB);
+        if (XR * kWave == 2 * RC * 16 * NB || of < 2u * RC) *(u32x4_t *)(rows_lds + of * PITCH + 16u * at) = x[i];
       }
       f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -548,10 +539,20 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const uint32_t of = 2u * h + p;
-        if (of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * p] + acc[2 * p + 1];
+        if (live && of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * p] + acc[2 * p + 1];
       }
+    };
+    tile(st.x, 0);
+    if (live) {
+      for (uint32_t t0 = RC; t0 < rows; t0 += RC) {   // more tokens than are requested ahead
+        u32x4_t x[XR];
+        request_x(x, row + t0, rows - t0, now.kb0, 0);
+#pragma unroll
+        for (int i = 0; i < XR; ++i) asm volatile("" : "+v"(x[i]));   // awaited here, not behind the branch
+        tile(x, t0);
+      }
+      advance(now);
     }
-    if (live) advance(now);
   };
 
   // ---- the biases of this thread's outputs by their gate weights, eight picks requested at a time
