@@ -417,7 +417,7 @@ constexpr int kMoeDownPitch = 256 * NB + 16;   // bytes of a row of h in a wave'
 // h comes as a few dense requests and goes through LDS, a buffer per wave, to where the MFMAs want it: requested in their layout
 // it takes four requests per block, most lanes of which bring nothing, and a request costs the CU about 20 cycles whatever it
 // brings (16 tokens of 128 experts of 2880 x 2880: 90 us, 50 without these requests, TODO now).
-template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D>
+template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D, bool ROUNDS>
 __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
   typedef ExpertWeights<BLOCKS, SHUFFLED> Weights;
@@ -443,74 +443,87 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
   const Buffer planes((const uint8_t *)a.workspace + kMoeTableBytes, (int64_t)slots * 4 * K);
   const uint32_t strip = blockIdx.x >> 1, f = blockIdx.x & 1u, n_kb = (uint32_t)(K + 127) / 128u, groups = (uint32_t)K / 32u;
 
-  // ---- a stage is an expert and up to 8 NB blocks of K, cut evenly: the wave's are kb0 .. kb0 + n - 1
-  struct Cursor {
-    uint32_t at, k0, kb0, n;
-  };
-  const auto part = [&](Cursor &p) {
-    const uint32_t here = n_kb - p.k0 < 8u * NB ? n_kb - p.k0 : 8u * NB, from = here * (uint32_t)wave / W;
-    p.kb0 = p.k0 + from, p.n = here * (uint32_t)(wave + 1) / W - from;
-  };
-  const auto advance = [&](Cursor &p) {
-    p.k0 += 8 * NB;
-    if (p.k0 >= n_kb) p.k0 = 0, ++p.at;
-    if (8 * NB < n_kb) part(p);
-  };
+  // ---- a stage is an expert and, with ROUNDS, 8 NB blocks of K from k0 on; these are cut evenly.  What a lane adds to the offsets
+  // depends on the place in K alone: made once, or once per stage with ROUNDS.
   const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
     row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
     rows = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at + 1]) - row;
+  };
+  struct Place {
+    uint32_t kb0, code_off[NB], scale_off[NS], x_off[XR];
+  };
+  const Weights form(a.down, 0, K, N);
+  const auto place_at = [&](uint32_t k0) {
+    Place p;
+    const uint32_t here = n_kb - k0 < 8u * NB ? n_kb - k0 : 8u * NB, from = here * (uint32_t)wave / W, n = here * (uint32_t)(wave + 1) / W - from;
+    p.kb0 = k0 + from;
+    const uint32_t code = form.code_offset(strip, f, c, h), scale = form.scale_offset(strip, f, c, h);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) p.code_off[i] = (uint32_t)i < n && (BLOCKS || 4u * (p.kb0 + i) + h < groups) ? code : kMoeOob;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if constexpr (SHUFFLED) p.scale_off[i] = 2u * ((p.kb0 >> 1) + i) < n_kb ? scale & ~3u : kMoeOob;   // blocks 2 (kb0 / 2 + i) and the next
+      else p.scale_off[i] = (uint32_t)i < n && 4u * (p.kb0 + i) + h < groups ? scale : kMoeOob;
+    }
+    // 16-byte chunk i * 64 + lane of the rows: row by row, 16 NB chunks each; zeros past K
+#pragma unroll
+    for (int i = 0; i < XR; ++i) {
+      const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), k = 128u * p.kb0 + 8u * (chunk % (16u * NB));
+      p.x_off[i] = of < 2u * RC && k < (uint32_t)K ? of * (uint32_t)(2 * K) + 2u * k : kMoeOob;
+    }
+    return p;
   };
   struct Stage {
     u32x4_t q[NB], x[XR];
     uint32_t s[NS];
   };
-  // 16-byte chunk i * 64 + lane of the rows: row by row, 16 NB chunks each; zeros past K and past the rows
-  const auto request_x = [&](u32x4_t (&to)[XR], uint32_t row, uint32_t rows, uint32_t kb0, uint32_t dead) {
+  const auto request_x = [&](u32x4_t (&to)[XR], const Place &p, uint32_t row, uint32_t rows) {
 #pragma unroll
     for (int i = 0; i < XR; ++i) {
-      const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), at = chunk % (16u * NB), k = 128u * kb0 + 8u * at;
-      uint32_t off = of < 2u * rows && of < 2u * RC && k < (uint32_t)K ? (2u * row + of) * (uint32_t)(2 * K) + 2u * k : kMoeOob;
+      const uint32_t of = (uint32_t)(i * kWave + lane) / (16u * NB);
+      uint32_t off = of < 2u * rows ? p.x_off[i] : kMoeOob;
       asm volatile("" : "+v"(off));   // (as in dead_unless)
-      to[i] = planes.load16(off + (off == kMoeOob ? 0u : dead));
+      to[i] = planes.load16(off, row * (uint32_t)(4 * K));
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  Cursor ask{0, 0, 0, 0}, now;
-  part(ask);
-  now = ask;
-  const uint32_t code_off = Weights(a.down, 0, K, N).code_offset(strip, f, c, h), scale_off = Weights(a.down, 0, K, N).scale_offset(strip, f, c, h);
+  uint32_t ask_at = 0, ask_k0 = 0, now_at = 0, now_k0 = 0;
+  const Place fixed = place_at(0);
   const auto request = [&](Stage &st) {
-    const bool live = ask.at < n_active;
-    const uint32_t at = live ? ask.at : 0u;
-    const Weights w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[at]), K, N);
+    const bool live = ask_at < n_active;
+    const uint32_t at = live ? ask_at : 0u;
+    Weights w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[at]), K, N);
+    if (!live) w.w = w.sc = Buffer(a.down.w, 0);   // (empty buffers: zeros)
     uint32_t row, rows;
     rows_at(at, row, rows);
-    request_x(st.x, row, rows, ask.kb0, dead_unless(live));
+    const Place p = ROUNDS ? place_at(ask_k0) : fixed;
+    request_x(st.x, p, row, live ? rows : 0u);
+    const uint32_t code_s = form.code_block(strip, p.kb0);
 #pragma unroll
     for (int i = 0; i < NB; ++i) {   // (one order wherever this is expanded: the waits are counted from it)
-      const uint32_t kb = ask.kb0 + i, dead = dead_unless(live && i < (int)ask.n);
-      if constexpr (BLOCKS) st.q[i] = w.w.template load16<2>(code_off + dead, w.code_block(strip, kb));
-      else st.q[i] = w.w.template load16<2>(4u * kb + h < groups ? code_off + dead : kMoeOob, w.code_block(strip, kb));
+      st.q[i] = w.w.template load16<2>(p.code_off[i], code_s + (BLOCKS ? 4096u : 64u) * i);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (!SHUFFLED) {
-        st.s[i] = w.sc.load1(4u * kb + h < groups ? scale_off + dead : kMoeOob, w.scale_block(strip, kb));
-        __builtin_amdgcn_sched_barrier(0);
-      }
     }
-    if constexpr (SHUFFLED) {
+    const uint32_t scale_s = SHUFFLED ? form.scale_block(strip, p.kb0 & ~1u) : form.scale_block(strip, p.kb0);
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {   // blocks 2 (kb0 / 2 + i) and the next
-        const uint32_t pair = (ask.kb0 >> 1) + i;
-        st.s[i] = w.sc.load4((scale_off & ~3u) + dead_unless(live && 2u * pair < n_kb), w.scale_block(strip, 2u * pair));
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int i = 0; i < NS; ++i) {
+      if constexpr (SHUFFLED) st.s[i] = w.sc.load4(p.scale_off[i], scale_s + 256u * i);
+      else st.s[i] = w.sc.load1(p.scale_off[i], scale_s + 4u * i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (live) advance(ask);
+    if (ROUNDS) {
+      ask_k0 += 8 * NB;
+      if (ask_k0 >= n_kb) ask_k0 = 0, ++ask_at;
+    } else {
+      ++ask_at;
+    }
   };
+  const uint32_t a_row = (c & (2u * RC - 1u)) * PITCH + 64u * h;   // (rows past the buffer's repeat: no one reads their sums)
   const auto multiply = [&](const Stage &st) {
-    const bool live = now.at < n_active;
+    const bool live = now_at < n_active;
     uint32_t row, rows;
-    rows_at(live ? now.at : 0u, row, rows);
+    rows_at(live ? now_at : 0u, row, rows);
+    const Place p = ROUNDS ? place_at(now_k0) : fixed;
     const auto tile = [&](const u32x4_t (&x)[XR], uint32_t t0) {
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
@@ -520,38 +533,40 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
       f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const uint32_t kb = now.kb0 + i;
         uint32_t scale;
         if constexpr (SHUFFLED) {
-          const uint32_t word0 = st.s[i / 2], word1 = st.s[i & 1 ? (i / 2 + 1 < NS ? i / 2 + 1 : i / 2) : i / 2];
-          scale = (now.kb0 & 1u ? word1 : word0) >> (8u * (((2u * c + f) >> 4) + 2u * (kb & 1u))) & 0xFFu;
+          const uint32_t odd = p.kb0 & 1u, word0 = st.s[i / 2], word1 = st.s[i & 1 ? (i / 2 + 1 < NS ? i / 2 + 1 : i / 2) : i / 2];
+          scale = (odd ? word1 : word0) >> (8u * ((2u * c + f) >> 4) + 16u * ((odd + i) & 1u)) & 0xFFu;
         } else {
           scale = st.s[i];
         }
         const float factor = bits_to_f32(scale << 23);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {   // (rows past the buffer's repeat: no one reads their sums)
-          const u32x4_t xv = *(const u32x4_t *)(rows_lds + (c & (2u * RC - 1u)) * PITCH + 256u * i + 64u * h + 16u * j);
-          acc = Mma16<XDT>::mma(as_frag<XDT>(xv), M::expand(st.q[i][j], factor), acc);
-        }
+        for (int j = 0; j < 4; ++j)
+          acc = Mma16<XDT>::mma(as_frag<XDT>(*(const u32x4_t *)(rows_lds + a_row + 256u * i + 16u * j)), M::expand(st.q[i][j], factor), acc);
       }
       // elements 2 p and 2 p + 1 of lane (c, h) are the planes of token 2 h + p of the tile
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint32_t of = 2u * h + p;
-        if (live && of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * p] + acc[2 * p + 1];
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t of = 2u * h + e;
+        if (live && of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * e] + acc[2 * e + 1];
       }
     };
     tile(st.x, 0);
     if (live) {
       for (uint32_t t0 = RC; t0 < rows; t0 += RC) {   // more tokens than are requested ahead
         u32x4_t x[XR];
-        request_x(x, row + t0, rows - t0, now.kb0, 0);
+        request_x(x, p, row + t0, rows - t0);
 #pragma unroll
         for (int i = 0; i < XR; ++i) asm volatile("" : "+v"(x[i]));   // awaited here, not behind the branch
         tile(x, t0);
       }
-      advance(now);
+    }
+    if (ROUNDS) {
+      now_k0 += 8 * NB;
+      if (now_k0 >= n_kb) now_k0 = 0, ++now_at;
+    } else {
+      ++now_at;
     }
   };
 
@@ -583,7 +598,7 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
   Stage st[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) request(st[d]);
-  while (now.at < n_active) {
+  while (now_at < n_active) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       multiply(st[d]);
@@ -639,7 +654,8 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
 
 template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D>
 int launch_moe_down_of(const tamd_moe_layer_args &a, hipStream_t st) {
-  const auto kernel = moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D>;
+  const bool rounds = 8 * NB < (a.inter + 127) / 128;
+  const auto kernel = rounds ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, true> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, false>;
   const size_t lds = sizeof(MoeDownLds) + 8 * 2 * RC * kMoeDownPitch<NB, RC> + (size_t)a.n_tokens * 8 * 16 * 4;
   if (lds > 64 * 1024)
     if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
