@@ -38,15 +38,20 @@ struct Abi {
                   void *, int64_t, int64_t, int, void *);
   int (*upcast)(const void *, int, int64_t, int64_t, const void *, int64_t, int64_t, void *, int, int64_t, int64_t, int64_t,
                 int64_t, int64_t, int64_t, void *);
+  int (*moe_layer)(const tamd_moe_layer_args *, size_t, void *);
+  int64_t (*moe_layer_workspace)(int, int, int);
+  int (*matvec)(const tamd_matvec_args *, size_t, void *);
+  int (*sample)(const tamd_sample_args *, size_t, void *);
+  int64_t (*sample_workspace)(int, int);
 } abi;
-PyObject *cls_tensor, *cls_value_layout, *cls_scale_layout, *obj_fp4, *ctx_constraints, *ctx_flags;
+PyObject *cls_tensor, *cls_value_layout, *cls_scale_layout, *obj_fp4, *ctx_constraints, *ctx_flags, *cls_int4, *obj_plain_flex;
 
 struct Names {
   PyObject *storage, *data, *layout, *dtype, *shape, *c_mx_scale, *c_microblock_size, *c_value_pack_factor, *a_mx_tensor_scale,
       *b_mx_tensor_scale, *acc_scale, *a_mx_scale, *a_microblock_size, *b_mx_scale, *b_microblock_size, *flex_ctx, *lhs_data,
       *rhs_data, *out_data, *acc_data, *scale, *expected_scale, *actual_scale, *checksum_scale, *out_dtype,
       *flexpoint_saturate_inf, *specs, *name, *fn_arg_names, *fn_args, *reduction_n, *slice_sizes, *slice_offs,
-      *block_offs_data, *block_schedule_data, *expected_slice_size, *native;
+      *block_offs_data, *block_schedule_data, *expected_slice_size, *native, *scales, *zeros, *group_size;
 } nm;
 
 // ------------------------------------------------------------------ small helpers
@@ -704,6 +709,205 @@ PyObject *py_upcast(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
   });
 }
 
+// ------------------------------------------------------------------ operators of a decoding step
+// (Tensors of another device than the current one are the general path's, which changes to theirs.)
+inline const at::Tensor &current_gpu_tensor(PyObject *o, int &dev) {
+  const at::Tensor &t = gpu_tensor(o, dev);
+  need(dev == (int)c10::hip::current_device());
+  return t;
+}
+inline bool plain_code(int c) { return c == TAMD_F32 || c == TAMD_BF16 || c == TAMD_F16; }
+
+// MXFP4 weights [E, K, N] of one product of a whole layer, with the scales of its PrecisionConfig and its bias.
+void moe_weights(PyObject *w_o, PyObject *pc, PyObject *bias_o, int64_t E, int64_t K, int64_t N, int dev, tamd_moe_weights &g) {
+  {
+    Ref fc(attr(pc, nm.flex_ctx));
+    need(fc.p == obj_plain_flex);
+    for (PyObject *n : {nm.a_mx_scale, nm.c_mx_scale, nm.a_mx_tensor_scale, nm.b_mx_tensor_scale, nm.out_dtype}) {
+      Ref r(attr(pc, n));
+      need(r.none());
+    }
+    Ref acc(attr(pc, nm.acc_scale)), mb(attr(pc, nm.b_microblock_size));
+    need(as_double(acc.p) == 1.0 && !mb.none() && as_int(mb.p) == 32);
+  }
+  const auto shape_is = [](PyObject *sh, int64_t a, int64_t b, int64_t c) {
+    return PyList_Check(sh) && PyList_GET_SIZE(sh) == 3 && as_int(PyList_GET_ITEM(sh, 0)) == a && as_int(PyList_GET_ITEM(sh, 1)) == b &&
+           as_int(PyList_GET_ITEM(sh, 2)) == c;
+  };
+  if (Py_TYPE(w_o) == (PyTypeObject *)cls_tensor) {
+    Ref dt(attr(w_o, nm.dtype)), st(attr(w_o, nm.storage)), sh(attr(w_o, nm.shape));
+    Ref lay(attr(st.p, nm.layout)), data(attr(st.p, nm.data));
+    need(dt.p == obj_fp4 && shape_is(sh.p, E, K, N) && Py_TYPE(lay.p) == (PyTypeObject *)cls_value_layout);
+    const at::Tensor &w = gpu_tensor(data.p, dev);
+    need(w.dim() == 3 && w.is_contiguous() && w.scalar_type() == at::kByte && w.size(0) == E && w.size(1) == (N + 63) / 64 &&
+         w.size(2) == (K + 127) / 128 * 4096);
+    g.w = w.data_ptr(), g.w_layout = TAMD_W_CDNA4_BLOCKS, g.w_stride_e = w.stride(0);
+  } else {
+    const at::Tensor &w = gpu_tensor(w_o, dev);
+    need(w.dim() == 3 && w.scalar_type() == at::kByte && w.size(0) == E && w.size(1) == K / 2 && w.size(2) == N && w.stride(1) == 1);
+    g.w = w.data_ptr(), g.w_layout = TAMD_W_STRIDED, g.w_stride_e = w.stride(0), g.w_stride_n = w.stride(2);
+  }
+  Ref sc(attr(pc, nm.b_mx_scale));
+  if (Py_TYPE(sc.p) == (PyTypeObject *)cls_tensor) {
+    Ref st(attr(sc.p, nm.storage)), sh(attr(sc.p, nm.shape));
+    Ref lay(attr(st.p, nm.layout)), data(attr(st.p, nm.data));
+    need(shape_is(sh.p, E, K / 32, N) && Py_TYPE(lay.p) == (PyTypeObject *)cls_scale_layout);
+    const at::Tensor &s = gpu_tensor(data.p, dev);
+    need(s.scalar_type() == at::kByte && s.dim() == 3 && s.size(0) == E && s.size(1) == (K / 32 + 7) / 8 * 8 * 32 && s.size(2) == (N + 31) / 32 &&
+         s.stride(1) == 1 && s.stride(2) == s.size(1));
+    g.scale = (const uint8_t *)s.data_ptr(), g.scale_layout = TAMD_SCALE_CDNA4, g.scale_stride_e = s.stride(0);
+  } else {
+    const at::Tensor &s = gpu_tensor(sc.p, dev);
+    need(s.scalar_type() == at::kByte && s.dim() == 3 && s.size(0) == E && s.size(1) == K / 32 && s.size(2) == N && (s.stride(1) == 1 || K == 32));
+    g.scale = (const uint8_t *)s.data_ptr(), g.scale_layout = TAMD_SCALE_STRIDED, g.scale_stride_e = s.stride(0), g.scale_stride_n = s.stride(2);
+  }
+  if (bias_o != Py_None) {
+    const at::Tensor &b = gpu_tensor(bias_o, dev);
+    need(b.dim() == 2 && b.size(0) == E && b.size(1) == N && b.stride(1) == 1);
+    g.bias = b.data_ptr(), g.bias_dtype = type_code(b.scalar_type()), g.bias_stride_e = b.stride(0);
+    need(plain_code(g.bias_dtype) && (uintptr_t)g.bias % 4 == 0 && g.bias_stride_e % 2 == 0);
+  }
+}
+
+// (x, logits, picks, w1, bias1, w2, bias2, precision config of either, activation): the whole layer into a new tensor.
+PyObject *py_moe_layer(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 10);
+    int dev = -1;
+    const at::Tensor &x = current_gpu_tensor(v[0], dev), &logits = gpu_tensor(v[1], dev);
+    need(x.dim() == 2 && logits.dim() == 2 && x.stride(1) == 1 && logits.stride(1) == 1 && logits.size(0) == x.size(0));
+    const int64_t T = x.size(0), H = x.size(1), E = logits.size(1), k = as_int(v[2]);
+    need(T >= 1 && T <= 64 && E <= 512 && k >= 1 && k <= 16 && k <= E && T * k <= 512 && H >= 32 && H % 32 == 0 && H <= 1 << 20);
+    need((T == 1 || (x.stride(0) % 8 == 0 && x.stride(0) < 1 << 17)) && (uintptr_t)x.data_ptr() % 16 == 0);
+    tamd_moe_layer_args g;
+    std::memset(&g, 0, sizeof g);
+    g.x_dtype = type_code(x.scalar_type()), g.logits_dtype = type_code(logits.scalar_type());
+    need((g.x_dtype == TAMD_BF16 || g.x_dtype == TAMD_F16) && plain_code(g.logits_dtype));
+    {
+      Ref sp(attr(v[9], nm.specs)), args(attr(v[9], nm.fn_args));
+      Ref n(attr(sp.p, nm.name)), names(attr(sp.p, nm.fn_arg_names));
+      need(PyUnicode_Check(n.p) && PyUnicode_CompareWithASCIIString(n.p, "swiglu") == 0 && PyTuple_Check(names.p) && PyTuple_Check(args.p) &&
+           PyTuple_GET_SIZE(names.p) == 2 && PyTuple_GET_SIZE(args.p) == 2);
+      need(PyUnicode_Check(PyTuple_GET_ITEM(names.p, 0)) && PyUnicode_Check(PyTuple_GET_ITEM(names.p, 1)) &&
+           PyUnicode_CompareWithASCIIString(PyTuple_GET_ITEM(names.p, 0), "alpha") == 0 &&
+           PyUnicode_CompareWithASCIIString(PyTuple_GET_ITEM(names.p, 1), "limit") == 0);
+      g.act_alpha = (float)as_double(PyTuple_GET_ITEM(args.p, 0));
+      PyObject *lim = PyTuple_GET_ITEM(args.p, 1);
+      g.act_has_limit = lim != Py_None;
+      g.act_limit = lim != Py_None ? (float)as_double(lim) : 0.f;
+    }
+    int64_t two_inter;
+    if (Py_TYPE(v[3]) == (PyTypeObject *)cls_tensor) {
+      Ref sh(attr(v[3], nm.shape));
+      need(PyList_Check(sh.p) && PyList_GET_SIZE(sh.p) == 3);
+      two_inter = as_int(PyList_GET_ITEM(sh.p, 2));
+    } else {
+      const at::Tensor &w = gpu_tensor(v[3], dev);
+      need(w.dim() == 3);
+      two_inter = w.size(2);
+    }
+    need(two_inter >= 64 && two_inter % 64 == 0 && two_inter <= 1 << 21);
+    moe_weights(v[3], v[7], v[4], E, H, two_inter, dev, g.up);
+    moe_weights(v[5], v[8], v[6], E, two_inter / 2, H, dev, g.down);
+    at::Tensor out = new_empty({T, H}, x.scalar_type(), dev);
+    at::Tensor ws = new_empty({abi.moe_layer_workspace((int)T, (int)k, (int)(two_inter / 2))}, at::kByte, dev);
+    g.x = x.data_ptr(), g.x_stride_m = T > 1 ? x.stride(0) : H, g.logits = logits.data_ptr(), g.logits_stride = logits.stride(0);
+    g.y = out.data_ptr(), g.y_stride_m = H, g.workspace = ws.data_ptr();
+    g.n_tokens = (int)T, g.n_experts = (int)E, g.n_picks = (int)k, g.hidden = (int)H, g.inter = (int)(two_inter / 2);
+    void *st = stream_of(dev);
+    const int rc = without_gil([&] { return abi.moe_layer(&g, sizeof g, st); });
+    if (rc != 0) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// (x [M, K], Int4Weights, bias, out_dtype or None): their product in a new tensor.
+PyObject *py_matvec(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 4 && Py_TYPE(v[1]) == (PyTypeObject *)cls_int4);
+    int dev = -1;
+    const at::Tensor &x = current_gpu_tensor(v[0], dev);
+    need(x.dim() == 2 && x.stride(1) == 1);
+    const int64_t M = x.size(0), K = x.size(1);
+    Ref d_o(attr(v[1], nm.data)), s_o(attr(v[1], nm.scales)), z_o(attr(v[1], nm.zeros)), sh(attr(v[1], nm.shape)), gs(attr(v[1], nm.group_size));
+    need(PyTuple_Check(sh.p) && PyTuple_GET_SIZE(sh.p) == 2 && as_int(PyTuple_GET_ITEM(sh.p, 0)) == K);
+    const int64_t N = as_int(PyTuple_GET_ITEM(sh.p, 1)), group = as_int(gs.p);
+    need(M >= 1 && N >= 1 && M <= 1 << 20 && N <= 1 << 30 && K >= 32 && K <= 1 << 20 && (group == 32 || group == 64 || group == 128));
+    need((M == 1 || (x.stride(0) % 8 == 0 && x.stride(0) < 1 << 23)) && (uintptr_t)x.data_ptr() % 16 == 0);
+    const int64_t S = (N + 15) / 16, B = (K + 127) / 128, per = 128 / group;
+    tamd_matvec_args g;
+    std::memset(&g, 0, sizeof g);
+    const at::Tensor &d = gpu_tensor(d_o.p, dev), &sc = gpu_tensor(s_o.p, dev);
+    const auto scales_like = [&](const at::Tensor &t) {
+      return t.dim() == 4 && t.size(0) == S && t.size(1) == B && t.size(2) == 16 && t.size(3) == per && t.is_contiguous();
+    };
+    need(d.scalar_type() == at::kByte && d.dim() == 3 && d.size(0) == S && d.size(1) == B && d.size(2) == 1024 && d.is_contiguous() && scales_like(sc));
+    if (!z_o.none()) {
+      const at::Tensor &z = gpu_tensor(z_o.p, dev);
+      need(z.scalar_type() == at::kByte && scales_like(z));
+      g.zeros = (const uint8_t *)z.data_ptr();
+    }
+    if (v[2] != Py_None) {
+      const at::Tensor &b = gpu_tensor(v[2], dev);
+      need(b.dim() == 1 && b.size(0) == N && b.is_contiguous());
+      g.bias = b.data_ptr(), g.bias_dtype = type_code(b.scalar_type());
+      need(plain_code(g.bias_dtype));
+    }
+    const at::ScalarType out_type = v[3] == Py_None ? x.scalar_type() : dtype_of(v[3]);
+    g.x_dtype = type_code(x.scalar_type()), g.scale_dtype = type_code(sc.scalar_type()), g.y_dtype = type_code(out_type);
+    need((g.x_dtype == TAMD_BF16 || g.x_dtype == TAMD_F16) && (g.scale_dtype == TAMD_BF16 || g.scale_dtype == TAMD_F16) && plain_code(g.y_dtype));
+    at::Tensor out = new_empty({M, N}, out_type, dev);
+    g.x = x.data_ptr(), g.x_stride_m = M > 1 ? x.stride(0) : K, g.codes = (const uint8_t *)d.data_ptr(), g.scales = sc.data_ptr();
+    g.y = out.data_ptr(), g.y_stride_m = N, g.M = (int)M, g.N = (int)N, g.K = (int)K, g.group = (int)group;
+    void *st = stream_of(dev);
+    const int rc = without_gil([&] { return abi.matvec(&g, sizeof g, st); });
+    if (rc != 0) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// (logits, u, temperature, top_k, top_p, min_p): tokens in a new tensor.
+PyObject *py_sample(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 6);
+    int dev = -1;
+    const at::Tensor &x = current_gpu_tensor(v[0], dev), &u = gpu_tensor(v[1], dev);
+    need(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1));
+    const int64_t R = x.size(0), V = x.size(1);
+    need(R >= 1 && R <= 1 << 20 && V >= 1 && V <= 1 << 20 && u.dim() == 1 && u.size(0) == R && u.scalar_type() == at::kFloat && u.is_contiguous());
+    tamd_sample_args g;
+    std::memset(&g, 0, sizeof g);
+    g.logits_dtype = type_code(x.scalar_type());
+    need(plain_code(g.logits_dtype));
+    // a number of the range that the general path lets pass, or a tensor of one per row
+    const auto setting = [&](PyObject *o, at::ScalarType t, double most, double &number) -> const void * {
+      if (PyFloat_CheckExact(o) || PyLong_CheckExact(o)) {
+        number = as_double(o);
+        need(number >= 0 && number <= most);
+        return nullptr;
+      }
+      const at::Tensor &s = gpu_tensor(o, dev);
+      need(s.dim() == 1 && s.size(0) == R && s.scalar_type() == t && s.is_contiguous());
+      return s.data_ptr();
+    };
+    double t = 0, p = 0, m = 0, k = 0;
+    g.temperature = (const float *)setting(v[2], at::kFloat, HUGE_VAL, t);
+    need(!PyFloat_Check(v[3]));
+    g.top_k = (const int32_t *)setting(v[3], at::kInt, HUGE_VAL, k);
+    g.top_p = (const float *)setting(v[4], at::kFloat, HUGE_VAL, p);
+    g.min_p = (const float *)setting(v[5], at::kFloat, 1.0, m);
+    g.temperature_value = (float)t, g.top_k_value = k < 1 << 20 ? (int)k : 1 << 20, g.top_p_value = (float)p, g.min_p_value = (float)m;
+    at::Tensor tokens = new_empty({R}, at::kInt, dev);
+    at::Tensor ws = new_empty({abi.sample_workspace((int)R, (int)V)}, at::kByte, dev);
+    g.logits = x.data_ptr(), g.logits_stride = x.stride(0), g.u = (const float *)u.data_ptr();
+    g.tokens = (int32_t *)tokens.data_ptr(), g.workspace = ws.data_ptr(), g.R = (int)R, g.V = (int)V;
+    void *st = stream_of(dev);
+    const int rc = without_gil([&] { return abi.sample(&g, sizeof g, st); });
+    if (rc != 0) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(tokens);
+  });
+}
+
 // ------------------------------------------------------------------ module
 PyObject *py_choose_block_m(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
   return covered([&]() -> PyObject * {
@@ -757,13 +961,13 @@ PyObject *py_routing_block_rows(PyObject *, PyObject *const *v, Py_ssize_t nargs
 }
 
 // (addresses of the C ABI functions by name, Tensor, CDNA4MXValueLayout, CDNA4MXScaleLayout, FP4, constraints ContextVar,
-//  flags ContextVar)
+//  flags ContextVar, Int4Weights, the FlexCtx of a PrecisionConfig without one)
 PyObject *py_init(PyObject *, PyObject *args) {
   PyObject *addr;
-  if (!PyArg_ParseTuple(args, "O!OOOOOO", &PyDict_Type, &addr, &cls_tensor, &cls_value_layout, &cls_scale_layout, &obj_fp4,
-                        &ctx_constraints, &ctx_flags))
+  if (!PyArg_ParseTuple(args, "O!OOOOOOOO", &PyDict_Type, &addr, &cls_tensor, &cls_value_layout, &cls_scale_layout, &obj_fp4,
+                        &ctx_constraints, &ctx_flags, &cls_int4, &obj_plain_flex))
     return nullptr;
-  for (PyObject *o : {cls_tensor, cls_value_layout, cls_scale_layout, obj_fp4, ctx_constraints, ctx_flags}) Py_INCREF(o);
+  for (PyObject *o : {cls_tensor, cls_value_layout, cls_scale_layout, obj_fp4, ctx_constraints, ctx_flags, cls_int4, obj_plain_flex}) Py_INCREF(o);
   auto take = [&](const char *name, void *slot) {
     PyObject *o = PyDict_GetItemString(addr, name);
     void *p = o ? PyLong_AsVoidPtr(o) : nullptr;
@@ -771,7 +975,9 @@ PyObject *py_init(PyObject *, PyObject *args) {
     return p != nullptr;
   };
   if (!take("tamd_matmul_sized", &abi.matmul) || !take("tamd_routing_gates", &abi.routing) || !take("tamd_reduce", &abi.reduce) ||
-      !take("tamd_downcast_mxfp", &abi.downcast) || !take("tamd_upcast_mxfp", &abi.upcast)) {
+      !take("tamd_downcast_mxfp", &abi.downcast) || !take("tamd_upcast_mxfp", &abi.upcast) || !take("tamd_moe_layer", &abi.moe_layer) ||
+      !take("tamd_moe_layer_workspace", &abi.moe_layer_workspace) || !take("tamd_matvec", &abi.matvec) || !take("tamd_sample", &abi.sample) ||
+      !take("tamd_sample_workspace", &abi.sample_workspace)) {
     PyErr_SetString(PyExc_RuntimeError, "an entry point of the library is missing");
     return nullptr;
   }
@@ -783,7 +989,8 @@ PyObject *py_init(PyObject *, PyObject *args) {
       TAMD_NAME(acc_data), TAMD_NAME(scale), TAMD_NAME(expected_scale), TAMD_NAME(actual_scale), TAMD_NAME(checksum_scale),
       TAMD_NAME(out_dtype), TAMD_NAME(flexpoint_saturate_inf), TAMD_NAME(specs), TAMD_NAME(name), TAMD_NAME(fn_arg_names),
       TAMD_NAME(fn_args), TAMD_NAME(reduction_n), TAMD_NAME(slice_sizes), TAMD_NAME(slice_offs), TAMD_NAME(block_offs_data),
-      TAMD_NAME(block_schedule_data), TAMD_NAME(expected_slice_size), TAMD_NAME(native);
+      TAMD_NAME(block_schedule_data), TAMD_NAME(expected_slice_size), TAMD_NAME(native), TAMD_NAME(scales), TAMD_NAME(zeros),
+      TAMD_NAME(group_size);
 #undef TAMD_NAME
   Py_RETURN_NONE;
 }
@@ -798,6 +1005,9 @@ PyMethodDef methods[] = {{"init", py_init, METH_VARARGS, nullptr},
                          {"reduce", TAMD_FAST(py_reduce)},
                          {"downcast", TAMD_FAST(py_downcast)},
                          {"upcast", TAMD_FAST(py_upcast)},
+                         {"moe_layer", TAMD_FAST(py_moe_layer)},
+                         {"matvec", TAMD_FAST(py_matvec)},
+                         {"sample", TAMD_FAST(py_sample)},
                          {"choose_block_m", TAMD_FAST(py_choose_block_m)},
                          {"blocks_of_16_stream", TAMD_FAST(py_blocks_of_16_stream)},
                          {"dense_block_m", TAMD_FAST(py_dense_block_m)},

@@ -8,7 +8,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, _native
 
 GROUP_SIZES = (32, 64, 128)
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -80,6 +80,12 @@ def matvec(x: torch.Tensor, w: Int4Weights, bias: Optional[torch.Tensor] = None,
     bias: [N] or None; out_dtype: float32, bfloat16 or float16 (default: x's type); out: where the result goes, which must not overlap
     an input.  Weights are not rounded, sums are float32, the result is rounded once.  The kernel is made for up to 64 rows;
     every further 64 read the weights again."""
+    if out is None:
+        done = _native.matvec(x, w, bias, out_dtype)
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done, "matvec")
+            return done
     _lib.require_gpu(x, "x")
     if x.ndim == 1:
         return matvec(x[None], w, bias, out_dtype, None if out is None else out[None])[0]

@@ -10,7 +10,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, _native
 from .matmul import FusedActivation, PrecisionConfig
 from .tensor import FP4, Tensor
 from .tensor_details.layout import CDNA4MXScaleLayout, CDNA4MXValueLayout
@@ -92,6 +92,12 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, n_expts_act: int, w1, bias1
     bias1: [E, 2 I], bias2: [E, H] or None.  fused_activation: "swiglu" with (alpha, limit), over the column pairs of w1.
     Returns [T, H] in x's type (`out`, if given, which must not overlap an input); sums are float32, the result is rounded once.
     More tokens: `routing`, `matmul`, `matmul`, `reduce`."""
+    if out is None:
+        done = _native.moe_layer(x, logits, n_expts_act, w1, bias1, w2, bias2, precision_config1, precision_config2, fused_activation)
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done, "moe_layer")
+            return done
     _lib.require_gpu(x, "x")
     assert x.ndim == 2 and logits.ndim == 2 and logits.shape[0] == x.shape[0], "x is [tokens, hidden], logits [tokens, experts]"
     if x.dtype not in (torch.bfloat16, torch.float16):

@@ -6,7 +6,7 @@ from typing import Union
 
 import torch
 
-from . import _lib
+from . import _lib, _native
 
 MAX_VOCABULARY = MAX_ROWS = 1 << 20
 
@@ -27,6 +27,11 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     first of the order.  NaN logits count as -inf; a row with nothing but -inf gives -1; +inf logits share the mass alike.
     In tensors, which are not looked at on the host, a temperature below 0 or NaN counts as 0, a NaN top_p as 1, min_p is
     clamped to [0, 1], u to [0, 1)."""
+    done = _native.sample(logits, u, temperature, top_k, top_p, min_p)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "sample")
+        return done
     _lib.require_gpu(logits, "logits")
     assert logits.ndim == 2, "logits are [rows, vocabulary]"
     R, V = logits.shape
