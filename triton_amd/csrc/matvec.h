@@ -16,7 +16,7 @@
 
 namespace tamd {
 
-constexpr int kMatvecRows = 64;   // rows of a workgroup's tiles: more rows read the weights again
+constexpr int kMatvecRows = 64;   // rows that are addressed together
 
 template <int XDT>
 struct Int4;
@@ -44,105 +44,324 @@ TAMD_DEVICE typename Mma<XDT>::frag_t codes_plus_16(uint32_t d) {
   return as_frag<XDT>(v);
 }
 
-// MT tiles of 16 rows; PER = groups of a block (4, 2, 1); eight waves split K, U blocks requested together.
-template <int XDT, int MT, int PER, bool ZEROS, int U>
-__global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_kernel(tamd_matvec_args a) {
+// Where the blocks of a wave lie in K: n of the n_kb blocks from kb0 on, an eighth of them.
+struct MatvecPart {
+  uint32_t kb0, n;
+  TAMD_DEVICE MatvecPart(uint32_t n_kb, uint32_t wave) : kb0(n_kb * wave / 8u), n(n_kb * (wave + 1u) / 8u - kb0) {}
+};
+
+// A strip's sums over the eight waves: row m of a tile, column `col`, from the waves' accumulators of that tile.
+TAMD_DEVICE float matvec_sum(const f32x4_t (*red)[kWave], int m, int col) {
+  float v = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) v += ((const float *)&red[w][(m >> 2) * 16 + col])[m & 3];
+  return v;
+}
+// A mask for a buffer's length (a uniform value), hidden from the compiler as in dead_unless.
+TAMD_DEVICE uint32_t all_ones_if(bool b) {
+  uint32_t v = (uint32_t)__builtin_amdgcn_readfirstlane(b ? 0x7FFFFFFF : 0);
+  asm volatile("" : "+s"(v));
+  return v;
+}
+TAMD_DEVICE float scale_of(uint32_t bits, bool f16) { return f16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits); }
+
+// Up to 16 rows and NB blocks per wave.  A workgroup per CU (two where a wave has few blocks) walks over a contiguous part of the
+// strips; its eight waves split K, and a wave's part of x stays in registers.  The codes of D strips are in flight, the waves'
+// sums meet in LDS, a barrier per strip.  Scales and zero points of four blocks come with one request, each quarter of the lanes bringing
+// those of one block, and change lanes from there: a request costs the CU about 20 cycles whatever it brings.
+// One strip per workgroup, x requested with the codes: 70 us for 1 x 4096 x 131072, TODO now.
+template <int XDT, int PER, bool ZEROS, int NB, int D>
+__global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
+  constexpr int SQ = (NB + 3) / 4, STEPS = 4 / PER;
+  constexpr bool KEEP = NB * PER <= 8;   // the sums of x stay in registers too
+  __shared__ f32x4_t red[2][8][kWave];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const uint32_t c = lane & 15, h = lane >> 4, K = (uint32_t)a.K, n_kb = (K + 127) / 128;
+  const MatvecPart part(n_kb, (uint32_t)wave);
+  const int64_t strips = (a.N + 15) / 16;
+  const int64_t begin = strips * blockIdx.x / gridDim.x, end = strips * (blockIdx.x + 1) / gridDim.x;
+  const bool scale_f16 = a.scale_dtype == TAMD_F16;
+  const u32x4_t ones = {Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne};
+
+  struct Stage {
+    u32x4_t q[NB];
+    uint32_t s[SQ][PER == 4 ? 2 : 1], z[SQ];
+  };
+  uint32_t code_off[NB], group_off[SQ];   // of the lane; group_off in groups
+#pragma unroll
+  for (int i = 0; i < NB; ++i) code_off[i] = (uint32_t)i < part.n ? (part.kb0 + i) * 1024u + 16u * lane : kMoeOob;
+#pragma unroll
+  for (int i = 0; i < SQ; ++i) group_off[i] = 4u * i + h < part.n ? ((part.kb0 + 4u * i + h) * 16u + c) * PER : kMoeOob / 4u;
+  int64_t ask = begin;
+  const auto request = [&](Stage &st) {   // (an empty buffer past the last strip: no branch around requests)
+    const bool live = ask < end;
+    const int64_t at = live ? ask : 0, blocks = live ? n_kb : 0;
+    const Buffer codes(a.codes + at * n_kb * 1024, blocks * 1024), scales((const uint8_t *)a.scales + at * n_kb * (32 * PER), blocks * (32 * PER));
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      st.q[i] = codes.template load16<2>(code_off[i]);
+      __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
+    }
+#pragma unroll
+    for (int i = 0; i < SQ; ++i) {
+      if constexpr (PER == 4) {
+        const u32x2_t v = scales.load8(2u * group_off[i]);
+        st.s[i][0] = v.x, st.s[i][1] = v.y;
+      } else if constexpr (PER == 2) {
+        st.s[i][0] = scales.load4(2u * group_off[i]);
+      } else {
+        st.s[i][0] = scales.load2(2u * group_off[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (ZEROS) {
+        const Buffer zeros(a.zeros + at * n_kb * (16 * PER), blocks * (16 * PER));
+        if constexpr (PER == 4) st.z[i] = zeros.load4(group_off[i]);
+        else if constexpr (PER == 2) st.z[i] = zeros.load2(group_off[i]);
+        else st.z[i] = zeros.load1(group_off[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    ++ask;
+  };
+
+  // ---- x, and the sums of its groups
+  u32x4_t xr[NB][4];
+  {
+    const Buffer x(a.x, (int64_t)(a.M - 1) * a.x_stride_m * 2 + 2 * (int64_t)K);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t k = 128u * (part.kb0 + i) + 32u * j;
+        xr[i][j] = x.load16((int)c < a.M && (uint32_t)i < part.n && k < K ? c * (uint32_t)a.x_stride_m * 2u + 2u * k + 16u * h : kMoeOob);
+      }
+  }
+  Stage st[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) request(st[d]);
+  const auto x_sum = [&](int i, int g) {
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) v = Mma16<XDT>::mma(as_frag<XDT>(xr[i][g * STEPS + j]), as_frag<XDT>(ones), v);
+    return v;
+  };
+  f32x4_t kept[KEEP ? NB : 1][PER];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int g = 0; g < PER; ++g) kept[i][g] = x_sum(i, g);
+  }
+
+  int64_t now = begin;
+  int turn = 0;
+  const auto multiply = [&](const Stage &st) {
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int from = 4 * (int)(16u * (i & 3) + c);
+      const uint32_t s0 = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)st.s[i / 4][0]);
+      const uint32_t s1 = PER == 4 ? (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)st.s[i / 4][PER == 4 ? 1 : 0]) : 0u;
+      const uint32_t z = ZEROS ? (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)st.z[i / 4]) : 0u;
+#pragma unroll
+      for (int g = 0; g < PER; ++g) {
+        const float scale = scale_of((g < 2 ? s0 : s1) >> (16 * (g & 1)) & 0xFFFFu, scale_f16);
+        const float offset = ZEROS ? -16.f - (float)(z >> (8 * g) & 0xFFu) : -24.f;
+        f32x4_t p;
+        if constexpr (KEEP) p = kept[i][g];
+        else p = x_sum(i, g);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) p[v] *= offset;
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) p = Mma16<XDT>::mma(as_frag<XDT>(xr[i][g * STEPS + j]), codes_plus_16<XDT>(st.q[i][g * STEPS + j]), p);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) y[v] = __builtin_fmaf(scale, p[v], y[v]);
+      }
+    }
+    red[turn][wave][lane] = y;
+    sync_threads();
+    const int m = tid >> 4, col = tid & 15;
+    const int64_t n = 16 * now + col;
+    if (m < a.M && now < end && n < a.N) {
+      float v = matvec_sum(red[turn], m, col);
+      if (a.bias) v += load_any_f32(a.bias, a.bias_dtype, n);
+      store_any(a.y, a.y_dtype, m * a.y_stride_m + n, v);
+    }
+    turn ^= 1;   // (one barrier between two uses of either half)
+    ++now;
+  };
+  while (now < end) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      multiply(st[d]);
+      request(st[d]);
+    }
+  }
+}
+
+// Any number of rows and any K: a workgroup has C strips and MT tiles of 16 rows, its eight waves split K and read their part of x once,
+// with the codes, U blocks at a time and twice that in flight.  Each block of x serves C strips.
+// (One strip, U = 2 and nothing ahead: 51 us for 48 x 8192 x 8192, TODO now.)
+template <int XDT, int MT, int C, int PER, bool ZEROS, int U>
+__global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a) {
+  constexpr int STEPS = 4 / PER;
   __shared__ f32x4_t red[8][kWave];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  const uint32_t c = lane & 15, h = lane >> 4;
-  const int64_t strip = blockIdx.x;
-  const int m0 = blockIdx.y * kMatvecRows, rows = a.M - m0 < kMatvecRows ? a.M - m0 : kMatvecRows;
-  const uint32_t K = (uint32_t)a.K, n_kb = (K + 127) / 128;
-  const Buffer x((const uint8_t *)a.x + m0 * a.x_stride_m * 2, (int64_t)(rows - 1) * a.x_stride_m * 2 + 2 * (int64_t)K);
-  const Buffer codes(a.codes + strip * n_kb * 1024, (int64_t)n_kb * 1024);
-  const Buffer scales((const uint8_t *)a.scales + strip * n_kb * (32 * PER), (int64_t)n_kb * (32 * PER));
-  const Buffer zeros((const uint8_t *)a.zeros + (ZEROS ? strip * n_kb * (16 * PER) : 0), ZEROS ? (int64_t)n_kb * (16 * PER) : 0);
+  const uint32_t c = lane & 15, h = lane >> 4, K = (uint32_t)a.K, n_kb = (K + 127) / 128;
+  const MatvecPart part(n_kb, (uint32_t)wave);
+  const int64_t strips = (a.N + 15) / 16, strip = (int64_t)blockIdx.x * C;
+  const int m0 = blockIdx.y * (16 * MT), rows = a.M - m0 < 16 * MT ? a.M - m0 : 16 * MT;
   const bool scale_f16 = a.scale_dtype == TAMD_F16;
-  uint32_t x_row[MT];
-  f32x4_t y[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    x_row[t] = 16 * t + (int)c < rows ? (uint32_t)((16 * t + c) * (uint32_t)a.x_stride_m * 2u) + 16u * h : kMoeOob;
-    y[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
   const u32x4_t ones = {Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne};
-  const uint32_t end = n_kb * (uint32_t)(wave + 1) / 8u;
-  for (uint32_t kb = n_kb * (uint32_t)wave / 8u; kb < end; kb += U) {
-    u32x4_t q[U];
-    uint32_t s[U][PER > 2 ? 2 : 1], z[U];
+  const int64_t here = strips - strip < C ? strips - strip : C, blocks = here * n_kb;
+  const uint8_t *const x_at = (const uint8_t *)a.x + m0 * a.x_stride_m * 2, *const codes_at = a.codes + strip * n_kb * 1024;
+  const uint8_t *const scales_at = (const uint8_t *)a.scales + strip * n_kb * (32 * PER), *const zeros_at = ZEROS ? a.zeros + strip * n_kb * (16 * PER) : nullptr;
+  const int64_t x_bytes = (int64_t)(rows - 1) * a.x_stride_m * 2 + 2 * (int64_t)K;
+  uint32_t x_row[MT];
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (kb + i < end) {
-        q[i] = codes.template load16<2>(16u * lane, (kb + i) * 1024u);
-        if constexpr (PER == 4) {
-          const u32x2_t v = scales.load8(8u * c, (kb + i) * 128u);
-          s[i][0] = v.x, s[i][1] = v.y;
-        } else if constexpr (PER == 2) {
-          s[i][0] = scales.load4(4u * c, (kb + i) * 64u);
-        } else {
-          s[i][0] = scales.load2(2u * c, (kb + i) * 32u);
-        }
-        if constexpr (ZEROS) {
-          if constexpr (PER == 4) z[i] = zeros.load4(4u * c, (kb + i) * 64u);
-          else if constexpr (PER == 2) z[i] = zeros.load2(2u * c, (kb + i) * 32u);
-          else z[i] = zeros.load1(c, (kb + i) * 16u);
+  for (int t = 0; t < MT; ++t) x_row[t] = 16 * t + (int)c < rows ? (16u * t + c) * (uint32_t)a.x_stride_m * 2u + 16u * h : kMoeOob;
+  struct Stage {
+    u32x4_t q[U][C], x[U][MT][4];
+    uint32_t s[U][C][PER == 4 ? 2 : 1], z[U][C];
+  };
+  uint32_t ask = 0;
+  const auto request = [&](Stage &st) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      // (what is not there comes from an empty buffer: no branch around requests)
+      const uint32_t kb = part.kb0 + ask + i, there = all_ones_if(ask + i < part.n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Buffer x(x_at, x_bytes & (int64_t)(there & all_ones_if(128u * kb + 32u * j < K)));
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          st.x[i][t][j] = x.load16(x_row[t], 256u * kb + 64u * j);
+          __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
         }
       }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      u32x4_t xr[U][4];
+      for (int s = 0; s < C; ++s) {   // (the scalar offset is no part of the range check)
+        const int64_t mask = (int64_t)(there & all_ones_if(s < here));
+        const Buffer codes(codes_at, (blocks * 1024) & mask), scales(scales_at, (blocks * 32 * PER) & mask);
+        st.q[i][s] = codes.template load16<2>(16u * lane, (s * n_kb + kb) * 1024u);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (PER == 4) {
+          const u32x2_t v = scales.load8(8u * c, (s * n_kb + kb) * 128u);
+          st.s[i][s][0] = v.x, st.s[i][s][1] = v.y;
+        } else if constexpr (PER == 2) {
+          st.s[i][s][0] = scales.load4(4u * c, (s * n_kb + kb) * 64u);
+        } else {
+          st.s[i][s][0] = scales.load2(2u * c, (s * n_kb + kb) * 32u);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (ZEROS) {
+          const Buffer zeros(zeros_at, (blocks * 16 * PER) & mask);
+          if constexpr (PER == 4) st.z[i][s] = zeros.load4(4u * c, (s * n_kb + kb) * 64u);
+          else if constexpr (PER == 2) st.z[i][s] = zeros.load2(2u * c, (s * n_kb + kb) * 32u);
+          else st.z[i][s] = zeros.load1(c, (s * n_kb + kb) * 16u);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    ask += U;
+  };
+  f32x4_t y[MT][C];
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (kb + i < end) {
+  for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) xr[i][j] = x.load16(128u * (kb + i) + 32u * j < K ? x_row[t] + 256u * (kb + i) + 64u * j : kMoeOob);
+    for (int s = 0; s < C; ++s) y[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const auto multiply = [&](const Stage &st) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int g = 0; g < PER; ++g) {
+        f32x4_t of_x[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          of_x[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j) of_x[t] = Mma16<XDT>::mma(as_frag<XDT>(st.x[i][t][g * STEPS + j]), as_frag<XDT>(ones), of_x[t]);
         }
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (kb + i < end) {
+        for (int s = 0; s < C; ++s) {
+          const float scale = scale_of(st.s[i][s][g / 2] >> (16 * (g & 1)) & 0xFFFFu, scale_f16);
+          const float offset = ZEROS ? -16.f - (float)(st.z[i][s] >> (8 * g) & 0xFFu) : -24.f;
+          typename Mma<XDT>::frag_t w[STEPS];
 #pragma unroll
-          for (int g = 0; g < PER; ++g) {
-            const uint32_t bits = s[i][g / 2] >> (16 * (g & 1)) & 0xFFFFu;
-            const float scale = scale_f16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
-            const float offset = ZEROS ? -16.f - (float)(z[i] >> (8 * g) & 0xFFu) : -24.f;
-            f32x4_t of_x = {0.f, 0.f, 0.f, 0.f}, p;
+          for (int j = 0; j < STEPS; ++j) w[j] = codes_plus_16<XDT>(st.q[i][s][g * STEPS + j]);
 #pragma unroll
-            for (int j = 0; j < 4 / PER; ++j) of_x = Mma16<XDT>::mma(as_frag<XDT>(xr[i][g * (4 / PER) + j]), as_frag<XDT>(ones), of_x);
+          for (int t = 0; t < MT; ++t) {
+            f32x4_t p;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) p[v] = offset * of_x[v];
+            for (int v = 0; v < 4; ++v) p[v] = offset * of_x[t][v];
 #pragma unroll
-            for (int j = 0; j < 4 / PER; ++j)
-              p = Mma16<XDT>::mma(as_frag<XDT>(xr[i][g * (4 / PER) + j]), codes_plus_16<XDT>(q[i][g * (4 / PER) + j]), p);
+            for (int j = 0; j < STEPS; ++j) p = Mma16<XDT>::mma(as_frag<XDT>(st.x[i][t][g * STEPS + j]), w[j], p);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) y[t][v] = __builtin_fmaf(scale, p[v], y[t][v]);
+            for (int v = 0; v < 4; ++v) y[t][s][v] = __builtin_fmaf(scale, p[v], y[t][s][v]);
           }
         }
-    }
+      }
+  };
+  Stage s0, s1;
+  request(s0);
+  request(s1);
+  for (uint32_t k = 0; k < part.n; k += 2 * U) {   // (blocks past the wave's last: zeros)
+    multiply(s0);
+    request(s0);
+    multiply(s1);
+    request(s1);
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    red[wave][lane] = y[t];
-    sync_threads();
-    const int m = tid >> 4, col = tid & 15;
-    const int64_t n = 16 * strip + col;
-    if (m < 16 && 16 * t + m < rows && n < a.N) {
-      float v = 0.f;
+  for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int w = 0; w < 8; ++w) v += ((const float *)&red[w][(m >> 2) * 16 + col])[m & 3];
-      if (a.bias) v += load_any_f32(a.bias, a.bias_dtype, n);
-      store_any(a.y, a.y_dtype, (m0 + 16 * t + m) * a.y_stride_m + n, v);
+    for (int s = 0; s < C; ++s) {
+      red[wave][lane] = y[t][s];
+      sync_threads();
+      const int m = tid >> 4, col = tid & 15;
+      const int64_t n = 16 * (strip + s) + col;
+      if (m < 16 && 16 * t + m < rows && n < a.N) {
+        float v = matvec_sum(red, m, col);
+        if (a.bias) v += load_any_f32(a.bias, a.bias_dtype, n);
+        store_any(a.y, a.y_dtype, (m0 + 16 * t + m) * a.y_stride_m + n, v);
+      }
+      sync_threads();
     }
-    sync_threads();
-  }
+}
+
+template <int XDT, int PER, bool ZEROS, int NB, int D>
+int launch_matvec_kept(const tamd_matvec_args &a, int cus, hipStream_t st) {
+  const int64_t strips = (a.N + 15) / 16;
+  matvec_kernel<XDT, PER, ZEROS, NB, D><<<(unsigned)(strips < cus ? strips : cus), 512, 0, st>>>(a);
+  return launch_status();
+}
+template <int XDT, int PER, bool ZEROS, int MT, int C, int U>
+int launch_matvec_rows(const tamd_matvec_args &a, hipStream_t st) {
+  const int64_t strips = (a.N + 15) / 16;
+  const dim3 grid((unsigned)((strips + C - 1) / C), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+  matvec_rows_kernel<XDT, MT, C, PER, ZEROS, U><<<grid, 512, 0, st>>>(a);
+  return launch_status();
 }
 
 template <int XDT, int PER, bool ZEROS>
 int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.M + kMatvecRows - 1) / kMatvecRows));
-  if (a.M <= 16) matvec_kernel<XDT, 1, PER, ZEROS, 4><<<grid, 512, 0, st>>>(a);
-  else if (a.M <= 32) matvec_kernel<XDT, 2, PER, ZEROS, 4><<<grid, 512, 0, st>>>(a);
-  else matvec_kernel<XDT, 4, PER, ZEROS, 2><<<grid, 512, 0, st>>>(a);
-  return launch_status();
+  int cus = 0;
+  if (int rc = cu_count(cus)) return rc;
+  const int64_t strips = (a.N + 15) / 16;
+  if (a.M <= 16) {   // x of a wave in registers, up to six blocks
+    const int nb = ((a.K + 127) / 128 + 7) / 8;
+    if (nb <= 1) return launch_matvec_kept<XDT, PER, ZEROS, 1, 4>(a, cus, st);
+    if (nb <= 2) return launch_matvec_kept<XDT, PER, ZEROS, 2, 4>(a, cus, st);
+    if (nb <= 3) return launch_matvec_kept<XDT, PER, ZEROS, 3, 4>(a, cus, st);
+    if (nb <= 4) return launch_matvec_kept<XDT, PER, ZEROS, 4, 3>(a, cus, st);
+    if constexpr (PER < 4)
+      if (nb <= 6) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
+    return strips >= 2 * cus ? launch_matvec_rows<XDT, PER, ZEROS, 1, 2, 2>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 2>(a, st);
+  }
+  // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
+  // registers with two strips: one strip, and above 48 rows parts of 32, which read the weights again from the caches.)
+  const bool two = strips >= 2 * cus;
+  if (a.M > 32 && a.M <= 48) return PER < 4 && two ? launch_matvec_rows<XDT, PER, ZEROS, 3, PER < 4 ? 2 : 1, 1>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 3, 1, 1>(a, st);
+  return two ? launch_matvec_rows<XDT, PER, ZEROS, 2, 2, 1>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 2, 1, 1>(a, st);
 }
 
 template <int XDT>
