@@ -182,7 +182,7 @@ __global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
     sync_threads();
     const int m = tid >> 4, col = tid & 15;
     const int64_t n = 16 * now + col;
-    if (m < a.M && now < end && n < a.N) {
+    if (m < a.M && n < a.N) {
       float v = matvec_sum(red[turn], m, col);
       if (a.bias) v += load_any_f32(a.bias, a.bias_dtype, n);
       store_any(a.y, a.y_dtype, m * a.y_stride_m + n, v);
@@ -193,8 +193,8 @@ __global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
   while (now < end) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      multiply(st[d]);
-      request(st[d]);
+      if (now < end) multiply(st[d]);
+      if (D > 1 || now < end) request(st[d]);
     }
   }
 }
@@ -204,8 +204,9 @@ __global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
 // (One strip, U = 2 and nothing ahead: 51 us for 48 x 8192 x 8192, TODO now.)
 template <int XDT, int MT, int C, int PER, bool ZEROS, int U>
 __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a) {
-  constexpr int STEPS = 4 / PER;
-  __shared__ f32x4_t red[8][kWave];
+  constexpr int STEPS = 4 / PER, PITCH = 256 + 16;   // bytes of a row of a block in LDS: rows 16 bytes apart on the banks
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  f32x4_t (*const red)[kWave] = (f32x4_t (*)[kWave])lds;   // (used after the loop)
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const uint32_t c = lane & 15, h = lane >> 4, K = (uint32_t)a.K, n_kb = (K + 127) / 128;
   const MatvecPart part(n_kb, (uint32_t)wave);
@@ -217,9 +218,18 @@ __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a)
   const uint8_t *const x_at = (const uint8_t *)a.x + m0 * a.x_stride_m * 2, *const codes_at = a.codes + strip * n_kb * 1024;
   const uint8_t *const scales_at = (const uint8_t *)a.scales + strip * n_kb * (32 * PER), *const zeros_at = ZEROS ? a.zeros + strip * n_kb * (16 * PER) : nullptr;
   const int64_t x_bytes = (int64_t)(rows - 1) * a.x_stride_m * 2 + 2 * (int64_t)K;
-  uint32_t x_row[MT];
+  // A block's part of x: request i of tile t brings rows 16 t + 4 i .. + 3, 256 bytes each, which go through LDS to the lanes that
+  // multiply them.  (Requested where they are multiplied, 64 bytes of 16 rows at a time, 48 rows of 8192 took 18 of 31 us.)
+  uint8_t *const x_lds = lds + wave * (U * MT * 16 * PITCH);
+  uint32_t x_row[MT][4];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) x_row[t] = 16 * t + (int)c < rows ? (16u * t + c) * (uint32_t)a.x_stride_m * 2u + 16u * h : kMoeOob;
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * t + 4 * i + (int)h;
+      x_row[t][i] = row < rows ? (uint32_t)row * (uint32_t)a.x_stride_m * 2u + 16u * c : kMoeOob;
+    }
+  const uint32_t tail = K - 128u * (n_kb - 1u);   // K of the last block
   struct Stage {
     u32x4_t q[U][C], x[U][MT][4];
     uint32_t s[U][C][PER == 4 ? 2 : 1], z[U][C];
@@ -230,15 +240,15 @@ __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a)
     for (int i = 0; i < U; ++i) {
       // (what is not there comes from an empty buffer: no branch around requests)
       const uint32_t kb = part.kb0 + ask + i, there = all_ones_if(ask + i < part.n);
+      const Buffer x(x_at, x_bytes & (int64_t)there);
+      const uint32_t beyond = all_ones_if(kb + 1u == n_kb) & (8u * c >= tail ? kMoeOob : 0u);   // (K past the last block's)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const Buffer x(x_at, x_bytes & (int64_t)(there & all_ones_if(128u * kb + 32u * j < K)));
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          st.x[i][t][j] = x.load16(x_row[t], 256u * kb + 64u * j);
+        for (int j = 0; j < 4; ++j) {
+          st.x[i][t][j] = x.load16(x_row[t][j] | beyond, 256u * kb);
           __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
         }
-      }
 #pragma unroll
       for (int s = 0; s < C; ++s) {   // (the scalar offset is no part of the range check)
         const int64_t mask = (int64_t)(there & all_ones_if(s < here));
@@ -274,13 +284,22 @@ __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a)
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(u32x4_t *)(x_lds + ((i * MT + t) * 16 + 4 * j + h) * PITCH + 16u * c) = st.x[i][t][j];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
       for (int g = 0; g < PER; ++g) {
         f32x4_t of_x[MT];
+        u32x4_t xf[MT][STEPS];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j) xf[t][j] = *(const u32x4_t *)(x_lds + ((i * MT + t) * 16 + c) * PITCH + 64u * (g * STEPS + j) + 16u * h);
           of_x[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < STEPS; ++j) of_x[t] = Mma16<XDT>::mma(as_frag<XDT>(st.x[i][t][g * STEPS + j]), as_frag<XDT>(ones), of_x[t]);
+          for (int j = 0; j < STEPS; ++j) of_x[t] = Mma16<XDT>::mma(as_frag<XDT>(xf[t][j]), as_frag<XDT>(ones), of_x[t]);
         }
 #pragma unroll
         for (int s = 0; s < C; ++s) {
@@ -295,7 +314,7 @@ __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a)
 #pragma unroll
             for (int v = 0; v < 4; ++v) p[v] = offset * of_x[t][v];
 #pragma unroll
-            for (int j = 0; j < STEPS; ++j) p = Mma16<XDT>::mma(as_frag<XDT>(st.x[i][t][g * STEPS + j]), w[j], p);
+            for (int j = 0; j < STEPS; ++j) p = Mma16<XDT>::mma(as_frag<XDT>(xf[t][j]), w[j], p);
 #pragma unroll
             for (int v = 0; v < 4; ++v) y[t][s][v] = __builtin_fmaf(scale, p[v], y[t][s][v]);
           }
@@ -311,6 +330,7 @@ __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a)
     multiply(s1);
     request(s1);
   }
+  sync_threads();
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -331,14 +351,21 @@ __global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a)
 template <int XDT, int PER, bool ZEROS, int NB, int D>
 int launch_matvec_kept(const tamd_matvec_args &a, int cus, hipStream_t st) {
   const int64_t strips = (a.N + 15) / 16;
-  matvec_kernel<XDT, PER, ZEROS, NB, D><<<(unsigned)(strips < cus ? strips : cus), 512, 0, st>>>(a);
+  // up to two strips per CU: a workgroup each, side by side (1 x 2880 x 5120: 5.7 us, 9.0 with one per CU that walks)
+  if (strips <= 2 * cus) matvec_kernel<XDT, PER, ZEROS, NB, 1><<<(unsigned)strips, 512, 0, st>>>(a);
+  else matvec_kernel<XDT, PER, ZEROS, NB, D><<<(unsigned)cus, 512, 0, st>>>(a);
   return launch_status();
 }
 template <int XDT, int PER, bool ZEROS, int MT, int C, int U>
 int launch_matvec_rows(const tamd_matvec_args &a, hipStream_t st) {
   const int64_t strips = (a.N + 15) / 16;
   const dim3 grid((unsigned)((strips + C - 1) / C), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-  matvec_rows_kernel<XDT, MT, C, PER, ZEROS, U><<<grid, 512, 0, st>>>(a);
+  const auto kernel = matvec_rows_kernel<XDT, MT, C, PER, ZEROS, U>;
+  constexpr int lds = 8 * U * MT * 16 * (256 + 16);
+  static_assert(lds >= 8 * kWave * 16 && lds <= 160 * 1024);
+  if (lds > 64 * 1024)
+    if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
+  kernel<<<grid, 512, lds, st>>>(a);
   return launch_status();
 }
 
@@ -355,7 +382,7 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
     if (nb <= 4) return launch_matvec_kept<XDT, PER, ZEROS, 4, 3>(a, cus, st);
     if constexpr (PER < 4)
       if (nb <= 6) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
-    return strips >= 2 * cus ? launch_matvec_rows<XDT, PER, ZEROS, 1, 2, 2>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 2>(a, st);
+    return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 2>(a, st);
   }
   // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
   // registers with two strips: one strip, and above 48 rows parts of 32, which read the weights again from the caches.)
