@@ -71,9 +71,9 @@ TAMD_DEVICE float scale_of(uint32_t bits, bool f16) { return f16 ? f16_bits_to_f
 // those of one block, and change lanes from there: a request costs the CU about 20 cycles whatever it brings.
 // One strip per workgroup, x requested with the codes: 70 us for 1 x 4096 x 131072, TODO now.
 template <int XDT, int PER, bool ZEROS, int NB, int D>
-__global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
+__global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec_args a) {
   constexpr int SQ = (NB + 3) / 4, STEPS = 4 / PER;
-  constexpr bool KEEP = NB * PER <= 8;   // the sums of x stay in registers too
+  constexpr bool KEEP = D > 1 && NB * PER <= 8;   // the sums of x stay in registers too
   __shared__ f32x4_t red[2][8][kWave];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const uint32_t c = lane & 15, h = lane >> 4, K = (uint32_t)a.K, n_kb = (K + 127) / 128;
@@ -124,6 +124,9 @@ __global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
     ++ask;
   };
 
+  Stage st[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) request(st[d]);
   // ---- x, and the sums of its groups
   u32x4_t xr[NB][4];
   {
@@ -136,9 +139,6 @@ __global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
         xr[i][j] = x.load16((int)c < a.M && (uint32_t)i < part.n && k < K ? c * (uint32_t)a.x_stride_m * 2u + 2u * k + 16u * h : kMoeOob);
       }
   }
-  Stage st[D];
-#pragma unroll
-  for (int d = 0; d < D; ++d) request(st[d]);
   const auto x_sum = [&](int i, int g) {
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -190,11 +190,15 @@ __global__ __launch_bounds__(512, 2) void matvec_kernel(tamd_matvec_args a) {
     turn ^= 1;   // (one barrier between two uses of either half)
     ++now;
   };
-  while (now < end) {
+  if constexpr (D == 1) {   // (a workgroup per strip)
+    multiply(st[0]);
+  } else {
+    while (now < end) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (now < end) multiply(st[d]);
-      if (D > 1 || now < end) request(st[d]);
+      for (int d = 0; d < D; ++d) {
+        if (now < end) multiply(st[d]);
+        request(st[d]);
+      }
     }
   }
 }
@@ -352,8 +356,12 @@ template <int XDT, int PER, bool ZEROS, int NB, int D>
 int launch_matvec_kept(const tamd_matvec_args &a, int cus, hipStream_t st) {
   const int64_t strips = (a.N + 15) / 16;
   // up to two strips per CU: a workgroup each, side by side (1 x 2880 x 5120: 5.7 us, 9.0 with one per CU that walks)
-  if (strips <= 2 * cus) matvec_kernel<XDT, PER, ZEROS, NB, 1><<<(unsigned)strips, 512, 0, st>>>(a);
-  else matvec_kernel<XDT, PER, ZEROS, NB, D><<<(unsigned)cus, 512, 0, st>>>(a);
+  if constexpr (NB <= 4)
+    if (strips <= 2 * cus) {
+      matvec_kernel<XDT, PER, ZEROS, NB, 1><<<(unsigned)strips, 512, 0, st>>>(a);
+      return launch_status();
+    }
+  matvec_kernel<XDT, PER, ZEROS, NB, D><<<(unsigned)(strips < cus ? strips : cus), 512, 0, st>>>(a);
   return launch_status();
 }
 template <int XDT, int PER, bool ZEROS, int MT, int C, int U>
@@ -381,7 +389,7 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
     if (nb <= 3) return launch_matvec_kept<XDT, PER, ZEROS, 3, 4>(a, cus, st);
     if (nb <= 4) return launch_matvec_kept<XDT, PER, ZEROS, 4, 3>(a, cus, st);
     if constexpr (PER < 4)
-      if (nb <= 6) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
+      if (nb <= 6 && strips > 2 * cus) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
     return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 2>(a, st);
   }
   // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
