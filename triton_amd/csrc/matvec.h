@@ -207,7 +207,7 @@ __global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec
 // with the codes, U blocks at a time and twice that in flight.  Each block of x serves C strips.
 // (One strip, U = 2 and nothing ahead: 51 us for 48 x 8192 x 8192, TODO now.)
 template <int XDT, int MT, int C, int PER, bool ZEROS, int U>
-__global__ __launch_bounds__(512, 2) void matvec_rows_kernel(tamd_matvec_args a) {
+__global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_matvec_args a) {
   constexpr int STEPS = 4 / PER, PITCH = 256 + 16;   // bytes of a row of a block in LDS: rows 16 bytes apart on the banks
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   f32x4_t (*const red)[kWave] = (f32x4_t (*)[kWave])lds;   // (used after the loop)
@@ -390,7 +390,7 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
     if (nb <= 4) return launch_matvec_kept<XDT, PER, ZEROS, 4, 3>(a, cus, st);
     if constexpr (PER < 4)
       if (nb <= 6 && strips > 2 * cus) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
-    return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 2>(a, st);
+    return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1>(a, st);
   }
   // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
   // registers with two strips: one strip, and above 48 rows parts of 32, which read the weights again from the caches.)
