@@ -206,7 +206,7 @@ __global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec
 // Any number of rows and any K: a workgroup has C strips and MT tiles of 16 rows, its eight waves split K and read their part of x once,
 // with the codes, U blocks at a time and twice that in flight.  Each block of x serves C strips.
 // (One strip, U = 2 and nothing ahead: 51 us for 48 x 8192 x 8192, TODO now.)
-template <int XDT, int MT, int C, int PER, bool ZEROS, int U>
+template <int XDT, int MT, int XI, int C, int PER, bool ZEROS, int U>
 __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_matvec_args a) {
   constexpr int STEPS = 4 / PER, PITCH = 256 + 16;   // bytes of a row of a block in LDS: rows 16 bytes apart on the banks
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -222,20 +222,20 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
   const uint8_t *const x_at = (const uint8_t *)a.x + m0 * a.x_stride_m * 2, *const codes_at = a.codes + strip * n_kb * 1024;
   const uint8_t *const scales_at = (const uint8_t *)a.scales + strip * n_kb * (32 * PER), *const zeros_at = ZEROS ? a.zeros + strip * n_kb * (16 * PER) : nullptr;
   const int64_t x_bytes = (int64_t)(rows - 1) * a.x_stride_m * 2 + 2 * (int64_t)K;
-  // A block's part of x: request i of tile t brings rows 16 t + 4 i .. + 3, 256 bytes each, which go through LDS to the lanes that
+  // A block's part of x: request i of a tile's XI brings rows 16 t + 4 i .. + 3, 256 bytes each, which go through LDS to the lanes that
   // multiply them.  (Requested where they are multiplied, 64 bytes of 16 rows at a time, 48 rows of 8192 took 18 of 31 us.)
-  uint8_t *const x_lds = lds + wave * (U * MT * 16 * PITCH);
-  uint32_t x_row[MT][4];
+  uint8_t *const x_lds = lds + wave * (U * MT * 4 * XI * PITCH);
+  uint32_t x_row[MT][XI];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < XI; ++i) {
       const int row = 16 * t + 4 * i + (int)h;
       x_row[t][i] = row < rows ? (uint32_t)row * (uint32_t)a.x_stride_m * 2u + 16u * c : kMoeOob;
     }
   const uint32_t tail = K - 128u * (n_kb - 1u);   // K of the last block
   struct Stage {
-    u32x4_t q[U][C], x[U][MT][4];
+    u32x4_t q[U][C], x[U][MT][XI];
     uint32_t s[U][C][PER == 4 ? 2 : 1], z[U][C];
   };
   uint32_t ask = 0;
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < XI; ++j) {
           st.x[i][t][j] = x.load16(x_row[t][j] | beyond, 256u * kb);
           __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
         }
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *(u32x4_t *)(x_lds + ((i * MT + t) * 16 + 4 * j + h) * PITCH + 16u * c) = st.x[i][t][j];
+        for (int j = 0; j < XI; ++j) *(u32x4_t *)(x_lds + ((i * MT + t) * 4 * XI + 4 * j + h) * PITCH + 16u * c) = st.x[i][t][j];
 #pragma unroll
     for (int i = 0; i < U; ++i)
 #pragma unroll
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
-          for (int j = 0; j < STEPS; ++j) xf[t][j] = *(const u32x4_t *)(x_lds + ((i * MT + t) * 16 + c) * PITCH + 64u * (g * STEPS + j) + 16u * h);
+          for (int j = 0; j < STEPS; ++j) xf[t][j] = *(const u32x4_t *)(x_lds + ((i * MT + t) * 4 * XI + (c & (4u * XI - 1u))) * PITCH + 64u * (g * STEPS + j) + 16u * h);   // (rows past the last repeat)
           of_x[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < STEPS; ++j) of_x[t] = Mma16<XDT>::mma(as_frag<XDT>(xf[t][j]), as_frag<XDT>(ones), of_x[t]);
@@ -364,13 +364,13 @@ int launch_matvec_kept(const tamd_matvec_args &a, int cus, hipStream_t st) {
   matvec_kernel<XDT, PER, ZEROS, NB, D><<<(unsigned)(strips < cus ? strips : cus), 512, 0, st>>>(a);
   return launch_status();
 }
-template <int XDT, int PER, bool ZEROS, int MT, int C, int U>
+template <int XDT, int PER, bool ZEROS, int MT, int C, int U, int XI = 4>
 int launch_matvec_rows(const tamd_matvec_args &a, hipStream_t st) {
   const int64_t strips = (a.N + 15) / 16;
   const dim3 grid((unsigned)((strips + C - 1) / C), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-  const auto kernel = matvec_rows_kernel<XDT, MT, C, PER, ZEROS, U>;
-  constexpr int lds = 8 * U * MT * 16 * (256 + 16);
-  static_assert(lds >= 8 * kWave * 16 && lds <= 160 * 1024);
+  const auto kernel = matvec_rows_kernel<XDT, MT, XI, C, PER, ZEROS, U>;
+  constexpr int for_x = 8 * U * MT * 4 * XI * (256 + 16), lds = for_x > 8 * kWave * 16 ? for_x : 8 * kWave * 16;
+  static_assert(lds <= 160 * 1024);
   if (lds > 64 * 1024)
     if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
   kernel<<<grid, 512, lds, st>>>(a);
@@ -390,6 +390,8 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
     if (nb <= 4) return launch_matvec_kept<XDT, PER, ZEROS, 4, 3>(a, cus, st);
     if constexpr (PER < 4)
       if (nb <= 6 && strips > 2 * cus) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
+    if (a.M <= 4) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, PER < 4 ? 2 : 1, 1>(a, st);
+    if (a.M <= 8) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1, 2>(a, st);
     return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1>(a, st);
   }
   // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
