@@ -83,6 +83,7 @@ struct RowScale {
   }
   // (of -inf: infinite, or NaN at an infinite temperature; neither counts)
   TAMD_DEVICE double y_of(float v) const {
+#pragma clang fp contract(off)
     if (infinite) return v == __builtin_inff() ? 0.0 : 1e9;
     return (top - (double)v) * to_y;
   }
@@ -96,6 +97,7 @@ struct RowScale {
   // of the product.  (With exp() and conversions this took longer than reading the logits.  Fused by hand: the histogram and
   // the candidates have to agree to the last unit in every kernel.)
   TAMD_DEVICE uint64_t units_of(double y) const {
+#pragma clang fp contract(off)
     const uint64_t fixed = __builtin_bit_cast(uint64_t, y + 6144.0) & 0xFFFFFFFFFFFFull;   // 6144 = 1.5 * 2^12: the lowest bit is 2^-40
     const uint32_t whole = (uint32_t)(fixed >> 40) & 0x7FFu;
     const double r = (double)(uint32_t)fixed * (0.6931471805599453 * 0x1p-40);
@@ -422,15 +424,18 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
     }
 }
 
-// n <= kMost elements of `list` (room for the next power of two), largest first afterwards.  Up to 1024 by counting the larger ones of
-// each, all threads sharing the comparisons (a few hundred: one barrier or two instead of 45), else in steps of the bitonic network.
+// n <= kMost elements of `list` (room for the next power of two), largest first afterwards.  Up to kCounted by counting the larger ones of
+// each, all threads sharing the comparisons.  Up to kThreads every wave sorts 64 in its registers, and an element's place is how many
+// of every wave's are larger, which seven steps of halving tell.  The last launch takes 6.7 us with the first and 8.2 with the second
+// for one row of some hundred candidates, 16.4 and 9.9 for 64 rows of some 600.  Else steps of the bitonic network.
+constexpr int kCounted = 256;
 TAMD_DEVICE void sort_elements(uint64_t *list, int n, uint32_t *rank) {
-  const int tid = threadIdx.x;
-  if (n <= kThreads) {
+  const int tid = threadIdx.x, lane = tid % kWave;
+  if (n <= kCounted) {
     int wide = kWave;
     while (wide < n) wide *= 2;
     const int i = tid % wide, part = tid / wide, parts = kThreads / wide;
-    rank[tid] = 0;
+    if (tid < kCounted) rank[tid] = 0;
     sync_threads();
     const uint64_t e = i < n ? list[i] : 0;
     uint32_t larger = 0;
@@ -438,6 +443,39 @@ TAMD_DEVICE void sort_elements(uint64_t *list, int n, uint32_t *rank) {
     if (i < n && larger) atomicAdd(&rank[i], larger);
     sync_threads();
     if (tid < n) list[rank[tid]] = e;   // (wide >= n: thread tid holds element tid; all are different)
+    sync_threads();
+    return;
+  }
+  if (n <= kThreads) {
+    const int runs = (n + kWave - 1) / kWave;
+    uint64_t e = tid < n ? list[tid] : 0;   // (0: smaller than any element; the list's own are all different)
+    if (tid < runs * kWave) {
+#pragma unroll
+      for (int k = 2; k <= kWave; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j > 0; j /= 2) {
+          const uint64_t other = __shfl_xor(e, j);
+          const bool larger = ((lane & k) == 0) == ((lane & j) == 0);   // (k = 64: the largest come first)
+          e = (other > e) == larger ? other : e;
+        }
+      list[tid] = e;
+    }
+    sync_threads();
+    int place = lane;
+    if (tid < n) {   // (zeros are last of their run, behind all that count)
+      for (int g = 0; g < runs; g += 4) {
+        int at[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int step = kWave / 2; step > 0; step /= 2)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) at[q] += g + q < runs && list[(g + q) * kWave + at[q] + step - 1] > e ? step : 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (g + q < runs && g + q != tid / kWave) place += at[q] + (list[(g + q) * kWave + at[q]] > e);
+      }
+    }
+    sync_threads();
+    if (e) list[place] = e;
     sync_threads();
     return;
   }
@@ -675,7 +713,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Wo
 template <int DT>
 __global__ __launch_bounds__(kThreads) void short_row_kernel(tamd_sample_args a) {
   __shared__ uint64_t list[kMost];
-  __shared__ uint32_t rank[kThreads];
+  __shared__ uint32_t rank[kCounted];
   __shared__ double powers[256];
   __shared__ Shared sh;
   const int r = blockIdx.x, tid = threadIdx.x;
