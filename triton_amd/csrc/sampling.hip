@@ -68,38 +68,35 @@ TAMD_DEVICE void make_powers(double *powers, int V) {
   if (threadIdx.x < 256) powers[threadIdx.x] = exp2(fraction_bits(V) - (double)threadIdx.x * 0.00390625);
 }
 
-// Weights of a row whose largest logit is `top` (> -inf).  y = log2(1 / w).
+// Weights of a row whose largest logit is `top` (> -inf).  y = log2(1 / w).  An infinite logit is kHuge here: such ones weigh alike, and
+// nothing else does (y in steps of one, from kHuge).
+constexpr double kHuge = 1e300;
 struct RowScale {
   double top, to_y, to_bin;
   int fraction;
-  bool infinite;     // with infinite logits these weigh alike and nothing else does
   const double *powers;
   TAMD_DEVICE RowScale(double top_, double to_y_, double to_bin_, int V, const double *powers_)
-      : top(top_), to_y(to_y_), to_bin(to_bin_), fraction(fraction_bits(V)), infinite(top_ == __builtin_inf()), powers(powers_) {}
+      : top(top_), to_y(to_y_), to_bin(to_bin_), fraction(fraction_bits(V)), powers(powers_) {}
   TAMD_DEVICE RowScale(uint32_t top_key, uint32_t least_key, double t, int V, const double *powers_)
-      : top(logit_of(top_key)), to_y(1.4426950408889634 / t), fraction(fraction_bits(V)), infinite(logit_of(top_key) == __builtin_inff()), powers(powers_) {
+      : top(__builtin_fmin((double)logit_of(top_key), kHuge)), to_y(top == kHuge ? 1.0 : 1.4426950408889634 / t), fraction(fraction_bits(V)), powers(powers_) {
     const double most = y_of(logit_of(least_key)), range = most < fraction ? most : fraction;
     to_bin = range > 0.0 ? kBins / range : 0.0;
   }
   // (of -inf: infinite, or NaN at an infinite temperature; neither counts)
   TAMD_DEVICE double y_of(float v) const {
 #pragma clang fp contract(off)
-    if (infinite) return v == __builtin_inff() ? 0.0 : 1e9;
-    return (top - (double)v) * to_y;
+    return (top - __builtin_fmin((double)v, kHuge)) * to_y;
   }
   TAMD_DEVICE bool counts(double y) const { return y < fraction; }
-  TAMD_DEVICE int bin_of(double y) const {
-    const double b = y * to_bin;
-    return b >= kBins - 1 ? kBins - 1 : (int)b;
-  }
-  // 2^(fraction - y) of a y that counts, in units.  y in units of 2^-40 (the low bits of y + 1.5 * 2^12) is a whole number, eight bits for
+  TAMD_DEVICE int bin_of(double y) const { return (int)__builtin_fmin(y * to_bin, (double)(kBins - 1)); }
+  // 2^(fraction - y) of a y that counts, in units (of another: any number).  y in units of 2^-40 (the low bits of y + 1.5 * 2^12) is a whole number, eight bits for
   // the table and the rest r for the series of 2^-r, whose first four terms leave 2.3e-12 of w; adding 2^52 makes a whole number
   // of the product.  (With exp() and conversions this took longer than reading the logits.  Fused by hand: the histogram and
   // the candidates have to agree to the last unit in every kernel.)
   TAMD_DEVICE uint64_t units_of(double y) const {
 #pragma clang fp contract(off)
     const uint64_t fixed = __builtin_bit_cast(uint64_t, y + 6144.0) & 0xFFFFFFFFFFFFull;   // 6144 = 1.5 * 2^12: the lowest bit is 2^-40
-    const uint32_t whole = (uint32_t)(fixed >> 40) & 0x7FFu;
+    const uint32_t whole = (uint32_t)(fixed >> 40) & 0x3Fu;
     const double r = (double)(uint32_t)fixed * (0.6931471805599453 * 0x1p-40);
     double p = __builtin_fma(r, -1.0 / 6.0, 0.5);
     p = __builtin_fma(r, p, -1.0);
@@ -304,6 +301,7 @@ struct Chunk {
       }
     }
   }
+  // use(v, index): four logits of consecutive indexes
   template <typename F>
   TAMD_DEVICE void each(F use) {
     while (at < end) {
@@ -314,7 +312,9 @@ struct Chunk {
       at += kStep;
       if (at < end) request();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) use(from + (j / 4) * 4 * kThreads + j % 4, now[j] != now[j] ? -__builtin_inff() : now[j]);
+      for (int j = 0; j < 8; ++j) now[j] = now[j] != now[j] ? -__builtin_inff() : now[j];
+      use(now, from);
+      use(now + 4, from + 4 * kThreads);
     }
   }
 };
@@ -354,11 +354,14 @@ __global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, 
   if (c == 0 && tid == 0) ws.collected[r] = 0;
   uint64_t first = 0;
   uint32_t least = 0xFFFFFFFFu;
-  logits.each([&](int i, float v) {
-    const uint32_t key = ordered_bits(v);
-    const uint64_t e = element_of(key, i);
-    first = e > first ? e : first;
-    least = key > kNothing && key < least ? key : least;
+  logits.each([&](const float *v, int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t key = ordered_bits(v[j]);
+      const uint64_t e = element_of(key, i + j);
+      first = e > first ? e : first;
+      least = key > kNothing && key < least ? key : least;
+    }
   });
 #pragma unroll
   for (int o = 1; o < kWave; o *= 2) {
@@ -408,12 +411,21 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
   for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
   const RowScale scale(key_of(first), least, s.t, a.V, powers);
   sync_threads();
-  logits.each([&](int, float v) {
-    const double y = scale.y_of(v);
-    if (scale.counts(y)) {
-      const int b = scale.bin_of(y);
-      atomicAdd((unsigned long long *)&mass[b], (unsigned long long)scale.units_of(y));
-      if (s.top_k) atomicAdd(&count[b], 1u);   // (nothing else asks for counts)
+  // (no branch but around the additions: a logit at a time, each waiting for its power, 64 rows of 131072 took 14.7 us and 256 of 100000
+  // 31.0, so 14.4 and 30.5: the additions in LDS and the logits are what is left)
+  logits.each([&](const float *v, int) {
+    double y[4];
+    uint64_t units[4];
+    int bin[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = scale.y_of(v[j]), bin[j] = scale.bin_of(y[j]), units[j] = scale.units_of(y[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (scale.counts(y[j])) atomicAdd((unsigned long long *)&mass[bin[j]], (unsigned long long)units[j]);
+    if (s.top_k) {   // (nothing else asks for counts)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (scale.counts(y[j])) atomicAdd(&count[bin[j]], 1u);
     }
   });
   sync_threads();
@@ -658,17 +670,27 @@ __global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, W
   const RowScale scale(b.top, b.to_y, b.to_bin, a.V, nullptr);
   if (tid == 0) sh.n = 0;
   sync_threads();
-  logits.each([&](int i, float v) {
-    const double y = scale.y_of(v);
-    if (scale.counts(y)) {
-      const int bin = scale.bin_of(y);
-      bool is = false;
+  uint32_t from[4], more[4];   // (an empty range: from = kBins, and nothing is as large)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) is |= bin >= b.from[j] && bin <= b.to[j];
-      if (is) {
-        const uint32_t at = atomicAdd(&sh.n, 1u);
-        if (at < kMost) list[at] = element_of(ordered_bits(v), i);
-      }
+  for (int q = 0; q < 4; ++q) from[q] = (uint32_t)b.from[q], more[q] = b.to[q] > b.from[q] ? (uint32_t)(b.to[q] - b.from[q]) : 0u;
+  logits.each([&](const float *v, int i) {
+    bool is[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double y = scale.y_of(v[j]);
+      const uint32_t bin = (uint32_t)scale.bin_of(y);
+      is[j] = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) is[j] |= bin - from[q] <= more[q];
+      is[j] &= scale.counts(y);
+    }
+    if (is[0] | is[1] | is[2] | is[3]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (is[j]) {
+          const uint32_t at = atomicAdd(&sh.n, 1u);
+          if (at < kMost) list[at] = element_of(ordered_bits(v[j]), i + j);
+        }
     }
   });
   sync_threads();
