@@ -63,13 +63,20 @@ TAMD_DEVICE uint32_t all_ones_if(bool b) {
   asm volatile("" : "+s"(v));
   return v;
 }
-TAMD_DEVICE float scale_of(uint32_t bits, bool f16) { return f16 ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits); }
+// A scale of either type; f16 is all ones or zero, hidden from the compiler: behind a branch per scale it put off what the
+// accumulators are used for, until the registers did not suffice.
+TAMD_DEVICE uint32_t scale_type(int dtype) {
+  uint32_t v = (uint32_t)__builtin_amdgcn_readfirstlane(dtype == TAMD_F16 ? -1 : 0);
+  asm volatile("" : "+s"(v));
+  return v;
+}
+TAMD_DEVICE float scale_of(uint32_t bits, uint32_t f16) { return bits_to_f32((f32_to_bits(f16_bits_to_f32(bits)) & f16) | (bits << 16 & ~f16)); }
 
 // Up to 16 rows and NB blocks per wave.  A workgroup per CU (two where a wave has few blocks) walks over a contiguous part of the
 // strips; its eight waves split K, and a wave's part of x stays in registers.  The codes of D strips are in flight, the waves'
 // sums meet in LDS, a barrier per strip.  Scales and zero points of four blocks come with one request, each quarter of the lanes bringing
 // those of one block, and change lanes from there: a request costs the CU about 20 cycles whatever it brings.
-// One strip per workgroup, x requested with the codes: 70 us for 1 x 4096 x 131072, TODO now.
+// One strip per workgroup, x requested with the codes: 70 us for 1 x 4096 x 131072, 43 to 46 now.
 template <int XDT, int PER, bool ZEROS, int NB, int D>
 __global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec_args a) {
   constexpr int SQ = (NB + 3) / 4, STEPS = 4 / PER;
@@ -80,7 +87,7 @@ __global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec
   const MatvecPart part(n_kb, (uint32_t)wave);
   const int64_t strips = (a.N + 15) / 16;
   const int64_t begin = strips * blockIdx.x / gridDim.x, end = strips * (blockIdx.x + 1) / gridDim.x;
-  const bool scale_f16 = a.scale_dtype == TAMD_F16;
+  const uint32_t scale_f16 = scale_type(a.scale_dtype);
   const u32x4_t ones = {Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne};
 
   struct Stage {
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec
 
 // Any number of rows and any K: a workgroup has C strips and MT tiles of 16 rows, its eight waves split K and read their part of x once,
 // with the codes, U blocks at a time and twice that in flight.  Each block of x serves C strips.
-// (One strip, U = 2 and nothing ahead: 51 us for 48 x 8192 x 8192, TODO now.)
+// (One strip, U = 2 and nothing ahead: 51 us for 48 x 8192 x 8192, 21 now.)
 template <int XDT, int MT, int XI, int C, int PER, bool ZEROS, int U>
 __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_matvec_args a) {
   constexpr int STEPS = 4 / PER, PITCH = 256 + 16;   // bytes of a row of a block in LDS: rows 16 bytes apart on the banks
@@ -216,7 +223,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
   const MatvecPart part(n_kb, (uint32_t)wave);
   const int64_t strips = (a.N + 15) / 16, strip = (int64_t)blockIdx.x * C;
   const int m0 = blockIdx.y * (16 * MT), rows = a.M - m0 < 16 * MT ? a.M - m0 : 16 * MT;
-  const bool scale_f16 = a.scale_dtype == TAMD_F16;
+  const uint32_t scale_f16 = scale_type(a.scale_dtype);
   const u32x4_t ones = {Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne};
   const int64_t here = strips - strip < C ? strips - strip : C, blocks = here * n_kb;
   const uint8_t *const x_at = (const uint8_t *)a.x + m0 * a.x_stride_m * 2, *const codes_at = a.codes + strip * n_kb * 1024;
@@ -323,6 +330,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
             for (int v = 0; v < 4; ++v) y[t][s][v] = __builtin_fmaf(scale, p[v], y[t][s][v]);
           }
         }
+        if constexpr (U > 1) __builtin_amdgcn_sched_barrier(0);   // (or a later group's x is read at once, and 128 registers do not suffice)
       }
   };
   Stage s0, s1;
@@ -352,6 +360,165 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
     }
 }
 
+// Several tiles of rows and many columns: a workgroup has MT tiles and 2 WN strips.  Its waves are WN pairs of strips times 8 / WN parts of K;
+// a block of x goes through LDS once for all waves of its part, two blocks deep, and with the codes is requested two blocks ahead.
+// (64 x 4096 x 131072: 269 us by matvec_rows_kernel, where x comes from the caches for every second strip, 125 so; 149 with three blocks
+// ahead, which leave room for one workgroup per CU.  The matrix products, the codes' arithmetic and LDS take about 40 us each.)
+template <int XDT, int MT, int WN, int PER, bool ZEROS>
+__global__ __launch_bounds__(512, 2) void matvec_wide_kernel(tamd_matvec_args a) {
+  constexpr int C = 2, D = 2, WK = 8 / WN, STEPS = 4 / PER, PITCH = 256 + 16, XL = (4 * MT + WN - 1) / WN;
+  constexpr uint32_t TILE = XL * 4 * WN * PITCH;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const uint32_t c = lane & 15, h = lane >> 4, K = (uint32_t)a.K, n_kb = (K + 127) / 128;
+  const uint32_t n = (n_kb + WK - 1) / WK, kb0 = (uint32_t)(wave / WN) * n;
+  const int64_t strips = (a.N + 15) / 16, strip = ((int64_t)blockIdx.x * WN + wave % WN) * C;
+  const int m0 = blockIdx.y * (16 * MT), rows = a.M - m0 < 16 * MT ? a.M - m0 : 16 * MT;
+  const uint32_t scale_f16 = scale_type(a.scale_dtype);
+  const u32x4_t ones = {Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne, Int4<XDT>::kOne};
+  const int64_t here = strips - strip < C ? (strips > strip ? strips - strip : 0) : C, first = here ? strip : 0, blocks = here * n_kb;
+  const uint8_t *const x_at = (const uint8_t *)a.x + m0 * a.x_stride_m * 2, *const codes_at = a.codes + first * n_kb * 1024;
+  const uint8_t *const scales_at = (const uint8_t *)a.scales + first * n_kb * (32 * PER), *const zeros_at = ZEROS ? a.zeros + first * n_kb * (16 * PER) : nullptr;
+  const int64_t x_bytes = (int64_t)(rows - 1) * a.x_stride_m * 2 + 2 * (int64_t)K;
+  uint8_t *const x_lds = lds + (wave / WN) * 2 * TILE;
+  uint32_t x_row[XL];   // request i of a wave brings four rows
+#pragma unroll
+  for (int i = 0; i < XL; ++i) {
+    const int row = 4 * (i * WN + wave % WN) + (int)h;
+    x_row[i] = row < rows ? (uint32_t)row * (uint32_t)a.x_stride_m * 2u + 16u * c : kMoeOob;
+  }
+  const uint32_t tail = K - 128u * (n_kb - 1u);   // K of the last block
+  struct Stage {
+    u32x4_t q[C], x[XL];
+    uint32_t s[C][PER == 4 ? 2 : 1], z[C];
+  };
+  uint32_t ask = 0;
+  const auto request = [&](Stage &st) {   // (what is not there comes from an empty buffer: no branch around requests)
+    const uint32_t kb = kb0 + ask, there = all_ones_if(ask < n && kb < n_kb);
+    const Buffer x(x_at, x_bytes & (int64_t)there);
+    const uint32_t beyond = all_ones_if(kb + 1u == n_kb) & (8u * c >= tail ? kMoeOob : 0u);   // (K past the last block's)
+#pragma unroll
+    for (int j = 0; j < XL; ++j) {
+      st.x[j] = x.load16(x_row[j] | beyond, 256u * kb);
+      __builtin_amdgcn_sched_barrier(0);   // (one order wherever this is expanded: the waits are counted from it)
+    }
+#pragma unroll
+    for (int s = 0; s < C; ++s) {   // (the scalar offset is no part of the range check)
+      const int64_t mask = (int64_t)(there & all_ones_if(s < here));
+      const Buffer codes(codes_at, (blocks * 1024) & mask), scales(scales_at, (blocks * 32 * PER) & mask);
+      st.q[s] = codes.template load16<2>(16u * lane, (s * n_kb + kb) * 1024u);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (PER == 4) {
+        const u32x2_t v = scales.load8(8u * c, (s * n_kb + kb) * 128u);
+        st.s[s][0] = v.x, st.s[s][1] = v.y;
+      } else if constexpr (PER == 2) {
+        st.s[s][0] = scales.load4(4u * c, (s * n_kb + kb) * 64u);
+      } else {
+        st.s[s][0] = scales.load2(2u * c, (s * n_kb + kb) * 32u);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (ZEROS) {
+        const Buffer zeros(zeros_at, (blocks * 16 * PER) & mask);
+        if constexpr (PER == 4) st.z[s] = zeros.load4(4u * c, (s * n_kb + kb) * 64u);
+        else if constexpr (PER == 2) st.z[s] = zeros.load2(2u * c, (s * n_kb + kb) * 32u);
+        else st.z[s] = zeros.load1(c, (s * n_kb + kb) * 16u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    ++ask;
+  };
+  f32x4_t y[MT][C];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int s = 0; s < C; ++s) y[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const auto keep = [&](const Stage &st, uint32_t at) {
+#pragma unroll
+    for (int i = 0; i < XL; ++i) *(u32x4_t *)(x_lds + at + (4 * (i * WN + wave % WN) + h) * PITCH + 16u * c) = st.x[i];
+  };
+  const auto multiply = [&](const Stage &st, uint32_t at) {
+#pragma unroll
+    for (int g = 0; g < PER; ++g) {
+      f32x4_t of_x[MT], p[MT][C];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        of_x[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < C; ++s) p[t][s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int j = 0; j < STEPS; ++j) {
+        u32x4_t xf[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) xf[t] = *(const u32x4_t *)(x_lds + at + (16 * t + c) * PITCH + 64u * (g * STEPS + j) + 16u * h);
+        typename Mma<XDT>::frag_t w[C];
+#pragma unroll
+        for (int s = 0; s < C; ++s) w[s] = codes_plus_16<XDT>(st.q[s][g * STEPS + j]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          of_x[t] = Mma16<XDT>::mma(as_frag<XDT>(xf[t]), as_frag<XDT>(ones), of_x[t]);
+#pragma unroll
+          for (int s = 0; s < C; ++s) p[t][s] = Mma16<XDT>::mma(as_frag<XDT>(xf[t]), w[s], p[t][s]);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < C; ++s) {
+        const float scale = scale_of(st.s[s][g / 2] >> (16 * (g & 1)) & 0xFFFFu, scale_f16);
+        const float offset = ZEROS ? -16.f - (float)(st.z[s] >> (8 * g) & 0xFFu) : -24.f;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) y[t][s][v] = __builtin_fmaf(scale, __builtin_fmaf(offset, of_x[t][v], p[t][s][v]), y[t][s][v]);
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (or a later group's x is read at once, and the registers do not suffice)
+    }
+  };
+  Stage st[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) request(st[d]);
+  keep(st[0], 0);
+  sync_threads();
+  uint32_t at = 0;
+  for (uint32_t k = 0; k < n; k += D) {   // (blocks past the last: zeros.  One barrier between two uses of either half of the part's LDS)
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      keep(st[(d + 1) % D], TILE - at);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(st[d], at);
+      request(st[d]);
+      at = TILE - at;
+      sync_threads();
+    }
+  }
+  f32x4_t (*const red)[MT][C][kWave] = (f32x4_t (*)[MT][C][kWave])lds;
+  if constexpr (WK > 1) {
+    if (wave >= WN) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int s = 0; s < C; ++s) red[wave - WN][t][s][lane] = y[t][s];
+    }
+    sync_threads();
+    if (wave >= WN) return;
+  }
+#pragma unroll
+  for (int s = 0; s < C; ++s) {
+    const int64_t col = 16 * (strip + s) + c;
+    if (col >= a.N) continue;
+    const float bias = a.bias ? load_any_f32(a.bias, a.bias_dtype, col) : 0.f;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int q = 1; q < WK; ++q) y[t][s] += red[(q - 1) * WN + wave][t][s][lane];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int m = 16 * t + 4 * (int)h + v;
+        if (m < rows) store_any(a.y, a.y_dtype, (m0 + m) * a.y_stride_m + col, y[t][s][v] + bias);
+      }
+    }
+  }
+}
+
 template <int XDT, int PER, bool ZEROS, int NB, int D>
 int launch_matvec_kept(const tamd_matvec_args &a, int cus, hipStream_t st) {
   const int64_t strips = (a.N + 15) / 16;
@@ -377,6 +544,20 @@ int launch_matvec_rows(const tamd_matvec_args &a, hipStream_t st) {
   return launch_status();
 }
 
+template <int XDT, int PER, bool ZEROS, int MT, int WN>
+int launch_matvec_wide(const tamd_matvec_args &a, hipStream_t st) {
+  const int64_t strips = (a.N + 15) / 16;
+  const dim3 grid((unsigned)((strips + 2 * WN - 1) / (2 * WN)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+  const auto kernel = matvec_wide_kernel<XDT, MT, WN, PER, ZEROS>;
+  constexpr int WK = 8 / WN, for_x = WK * 2 * ((4 * MT + WN - 1) / WN) * 4 * WN * (256 + 16), for_sums = (8 - WN) * MT * 2 * kWave * 16;
+  constexpr int lds = for_x > for_sums ? for_x : for_sums;
+  static_assert(lds <= 160 * 1024);
+  if (lds > 64 * 1024)
+    if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
+  kernel<<<grid, 512, lds, st>>>(a);
+  return launch_status();
+}
+
 template <int XDT, int PER, bool ZEROS>
 int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
   int cus = 0;
@@ -390,12 +571,19 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
     if (nb <= 4) return launch_matvec_kept<XDT, PER, ZEROS, 4, 3>(a, cus, st);
     if constexpr (PER < 4)
       if (nb <= 6 && strips > 2 * cus) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
-    if (a.M <= 4) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, PER < 4 ? 2 : 1, 1>(a, st);
+    if (a.M <= 4) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, PER < 2 ? 2 : 1, 1>(a, st);
     if (a.M <= 8) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1, 2>(a, st);
     return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1>(a, st);
   }
   // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
   // registers with two strips: one strip, and above 48 rows parts of 32, which read the weights again from the caches.)
+  // Waves with strips of their own from five strips per CU on, eight per workgroup: 64 x 4096 x 20480 takes 32 us so and 45 with the
+  // other kernel, 20 x 8192 x 20480 41 either way; with four per CU 20 x 8192 x 16384 takes 41 and 29.
+  if (strips >= 5 * cus) {
+    if (a.M <= 32) return launch_matvec_wide<XDT, PER, ZEROS, 2, 4>(a, st);
+    if (a.M <= 48) return launch_matvec_wide<XDT, PER, ZEROS, 3, 4>(a, st);
+    return launch_matvec_wide<XDT, PER, ZEROS, 4, 4>(a, st);
+  }
   const bool two = strips >= 2 * cus;
   if (a.M > 32 && a.M <= 48) return PER < 4 && two ? launch_matvec_rows<XDT, PER, ZEROS, 3, PER < 4 ? 2 : 1, 1>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 3, 1, 1>(a, st);
   return two ? launch_matvec_rows<XDT, PER, ZEROS, 2, 2, 1>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 2, 1, 1>(a, st);
