@@ -1,4 +1,4 @@
-"""GPU: `matvec` of more than 16 rows and so many columns that waves have strips of their own, against the formula in 64 bits
+"""GPU: `matvec` of more than a few rows and so many columns that waves have strips of their own, against the formula in 64 bits
 (the bound is the one of test_gpu_matvec: no element passes more additions here, and two parts of K meet in one more)."""
 import pytest
 import torch
@@ -51,3 +51,10 @@ def test_padding_is_left_alone(device):
     bad[7, 3] = float("nan")
     again = matvec(bad, w, b, out_dtype=torch.float32)
     assert torch.isnan(again[7]).all() and torch.equal(again[:7], y[:7]) and torch.equal(again[8:], y[8:])
+
+
+@pytest.mark.parametrize("M,group", [(9, 32), (12, 128), (16, 64)])
+def test_rows_whose_inner_dimension_is_long(M, group, device):
+    w, dense, mag = make(6272, columns(device, 9), group, True, torch.bfloat16, device)
+    x = rows(M, 6272, torch.float16, device)
+    check(matvec(x, w), x, dense, 2 * mag)   # (6272 rows pass half as many groups again as the bound's 4096)

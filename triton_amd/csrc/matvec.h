@@ -360,7 +360,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
     }
 }
 
-// Several tiles of rows and many columns: a workgroup has MT tiles and 2 WN strips.  Its waves are WN pairs of strips times 8 / WN parts of K;
+// Many columns: a workgroup has MT tiles of 16 rows and 2 WN strips.  Its waves are WN pairs of strips times 8 / WN parts of K;
 // a block of x goes through LDS once for all waves of its part, two blocks deep, and with the codes is requested two blocks ahead.
 // (64 x 4096 x 131072: 269 us by matvec_rows_kernel, where x comes from the caches for every second strip, 125 so; 149 with three blocks
 // ahead, which leave room for one workgroup per CU.  The matrix products, the codes' arithmetic and LDS take about 40 us each.)
@@ -573,6 +573,8 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
       if (nb <= 6 && strips > 2 * cus) return launch_matvec_kept<XDT, PER, ZEROS, 6, 2>(a, cus, st);
     if (a.M <= 4) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, PER < 2 ? 2 : 1, 1>(a, st);
     if (a.M <= 8) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1, 2>(a, st);
+    // (16 x 8192 x 28672: 33 us, 43 by the next; 5 rows take 39 and 34)
+    if (strips >= 5 * cus) return launch_matvec_wide<XDT, PER, ZEROS, 1, 4>(a, st);
     return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1>(a, st);
   }
   // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
