@@ -9,14 +9,14 @@
 // What rounds to zero is not there at all: it cannot be drawn, and adds nothing to what top-k keeps.
 //
 // Five launches, three of them over (chunk of a row, row):
-//   extremes   the largest logit with its index, and the smallest;
+//   extremes   the largest logit (of greedy rows with its index) and the smallest;
 //   histogram  mass (and for top-k count) of the logits in 2048 bins of equal width between the two, or down to where w is zero;
 //   bounds     a workgroup per row finds in the histogram the few bins in which the ends of top-k, top-p and min-p and the token
 //              can lie;
 //   collect    gathers the logits of those, a few hundred of the whole vocabulary;
 //   finish     a workgroup per row sorts them and answers the questions exactly.
-// Rows of up to 4096 logits are sorted as they are, in one launch.  A row that has more than 4096 logits in those bins -- many
-// equal or nearly equal ones -- is searched by the bits of its keys (search_row): slower, but right for any row.
+// Where that is faster a workgroup goes through all of it for a row, in one launch (sample_whole).  A row that has more than 4096 logits in those
+// bins -- many equal or nearly equal ones -- is searched by the bits of its keys (search_row): slower, but right for any row.
 #include "common.h"
 
 namespace tamd {
@@ -25,7 +25,15 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / kWave;
 constexpr int kBins = 2048, kMost = 4096;   // candidates that are sorted
 constexpr int kChunk = 8192, kMaxChunks = 64;
+constexpr int kShort = 24000;
 constexpr int kRowsAtOnce = 4096;           // of one round of launches (the workspace holds as many)
+
+// Whether a workgroup does a row alone.  That takes about 9 us and one for every 2000 logits, as often as there are rows for a CU; the
+// five launches take 24 and one for every 1600 logits of a CU's share.  Measured: 1 row of 8192 13.7 and 24.0, of 32000 25.0 and 25.0,
+// of 65536 41 and 26; 256 rows of 65536 48 and 63.
+inline bool sample_whole(int R, int V, int cus) {
+  return V <= kShort || (int64_t)((R + cus - 1) / cus) * (18000 + V) <= 48000 + (int64_t)R * V / cus * 5 / 4;
+}
 
 struct RowSettings {
   double t;          // temperature
@@ -344,25 +352,31 @@ inline Workspace workspace_of(void *p, int rows) {
   return w;
 }
 
+// Largest element (its index for greedy rows only: that takes four times the instructions) and smallest key above -inf of a
+// workgroup's part of a row; every thread gets them.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, Workspace ws, int chunk) {
-  __shared__ uint64_t s_first[kWaves];
-  __shared__ uint32_t s_least[kWaves];
-  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
-  Chunk<DT> logits(a, r, c, chunk);
-  for (int b = c * kThreads + tid; b < kBins; b += gridDim.x * kThreads) ws.mass[(int64_t)r * kBins + b] = 0, ws.count[(int64_t)r * kBins + b] = 0;
-  if (c == 0 && tid == 0) ws.collected[r] = 0;
-  uint64_t first = 0;
-  uint32_t least = 0xFFFFFFFFu;
-  logits.each([&](const float *v, int i) {
+TAMD_DEVICE void extremes_of(Chunk<DT> &logits, bool greedy, uint64_t &first, uint32_t &least, uint64_t *s_first, uint32_t *s_least) {
+  const int tid = threadIdx.x;
+  first = 0, least = 0xFFFFFFFFu;
+  if (greedy) {
+    logits.each([&](const float *v, int i) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t key = ordered_bits(v[j]);
-      const uint64_t e = element_of(key, i + j);
-      first = e > first ? e : first;
-      least = key > kNothing && key < least ? key : least;
-    }
-  });
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t e = element_of(ordered_bits(v[j]), i + j);
+        first = e > first ? e : first;
+      }
+    });
+  } else {
+    float most = -__builtin_inff(), fewest = __builtin_inff();
+    logits.each([&](const float *v, int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        most = __builtin_fmaxf(most, v[j]);
+        fewest = __builtin_fminf(fewest, v[j] > -__builtin_inff() ? v[j] : __builtin_inff());
+      }
+    });
+    first = element_of(ordered_bits(most), 0), least = ordered_bits(fewest);
+  }
 #pragma unroll
   for (int o = 1; o < kWave; o *= 2) {
     const uint64_t e = __shfl_xor(first, o);
@@ -372,13 +386,25 @@ __global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, 
   }
   if (tid % kWave == 0) s_first[tid / kWave] = first, s_least[tid / kWave] = least;
   sync_threads();
-  if (tid == 0) {
-    for (int w = 0; w < kWaves; ++w) {
-      first = s_first[w] > first ? s_first[w] : first;
-      least = s_least[w] < least ? s_least[w] : least;
-    }
-    ws.first[r * kMaxChunks + c] = first, ws.least[r * kMaxChunks + c] = least;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    first = s_first[w] > first ? s_first[w] : first;
+    least = s_least[w] < least ? s_least[w] : least;
   }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void extremes_kernel(tamd_sample_args a, Workspace ws, int chunk) {
+  __shared__ uint64_t s_first[kWaves];
+  __shared__ uint32_t s_least[kWaves];
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  Chunk<DT> logits(a, r, c, chunk);
+  for (int b = c * kThreads + tid; b < kBins; b += gridDim.x * kThreads) ws.mass[(int64_t)r * kBins + b] = 0, ws.count[(int64_t)r * kBins + b] = 0;
+  if (c == 0 && tid == 0) ws.collected[r] = 0;
+  uint64_t first;
+  uint32_t least;
+  extremes_of<DT>(logits, settings_of(a, r).greedy, first, least, s_first, s_least);
+  if (tid == 0) ws.first[r * kMaxChunks + c] = first, ws.least[r * kMaxChunks + c] = least;
 }
 
 // A row's extremes from its chunks', by every thread.
@@ -393,6 +419,28 @@ TAMD_DEVICE void row_extremes(const Workspace &ws, int r, int chunks, uint64_t &
     first = e > first ? e : first;
     least = l < least ? l : least;
   }
+}
+
+// Adds a workgroup's part of a row to a histogram in LDS.
+template <int DT>
+TAMD_DEVICE void add_to_histogram(Chunk<DT> &logits, const RowScale &scale, bool counting, uint64_t *mass, uint32_t *count) {
+  // (no branch but around the additions: a logit at a time, each waiting for its power, 64 rows of 131072 took 14.7 us and 256 of 100000
+  // 31.0, so 14.4 and 30.5: the additions in LDS and the logits are what is left)
+  logits.each([&](const float *v, int) {
+    double y[4];
+    uint64_t units[4];
+    int bin[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = scale.y_of(v[j]), bin[j] = scale.bin_of(y[j]), units[j] = scale.units_of(y[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (scale.counts(y[j])) atomicAdd((unsigned long long *)&mass[bin[j]], (unsigned long long)units[j]);
+    if (counting) {   // (only top-k asks for counts)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (scale.counts(y[j])) atomicAdd(&count[bin[j]], 1u);
+    }
+  });
 }
 
 template <int DT>
@@ -411,23 +459,7 @@ __global__ __launch_bounds__(kThreads) void histogram_kernel(tamd_sample_args a,
   for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
   const RowScale scale(key_of(first), least, s.t, a.V, powers);
   sync_threads();
-  // (no branch but around the additions: a logit at a time, each waiting for its power, 64 rows of 131072 took 14.7 us and 256 of 100000
-  // 31.0, so 14.4 and 30.5: the additions in LDS and the logits are what is left)
-  logits.each([&](const float *v, int) {
-    double y[4];
-    uint64_t units[4];
-    int bin[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = scale.y_of(v[j]), bin[j] = scale.bin_of(y[j]), units[j] = scale.units_of(y[j]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (scale.counts(y[j])) atomicAdd((unsigned long long *)&mass[bin[j]], (unsigned long long)units[j]);
-    if (s.top_k) {   // (nothing else asks for counts)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (scale.counts(y[j])) atomicAdd(&count[bin[j]], 1u);
-    }
-  });
+  add_to_histogram<DT>(logits, scale, s.top_k != 0, mass, count);
   sync_threads();
   for (int b = tid; b < kBins; b += kThreads)
     if (mass[b]) {
@@ -506,10 +538,20 @@ TAMD_DEVICE void sort_elements(uint64_t *list, int n, uint32_t *rank) {
     }
 }
 
-// The token, from n <= kMost sorted candidates.  before_mass / before_rank: what lies in front of every bin (null: the candidates are the
-// whole row); min_lo, min_hi: the bins in which min-p ends, min_mass: what lies in front of them.
-TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const uint64_t *list, int n, const uint64_t *before_mass, const uint32_t *before_rank,
-                           uint64_t total_mass, uint32_t total_count, int min_lo, int min_hi, uint64_t min_mass, uint64_t *bin_mass, uint32_t *bin_rank, Shared &sh) {
+// What is known of a row in front of the gathering.
+struct Bounds {
+  int from[4], to[4];      // bins of the candidates: the ends of top-k, top-p and min-p, and the token
+  uint64_t mass, min_mass; // of the row; in front of the bins in which min-p ends
+  double top, to_y, to_bin;
+  uint32_t count;
+  int done;                // the token is known
+};
+static_assert(sizeof(Bounds) <= 96);
+
+// The token, from n <= kMost sorted candidates.  before_mass / before_rank: what lies in front of every bin; bin_mass / bin_rank: room for as
+// many, or the same.
+TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const Bounds &b, const uint64_t *list, int n, const uint64_t *before_mass,
+                           const uint32_t *before_rank, uint64_t *bin_mass, uint32_t *bin_rank, Shared &sh) {
   constexpr int PER = kMost / kThreads;
   const int tid = threadIdx.x;
   uint64_t units[PER], before[PER], run = 0, enough = 0;
@@ -524,28 +566,26 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
     bin[j] = scale.counts(y) ? scale.bin_of(y) : -1;
     before[j] = run;
     run += units[j];
-    enough += bin[j] >= min_lo && bin[j] <= min_hi && units[j] >= least ? units[j] : 0;
+    enough += bin[j] >= b.from[2] && bin[j] <= b.to[2] && units[j] >= least ? units[j] : 0;
   }
   const uint64_t start = block_scan<uint64_t>(run, sh.tmp) - run;
-  if (before_mass) {   // the first candidate of a bin leaves what the running sums of the bin's candidates lack
+  // the first candidate of a bin leaves what the running sums of the bin's candidates lack
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int i = PER * tid + j;
-      if (bin[j] >= 0 && (i == 0 || scale.bin_of(scale.y_of(logit_of(key_of(list[i - 1])))) != bin[j])) {
-        bin_mass[bin[j]] = before_mass[bin[j]] - (start + before[j]);
-        if (s.top_k) bin_rank[bin[j]] = before_rank[bin[j]] - (uint32_t)i;
-      }
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * tid + j;
+    if (bin[j] >= 0 && (i == 0 || scale.bin_of(scale.y_of(logit_of(key_of(list[i - 1])))) != bin[j])) {
+      bin_mass[bin[j]] = before_mass[bin[j]] - (start + before[j]);
+      if (s.top_k) bin_rank[bin[j]] = before_rank[bin[j]] - (uint32_t)i;
     }
   }
-  if (tid == 0) sh.sum = total_mass, sh.token = -1;
+  if (tid == 0) sh.sum = b.mass, sh.token = -1;
   sync_threads();
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const bool adds = before_mass && bin[j] >= 0;
-    before[j] += start + (adds ? bin_mass[bin[j]] : 0);
-    rank[j] = (uint32_t)(PER * tid + j) + (adds && s.top_k ? bin_rank[bin[j]] : 0u);
+    before[j] += start + (bin[j] >= 0 ? bin_mass[bin[j]] : 0);
+    rank[j] = (uint32_t)(PER * tid + j) + (bin[j] >= 0 && s.top_k ? bin_rank[bin[j]] : 0u);
   }
-  if (s.top_k && (uint32_t)s.top_k < total_count) {
+  if (s.top_k && (uint32_t)s.top_k < b.count) {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (bin[j] >= 0 && rank[j] == (uint32_t)s.top_k - 1) sh.sum = before[j] + units[j];
@@ -561,7 +601,7 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const ui
   }
   uint64_t sum = sh.sum;
   if (s.min_p > 0.0) {
-    const uint64_t has = min_mass + block_sum<uint64_t>(enough, sh.tmp);
+    const uint64_t has = b.min_mass + block_sum<uint64_t>(enough, sh.tmp);
     sum = has < sum ? has : sum;
   }
   const uint64_t target = token_target(s.u, sum);
@@ -587,44 +627,18 @@ TAMD_DEVICE int bin_reaching(const T *before, T target, int &slot) {
   return found;
 }
 
-// What the last two launches are told about a row.
-struct Bounds {
-  int from[4], to[4];      // bins of the candidates: the ends of top-k, top-p and min-p, and the token
-  uint64_t mass, min_mass; // of the row; in front of the bins in which min-p ends
-  double top, to_y, to_bin;
-  uint32_t count;
-  int done;                // the token is known
-};
-static_assert(sizeof(Bounds) <= 96);
-
-// The bins in which the ends of what is kept and the token can lie: lo and hi enclose the sum of what is kept.  The row's histogram
-// becomes what lies in front of every bin.  (In a launch of its own: done by every workgroup of the next two, as at first, these took
-// 40 us for 64 rows of 131072; the three now take 33, for one row 18 instead of 21.)
-__global__ __launch_bounds__(kThreads) void bounds_kernel(tamd_sample_args a, Workspace ws, int chunks) {
-  __shared__ uint64_t mass[kBins + 1];
-  __shared__ uint32_t rank[kBins + 1];
-  __shared__ Shared sh;
+// The bins in which the ends of what is kept and the token can lie: lo and hi enclose the sum of what is kept.  A thread brings two bins of
+// the row's histogram; mass and rank become what lies in front of every bin.
+TAMD_DEVICE Bounds find_bounds(const RowSettings &s, const RowScale &scale, uint64_t m0, uint64_t m1, uint32_t n0, uint32_t n1, uint64_t *mass, uint32_t *rank,
+                               Shared &sh) {
   static_assert(kBins == 2 * kThreads);
-  const int r = blockIdx.x, tid = threadIdx.x;
-  const int64_t h = (int64_t)r * kBins + 2 * tid;
-  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1];
-  const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1];
-  uint64_t first;
-  uint32_t least;
-  row_extremes(ws, r, chunks, first, least);
-  const RowSettings s = settings_of(a, r);
-  Bounds *out = (Bounds *)ws.bounds + r;
-  if (s.greedy || key_of(first) <= kNothing) {
-    if (tid == 0) out->done = 1, a.tokens[r] = key_of(first) <= kNothing ? -1 : index_of(first);
-    return;
-  }
-  const RowScale scale(key_of(first), least, s.t, a.V, nullptr);
+  const int tid = threadIdx.x;
   const uint64_t upto = block_scan<uint64_t>(m0 + m1, sh.tmp);
-  ws.mass[h] = mass[2 * tid] = upto - m0 - m1, ws.mass[h + 1] = mass[2 * tid + 1] = upto - m1;
+  mass[2 * tid] = upto - m0 - m1, mass[2 * tid + 1] = upto - m1;
   if (tid == kThreads - 1) mass[kBins] = upto;
   if (s.top_k) {
     const uint32_t n = block_scan<uint32_t>(n0 + n1, (uint32_t *)sh.tmp);
-    ws.count[h] = rank[2 * tid] = n - n0 - n1, ws.count[h + 1] = rank[2 * tid + 1] = n - n1;
+    rank[2 * tid] = n - n0 - n1, rank[2 * tid + 1] = n - n1;
     if (tid == kThreads - 1) rank[kBins] = n;
   }
   sync_threads();
@@ -654,22 +668,38 @@ __global__ __launch_bounds__(kThreads) void bounds_kernel(tamd_sample_args a, Wo
   }
   b.from[3] = bin_reaching<uint64_t>(mass, token_target(s.u, lo), sh.at[0]);
   b.to[3] = lo == hi ? b.from[3] : bin_reaching<uint64_t>(mass, token_target(s.u, hi), sh.at[1]);
+  return b;
+}
+
+// (In a launch of its own: done by every workgroup of the next two, as at first, these took 40 us for 64 rows of 131072; the three
+// now take 26, for one row 18 instead of 21.)
+__global__ __launch_bounds__(kThreads) void bounds_kernel(tamd_sample_args a, Workspace ws, int chunks) {
+  __shared__ uint64_t mass[kBins + 1];
+  __shared__ uint32_t rank[kBins + 1];
+  __shared__ Shared sh;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const int64_t h = (int64_t)r * kBins + 2 * tid;
+  const uint64_t m0 = ws.mass[h], m1 = ws.mass[h + 1];
+  const uint32_t n0 = ws.count[h], n1 = ws.count[h + 1];
+  uint64_t first;
+  uint32_t least;
+  row_extremes(ws, r, chunks, first, least);
+  const RowSettings s = settings_of(a, r);
+  Bounds *out = (Bounds *)ws.bounds + r;
+  if (s.greedy || key_of(first) <= kNothing) {
+    if (tid == 0) out->done = 1, a.tokens[r] = key_of(first) <= kNothing ? -1 : index_of(first);
+    return;
+  }
+  const RowScale scale(key_of(first), least, s.t, a.V, nullptr);
+  const Bounds b = find_bounds(s, scale, m0, m1, n0, n1, mass, rank, sh);
+  ws.mass[h] = mass[2 * tid], ws.mass[h + 1] = mass[2 * tid + 1];
+  if (s.top_k) ws.count[h] = rank[2 * tid], ws.count[h + 1] = rank[2 * tid + 1];
   if (tid == 0) *out = b;
 }
 
-// A chunk's candidates, gathered in LDS first: an atomic on the row's counter takes a trip to memory, and they take turns (one per
-// candidate: 282 us for 64 rows of 131072).  More than kMost are only counted.
+// Gathers the candidates of a workgroup's part of a row in LDS; more than kMost are only counted.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, Workspace ws, int chunk) {
-  __shared__ uint64_t list[kMost];
-  __shared__ Shared sh;
-  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
-  Chunk<DT> logits(a, r, c, chunk);
-  const Bounds b = ((const Bounds *)ws.bounds)[r];
-  if (b.done) return;
-  const RowScale scale(b.top, b.to_y, b.to_bin, a.V, nullptr);
-  if (tid == 0) sh.n = 0;
-  sync_threads();
+TAMD_DEVICE void gather(Chunk<DT> &logits, const Bounds &b, const RowScale &scale, uint64_t *list, Shared &sh) {
   uint32_t from[4], more[4];   // (an empty range: from = kBins, and nothing is as large)
 #pragma unroll
   for (int q = 0; q < 4; ++q) from[q] = (uint32_t)b.from[q], more[q] = b.to[q] > b.from[q] ? (uint32_t)(b.to[q] - b.from[q]) : 0u;
@@ -693,6 +723,22 @@ __global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, W
         }
     }
   });
+}
+
+// (In LDS first: an atomic on the row's counter takes a trip to memory, and they take turns; one per candidate took 282 us for 64 rows
+// of 131072.)
+template <int DT>
+__global__ __launch_bounds__(kThreads) void collect_kernel(tamd_sample_args a, Workspace ws, int chunk) {
+  __shared__ uint64_t list[kMost];
+  __shared__ Shared sh;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+  Chunk<DT> logits(a, r, c, chunk);
+  const Bounds b = ((const Bounds *)ws.bounds)[r];
+  if (b.done) return;
+  const RowScale scale(b.top, b.to_y, b.to_bin, a.V, nullptr);
+  if (tid == 0) sh.n = 0;
+  sync_threads();
+  gather<DT>(logits, b, scale, list, sh);
   sync_threads();
   const uint32_t n = sh.n, stored = n < kMost ? n : kMost;
   if (n == 0) return;
@@ -726,47 +772,65 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Wo
     const int n = (int)collected;
     for (int i = tid; i < n; i += kThreads) list[i] = ws.candidates[(int64_t)r * kMost + i];
     sort_elements(list, n, bin_rank);
-    token = pick_among(s, scale, list, n, ws.mass + (int64_t)r * kBins, ws.count + (int64_t)r * kBins, b.mass, b.count, b.from[2], b.to[2], b.min_mass, bin_mass, bin_rank, sh);
+    token = pick_among(s, scale, b, list, n, ws.mass + (int64_t)r * kBins, ws.count + (int64_t)r * kBins, bin_mass, bin_rank, sh);
   }
   if (tid == 0) a.tokens[r] = token;
 }
 
-// Rows of up to kMost logits: all of them are candidates.
+// All of it for a row, in LDS: three reads of the row, and what bounds it is their arithmetic, some 70 instructions a logit.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void short_row_kernel(tamd_sample_args a) {
-  __shared__ uint64_t list[kMost];
-  __shared__ uint32_t rank[kCounted];
+__global__ __launch_bounds__(kThreads) void whole_row_kernel(tamd_sample_args a) {
+  __shared__ uint64_t list[kMost], mass[kBins + 1];
+  __shared__ uint32_t rank[kBins + 1], places[kCounted];
   __shared__ double powers[256];
   __shared__ Shared sh;
+  static_assert(kCounted >= kWaves);
   const int r = blockIdx.x, tid = threadIdx.x;
   const RowSettings s = settings_of(a, r);
-  make_powers(powers, a.V);
-  for (int i = tid; i < a.V; i += kThreads) list[i] = element_of(key_at<DT>(a.logits, r * a.logits_stride + i), i);
-  sort_elements(list, a.V, rank);
-  const uint32_t top = key_of(list[0]);
-  int token = -1;
-  if (top > kNothing) {
-    if (s.greedy) {
-      token = index_of(list[0]);
-    } else {
-      const RowScale scale(top, top, s.t, a.V, powers);   // (one bin)
-      uint64_t mine = 0;
-      for (int i = tid; i < a.V; i += kThreads) mine += scale.units(key_of(list[i]));
-      const uint64_t total = block_sum<uint64_t>(mine, sh.tmp);
-      token = pick_among(s, scale, list, a.V, nullptr, nullptr, total, (uint32_t)a.V, 0, kBins, 0, nullptr, nullptr, sh);
-    }
+  uint64_t first;
+  uint32_t least;
+  {
+    Chunk<DT> logits(a, r, 0, a.V);
+    mass[2 * tid] = mass[2 * tid + 1] = 0, rank[2 * tid] = rank[2 * tid + 1] = 0;
+    if (tid == 0) sh.n = 0;
+    make_powers(powers, a.V);
+    extremes_of<DT>(logits, s.greedy, first, least, sh.tmp, places);
+  }
+  if (s.greedy || key_of(first) <= kNothing) {
+    if (tid == 0) a.tokens[r] = key_of(first) <= kNothing ? -1 : index_of(first);
+    return;
+  }
+  const RowScale scale(key_of(first), least, s.t, a.V, powers);
+  {
+    Chunk<DT> logits(a, r, 0, a.V);
+    add_to_histogram<DT>(logits, scale, s.top_k != 0, mass, rank);
+  }
+  Chunk<DT> logits(a, r, 0, a.V);
+  sync_threads();
+  const uint64_t m0 = mass[2 * tid], m1 = mass[2 * tid + 1];
+  const uint32_t n0 = rank[2 * tid], n1 = rank[2 * tid + 1];
+  const Bounds b = find_bounds(s, scale, m0, m1, n0, n1, mass, rank, sh);   // (a barrier before either is written)
+  gather<DT>(logits, b, scale, list, sh);
+  sync_threads();
+  int token;
+  if (sh.n > kMost) {
+    token = search_row<DT>(a, r, s, scale, list, sh);
+  } else {
+    const int n = (int)sh.n;
+    sort_elements(list, n, places);
+    token = pick_among(s, scale, b, list, n, mass, rank, mass, rank, sh);
   }
   if (tid == 0) a.tokens[r] = token;
 }
 
 template <int DT>
 int launch_sample(const tamd_sample_args &args, hipStream_t st) {
-  if (args.V <= kMost) {
-    short_row_kernel<DT><<<args.R, kThreads, 0, st>>>(args);
-    return launch_status();
-  }
   int cus = 0;
   if (int rc = cu_count(cus)) return rc;
+  if (sample_whole(args.R, args.V, cus)) {
+    whole_row_kernel<DT><<<args.R, kThreads, 0, st>>>(args);
+    return launch_status();
+  }
   for (int r = 0; r < args.R; r += kRowsAtOnce) {
     tamd_sample_args a = args;
     a.R = args.R - r < kRowsAtOnce ? args.R - r : kRowsAtOnce;
@@ -800,7 +864,7 @@ using namespace tamd;
 
 extern "C" int64_t tamd_sample_workspace(int R, int V) {
   if (R < 0 || V < 0) return TAMD_E_INVALID;
-  return V <= kMost ? 16 : (R < kRowsAtOnce ? R : kRowsAtOnce) * kRowBytes + 16;
+  return V <= kShort ? 16 : (R < kRowsAtOnce ? R : kRowsAtOnce) * kRowBytes + 16;
 }
 
 extern "C" int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream) {
