@@ -42,6 +42,7 @@ struct MoeTables {
   uint8_t token[kMoeSlots];         // of a row of h
 };
 constexpr int64_t kMoeTableBytes = (sizeof(MoeTables) + 255) / 256 * 256;
+constexpr int kMoeShares = 256;   // workgroups between which the down projection is dealt out; two partial sums of 16 columns each, behind h
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -406,6 +407,16 @@ struct MoeDownLds {
   uint8_t token[kMoeSlots];
 };
 static_assert(sizeof(MoeDownLds) % 16 == 0);
+// The experts of all strips of 16 columns, strip by strip, are dealt out evenly to up to `shares` workgroups, none of which has none:
+// where one begins, and whose an expert of a strip is.
+struct MoeDeal {
+  uint32_t items, shares;
+  TAMD_DEVICE MoeDeal(uint32_t n_active, int N, uint32_t shares_) : items(n_active * ((uint32_t)N / 16u)), shares(shares_ < items ? shares_ : items) {}
+  TAMD_DEVICE uint32_t begin(uint32_t w) const { return (uint32_t)((uint64_t)items * w / shares); }
+  TAMD_DEVICE uint32_t owner(uint32_t at) const { return (uint32_t)((((uint64_t)at + 1u) * shares - 1u) / items); }
+};
+__host__ __device__ inline int64_t moe_partial_at(int64_t slots, int64_t inter) { return kMoeTableBytes + (slots * inter * 4 + 15) / 16 * 16; }
+
 template <int NB, int RC>
 constexpr int kMoeDownPitch = 256 * NB + 16;   // bytes of a row of h in a wave's buffer (rows 16 bytes apart on the banks)
 
@@ -417,7 +428,7 @@ constexpr int kMoeDownPitch = 256 * NB + 16;   // bytes of a row of h in a wave'
 // h comes as a few dense requests and goes through LDS, a buffer per wave, to where the MFMAs want it: requested in their layout
 // it takes four requests per block, most lanes of which bring nothing, and a request costs the CU about 20 cycles whatever it
 // brings (16 tokens of 128 experts of 2880 x 2880: 90 us, 50 without these requests, TODO now).
-template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D, bool ROUNDS>
+template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D, bool ROUNDS, bool DEALT>
 __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
   typedef ExpertWeights<BLOCKS, SHUFFLED> Weights;
@@ -433,6 +444,13 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
   const MoeTables *tab = (const MoeTables *)a.workspace;
   const int slots = T * a.n_picks;
   const uint32_t n_active = (uint32_t)__builtin_amdgcn_readfirstlane(tab->n_active);
+  uint32_t strip = blockIdx.x, ask_at = 0, left = n_active;   // from this expert of this strip on, so many experts of strips
+  if constexpr (DEALT) {
+    const MoeDeal deal(n_active, N, gridDim.x);
+    if (blockIdx.x >= deal.shares) return;
+    const uint32_t begin = deal.begin(blockIdx.x);
+    strip = begin / n_active, ask_at = begin - strip * n_active, left = deal.begin(blockIdx.x + 1) - begin;
+  }
   if (tid < slots) {   // (no more experts than slots)
     s.expert[tid] = tab->expert[tid], s.start[tid] = (uint32_t)tid < n_active ? tab->start[tid] : (uint16_t)slots;
     s.gate[tid] = tab->gate[tid], s.pick[tid] = tab->pick[tid], s.token[tid] = tab->token[tid];
@@ -441,9 +459,9 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
   for (int i = tid; i < W * T * 16; i += 64 * W) sums[i] = 0.f;
   sync_threads();
   const Buffer planes((const uint8_t *)a.workspace + kMoeTableBytes, (int64_t)slots * 4 * K);
-  const uint32_t strip = blockIdx.x >> 1, f = blockIdx.x & 1u, n_kb = (uint32_t)(K + 127) / 128u, groups = (uint32_t)K / 32u;
+  const uint32_t n_kb = (uint32_t)(K + 127) / 128u, groups = (uint32_t)K / 32u;
 
-  // ---- a stage is an expert and, with ROUNDS, 8 NB blocks of K from k0 on; these are cut evenly.  What a lane adds to the offsets
+  // ---- a stage is an expert of a strip and, with ROUNDS, 8 NB blocks of K from k0 on; these are cut evenly.  What a lane adds to the offsets
   // depends on the place in K alone: made once, or once per stage with ROUNDS.
   const auto rows_at = [&](uint32_t at, uint32_t &row, uint32_t &rows) {
     row = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.start[at]);
@@ -453,7 +471,8 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
     uint32_t kb0, code_off[NB], scale_off[NS], x_off[XR];
   };
   const Weights form(a.down, 0, K, N);
-  const auto place_at = [&](uint32_t k0) {
+  const auto place_at = [&](uint32_t of_16, uint32_t k0) {
+    const uint32_t strip = of_16 >> 1, f = of_16 & 1u;
     Place p;
     const uint32_t here = n_kb - k0 < 8u * NB ? n_kb - k0 : 8u * NB, from = here * (uint32_t)wave / W, n = here * (uint32_t)(wave + 1) / W - from;
     p.kb0 = k0 + from;
@@ -487,24 +506,25 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  uint32_t ask_at = 0, ask_k0 = 0, now_at = 0, now_k0 = 0;
-  const Place fixed = place_at(0);
+  // where the next request and the next product are
+  uint32_t asked = strip, now_at = ask_at, ask_k0 = 0, now_k0 = 0, to_ask = left, to_do = left;
+  Place fixed = place_at(asked, 0);
   const auto request = [&](Stage &st) {
-    const bool live = ask_at < n_active;
+    const bool live = to_ask > 0;
     const uint32_t at = live ? ask_at : 0u;
     Weights w(a.down, __builtin_amdgcn_readfirstlane((int)s.expert[at]), K, N);
     if (!live) w.w = w.sc = Buffer(a.down.w, 0);   // (empty buffers: zeros)
     uint32_t row, rows;
     rows_at(at, row, rows);
-    const Place p = ROUNDS ? place_at(ask_k0) : fixed;
+    const Place p = ROUNDS ? place_at(asked, ask_k0) : fixed;
     request_x(st.x, p, row, live ? rows : 0u);
-    const uint32_t code_s = form.code_block(strip, p.kb0);
+    const uint32_t code_s = form.code_block(asked >> 1, p.kb0);
 #pragma unroll
     for (int i = 0; i < NB; ++i) {   // (one order wherever this is expanded: the waits are counted from it)
       st.q[i] = w.w.template load16<2>(p.code_off[i], code_s + (BLOCKS ? 4096u : 64u) * i);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const uint32_t scale_s = SHUFFLED ? form.scale_block(strip, p.kb0 & ~1u) : form.scale_block(strip, p.kb0);
+    const uint32_t scale_s = SHUFFLED ? form.scale_block(asked >> 1, p.kb0 & ~1u) : form.scale_block(asked >> 1, p.kb0);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       if constexpr (SHUFFLED) st.s[i] = w.sc.load4(p.scale_off[i], scale_s + 256u * i);
@@ -513,17 +533,25 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
     }
     if (ROUNDS) {
       ask_k0 += 8 * NB;
-      if (ask_k0 >= n_kb) ask_k0 = 0, ++ask_at;
-    } else {
-      ++ask_at;
+      if (ask_k0 < n_kb) return;
+      ask_k0 = 0;
+    }
+    ++ask_at;
+    if (live) --to_ask;
+    if constexpr (DEALT) {
+      if (ask_at >= n_active) {
+        ask_at = 0, ++asked;
+        if (!ROUNDS) fixed = place_at(asked, 0);
+      }
     }
   };
   const uint32_t a_row = (c & (2u * RC - 1u)) * PITCH + 64u * h;   // (rows past the buffer's repeat: no one reads their sums)
   const auto multiply = [&](const Stage &st) {
-    const bool live = now_at < n_active;
+    const bool live = to_do > 0;
+    const uint32_t f = strip & 1u;
     uint32_t row, rows;
     rows_at(live ? now_at : 0u, row, rows);
-    const Place p = ROUNDS ? place_at(now_k0) : fixed;
+    const Place p = ROUNDS ? place_at(strip, now_k0) : fixed;   // (of `fixed` what lies along K is used: the same for all strips)
     const auto tile = [&](const u32x4_t (&x)[XR], uint32_t t0) {
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
@@ -562,18 +590,12 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
         tile(x, t0);
       }
     }
-    if (ROUNDS) {
-      now_k0 += 8 * NB;
-      if (now_k0 >= n_kb) now_k0 = 0, ++now_at;
-    } else {
-      ++now_at;
-    }
   };
 
   // ---- the biases of this thread's outputs by their gate weights, eight picks requested at a time
   const auto bias_of = [&](int i) {
     float v = 0.f;
-    const int64_t n = 32 * (int64_t)strip + 2 * (i & 15) + f;
+    const int64_t n = 32 * (int64_t)(strip >> 1) + 2 * (i & 15) + (strip & 1u);
     for (int j0 = 0; j0 < a.n_picks; j0 += 8) {
       float b[8], g[8];
 #pragma unroll
@@ -588,33 +610,79 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
     return v;
   };
   static_assert(kMoeTokens * 16 <= 2 * 64 * W);   // two outputs per thread at most
+  bool from_start = !DEALT || now_at == 0;   // the strip's first expert is this workgroup's
   float from_bias[2] = {0.f, 0.f};
-  if (a.down.bias) {
+  if (a.down.bias && from_start) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
       if (tid + m * 64 * W < T * 16) from_bias[m] = bias_of(tid + m * 64 * W);
   }
+  // Behind the strip's last expert here: the waves' sums go to y, or, where other workgroups have experts of it, to the workspace.
+  float *const partial = (float *)((uint8_t *)a.workspace + moe_partial_at(slots, K)) + (int64_t)blockIdx.x * 2 * (T * 16);
+  const auto finish = [&](bool last) {
+    sync_threads();
+    const bool whole = !DEALT || (from_start && now_at == n_active);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int i = tid + m * 64 * W;
+      if (i < T * 16) {
+        float v = from_bias[m];
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += sums[w * T * 16 + i];
+        if (whole) store_any(a.y, XDT, (i >> 4) * a.y_stride_m + 32 * (int64_t)(strip >> 1) + 2 * (i & 15) + (strip & 1u), v);
+        else partial[(from_start ? T * 16 : 0) + i] = v;
+        if (!last) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) sums[w * T * 16 + i] = 0.f;
+        }
+      }
+    }
+    if (!last) {
+      ++strip, now_at = 0, from_start = true;
+      if (a.down.bias) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+          if (tid + m * 64 * W < T * 16) from_bias[m] = bias_of(tid + m * 64 * W);
+      }
+      sync_threads();
+    }
+  };
 
   Stage st[D];
 #pragma unroll
   for (int d = 0; d < D; ++d) request(st[d]);
-  while (now_at < n_active) {
+  while (to_do > 0) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       multiply(st[d]);
       request(st[d]);
+      if (to_do > 0) {
+        if (ROUNDS) now_k0 += 8 * NB;
+        if (!ROUNDS || now_k0 >= n_kb) {
+          now_k0 = 0, ++now_at, --to_do;
+          if constexpr (DEALT)
+            if (to_do > 0 && now_at == n_active) finish(false);
+        }
+      }
     }
   }
-  sync_threads();
-#pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const int i = tid + m * 64 * W;
-    if (i < T * 16) {
-      float v = from_bias[m];
-#pragma unroll
-      for (int w = 0; w < W; ++w) v += sums[w * T * 16 + i];
-      store_any(a.y, XDT, (i >> 4) * a.y_stride_m + 32 * (int64_t)strip + 2 * (i & 15) + f, v);
-    }
+  finish(true);
+}
+
+// Adds up what several workgroups have of 16 columns; those that one has alone are in y already.
+template <int XDT>
+__global__ __launch_bounds__(256) void moe_join_kernel(tamd_moe_layer_args a, uint32_t shares) {
+  const MoeTables *tab = (const MoeTables *)a.workspace;
+  const uint32_t n_active = (uint32_t)__builtin_amdgcn_readfirstlane(tab->n_active), strip = blockIdx.x;
+  const MoeDeal deal(n_active, a.hidden, shares);
+  const uint32_t from = deal.owner(strip * n_active), to = deal.owner(strip * n_active + n_active - 1u);
+  if (from == to) return;
+  const int outs = a.n_tokens * 16;
+  const float *const partial = (const float *)((const uint8_t *)a.workspace + moe_partial_at(a.n_tokens * a.n_picks, a.inter));
+  for (int i = threadIdx.x; i < outs; i += 256) {
+    float v = partial[(int64_t)(2 * from + 1) * outs + i];
+    for (uint32_t w = from + 1; w <= to; ++w) v += partial[(int64_t)(2 * w) * outs + i];
+    store_any(a.y, XDT, (i >> 4) * a.y_stride_m + 32 * (int64_t)(strip >> 1) + 2 * (i & 15) + (strip & 1u), v);
   }
 }
 
@@ -654,12 +722,21 @@ int launch_moe_up(const tamd_moe_layer_args &a, hipStream_t st) {
 
 template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D>
 int launch_moe_down_of(const tamd_moe_layer_args &a, hipStream_t st) {
-  const bool rounds = 8 * NB < (a.inter + 127) / 128;
-  const auto kernel = rounds ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, true> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, false>;
+  int cus = 0;
+  if (int rc = cu_count(cus)) return rc;
+  // One strip per workgroup, or the experts of all strips dealt out: where nine experts or more of a strip that no CU has to do meanwhile are
+  // saved the join costs less.  16 tokens of 128 experts of 2880 x 2880 (19 saved) take 129 us and 126, 32 of 32 (10) 138 and 122,
+  // 64 of 128 of 512 x 1024 (96) 129 and 74, but 2 of 64 of 1024 x 2048 (8) 23 and 26, one of 2880 x 2880 (1) 22 and 27.
+  const int64_t strips = a.hidden / 16, slots = (int64_t)a.n_tokens * a.n_picks, most = slots < a.n_experts ? slots : a.n_experts;
+  const int64_t shares = cus < kMoeShares ? cus : kMoeShares;
+  const bool rounds = 8 * NB < (a.inter + 127) / 128, dealt = ((strips + shares - 1) / shares * shares - strips) * most >= 9 * shares;
+  const auto kernel = dealt ? (rounds ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, true, true> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, false, true>)
+                            : (rounds ? moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, true, false> : moe_down_kernel<XDT, BLOCKS, SHUFFLED, NB, RC, D, false, false>);
   const size_t lds = sizeof(MoeDownLds) + 8 * 2 * RC * kMoeDownPitch<NB, RC> + (size_t)a.n_tokens * 8 * 16 * 4;
   if (lds > 64 * 1024)
     if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
-  kernel<<<dim3((unsigned)(a.hidden / 16)), 512, lds, st>>>(a);
+  kernel<<<(unsigned)(dealt ? shares : strips), 512, lds, st>>>(a);
+  if (dealt) moe_join_kernel<XDT><<<(unsigned)strips, 256, 0, st>>>(a, (uint32_t)shares);
   return launch_status();
 }
 

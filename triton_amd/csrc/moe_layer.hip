@@ -28,7 +28,7 @@ using namespace tamd;
 
 extern "C" int64_t tamd_moe_layer_workspace(int n_tokens, int n_picks, int inter) {
   if (n_tokens < 0 || n_picks < 0 || inter < 0) return TAMD_E_INVALID;
-  return kMoeTableBytes + (int64_t)n_tokens * n_picks * inter * 4;
+  return moe_partial_at((int64_t)n_tokens * n_picks, inter) + (int64_t)kMoeShares * 2 * n_tokens * 16 * 4;
 }
 
 extern "C" int tamd_moe_layer(const tamd_moe_layer_args *args, size_t args_size, void *stream) {
