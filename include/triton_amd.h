@@ -385,7 +385,7 @@ int tamd_swiglu(const void *a, int dtype, int64_t M, int64_t N_out, int64_t a_st
                 int64_t out_stride_m, float alpha, float limit, int has_limit, void *stream);
 
 /*
- * A whole mixture-of-experts layer for a few tokens, in two launches (no counterpart in the reference, which chains topk,
+ * A whole mixture-of-experts layer for a few tokens, in two or three launches (no counterpart in the reference, which chains topk,
  * metadata, two products and a reduction):
  *
  *   y[t] = sum_j g[t,j] * (h[t,j] W_down[e] + b_down[e]),   h[t,j] = swiglu(x[t] W_up[e] + b_up[e]),   e = pick j of token t

@@ -16,7 +16,7 @@ extern "C" int tamd_matvec(const tamd_matvec_args *args, size_t args_size, void 
   if (a.M == 0 || a.N == 0) return 0;
   if (!a.x || !a.codes || !a.scales || !a.y || a.x_stride_m < 0 || a.y_stride_m < 0) return TAMD_E_INVALID;
   if (!aligned(a.x, 16) || a.x_stride_m % 8 != 0 || !aligned(a.codes, 16) || !aligned(a.scales, 16) || !aligned(a.zeros, 16)) return TAMD_E_ALIGNMENT;
-  if (a.K > (1 << 20) || a.M > kMatvecRows * 65535 || a.N > (1 << 30)) return TAMD_E_UNSUPPORTED;   // (a strip and the grid stay in 31 bits)
+  if (a.K > (1 << 20) || a.M > 32 * 65535 || a.N > (1 << 30)) return TAMD_E_UNSUPPORTED;   // (a strip and the grid stay in 31 bits)
   if (a.x_stride_m >= ((int64_t)kMoeOob - 2 * a.K) / (2 * kMatvecRows)) return TAMD_E_UNSUPPORTED;  // 64 rows are addressed with 32 bits
   hipStream_t st = (hipStream_t)stream;
   return a.x_dtype == TAMD_BF16 ? matvec_bf16(a, st) : matvec_f16(a, st);

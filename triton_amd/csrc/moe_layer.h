@@ -1,4 +1,4 @@
-// A whole mixture-of-experts layer for a few tokens in two launches: 16-bit activations x MXFP4 weights.
+// A whole mixture-of-experts layer for a few tokens in two or three launches: 16-bit activations x MXFP4 weights.
 //
 //   y[t] = sum_j g[t,j] * (W2[e]^T h[t,j] + b2[e]),   h[t,j] = swiglu(W1[e]^T x[t] + b1[e]),   e = pick j of token t,
 //
@@ -7,11 +7,11 @@
 // to the bytes are launches and the latencies in front of the first weight.
 //
 //   moe_up_kernel    every workgroup picks the experts by itself (a few hundred logits, no launch for them), then walks
-//                    over (picked expert, strip of 32 columns = 16 gate / linear pairs).  Its eight waves split K; the partial
-//                    sums meet in LDS; h times its gate weight goes to memory.
-//   moe_down_kernel  a workgroup owns 16 columns of y.  Its sixteen waves cut the list of (picked expert, 128 K) into equal
-//                    parts; a row of the matrix cores' tile is a token, so the sum over the experts is the sum in the
-//                    accumulators: no partial results in memory, no atomics, one rounding.
+//                    over its part of the (picked expert, strip of 32 columns = 16 gate / linear pairs).  Its eight waves split K; the
+//                    partial sums meet in LDS; h times its gate weight goes to memory.
+//   moe_down_kernel  a workgroup owns 16 columns of y and walks over the picked experts, its eight waves splitting K; the
+//                    tokens' sums stay in LDS.  Where that leaves CUs without work the experts of all strips are dealt out evenly.
+//   moe_join_kernel  then adds up what several workgroups have of a strip, in a fixed order.
 //
 // h is kept as two 16-bit planes, its rounding and what that leaves (16 bits more), each a row of its own in the tile of the
 // down projection: with up to eight tokens these rows are there anyhow, and the layer's error is that of its one rounding
@@ -59,10 +59,6 @@ struct Buffer {
   TAMD_DEVICE uint32_t load2(uint32_t off, uint32_t uniform = 0) const { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, uniform, 0); }
   TAMD_DEVICE uint32_t load1(uint32_t off, uint32_t uniform = 0) const { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, off, uniform, 0); }
 };
-
-TAMD_DEVICE uint64_t uniform64(uint64_t v) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32;
-}
 
 template <int XDT>
 TAMD_DEVICE typename Mma<XDT>::frag_t as_frag(u32x4_t v) { return __builtin_bit_cast(typename Mma<XDT>::frag_t, v); }
@@ -228,7 +224,7 @@ TAMD_DEVICE float swiglu_keeping_nan(const tamd_moe_layer_args &a, float g, floa
 // rows of x then stay in registers.  Its eight waves split K, NB blocks of 128 each; the weights of two units are in flight
 // (48 KB per CU with NB = 3), their partial sums meet in LDS, a barrier per unit.  A stage is a unit, 16 of its rows and 8 * NB
 // blocks of K; with ROUNDS (long K, many rows per expert) a unit may have several of K and x travels with the weights.
-// As a loop without requests ahead, two workgroups per CU, 16 tokens of 128 experts of 2880 x 5760 took 154 us instead of TODO.
+// As a loop without requests ahead, two workgroups per CU, 16 tokens of 128 experts of 2880 x 5760 took 154 us, 76 so: 5.9 TB/s.
 template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, bool ROUNDS>
 __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
@@ -420,14 +416,14 @@ __host__ __device__ inline int64_t moe_partial_at(int64_t slots, int64_t inter) 
 template <int NB, int RC>
 constexpr int kMoeDownPitch = 256 * NB + 16;   // bytes of a row of h in a wave's buffer (rows 16 bytes apart on the banks)
 
-// A workgroup owns 16 columns of y; its eight waves split K, NB blocks of 128 each, and walk over the picked experts with the weights of
-// D experts in flight.  A row of a tile is a plane of one of the expert's tokens, RC tokens at a time; when these are multiplied
+// A workgroup has 16 columns of y at a time, all of the picked experts or (DEALT) some of them; its eight waves split K, NB blocks of 128 each, and walk over
+// the experts with the weights of D of them in flight.  A row of a tile is a plane of one of the expert's tokens, RC tokens at a time; when these are multiplied
 // a wave adds the tokens' sums to its own copy of the output in LDS, where the copies are added up at last: no atomics, and
 // NaN or infinite weights stay with the tokens that picked them.
 //
 // h comes as a few dense requests and goes through LDS, a buffer per wave, to where the MFMAs want it: requested in their layout
 // it takes four requests per block, most lanes of which bring nothing, and a request costs the CU about 20 cycles whatever it
-// brings (16 tokens of 128 experts of 2880 x 2880: 90 us, 50 without these requests, TODO now).
+// brings (16 tokens of 128 experts of 2880 x 2880: 90 us, 53 so, and 49 dealt out, 4.6 TB/s).
 template <int XDT, bool BLOCKS, bool SHUFFLED, int NB, int RC, int D, bool ROUNDS, bool DEALT>
 __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a) {
   typedef Mma<XDT> M;
