@@ -1,9 +1,9 @@
-"""`moe_layer`: a whole mixture-of-experts layer for a few tokens, in two launches.
+"""`moe_layer`: a whole mixture-of-experts layer for a few tokens, in two or three launches.
 
 The chain of `routing`, `matmul` (gathered rows, SwiGLU), `matmul` (gate weights, scatter) and `reduce` launches five or six
-kernels and writes its rows to memory three times; with a handful of tokens that is most of a layer's time.  The two kernels behind
-this function pick the experts themselves, read every picked expert's weights once and add the experts' rows up in the
-accumulators of the down projection.  Arguments and options are those of `routing` and `matmul`."""
+kernels and writes its rows to memory three times; with a handful of tokens that is most of a layer's time.  The kernels behind
+this function pick the experts themselves, read every picked expert's weights once and add the experts' rows up where
+they are made.  Arguments and options are those of `routing` and `matmul`."""
 import ctypes
 import math
 from typing import Optional
