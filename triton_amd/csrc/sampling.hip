@@ -178,12 +178,30 @@ TAMD_DEVICE Found find_in_row(const void *logits, int64_t row, int V, const RowS
     const int bits = shift ? 11 : 10;
     for (int b = tid; b < kBins; b += kThreads) mass[b] = 0, count[b] = 0;
     sync_threads();
-    for (int i = tid; i < V; i += kThreads) {
-      const uint32_t key = key_at<DT>(logits, row + i);
-      if (shift < 21 && key >> (shift + bits) != f.key >> (shift + bits)) continue;
+    for (int i0 = 0; i0 < V; i0 += kThreads) {
+      const int i = i0 + tid;
+      const uint32_t key = key_at<DT>(logits, row + (i < V ? i : 0));
+      bool on = i < V && (shift == 21 || key >> (shift + bits) == f.key >> (shift + bits));
       const uint32_t d = key >> shift & ((1u << bits) - 1u);
-      atomicAdd((unsigned long long *)&mass[d], (unsigned long long)scale.units(key));
-      atomicAdd(&count[d], 1u);
+      const uint64_t units = scale.units(key);
+      // (the two first keys of a wave once for all lanes that share them: rows that come here have few different ones, and additions to
+      // one place take turns; 131072 equal logits took 789 us, 340 so)
+      for (int j = 0; j < 2; ++j) {
+        const uint64_t left = __ballot(on);
+        if (left == 0) break;
+        const int first = __builtin_ctzll(left);
+        const uint32_t same = (uint32_t)__builtin_amdgcn_readlane((int)key, first);
+        const uint32_t n = (uint32_t)__popcll(__ballot(on && key == same));
+        if (tid % kWave == first) {
+          atomicAdd((unsigned long long *)&mass[d], (unsigned long long)(units * n));
+          atomicAdd(&count[d], n);
+        }
+        on = on && key != same;
+      }
+      if (on) {
+        atomicAdd((unsigned long long *)&mass[d], (unsigned long long)units);
+        atomicAdd(&count[d], 1u);
+      }
     }
     sync_threads();
     // from the largest digit down: thread t has the digits kBins - 1 - 2 t and the one below
