@@ -9,9 +9,9 @@ from triton_amd.matvec import matvec
 pytestmark = pytest.mark.gpu
 
 
-def columns(device, extra):
-    """Five strips per CU and `extra` columns: from here on strips are dealt out to waves."""
-    return 80 * torch.cuda.get_device_properties(device).multi_processor_count + extra
+def columns(device, extra, strips=5):
+    """Columns of so many strips of 16 per CU, and `extra`: from two on waves have a strip of their own, from five on two."""
+    return 16 * strips * torch.cuda.get_device_properties(device).multi_processor_count + extra
 
 
 @pytest.mark.parametrize("group,zeros", [(32, False), (32, True), (64, False), (64, True), (128, False), (128, True)])
@@ -58,3 +58,13 @@ def test_rows_whose_inner_dimension_is_long(M, group, device):
     w, dense, mag = make(6272, columns(device, 9), group, True, torch.bfloat16, device)
     x = rows(M, 6272, torch.float16, device)
     check(matvec(x, w), x, dense, 2 * mag)   # (6272 rows pass half as many groups again as the bound's 4096)
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, False), (128, True)])
+@pytest.mark.parametrize("M,K,strips,extra,dtype", [(17, 128, 2, 1, torch.bfloat16), (33, 384, 2, 50, torch.float16), (64, 1152, 3, 0, torch.bfloat16),
+                                                    (130, 256, 4, 15, torch.bfloat16), (40, 256, 1, 1, torch.float16), (64, 256, 2, 0, torch.bfloat16)])
+def test_fewer_strips(M, K, strips, extra, dtype, group, zeros, device):
+    w, dense, mag = make(K, columns(device, extra, strips), group, zeros, torch.float16, device)
+    x = rows(M, K, dtype, device)
+    for out in (dtype, torch.float32):
+        check(matvec(x, w, out_dtype=out), x, dense, mag)

@@ -360,13 +360,13 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
     }
 }
 
-// Many columns: a workgroup has MT tiles of 16 rows and 2 WN strips.  Its waves are WN pairs of strips times 8 / WN parts of K;
+// Many columns: a workgroup has MT tiles of 16 rows and C WN strips.  Its waves are WN, with C strips each, times 8 / WN parts of K;
 // a block of x goes through LDS once for all waves of its part, two blocks deep, and with the codes is requested two blocks ahead.
 // (64 x 4096 x 131072: 269 us by matvec_rows_kernel, where x comes from the caches for every second strip, 125 so; 149 with three blocks
 // ahead, which leave room for one workgroup per CU.  The matrix products, the codes' arithmetic and LDS take about 40 us each.)
-template <int XDT, int MT, int WN, int PER, bool ZEROS>
+template <int XDT, int MT, int WN, int C, int PER, bool ZEROS>
 __global__ __launch_bounds__(512, 2) void matvec_wide_kernel(tamd_matvec_args a) {
-  constexpr int C = 2, D = 2, WK = 8 / WN, STEPS = 4 / PER, PITCH = 256 + 16, XL = (4 * MT + WN - 1) / WN;
+  constexpr int D = 2, WK = 8 / WN, STEPS = 4 / PER, PITCH = 256 + 16, XL = (4 * MT + WN - 1) / WN;
   constexpr uint32_t TILE = XL * 4 * WN * PITCH;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
@@ -544,18 +544,25 @@ int launch_matvec_rows(const tamd_matvec_args &a, hipStream_t st) {
   return launch_status();
 }
 
-template <int XDT, int PER, bool ZEROS, int MT, int WN>
+template <int XDT, int PER, bool ZEROS, int MT, int WN, int C>
 int launch_matvec_wide(const tamd_matvec_args &a, hipStream_t st) {
   const int64_t strips = (a.N + 15) / 16;
-  const dim3 grid((unsigned)((strips + 2 * WN - 1) / (2 * WN)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-  const auto kernel = matvec_wide_kernel<XDT, MT, WN, PER, ZEROS>;
-  constexpr int WK = 8 / WN, for_x = WK * 2 * ((4 * MT + WN - 1) / WN) * 4 * WN * (256 + 16), for_sums = (8 - WN) * MT * 2 * kWave * 16;
+  const dim3 grid((unsigned)((strips + C * WN - 1) / (C * WN)), (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
+  const auto kernel = matvec_wide_kernel<XDT, MT, WN, C, PER, ZEROS>;
+  constexpr int WK = 8 / WN, for_x = WK * 2 * ((4 * MT + WN - 1) / WN) * 4 * WN * (256 + 16), for_sums = (8 - WN) * MT * C * kWave * 16;
   constexpr int lds = for_x > for_sums ? for_x : for_sums;
   static_assert(lds <= 160 * 1024);
   if (lds > 64 * 1024)
     if (int rc = raise_lds_limit_once((const void *)kernel)) return rc;
   kernel<<<grid, 512, lds, st>>>(a);
   return launch_status();
+}
+
+template <int XDT, int PER, bool ZEROS, int C>
+int launch_matvec_wide_of(const tamd_matvec_args &a, hipStream_t st) {
+  if (a.M <= 32) return launch_matvec_wide<XDT, PER, ZEROS, 2, 4, C>(a, st);
+  if (a.M <= 48) return launch_matvec_wide<XDT, PER, ZEROS, 3, 4, C>(a, st);
+  return launch_matvec_wide<XDT, PER, ZEROS, 4, 4, C>(a, st);
 }
 
 template <int XDT, int PER, bool ZEROS>
@@ -574,19 +581,17 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
     if (a.M <= 4) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, PER < 2 ? 2 : 1, 1>(a, st);
     if (a.M <= 8) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1, 2>(a, st);
     // (16 x 8192 x 28672: 33 us, 43 by the next; 5 rows take 39 and 34)
-    if (strips >= 5 * cus) return launch_matvec_wide<XDT, PER, ZEROS, 1, 4>(a, st);
+    if (strips >= 5 * cus) return launch_matvec_wide<XDT, PER, ZEROS, 1, 4, 2>(a, st);
     return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1>(a, st);
   }
-  // Two strips share x where these still give every CU a workgroup.  (Three tiles with groups of 32, and four of any, do not fit the
-  // registers with two strips: one strip, and above 48 rows parts of 32, which read the weights again from the caches.)
-  // Waves with strips of their own from five strips per CU on, eight per workgroup: 64 x 4096 x 20480 takes 32 us so and 45 with the
-  // other kernel, 20 x 8192 x 20480 41 either way; with four per CU 20 x 8192 x 16384 takes 41 and 29.
-  if (strips >= 5 * cus) {
-    if (a.M <= 32) return launch_matvec_wide<XDT, PER, ZEROS, 2, 4>(a, st);
-    if (a.M <= 48) return launch_matvec_wide<XDT, PER, ZEROS, 3, 4>(a, st);
-    return launch_matvec_wide<XDT, PER, ZEROS, 4, 4>(a, st);
-  }
-  const bool two = strips >= 2 * cus;
+  // Waves with strips of their own where there are more than two for a CU, from five on two for each: 64 x 4096 x 14336 takes 23 us so and 35
+  // with the other kernel, 48 x 512 x 16384 7 and 15, 64 x 4096 x 20480 32 and 45; at two per CU 48 x 8192 x 8192 takes 33 and 21.
+  if (strips >= 5 * cus) return launch_matvec_wide_of<XDT, PER, ZEROS, 2>(a, st);
+  if (strips > 2 * cus) return launch_matvec_wide_of<XDT, PER, ZEROS, 1>(a, st);
+  // Two strips share x where one each would be more than one workgroup per CU (24 x 2880 x 5120: 9.8 us, 13.2 with one each).  (Three tiles
+  // with groups of 32, and four of any, do not fit the registers with two strips: one strip, and above 48 rows parts of
+  // 32, which read the weights again from the caches.)
+  const bool two = strips > cus;
   if (a.M > 32 && a.M <= 48) return PER < 4 && two ? launch_matvec_rows<XDT, PER, ZEROS, 3, PER < 4 ? 2 : 1, 1>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 3, 1, 1>(a, st);
   return two ? launch_matvec_rows<XDT, PER, ZEROS, 2, 2, 1>(a, st) : launch_matvec_rows<XDT, PER, ZEROS, 2, 1, 1>(a, st);
 }
