@@ -25,10 +25,10 @@ def test_layer(T, E, k, H, I, dtype, values, scales, device):
         assert torch.equal(layer.call(x, logits, k, (values, values), (scales, scales)), y)
 
 
-@pytest.mark.parametrize("T,E,k", [(20, 12, 8), (3, 12, 8)])
-def test_rounds_of_blocks(T, E, k, device):
-    """More blocks of K than one round of the eight waves takes."""
-    layer = Layer(device, E, 64, 4128, spread=0.05)
+@pytest.mark.parametrize("T,E,k,I", [(20, 12, 8, 4128), (3, 12, 8, 4128), (16, 12, 3, 2880), (30, 12, 6, 2880), (7, 40, 1, 2336)])
+def test_rounds_of_blocks(T, E, k, I, device):
+    """More blocks of K than one round of the eight waves takes, or as many as three for each; one to fifteen rows per expert."""
+    layer = Layer(device, E, 64, I, spread=0.05)
     x, logits = inputs(T, E, 64, torch.bfloat16, device)
     got = layer.call(x, logits, k, ("blocks", "blocks"), ("shuffled", "shuffled")).cpu().double()
     want, err = layer.expected(x, logits, k)

@@ -721,7 +721,7 @@ int launch_moe_down_of(const tamd_moe_layer_args &a, hipStream_t st) {
   int cus = 0;
   if (int rc = cu_count(cus)) return rc;
   // One strip per workgroup, or the experts of all strips dealt out: where nine experts or more of a strip that no CU has to do meanwhile are
-  // saved the join costs less.  16 tokens of 128 experts of 2880 x 2880 (19 saved) take 129 us and 126, 32 of 32 (10) 138 and 122,
+  // saved the join costs less.  16 tokens of 128 experts of 2880 x 2880 (19 saved) take 129 us and 126, 32 of 32 (10; eight tokens ahead) 138 and 122,
   // 64 of 128 of 512 x 1024 (96) 129 and 74, but 2 of 64 of 1024 x 2048 (8) 23 and 26, one of 2880 x 2880 (1) 22 and 27.
   const int64_t strips = a.hidden / 16, slots = (int64_t)a.n_tokens * a.n_picks, most = slots < a.n_experts ? slots : a.n_experts;
   const int64_t shares = cus < kMoeShares ? cus : kMoeShares;
@@ -736,13 +736,15 @@ int launch_moe_down_of(const tamd_moe_layer_args &a, hipStream_t st) {
   return launch_status();
 }
 
-// Tokens of an expert that are requested ahead: two where more are rare, four, or eight.
+// Tokens of an expert that are requested ahead: two where more are rare, four, or eight.  Eight of three blocks do not fit the
+// registers, and two blocks are two rounds of K for as many columns: there four serve up to six rows on average (32 tokens of 32
+// experts of 2880 x 2880: 114 us, 132 with eight; with two blocks or one eight are better from 2.5 on, 64 of 128 of 2048 x 768: 110 and 119).
 template <int XDT, bool BLOCKS, bool SHUFFLED, int NB>
 int launch_moe_down_nb(const tamd_moe_layer_args &a, hipStream_t st) {
   const float rows = (float)(a.n_tokens * a.n_picks) / (float)a.n_experts;
   if (a.n_tokens <= 2 || rows <= 0.75f) return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB, 2, 4>(a, st);
-  if (a.n_tokens <= 4 || rows <= 2.5f) return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB, 4, 3>(a, st);
-  return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB < 3 ? NB : 2, 8, 2>(a, st);   // (eight tokens of three blocks do not fit the registers)
+  if (a.n_tokens <= 4 || rows <= (NB == 3 ? 6.f : 2.5f)) return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB, 4, 3>(a, st);
+  return launch_moe_down_of<XDT, BLOCKS, SHUFFLED, NB < 3 ? NB : 2, 8, 2>(a, st);
 }
 
 template <int XDT, bool BLOCKS, bool SHUFFLED>
