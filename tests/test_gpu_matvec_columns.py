@@ -26,10 +26,11 @@ def test_product(M, K, extra, dtype, group, zeros, device):
 
 @pytest.mark.parametrize("K,group", [(32, 32), (96, 32), (160, 32), (192, 64), (1056, 32)])
 def test_last_block_not_whole(K, group, device):
-    w, dense, mag = make(K, columns(device, 7), group, True, torch.float16, device)
-    for M in (20, 61):
-        x = rows(M, K, torch.bfloat16, device)
-        check(matvec(x, w, out_dtype=torch.float32), x, dense, mag)
+    for strips in (5, 2, 1):
+        w, dense, mag = make(K, columns(device, 7 if strips > 1 else -9, strips), group, True, torch.float16, device)
+        for M in (20, 40, 61):
+            x = rows(M, K, torch.bfloat16, device)
+            check(matvec(x, w, out_dtype=torch.float32), x, dense, mag)
 
 
 def test_padding_is_left_alone(device):
@@ -62,7 +63,9 @@ def test_rows_whose_inner_dimension_is_long(M, group, device):
 
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, False), (128, True)])
 @pytest.mark.parametrize("M,K,strips,extra,dtype", [(17, 128, 2, 1, torch.bfloat16), (33, 384, 2, 50, torch.float16), (64, 1152, 3, 0, torch.bfloat16),
-                                                    (130, 256, 4, 15, torch.bfloat16), (40, 256, 1, 1, torch.float16), (64, 256, 2, 0, torch.bfloat16)])
+                                                    (130, 256, 4, 15, torch.bfloat16), (40, 256, 1, 1, torch.float16), (64, 256, 2, 0, torch.bfloat16),
+                                                    (20, 1152, 1, 0, torch.bfloat16), (48, 384, 1, 0, torch.float16), (61, 128, 1, -7, torch.float16),
+                                                    (25, 2176, 1, 17, torch.bfloat16)])
 def test_fewer_strips(M, K, strips, extra, dtype, group, zeros, device):
     w, dense, mag = make(K, columns(device, extra, strips), group, zeros, torch.float16, device)
     x = rows(M, K, dtype, device)

@@ -588,6 +588,9 @@ int launch_matvec(const tamd_matvec_args &a, hipStream_t st) {
   // with the other kernel, 48 x 512 x 16384 7 and 15, 64 x 4096 x 20480 32 and 45; at two per CU 48 x 8192 x 8192 takes 33 and 21.
   if (strips >= 5 * cus) return launch_matvec_wide_of<XDT, PER, ZEROS, 2>(a, st);
   if (strips > 2 * cus) return launch_matvec_wide_of<XDT, PER, ZEROS, 1>(a, st);
+  // Few strips: every 16 rows a workgroup of their own, two of which a CU holds; the weights come again from the caches.  Up to three for two CUs:
+  // 33 x 5120 x 530 takes 6.3 us so and 11.2 as one, 48 x 4096 x 2048 7.7 and 10.4, at four for two 20 x 14336 x 4096 19.8 and 17.4.
+  if (2 * strips * ((a.M + 15) / 16) <= 3 * cus) return launch_matvec_rows<XDT, PER, ZEROS, 1, 1, 1>(a, st);
   // Two strips share x where one each would be more than one workgroup per CU (24 x 2880 x 5120: 9.8 us, 13.2 with one each).  (Three tiles
   // with groups of 32, and four of any, do not fit the registers with two strips: one strip, and above 48 rows parts of
   // 32, which read the weights again from the caches.)
