@@ -463,8 +463,9 @@ int tamd_matvec(const tamd_matvec_args *args, size_t args_size, void *stream);
  * Order of a row: by logit, the largest first, equal ones by index (as in tamd_topk_forward); w = exp((x - max) / temperature).  Kept is
  *   the first top_k (top_k <= 0: all), of these the shortest prefix with a sum of w of at least top_p times theirs (top_p >= 1: all),
  *   of these what has w >= min_p; the first always.
- * The token is the first kept one, in that order, whose running sum of w exceeds u times the sum of all kept.  Sums are exact to
- * 2^-37 of the row's and do not depend on how the work is cut.
+ * The token is the first kept one, in that order, whose running sum of w exceeds u times the sum of all kept.  Sums do not depend on
+ * how the work is cut: w is held to the nearest multiple of 2^-f, f = min(51, 62 - bits of V), so a sum over n logits is off by at most
+ * n 2^-(f + 1) and 2^-38 of itself (V = 2^17: 2^-28 of the largest w, 2^20: 2^-22; as roundings fall, 2^-36 and 2^-32), and what is below 2^-(f + 1) has no mass.
  * temperature <= 0 or NaN: the first of the order.  NaN logits count as -inf; a row of nothing but -inf gives -1; with +inf logits these
  * share the mass alike.  u is clamped to [0, 1), min_p to at most 1; a NaN top_p or min_p keeps all, a NaN u is 0.
  * temperature, top_k, top_p, min_p: per row if the pointer is given, else the value for all.  Limits: V <= 2^20, R <= 2^20.

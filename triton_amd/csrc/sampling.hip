@@ -4,9 +4,9 @@
 // a prefix of that order, and the token is the first of it whose running sum of w exceeds u times the sum of all kept: nothing
 // has to be sorted, every question is "where does the running count or sum reach this".
 //
-// w is taken in 64 bits and held as a whole number of units of 2^-fraction, 2^fraction * V < 2^62: sums of whole numbers do not depend on
-// their order, so the same row gives the same token however the work is cut, and they are off by less than 2^-37 of the row's mass.
-// What rounds to zero is not there at all: it cannot be drawn, and adds nothing to what top-k keeps.
+// w is taken in 64 bits and held as a whole number of units of 2^-fraction (sample_weights.h, with what that leaves of the sums): sums of whole
+// numbers do not depend on their order, so the same row gives the same token however the work is cut.  What rounds to zero is
+// not there at all: it cannot be drawn, and adds nothing to what top-k keeps.  Where min-p ends is decided by the logits, in 64 bits.
 //
 // Five launches, three of them over (chunk of a row, row):
 //   extremes   the largest logit (of greedy rows with its index) and the smallest;
@@ -18,6 +18,7 @@
 // Where that is faster a workgroup goes through all of it for a row, in one launch (sample_whole).  A row that has more than 4096 logits in those
 // bins -- many equal or nearly equal ones -- is searched by the bits of its keys (search_row): slower, but right for any row.
 #include "common.h"
+#include "sample_weights.h"
 
 namespace tamd {
 namespace {
@@ -65,12 +66,6 @@ TAMD_DEVICE uint32_t key_at(const void *logits, int64_t i) {
 }
 constexpr uint32_t kNothing = 0x007FFFFFu;   // key of -inf
 
-// Bits of a weight of one: a row's weights together stay below 2^62, one below 2^51 (units_of).
-TAMD_DEVICE int fraction_bits(int V) {
-  const int b = 62 - (32 - __builtin_clz((uint32_t)V));
-  return b < 51 ? b : 51;
-}
-
 // 2^(fraction - j / 256) by the threads of a workgroup.
 TAMD_DEVICE void make_powers(double *powers, int V) {
   if (threadIdx.x < 256) powers[threadIdx.x] = exp2(fraction_bits(V) - (double)threadIdx.x * 0.00390625);
@@ -87,7 +82,7 @@ struct RowScale {
       : top(top_), to_y(to_y_), to_bin(to_bin_), fraction(fraction_bits(V)), powers(powers_) {}
   TAMD_DEVICE RowScale(uint32_t top_key, uint32_t least_key, double t, int V, const double *powers_)
       : top(__builtin_fmin((double)logit_of(top_key), kHuge)), to_y(top == kHuge ? 1.0 : 1.4426950408889634 / t), fraction(fraction_bits(V)), powers(powers_) {
-    const double most = y_of(logit_of(least_key)), range = most < fraction ? most : fraction;
+    const double most = y_of(logit_of(least_key)), range = counts(most) ? most : fraction + 1;
     to_bin = range > 0.0 ? kBins / range : 0.0;
   }
   // (of -inf: infinite, or NaN at an infinite temperature; neither counts)
@@ -95,23 +90,9 @@ struct RowScale {
 #pragma clang fp contract(off)
     return (top - __builtin_fmin((double)v, kHuge)) * to_y;
   }
-  TAMD_DEVICE bool counts(double y) const { return y < fraction; }
+  TAMD_DEVICE bool counts(double y) const { return y < fraction + 1; }   // half a unit or more
   TAMD_DEVICE int bin_of(double y) const { return (int)__builtin_fmin(y * to_bin, (double)(kBins - 1)); }
-  // 2^(fraction - y) of a y that counts, in units (of another: any number).  y in units of 2^-40 (the low bits of y + 1.5 * 2^12) is a whole number, eight bits for
-  // the table and the rest r for the series of 2^-r, whose first four terms leave 2.3e-12 of w; adding 2^52 makes a whole number
-  // of the product.  (With exp() and conversions this took longer than reading the logits.  Fused by hand: the histogram and
-  // the candidates have to agree to the last unit in every kernel.)
-  TAMD_DEVICE uint64_t units_of(double y) const {
-#pragma clang fp contract(off)
-    const uint64_t fixed = __builtin_bit_cast(uint64_t, y + 6144.0) & 0xFFFFFFFFFFFFull;   // 6144 = 1.5 * 2^12: the lowest bit is 2^-40
-    const uint32_t whole = (uint32_t)(fixed >> 40) & 0x3Fu;
-    const double r = (double)(uint32_t)fixed * (0.6931471805599453 * 0x1p-40);
-    double p = __builtin_fma(r, -1.0 / 6.0, 0.5);
-    p = __builtin_fma(r, p, -1.0);
-    p = __builtin_fma(r, p, 1.0);
-    const double x = __builtin_fma(powers[(uint32_t)(fixed >> 32) & 0xFFu], p, 0x1p52);
-    return (__builtin_bit_cast(uint64_t, x) & 0xFFFFFFFFFFFFFull) >> whole;
-  }
+  TAMD_DEVICE uint64_t units_of(double y) const { return weight_units(y, powers); }
   TAMD_DEVICE uint64_t units(uint32_t key) const {
     const double y = y_of(logit_of(key));
     return counts(y) ? units_of(y) : 0;
@@ -218,10 +199,7 @@ TAMD_DEVICE Found find_in_row(const void *logits, int64_t row, int V, const RowS
   return f;
 }
 
-// Where the kept prefix ends, from the row's sums: with `least` units or more.
-TAMD_DEVICE uint64_t least_units(const RowSettings &s, const RowScale &scale) {
-  return s.min_p > 0.0 ? (uint64_t)ceil(s.min_p * (double)(1ull << scale.fraction)) : 1;
-}
+// Where the kept prefix ends, from the row's sums.
 TAMD_DEVICE uint64_t top_p_target(double top_p, uint64_t sum) {   // the prefix ends where the sum reaches it
   const double want = ceil(top_p * (double)sum);
   return want >= 1.0 ? (want < (double)sum ? (uint64_t)want : sum) : 1;
@@ -231,33 +209,30 @@ TAMD_DEVICE uint64_t token_target(double u, uint64_t sum) {       // the token i
   return at < sum ? at : sum;
 }
 
-// The token of a row whose largest logit is known, by the bits of the keys.
+// The token of a row whose largest logit is known, by the bits of the keys.  min_p_y as in Bounds.
 template <int DT>
-TAMD_DEVICE int search_row(const tamd_sample_args &a, int r, const RowSettings &s, const RowScale &scale, uint64_t *hist, Shared &sh) {
+TAMD_DEVICE int search_row(const tamd_sample_args &a, int r, const RowSettings &s, const RowScale &scale, double min_p_y, uint64_t *hist, Shared &sh) {
   const int tid = threadIdx.x, V = a.V;
   uint64_t *tmp = sh.tmp;
   const int64_t row = r * a.logits_stride;
-  const auto sum_of = [&](uint32_t above, uint64_t least) {   // of larger keys with at least that many units
+  const auto sum_of = [&](uint32_t above, double most) {   // of larger keys with no larger y
     uint64_t mine = 0;
     for (int i = tid; i < V; i += kThreads) {
       const uint32_t key = key_at<DT>(a.logits, row + i);
-      const uint64_t w = key > above ? scale.units(key) : 0;
-      mine += w >= least ? w : 0;
+      mine += key > above && scale.y_of(logit_of(key)) <= most ? scale.units(key) : 0;
     }
     return block_sum<uint64_t>(mine, tmp);
   };
   // the kept prefix: what has a larger key than `last`, and `ties` elements of it
   uint32_t last = kNothing + 1;
   int64_t ties = V;
-  uint64_t sum = s.top_k ? 0 : sum_of(kNothing, 0), target = 0;
+  uint64_t sum = s.top_k ? 0 : sum_of(kNothing, (double)__builtin_inff()), target = 0;
   Found f{0, 0, 0};
   // where top-k ends, where top-p ends, the token
 #pragma clang loop unroll(disable)
   for (int ask = s.top_k ? 0 : s.top_p < 1.0 ? 1 : 2; ask < 3; ask = ask == 0 && s.top_p < 1.0 ? 1 : ask == 2 ? 3 : 2) {
-    if (ask == 2) {
-      const uint64_t least = least_units(s, scale);
-      if (s.min_p > 0.0 && scale.units(last) < least) sum = sum_of(last, least);
-    }
+    // (of -inf y may be NaN)
+    if (ask == 2 && s.min_p > 0.0 && !(scale.y_of(logit_of(last)) <= min_p_y)) sum = sum_of(last, min_p_y);
     target = ask == 0 ? (uint64_t)s.top_k : ask == 1 ? top_p_target(s.top_p, sum) : token_target(s.u, sum);
     f = find_in_row<DT>(a.logits, row, V, scale, ask != 0, target, hist, sh);
     const uint64_t w = scale.units(f.key);
@@ -561,6 +536,7 @@ struct Bounds {
   int from[4], to[4];      // bins of the candidates: the ends of top-k, top-p and min-p, and the token
   uint64_t mass, min_mass; // of the row; in front of the bins in which min-p ends
   double top, to_y, to_bin;
+  double min_p_y;          // min-p keeps what has no larger y: w >= min_p is y <= log2(1 / min_p)
   uint32_t count;
   int done;                // the token is known
 };
@@ -575,7 +551,6 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const Bo
   uint64_t units[PER], before[PER], run = 0, enough = 0;
   uint32_t rank[PER];
   int bin[PER];
-  const uint64_t least = least_units(s, scale);
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int i = PER * tid + j;
@@ -584,7 +559,7 @@ TAMD_DEVICE int pick_among(const RowSettings &s, const RowScale &scale, const Bo
     bin[j] = scale.counts(y) ? scale.bin_of(y) : -1;
     before[j] = run;
     run += units[j];
-    enough += bin[j] >= b.from[2] && bin[j] <= b.to[2] && units[j] >= least ? units[j] : 0;
+    enough += bin[j] >= b.from[2] && bin[j] <= b.to[2] && y <= b.min_p_y ? units[j] : 0;
   }
   const uint64_t start = block_scan<uint64_t>(run, sh.tmp) - run;
   // the first candidate of a bin leaves what the running sums of the bin's candidates lack
@@ -663,7 +638,7 @@ TAMD_DEVICE Bounds find_bounds(const RowSettings &s, const RowScale &scale, uint
   Bounds b;
 #pragma unroll
   for (int j = 0; j < 4; ++j) b.from[j] = kBins, b.to[j] = -1;
-  b.mass = mass[kBins], b.count = s.top_k ? rank[kBins] : 0u, b.min_mass = 0, b.done = 0;
+  b.mass = mass[kBins], b.count = s.top_k ? rank[kBins] : 0u, b.min_mass = 0, b.min_p_y = 0.0, b.done = 0;
   b.top = scale.top, b.to_y = scale.to_y, b.to_bin = scale.to_bin;
   uint64_t lo = b.mass, hi = lo;
   if (s.top_k && (uint32_t)s.top_k < b.count) {
@@ -677,8 +652,8 @@ TAMD_DEVICE Bounds find_bounds(const RowSettings &s, const RowScale &scale, uint
     hi = mass[b.to[1] + 1] < hi ? mass[b.to[1] + 1] : hi;
   }
   if (s.min_p > 0.0) {
-    const double y = -log2(s.min_p);
-    const int at = scale.counts(y) ? scale.bin_of(y) : kBins - 1;
+    b.min_p_y = -log2(s.min_p);
+    const int at = scale.counts(b.min_p_y) ? scale.bin_of(b.min_p_y) : kBins - 1;
     b.from[2] = at > 0 ? at - 1 : 0, b.to[2] = at < kBins - 1 ? at + 1 : kBins - 1;
     b.min_mass = mass[b.from[2]];
     lo = b.min_mass < lo ? b.min_mass : lo;
@@ -785,7 +760,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Wo
   int token;
   if (collected > kMost) {
     sync_threads();
-    token = search_row<DT>(a, r, s, scale, list, sh);
+    token = search_row<DT>(a, r, s, scale, b.min_p_y, list, sh);
   } else {
     const int n = (int)collected;
     for (int i = tid; i < n; i += kThreads) list[i] = ws.candidates[(int64_t)r * kMost + i];
@@ -832,7 +807,7 @@ __global__ __launch_bounds__(kThreads) void whole_row_kernel(tamd_sample_args a)
   sync_threads();
   int token;
   if (sh.n > kMost) {
-    token = search_row<DT>(a, r, s, scale, list, sh);
+    token = search_row<DT>(a, r, s, scale, b.min_p_y, list, sh);
   } else {
     const int n = (int)sh.n;
     sort_elements(list, n, places);

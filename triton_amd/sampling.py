@@ -21,7 +21,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
       of these the shortest prefix that holds top_p of their mass (1 or more: all of them),
       of these what has w >= min_p, that is at least min_p times the largest probability,
     and always the first.  The token is the first kept one whose running sum of w exceeds u times the sum of all kept, so the same
-    u gives the same token however large the batch.  Sums are of 62 bits; the settings are taken as float32.
+    u gives the same token however large the batch.  w is held to the nearest multiple of 2^-44 of the largest for V up to 2^18 - 1, of 2^-41 for
+    2^20, which leaves sums of V logits within V / 2 of these (and 2^-38 of themselves); the settings are taken as float32.
 
     temperature, top_k, top_p, min_p: a number for all rows, or a tensor [R] (float32; top_k int32).  temperature 0 takes the
     first of the order.  NaN logits count as -inf; a row with nothing but -inf gives -1; +inf logits share the mass alike.
