@@ -11,6 +11,10 @@
 // and-or turn a pair into the 16-bit numbers 16 + q (the code is the top of the mantissa).  What is too much, (16 + z) times
 // the sum of the group's x, is what the group's accumulators start from; the sums of x come from one more MFMA against
 // ones.  (With 128 + q or 1024 + q the shift could go, but the difference would lose four or seven bits of the float32 sums.)
+//
+// With bf16 rows all of these numbers, and the ones, are 2^-12 of that, and the result is 2^12 times the sums: 128 values of up to 2^128 times up to
+// 31 stay within float32, so every finite row has finite sums before its scales come in.  (Without it one x from 1e37 on, or a
+// group of one sign from 1e35 on, made a row infinite or NaN.  At the other end products are no longer normal below |x| of 2^-117.)
 #pragma once
 #include "moe_layer.h"
 
@@ -22,16 +26,18 @@ template <int XDT>
 struct Int4;
 template <>
 struct Int4<TAMD_BF16> {
-  static constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u, kOne = 0x3F803F80u;
+  static constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x3B803B80u, kOne = 0x39803980u;   // 16 and 1 times 2^-12
+  static constexpr float kTimes = 0x1p12f;   // what the sums are multiplied by at last
   static constexpr int kUp = 3;   // place of a code in the mantissa
 };
 template <>
 struct Int4<TAMD_F16> {
   static constexpr uint32_t kMask = 0x03C003C0u, kSixteen = 0x4C004C00u, kOne = 0x3C003C00u;
+  static constexpr float kTimes = 1.f;
   static constexpr int kUp = 6;
 };
 
-// eight codes -> 16 + q
+// eight codes -> 16 + q, over kTimes
 template <int XDT>
 TAMD_DEVICE typename Mma<XDT>::frag_t codes_plus_16(uint32_t d) {
   typedef Int4<XDT> I;
@@ -51,11 +57,12 @@ struct MatvecPart {
 };
 
 // A strip's sums over the eight waves: row m of a tile, column `col`, from the waves' accumulators of that tile.
+template <int XDT>
 TAMD_DEVICE float matvec_sum(const f32x4_t (*red)[kWave], int m, int col) {
   float v = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) v += ((const float *)&red[w][(m >> 2) * 16 + col])[m & 3];
-  return v;
+  return Int4<XDT>::kTimes * v;
 }
 // A mask for a buffer's length (a uniform value), hidden from the compiler as in dead_unless.
 TAMD_DEVICE uint32_t all_ones_if(bool b) {
@@ -190,7 +197,7 @@ __global__ __launch_bounds__(512, D == 1 ? 4 : 2) void matvec_kernel(tamd_matvec
     const int m = tid >> 4, col = tid & 15;
     const int64_t n = 16 * now + col;
     if (m < a.M && n < a.N) {
-      float v = matvec_sum(red[turn], m, col);
+      float v = matvec_sum<XDT>(red[turn], m, col);
       if (a.bias) v += load_any_f32(a.bias, a.bias_dtype, n);
       store_any(a.y, a.y_dtype, m * a.y_stride_m + n, v);
     }
@@ -352,7 +359,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
       const int m = tid >> 4, col = tid & 15;
       const int64_t n = 16 * (strip + s) + col;
       if (m < 16 && 16 * t + m < rows && n < a.N) {
-        float v = matvec_sum(red, m, col);
+        float v = matvec_sum<XDT>(red, m, col);
         if (a.bias) v += load_any_f32(a.bias, a.bias_dtype, n);
         store_any(a.y, a.y_dtype, (m0 + 16 * t + m) * a.y_stride_m + n, v);
       }
@@ -513,7 +520,7 @@ __global__ __launch_bounds__(512, 2) void matvec_wide_kernel(tamd_matvec_args a)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int m = 16 * t + 4 * (int)h + v;
-        if (m < rows) store_any(a.y, a.y_dtype, (m0 + m) * a.y_stride_m + col, y[t][s][v] + bias);
+        if (m < rows) store_any(a.y, a.y_dtype, (m0 + m) * a.y_stride_m + col, Int4<XDT>::kTimes * y[t][s][v] + bias);
       }
     }
   }

@@ -78,7 +78,8 @@ def matvec(x: torch.Tensor, w: Int4Weights, bias: Optional[torch.Tensor] = None,
     y = x @ w + bias for a few rows x [M, K] (or one, [K]) of bf16 / fp16 and 4-bit weights of `pack_int4`.
 
     bias: [N] or None; out_dtype: float32, bfloat16 or float16 (default: x's type); out: where the result goes, which must not overlap
-    an input.  Weights are not rounded, sums are float32, the result is rounded once; a row of x with a NaN or an infinity gives NaN.  The kernel is made for up to 64 rows;
+    an input.  Weights are not rounded, sums are float32, the result is rounded once; a row of x with a NaN or an infinity gives NaN,
+    any finite one a finite result where float32 holds it (bf16: |x| below 2^-117 may count as 0).  The kernel is made for up to 64 rows;
     every further 64 read the weights again."""
     if out is None:
         done = _native.matvec(x, w, bias, out_dtype)
