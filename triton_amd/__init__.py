@@ -16,11 +16,11 @@ def install_as_triton_kernels():
     me = sys.modules[__name__]
     sys.modules.setdefault("triton_kernels", me)
     for sub in ("tensor", "topk", "routing", "numerics", "numerics_details", "numerics_details.mxfp", "matmul",
-                "matmul_details", "matmul_details.opt_flags", "swiglu", "reduce", "specialize", "testing",
+                "matmul_details", "matmul_details.opt_flags", "swiglu", "reduce", "moe_layer", "matvec", "sampling", "specialize", "testing",
                 "tensor_details", "tensor_details.layout", "tensor_details.ragged_tensor",
                 "tensor_details.bitmatrix", "tensor_details.dtype", "tensor_details.layout_details",
                 "tensor_details.layout_details.base", "tensor_details.layout_details.strided",
-                "tensor_details.layout_details.cdna4_scale", "target_info"):
+                "tensor_details.layout_details.cdna4_scale", "tensor_details.layout_details.cdna4_value", "target_info"):
         mod = importlib.import_module(f"{__name__}.{sub}")
         sys.modules.setdefault(f"triton_kernels.{sub}", mod)
     return me
