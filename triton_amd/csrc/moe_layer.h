@@ -482,11 +482,12 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
       if constexpr (SHUFFLED) p.scale_off[i] = 2u * ((p.kb0 >> 1) + i) < n_kb ? scale & ~3u : kMoeOob;   // blocks 2 (kb0 / 2 + i) and the next
       else p.scale_off[i] = (uint32_t)i < n && 4u * (p.kb0 + i) + h < groups ? scale : kMoeOob;
     }
-    // 16-byte chunk i * 64 + lane of the rows: row by row, 16 NB chunks each; zeros past K
+    // 16-byte chunk i * 64 + lane of the rows: row by row, 16 NB chunks each; zeros past K and past this wave's blocks (an infinite h
+    // times the zeros in place of another wave's codes would be NaN)
 #pragma unroll
     for (int i = 0; i < XR; ++i) {
-      const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), k = 128u * p.kb0 + 8u * (chunk % (16u * NB));
-      p.x_off[i] = of < 2u * RC && k < (uint32_t)K ? of * (uint32_t)(2 * K) + 2u * k : kMoeOob;
+      const uint32_t chunk = (uint32_t)(i * kWave + lane), of = chunk / (16u * NB), at = chunk % (16u * NB), k = 128u * p.kb0 + 8u * at;
+      p.x_off[i] = of < 2u * RC && at < 16u * n && k < (uint32_t)K ? of * (uint32_t)(2 * K) + 2u * k : kMoeOob;
     }
     return p;
   };
