@@ -239,6 +239,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
   // A block's part of x: request i of a tile's XI brings rows 16 t + 4 i .. + 3, 256 bytes each, which go through LDS to the lanes that
   // multiply them.  (Requested where they are multiplied, 64 bytes of 16 rows at a time, 48 rows of 8192 took 18 of 31 us.)
   uint8_t *const x_lds = lds + wave * (U * MT * 4 * XI * PITCH);
+  const uint32_t x_read = wave_lds_offset((c & (4u * XI - 1u)) * PITCH + 16u * h);   // (rows past the last repeat)
   uint32_t x_row[MT][XI];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(512, MT == 1 ? 4 : 2) void matvec_rows_kernel(tamd_
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
-          for (int j = 0; j < STEPS; ++j) xf[t][j] = *(const u32x4_t *)(x_lds + ((i * MT + t) * 4 * XI + (c & (4u * XI - 1u))) * PITCH + 64u * (g * STEPS + j) + 16u * h);   // (rows past the last repeat)
+          for (int j = 0; j < STEPS; ++j) xf[t][j] = *(const u32x4_t *)(x_lds + x_read + (i * MT + t) * 4 * XI * PITCH + 64u * (g * STEPS + j));
           of_x[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < STEPS; ++j) of_x[t] = Mma16<XDT>::mma(as_frag<XDT>(xf[t][j]), as_frag<XDT>(ones), of_x[t]);

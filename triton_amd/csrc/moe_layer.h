@@ -544,7 +544,7 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
       }
     }
   };
-  const uint32_t a_row = (c & (2u * RC - 1u)) * PITCH + 64u * h;   // (rows past the buffer's repeat: no one reads their sums)
+  const uint32_t a_row = wave_lds_offset((c & (2u * RC - 1u)) * PITCH + 64u * h);   // (rows past the buffer's repeat: no one reads their sums)
   const auto multiply = [&](const Stage &st) {
     const bool live = to_do > 0;
     const uint32_t f = strip & 1u;
