@@ -99,9 +99,8 @@ def matvec(x: torch.Tensor, w: Int4Weights, bias: Optional[torch.Tensor] = None,
         assert t is None or t.device == x.device, f"{name} must live on the device of x"
     per = 128 // w.group_size
     S, B = -(-N // 16), -(-K // 128)
-    assert tuple(w.data.shape) == (S, B, 1024) and tuple(w.scales.shape) == (S, B, 16, per) and w.data.is_contiguous() \
-        and w.scales.is_contiguous() and (w.zeros is None or (tuple(w.zeros.shape) == (S, B, 16, per) and w.zeros.is_contiguous())), \
-        "weights as pack_int4 returns them"
+    for t, shape, dtypes in ((w.data, (S, B, 1024), (torch.uint8,)), (w.scales, (S, B, 16, per), (torch.bfloat16, torch.float16)), (w.zeros, (S, B, 16, per), (torch.uint8,))):
+        assert t is None or (tuple(t.shape) == shape and t.dtype in dtypes and t.is_contiguous()), "weights as pack_int4 returns them"
     dtype = out_dtype or (out.dtype if out is not None else x.dtype)
     if dtype not in _TYPES:
         raise NotImplementedError(f"{dtype} outputs are not built")
