@@ -28,8 +28,9 @@ extern "C" {
 #endif
 
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
- * 3: tamd_moe_layer, tamd_matvec, tamd_sample */
-#define TAMD_VERSION 3
+ * 3: tamd_moe_layer, tamd_matvec, tamd_sample
+ * 4: tamd_sample_workspace_exact */
+#define TAMD_VERSION 4
 
 /* error codes (negative) */
 #define TAMD_E_INVALID (-1)     /* bad shape / stride / pointer / enum */
@@ -470,7 +471,8 @@ int tamd_matvec(const tamd_matvec_args *args, size_t args_size, void *stream);
  * temperature <= 0 or NaN: the first of the order.  NaN logits count as -inf; a row of nothing but -inf gives -1; with +inf logits these
  * share the mass alike.  u is clamped to [0, 1), min_p to at most 1; a NaN top_p or min_p keeps all, a NaN u is 0.
  * temperature, top_k, top_p, min_p: per row if the pointer is given, else the value for all.  Limits: V <= 2^20, R <= 2^20.
- * workspace: tamd_sample_workspace(R, V) bytes on a 16-byte boundary, any contents; calls that may run at the same time need one each.
+ * workspace: on a 16-byte boundary, any contents; calls that may run at the same time need one each.  tamd_sample_workspace(R, V) bytes serve
+ * calls of up to R rows of V logits, tamd_sample_workspace_exact(R, V) a call of exactly R: large batches need next to nothing, but fewer rows may need more.
  */
 typedef struct tamd_sample_args {
   const void *logits;
@@ -490,6 +492,7 @@ typedef struct tamd_sample_args {
 } tamd_sample_args;
 
 int64_t tamd_sample_workspace(int R, int V);
+int64_t tamd_sample_workspace_exact(int R, int V);
 /* args_size: sizeof(tamd_sample_args) as the caller was compiled; other sizes are refused */
 int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream);
 

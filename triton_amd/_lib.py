@@ -179,6 +179,7 @@ _SIGNATURES = {
     "tamd_moe_layer_workspace": ([_INT, _INT, _INT], C.c_int64),
     "tamd_moe_layer": ([C.POINTER(MoeLayerArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_sample_workspace": ([_INT, _INT], C.c_int64),
+    "tamd_sample_workspace_exact": ([_INT, _INT], C.c_int64),
     "tamd_sample": ([C.POINTER(SampleArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_matvec": ([C.POINTER(MatvecArgs), C.c_size_t, _PTR], C.c_int),
 }

@@ -38,7 +38,7 @@ def load():
                            "`python -m triton_amd.build`")
     addresses = {n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
                  for n in ("tamd_matmul_sized", "tamd_routing_gates", "tamd_reduce", "tamd_downcast_mxfp", "tamd_upcast_mxfp", "tamd_moe_layer",
-                           "tamd_moe_layer_workspace", "tamd_matvec", "tamd_sample", "tamd_sample_workspace")}
+                           "tamd_moe_layer_workspace", "tamd_matvec", "tamd_sample", "tamd_sample_workspace_exact")}
     host.init(addresses, Tensor, CDNA4MXValueLayout, CDNA4MXScaleLayout, FP4, opt_flags._opt_flags_constraints,
               opt_flags._opt_flags, Int4Weights, PrecisionConfig.flex_ctx)
     for name in _FUNCTIONS:

@@ -977,7 +977,7 @@ PyObject *py_init(PyObject *, PyObject *args) {
   if (!take("tamd_matmul_sized", &abi.matmul) || !take("tamd_routing_gates", &abi.routing) || !take("tamd_reduce", &abi.reduce) ||
       !take("tamd_downcast_mxfp", &abi.downcast) || !take("tamd_upcast_mxfp", &abi.upcast) || !take("tamd_moe_layer", &abi.moe_layer) ||
       !take("tamd_moe_layer_workspace", &abi.moe_layer_workspace) || !take("tamd_matvec", &abi.matvec) || !take("tamd_sample", &abi.sample) ||
-      !take("tamd_sample_workspace", &abi.sample_workspace)) {
+      !take("tamd_sample_workspace_exact", &abi.sample_workspace)) {
     PyErr_SetString(PyExc_RuntimeError, "an entry point of the library is missing");
     return nullptr;
   }

@@ -31,8 +31,9 @@ constexpr int kRowsAtOnce = 4096;           // of one round of launches (the wor
 
 // Whether a workgroup does a row alone.  That takes about 9 us and one for every 2000 logits, as often as there are rows for a CU; the
 // five launches take 24 and one for every 1600 logits of a CU's share.  Measured: 1 row of 8192 13.7 and 24.0, of 32000 25.0 and 25.0,
-// of 65536 41 and 26; 256 rows of 65536 48 and 63.
-inline bool sample_whole(int R, int V, int cus) {
+// of 65536 41 and 26; 256 rows of 65536 48 and 63.  (By the 256 CUs of a whole MI355X on any device: the size of the workspace goes by it.)
+inline bool sample_whole(int R, int V) {
+  constexpr int cus = 256;
   return V <= kShort || (int64_t)((R + cus - 1) / cus) * (18000 + V) <= 48000 + (int64_t)R * V / cus * 5 / 4;
 }
 
@@ -818,12 +819,12 @@ __global__ __launch_bounds__(kThreads) void whole_row_kernel(tamd_sample_args a)
 
 template <int DT>
 int launch_sample(const tamd_sample_args &args, hipStream_t st) {
-  int cus = 0;
-  if (int rc = cu_count(cus)) return rc;
-  if (sample_whole(args.R, args.V, cus)) {
+  if (sample_whole(args.R, args.V)) {
     whole_row_kernel<DT><<<args.R, kThreads, 0, st>>>(args);
     return launch_status();
   }
+  int cus = 0;
+  if (int rc = cu_count(cus)) return rc;
   for (int r = 0; r < args.R; r += kRowsAtOnce) {
     tamd_sample_args a = args;
     a.R = args.R - r < kRowsAtOnce ? args.R - r : kRowsAtOnce;
@@ -858,6 +859,11 @@ using namespace tamd;
 extern "C" int64_t tamd_sample_workspace(int R, int V) {
   if (R < 0 || V < 0) return TAMD_E_INVALID;
   return V <= kShort ? 16 : (R < kRowsAtOnce ? R : kRowsAtOnce) * kRowBytes + 16;
+}
+
+extern "C" int64_t tamd_sample_workspace_exact(int R, int V) {
+  if (R < 0 || V < 0) return TAMD_E_INVALID;
+  return sample_whole(R, V) ? 16 : tamd_sample_workspace(R, V);
 }
 
 extern "C" int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream) {

@@ -65,7 +65,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
         return tokens
     L = _lib.lib()
     with torch.cuda.device(logits.device):
-        workspace = torch.empty(L.tamd_sample_workspace(R, V), dtype=torch.uint8, device=logits.device)
+        workspace = torch.empty(L.tamd_sample_workspace_exact(R, V), dtype=torch.uint8, device=logits.device)
         a.logits, a.logits_stride, a.u = logits.data_ptr(), logits.stride(0), u.data_ptr()
         a.tokens, a.workspace = tokens.data_ptr(), workspace.data_ptr()
         _lib.check(L.tamd_sample(ctypes.byref(a), ctypes.sizeof(a), _lib.stream_ptr(logits.device)), "sample")
