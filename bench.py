@@ -69,17 +69,23 @@ CONFIG_RUNS = (("c1_dense", "c1_dense"), ("c2_routing", "c2_routing"), ("c4_deco
 
 
 # ---------------------------------------------------------------------------------------------------------------------
-# HBM traffic of the dominant kernels: measured with rocprofv3 counters outside this process and kept, with the digest
-# of the kernel sources it was measured on, in profiles/hbm_traffic.txt
+# HBM traffic of the dominant kernels, those of the grouped matmul: measured with rocprofv3 counters outside this process and kept, with the
+# digest of the sources that these are built from, in profiles/hbm_traffic.txt
 # ---------------------------------------------------------------------------------------------------------------------
 def kernel_sources_digest():
-    """sha256 over the kernel sources (csrc/*.h, *.hip, *.cpp and the C header), in name order."""
+    """sha256 over csrc/moe_matmul*.hip and what they include from that folder, in name order: other operators' sources may change
+    without these kernels (the C header only declares)."""
     h = hashlib.sha256()
     csrc = os.path.join(ROOT, "triton_amd", "csrc")
-    files = sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".h", ".hip", ".cpp")))
-    for path in files + [os.path.join(ROOT, "include", "triton_amd.h")]:
-        h.update(os.path.basename(path).encode())
-        h.update(open(path, "rb").read())
+    files, found = {}, [f for f in os.listdir(csrc) if f.startswith("moe_matmul") and f.endswith(".hip")]
+    while found:
+        name = found.pop()
+        with open(os.path.join(csrc, name), "rb") as f:
+            files[name] = f.read()
+        found += [i for i in re.findall(r'^#include "([^"/]+)"', files[name].decode(), re.M) if i not in files]
+    for name in sorted(files):
+        h.update(name.encode())
+        h.update(files[name])
     return h.hexdigest()[:16]
 
 
