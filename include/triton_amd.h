@@ -394,7 +394,7 @@ int tamd_swiglu(const void *a, int dtype, int64_t M, int64_t N_out, int64_t a_st
  * picks and g as tamd_topk_forward with softmax gives them (ties: lower column; g stays float32), swiglu over the column pairs
  * (2i, 2i+1) as in tamd_matmul, but a NaN passes the clamps.  x, y F16 or BF16 (one type), logits and biases F32 / F16 / BF16, weights MXFP4 contiguous
  * along K or in 4 KB blocks, scales strided or pre-shuffled, each product its own.  h is held in the workspace with twice the
- * bits of x's type (F16: to a multiple of 2^-24, infinite from 65520 on); sums and the activation are float32; y is rounded once.
+ * bits of x's type (F16: to a multiple of 2^-35, infinite from 65520 on); sums and the activation are float32; y is rounded once.
  * Limits: n_tokens <= 64, n_experts <= 512, 1 <= n_picks <= min(n_experts, 16), n_tokens * n_picks <= 512 (TAMD_E_TOO_LARGE);
  * hidden and inter multiples of 32; x rows and strided weight columns start on 16-byte boundaries (TAMD_E_ALIGNMENT).
  * workspace: tamd_moe_layer_workspace(n_tokens, n_picks, inter) bytes on a 16-byte boundary, any contents; calls that may

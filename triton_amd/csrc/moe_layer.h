@@ -15,7 +15,8 @@
 //
 // h is kept as two 16-bit planes, its rounding and what that leaves (16 bits more), each a row of its own in the tile of the
 // down projection: with up to eight tokens these rows are there anyhow, and the layer's error is that of its one rounding
-// at the end.  The gate weights enter h in float32 before that.
+// at the end.  The gate weights enter h in float32 before that.  With float16 the second plane is 2^11 times as large, which its sums are
+// divided by: what a rounding leaves is at most half of the value then, and not lost below float16's smallest step.
 //
 // v_mfma_f32_16x16x32: lane (c = lane % 16, h = lane / 16) is row c of A and column c of B.  A block of 128 K is read as
 // 16 bytes (32 codes, one scale) per lane: lane (c, h) takes group h of column c, consumed 8 K at a time by four MFMAs.
@@ -29,6 +30,8 @@ constexpr int kMoeTokens = 64;     // a token is a bit of a 64-bit mask per expe
 constexpr int kMoeExperts = 512;   // one thread each
 constexpr int kMoePicks = 16;
 constexpr int kMoeSlots = 512;     // picks of all tokens
+template <int XDT>
+constexpr float kMoeRest = XDT == TAMD_F16 ? 0x1p11f : 1.f;   // of the second plane of h
 constexpr uint32_t kMoeOob = 0x7FFFFFF0u;   // past the end of every buffer: such a load gives zeros
 
 // What the first launch hands to the second, at the start of the workspace.
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(512, 2) void moe_up_kernel(tamd_moe_layer_args a) {
       const float v = r.row_gate[row] * swiglu_keeping_nan(a, g, l);
       const uint32_t hi = XDT == TAMD_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
       const float rest = v - (XDT == TAMD_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi));
-      const float lo = rest - rest == 0.f ? rest : 0.f;   // (infinities leave nothing)
+      const float lo = rest - rest == 0.f ? kMoeRest<XDT> * rest : 0.f;   // (infinities leave nothing)
       uint16_t *p = planes + (int64_t)row * 2 * I + 16 * done.strip + pair;
       p[0] = (uint16_t)hi;
       p[I] = (uint16_t)(XDT == TAMD_BF16 ? f32_to_bf16_bits(lo) : f32_to_f16_bits(lo));
@@ -576,7 +579,7 @@ __global__ __launch_bounds__(512, 2) void moe_down_kernel(tamd_moe_layer_args a)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t of = 2u * h + e;
-        if (live && of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * e] + acc[2 * e + 1];
+        if (live && of < RC && t0 + of < rows) sums[(wave * T + s.token[row + t0 + of]) * 16 + (int)c] += acc[2 * e] + 1.f / kMoeRest<XDT> * acc[2 * e + 1];
       }
     };
     tile(st.x, 0);
