@@ -407,8 +407,8 @@ struct MoeDownLds {
 };
 static_assert(sizeof(MoeDownLds) % 16 == 0);
 // The experts of all strips of 16 columns, strip by strip, are dealt out evenly to up to `shares` workgroups, none of which has none:
-// where one begins, and whose an expert of a strip is.  (Less than 2^24 of them, so that 32 bits do: with divisions of 64 the two
-// launches took 2 us longer, 5 tokens of 32 experts of 2016 x 1056 33.2 instead of 31.0.)
+// where one begins, and whose an expert of a strip is.  (Less than 2^24 of them, so that 32 bits do.  Divisions of 64 take as long: 5 tokens of 32
+// experts of 2016 x 1056 15.2 us for the down projection and 3.9 for the join either way.)
 constexpr int64_t kMoeDealt = 1 << 24;
 struct MoeDeal {
   uint32_t items, shares;

@@ -771,7 +771,7 @@ __global__ __launch_bounds__(kThreads) void finish_kernel(tamd_sample_args a, Wo
   if (tid == 0) a.tokens[r] = token;
 }
 
-// All of it for a row, in LDS: three reads of the row, and what bounds it is their arithmetic, some 70 instructions a logit.
+// All of it for a row, in LDS: three reads of the row, and what bounds it is their arithmetic, 75 instructions a logit (13, 38 and 25).
 template <int DT>
 __global__ __launch_bounds__(kThreads) void whole_row_kernel(tamd_sample_args a) {
   __shared__ uint64_t list[kMost], mass[kBins + 1];
