@@ -440,8 +440,8 @@ int tamd_moe_layer(const tamd_moe_layer_args *args, size_t args_size, void *stre
  *   codes   uint8 [S, B, 4 h, 16 c, 4 t, 4]: dword t of lane (h, c) holds K 128 b + 32 t + 8 h .. + 8 of column 16 s + c, the code of the
  *           chunk's K 2 i in bits 4 i .. and that of K 2 i + 1 in bits 16 + 4 i ..;
  *   scales  [S, B, 16 c, 128 / group],  zeros  uint8, laid out like the scales.
- * A row of x with a NaN or an infinity gives NaN; finite rows of any size give what float32 holds of the result (BF16: |x| below 2^-117 may count
- * as 0).  What pads columns and K may hold anything but NaN and infinite scales; x rows start on 16-byte boundaries, codes, scales and
+ * A row of x with a NaN or an infinity gives NaN; finite rows of any size give what float32 holds of the result (BF16: to a
+ * multiple of 2^-137).  What pads columns and K may hold anything but NaN and infinite scales; x rows start on 16-byte boundaries, codes, scales and
  * zeros too.  Made for up to 64 rows: up to 16 read the weights once, and so do up to 64 where there are more than two strips per CU; with fewer strips 17 to 64 rows
  * are cut into parts of 16 to 48 that read them each, mostly from the caches.  More rows are cut alike, into parts of 64 at most.
  */

@@ -45,9 +45,14 @@ def test_largest_values(M, K, extra, strips, group, zeros, device):
 
 @pytest.mark.parametrize("M,K,extra,strips", CALLS)
 def test_small_values(M, K, extra, strips, device):
-    """Values of 2^-117 on: no bits lost."""
+    """Values of 2^-117 on, and of bfloat16's smallest normal and subnormal ones: no bits lost."""
     K = -(-K // 64) * 64
     N = columns(device, extra, strips) if strips else extra
     w, dense, mag = weights(K, N, 64, True, device, 2.0**20)
     x = (torch.randn(M, K, generator=torch.Generator().manual_seed(M)).abs() + 1).to(torch.bfloat16) * 2.0**-117
     check(matvec(x.to(device), w, out_dtype=torch.float32), x, dense, mag)
+    least = 2.0**-126 * (torch.arange(M * K).view(M, K) % 257 - 128).double() / 128   # (multiples of 2^-133, both signs)
+    for least in (least, least * (torch.arange(K) % 61 == 5)):
+        x = least.to(torch.bfloat16)
+        assert torch.equal(x.double(), least) and x.any()
+        check(matvec(x.to(device), w, out_dtype=torch.float32), x, dense, mag)

@@ -14,7 +14,8 @@
 //
 // With bf16 rows all of these numbers, and the ones, are 2^-12 of that, and the result is 2^12 times the sums: 128 values of up to 2^128 times up to
 // 31 stay within float32, so every finite row has finite sums before its scales come in.  (Without it one x from 1e37 on, or a
-// group of one sign from 1e35 on, made a row infinite or NaN.  At the other end products are no longer normal below |x| of 2^-117.)
+// group of one sign from 1e35 on, made a row infinite or NaN.  At the other end the matrix unit keeps subnormal numbers: products are exact down to
+// bf16's smallest, and sums of 2^-149 steps leave results to a multiple of 2^-137.)
 #pragma once
 #include "moe_layer.h"
 

@@ -79,7 +79,7 @@ def matvec(x: torch.Tensor, w: Int4Weights, bias: Optional[torch.Tensor] = None,
 
     bias: [N] or None; out_dtype: float32, bfloat16 or float16 (default: x's type); out: where the result goes, which must not overlap
     an input.  Weights are not rounded, sums are float32, the result is rounded once; a row of x with a NaN or an infinity gives NaN,
-    any finite one a finite result where float32 holds it (bf16: |x| below 2^-117 may count as 0).  The kernels are
+    any finite one a finite result where float32 holds it (bf16: to a multiple of 2^-137).  The kernels are
     made for up to 64 rows.  Up to 16 read the weights once, and so do up to 64 where there are more than 32 columns per CU; with fewer columns 17 to
     64 rows are cut into parts of 16 to 48 that read them each, mostly from the caches.  More rows are cut alike, into parts of 64 at most."""
     if out is None:
