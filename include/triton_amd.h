@@ -29,8 +29,9 @@ extern "C" {
 
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
  * 3: tamd_moe_layer, tamd_matvec, tamd_sample
- * 4: tamd_sample_workspace_exact */
-#define TAMD_VERSION 4
+ * 4: tamd_sample_workspace_exact
+ * 5: tamd_dispatch, tamd_combine */
+#define TAMD_VERSION 5
 
 /* error codes (negative) */
 #define TAMD_E_INVALID (-1)     /* bad shape / stride / pointer / enum */
@@ -496,6 +497,37 @@ int64_t tamd_sample_workspace(int R, int V);
 int64_t tamd_sample_workspace_exact(int R, int V);
 /* args_size: sizeof(tamd_sample_args) as the caller was compiled; other sizes are refused */
 int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Rows of tokens to the rows of their experts and back, and the gradients of both.  p[t,j] = row_indx[t * row_indx_stride + j] is the
+ * expert row of pick j of token t (outside [0, n_rows): none), g[t,j] its gate weight (1 without gates):
+ *   tamd_dispatch   dst[p[t,j], :] = g[t,j] src[t, :]             dots[t,j] = <src[t, :], other[p[t,j], :]>
+ *   tamd_combine    dst[t, :] = sum_j g[t,j] src[p[t,j], :]       dots[t,j] = <other[t, :], src[p[t,j], :]>
+ * Without a row a pick adds nothing, and its dot is 0; tamd_dispatch leaves rows of dst that no pick names as they are, and rows that
+ * several picks name hold one of them, or a mixture.  Sums are float32, in the order of j; results are rounded once.
+ * dots (and with it other): NULL, or [T, k] in gates_dtype.  src, dst and other are of `dtype` (float32, bfloat16, float16), with unit stride along
+ * H and any row pitch; rows that all start on 16-byte boundaries are the fast form.  dst overlaps nothing that is read.
+ */
+typedef struct tamd_token_rows_args {
+  const void *src;
+  int64_t src_stride;
+  void *dst;
+  int64_t dst_stride;
+  const int32_t *row_indx;
+  int64_t row_indx_stride;
+  const void *gates;
+  int64_t gates_stride;
+  const void *other;
+  int64_t other_stride;
+  void *dots;
+  int64_t dots_stride;
+  int dtype, gates_dtype;
+  int T, k, H, n_rows;
+} tamd_token_rows_args;
+
+/* args_size: sizeof(tamd_token_rows_args) as the caller was compiled; other sizes are refused */
+int tamd_dispatch(const tamd_token_rows_args *args, size_t args_size, void *stream);
+int tamd_combine(const tamd_token_rows_args *args, size_t args_size, void *stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ def install_as_triton_kernels():
     me = sys.modules[__name__]
     sys.modules.setdefault("triton_kernels", me)
     for sub in ("tensor", "topk", "routing", "numerics", "numerics_details", "numerics_details.mxfp", "matmul",
-                "matmul_details", "matmul_details.opt_flags", "swiglu", "reduce", "moe_layer", "matvec", "sampling", "specialize", "testing",
+                "matmul_details", "matmul_details.opt_flags", "swiglu", "reduce", "dispatch", "moe_layer", "matvec", "sampling", "specialize", "testing",
                 "tensor_details", "tensor_details.layout", "tensor_details.ragged_tensor",
                 "tensor_details.bitmatrix", "tensor_details.dtype", "tensor_details.layout_details",
                 "tensor_details.layout_details.base", "tensor_details.layout_details.strided",

@@ -146,6 +146,16 @@ class SampleArgs(C.Structure):
     ]
 
 
+class TokenRowsArgs(C.Structure):
+    """Mirror of `tamd_token_rows_args`."""
+    _fields_ = [
+        ("src", C.c_void_p), ("src_stride", C.c_int64), ("dst", C.c_void_p), ("dst_stride", C.c_int64),
+        ("row_indx", C.c_void_p), ("row_indx_stride", C.c_int64), ("gates", C.c_void_p), ("gates_stride", C.c_int64),
+        ("other", C.c_void_p), ("other_stride", C.c_int64), ("dots", C.c_void_p), ("dots_stride", C.c_int64),
+        ("dtype", C.c_int), ("gates_dtype", C.c_int), ("T", C.c_int), ("k", C.c_int), ("H", C.c_int), ("n_rows", C.c_int),
+    ]
+
+
 _I64, _INT, _PTR, _F = C.c_int64, C.c_int, C.c_void_p, C.c_float
 _SIGNATURES = {
     "tamd_version": ([], C.c_int),
@@ -182,6 +192,8 @@ _SIGNATURES = {
     "tamd_sample_workspace_exact": ([_INT, _INT], C.c_int64),
     "tamd_sample": ([C.POINTER(SampleArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_matvec": ([C.POINTER(MatvecArgs), C.c_size_t, _PTR], C.c_int),
+    "tamd_dispatch": ([C.POINTER(TokenRowsArgs), C.c_size_t, _PTR], C.c_int),
+    "tamd_combine": ([C.POINTER(TokenRowsArgs), C.c_size_t, _PTR], C.c_int),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -1,0 +1,301 @@
+// Rows of tokens to the rows of their experts and back, with gate weights, and the gradients of both.
+//
+// p[t, j] is the expert row of pick j of token t (anything outside [0, n_rows): none), g[t, j] its gate weight (1 without gates):
+//   spread    dst[p[t,j], :] = g[t,j] src[t, :]           dots[t,j] = <src[t, :], other[p[t,j], :]>
+//   collect   dst[t, :] = sum_j g[t,j] src[p[t,j], :]     dots[t,j] = <other[t, :], src[p[t,j], :]>
+// `spread` is the dispatch and, with dots, the gradient of the sum; `collect` the sum over the picks and, with dots, the gradient of
+// the dispatch.  Both go by token, so that a token's row is read (or written) once whatever k is, and its k expert rows are whole,
+// contiguous pieces of memory.  Sums are float32 in the order of j, a dot's partial sums are joined in a fixed order: no atomics.
+#include "common.h"
+
+using namespace tamd;
+
+namespace {
+
+constexpr int kPicks = 8;   // expert rows of a token that are handled together
+
+// 16 bytes of a row: V elements, aligned to 16 bytes or to an element only
+template <int DT>
+constexpr int kPiece = DT == TAMD_F32 ? 4 : 8;
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
+
+template <bool ALIGNED>
+TAMD_DEVICE u32x4_t load_raw(const void *row, int64_t i) {
+  if constexpr (ALIGNED) return *(const u32x4_t *)((const char *)row + i * 16);
+  else return *(const u32x4_by2_t *)((const char *)row + i * 16);
+}
+template <bool ALIGNED>
+TAMD_DEVICE void store_raw(void *row, int64_t i, u32x4_t q) {
+  if constexpr (ALIGNED) *(u32x4_t *)((char *)row + i * 16) = q;
+  else *(u32x4_by2_t *)((char *)row + i * 16) = q;
+}
+template <int DT>
+TAMD_DEVICE void widen(u32x4_t q, float (&v)[kPiece<DT>]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == TAMD_F32) {
+      v[e] = bits_to_f32(q[e]);
+    } else {
+      v[2 * e] = DT == TAMD_BF16 ? bf16_bits_to_f32(q[e] & 0xFFFFu) : f16_bits_to_f32(q[e] & 0xFFFFu);
+      v[2 * e + 1] = DT == TAMD_BF16 ? bf16_bits_to_f32(q[e] >> 16) : f16_bits_to_f32(q[e] >> 16);
+    }
+  }
+}
+template <int DT>
+TAMD_DEVICE u32x4_t narrow(const float (&v)[kPiece<DT>]) {
+  u32x4_t q;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (DT == TAMD_F32) q[e] = f32_to_bits(v[e]);
+    else if constexpr (DT == TAMD_BF16) q[e] = f32_to_bf16_bits(v[2 * e]) | (f32_to_bf16_bits(v[2 * e + 1]) << 16);
+    else q[e] = f32_to_f16_bits(v[2 * e]) | (f32_to_f16_bits(v[2 * e + 1]) << 16);
+  }
+  return q;
+}
+
+TAMD_DEVICE float load_gate(const void *p, int dt, int64_t i) {
+  return dt == TAMD_F32 ? load_as_f32<TAMD_F32>(p, i) : dt == TAMD_BF16 ? load_as_f32<TAMD_BF16>(p, i) : load_as_f32<TAMD_F16>(p, i);
+}
+TAMD_DEVICE void store_gate(void *p, int dt, int64_t i, float v) {
+  if (dt == TAMD_F32) store_from_f32<TAMD_F32>(p, i, v);
+  else if (dt == TAMD_BF16) store_from_f32<TAMD_BF16>(p, i, v);
+  else store_from_f32<TAMD_F16>(p, i, v);
+}
+
+TAMD_DEVICE float wave_sum(float v) {
+  return bits_to_f32(group_reduce<64>(f32_to_bits(v), [](uint32_t a, uint32_t b) { return f32_to_bits(bits_to_f32(a) + bits_to_f32(b)); }));
+}
+
+// What a wave (or the workgroup, WAVES of them) knows of its token: up to kPicks of its expert rows and their weights.
+struct Picks {
+  int32_t row[kPicks];
+  float gate[kPicks];
+};
+TAMD_DEVICE void load_picks(const tamd_token_rows_args &a, int64_t t, int j0, Picks &p) {
+#pragma unroll
+  for (int j = 0; j < kPicks; ++j) {
+    p.row[j] = -1;
+    p.gate[j] = 1.0f;
+    if (j0 + j < a.k) {
+      const int32_t r = __builtin_amdgcn_readfirstlane(a.row_indx[t * a.row_indx_stride + j0 + j]);
+      p.row[j] = (uint32_t)r < (uint32_t)a.n_rows ? r : -1;
+      if (a.gates) p.gate[j] = load_gate(a.gates, a.gates_dtype, t * a.gates_stride + j0 + j);
+    }
+  }
+}
+
+// dots of the picks j0 ..: the lanes' sums joined, and the waves' in their order
+template <int WAVES>
+TAMD_DEVICE void store_dots(const tamd_token_rows_args &a, int64_t t, int j0, const float (&dot)[kPicks], float *lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float all[kPicks];
+#pragma unroll
+  for (int j = 0; j < kPicks; ++j) all[j] = j0 + j < a.k ? wave_sum(dot[j]) : 0.f;
+  if constexpr (WAVES > 1) {
+    sync_threads();
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < kPicks; ++j) lds[wave * kPicks + j] = all[j];
+    }
+    sync_threads();
+#pragma unroll
+    for (int j = 0; j < kPicks; ++j) {
+      all[j] = lds[j];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) all[j] += lds[w * kPicks + j];
+    }
+    if (wave != 0) return;
+  }
+#pragma unroll
+  for (int j = 0; j < kPicks; ++j)
+    if (lane == j && j0 + j < a.k) store_gate(a.dots, a.gates_dtype, t * a.dots_stride + j0 + j, all[j]);
+}
+
+// WAVES waves to a token: 4 make a workgroup, or 1 of the 4 that a workgroup has.  Without gates rows are copied as bits.
+template <int DT, bool ALIGNED, int WAVES, bool DOTS, bool GATES>
+__global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
+  constexpr int V = kPiece<DT>, SIZE = 16 / V, LANES = 64 * WAVES;
+  __shared__ float lds[4 * kPicks];
+  const int64_t t = WAVES == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (t >= a.T) return;
+  const int at = threadIdx.x & (LANES - 1);
+  const char *const src = (const char *)a.src + t * a.src_stride * SIZE;
+  const int pieces = a.H / V, rest = a.H % V;
+  for (int j0 = 0; j0 < a.k; j0 += kPicks) {
+    Picks p;
+    load_picks(a, t, j0, p);
+    float dot[kPicks] = {};
+    for (int c = at; c < pieces; c += LANES) {
+      const u32x4_t q = load_raw<ALIGNED>(src, c);
+      float x[V];
+      widen<DT>(q, x);
+#pragma unroll
+      for (int j = 0; j < kPicks; ++j) {
+        if (p.row[j] < 0) continue;
+        if constexpr (DOTS) {
+          float y[V];
+          widen<DT>(load_raw<ALIGNED>((const char *)a.other + p.row[j] * a.other_stride * SIZE, c), y);
+#pragma unroll
+          for (int e = 0; e < V; ++e) dot[j] = __builtin_fmaf(x[e], y[e], dot[j]);
+        }
+        char *const row = (char *)a.dst + p.row[j] * a.dst_stride * SIZE;
+        if constexpr (GATES) {
+          float out[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) out[e] = x[e] * p.gate[j];
+          store_raw<ALIGNED>(row, c, narrow<DT>(out));
+        } else {
+          store_raw<ALIGNED>(row, c, q);
+        }
+      }
+    }
+    if (at < rest) {
+      const int64_t i = (int64_t)pieces * V + at;
+      const float x = load_as_f32<DT>(src, i);
+#pragma unroll
+      for (int j = 0; j < kPicks; ++j) {
+        if (p.row[j] < 0) continue;
+        if constexpr (DOTS) dot[j] = __builtin_fmaf(x, load_as_f32<DT>((const char *)a.other + p.row[j] * a.other_stride * SIZE, i), dot[j]);
+        char *const row = (char *)a.dst + p.row[j] * a.dst_stride * SIZE;
+        if constexpr (GATES) store_from_f32<DT>(row, i, x * p.gate[j]);
+        else if constexpr (DT == TAMD_F32) ((uint32_t *)row)[i] = ((const uint32_t *)src)[i];
+        else ((uint16_t *)row)[i] = ((const uint16_t *)src)[i];
+      }
+    }
+    if constexpr (DOTS) store_dots<WAVES>(a, t, j0, dot, lds);
+  }
+}
+
+template <int DT, bool ALIGNED, int WAVES, bool DOTS>
+__global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
+  constexpr int V = kPiece<DT>, SIZE = 16 / V, LANES = 64 * WAVES;
+  __shared__ float lds[4 * kPicks];
+  const int64_t t = WAVES == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (t >= a.T) return;
+  const int at = threadIdx.x & (LANES - 1);
+  char *const dst = (char *)a.dst + t * a.dst_stride * SIZE;
+  const char *const other = DOTS ? (const char *)a.other + t * a.other_stride * SIZE : nullptr;
+  const int pieces = a.H / V, rest = a.H % V;
+  const bool few = a.k <= kPicks;    // all picks at once: their dots come with the sum
+  Picks p;
+  load_picks(a, t, 0, p);
+  float dot[kPicks] = {};
+  for (int c = at; c < pieces; c += LANES) {
+    float sum[V] = {}, x[V];
+    if constexpr (DOTS) widen<DT>(load_raw<ALIGNED>(other, c), x);
+    for (int j0 = 0; j0 < a.k; j0 += kPicks) {
+      if (j0) load_picks(a, t, j0, p);
+#pragma unroll
+      for (int j = 0; j < kPicks; ++j) {
+        if (p.row[j] < 0) continue;
+        float y[V];
+        widen<DT>(load_raw<ALIGNED>((const char *)a.src + p.row[j] * a.src_stride * SIZE, c), y);
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] = __builtin_fmaf(y[e], p.gate[j], sum[e]);
+        if constexpr (DOTS) {
+          if (few) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) dot[j] = __builtin_fmaf(x[e], y[e], dot[j]);
+          }
+        }
+      }
+    }
+    if (!few) load_picks(a, t, 0, p);
+    store_raw<ALIGNED>(dst, c, narrow<DT>(sum));
+  }
+  if (at < rest) {
+    const int64_t i = (int64_t)pieces * V + at;
+    float sum = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+      const int32_t r = a.row_indx[t * a.row_indx_stride + j];
+      if ((uint32_t)r >= (uint32_t)a.n_rows) continue;
+      const float g = a.gates ? load_gate(a.gates, a.gates_dtype, t * a.gates_stride + j) : 1.0f;
+      sum = __builtin_fmaf(load_as_f32<DT>((const char *)a.src + r * a.src_stride * SIZE, i), g, sum);
+    }
+    store_from_f32<DT>(dst, i, sum);
+  }
+  if constexpr (DOTS) {
+    for (int j0 = 0; j0 < a.k; j0 += kPicks) {
+      if (!few) {
+        load_picks(a, t, j0, p);
+#pragma unroll
+        for (int j = 0; j < kPicks; ++j) dot[j] = 0.f;
+        for (int c = at; c < pieces; c += LANES) {
+          float x[V];
+          widen<DT>(load_raw<ALIGNED>(other, c), x);
+#pragma unroll
+          for (int j = 0; j < kPicks; ++j) {
+            if (p.row[j] < 0) continue;
+            float y[V];
+            widen<DT>(load_raw<ALIGNED>((const char *)a.src + p.row[j] * a.src_stride * SIZE, c), y);
+#pragma unroll
+            for (int e = 0; e < V; ++e) dot[j] = __builtin_fmaf(x[e], y[e], dot[j]);
+          }
+        }
+      }
+      if (at < rest) {
+        const int64_t i = (int64_t)pieces * V + at;
+        const float x = load_as_f32<DT>(other, i);
+#pragma unroll
+        for (int j = 0; j < kPicks; ++j)
+          if (p.row[j] >= 0) dot[j] = __builtin_fmaf(x, load_as_f32<DT>((const char *)a.src + p.row[j] * a.src_stride * SIZE, i), dot[j]);
+      }
+      store_dots<WAVES>(a, t, j0, dot, lds);
+    }
+  }
+}
+
+// Four waves to a token where one each would leave CUs idle or a wave with a long row.
+template <int DT, bool ALIGNED, bool DOTS, bool GATES>
+int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
+  const bool wide = a.T <= 4096;
+  const dim3 grid(wide ? (unsigned)a.T : (unsigned)(((int64_t)a.T + 3) / 4));
+  if (spread) {
+    if (wide) spread_kernel<DT, ALIGNED, 4, DOTS, GATES><<<grid, 256, 0, st>>>(a);
+    else spread_kernel<DT, ALIGNED, 1, DOTS, GATES><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (wide) collect_kernel<DT, ALIGNED, 4, DOTS><<<grid, 256, 0, st>>>(a);
+    else collect_kernel<DT, ALIGNED, 1, DOTS><<<grid, 256, 0, st>>>(a);
+  }
+  return launch_status();
+}
+template <int DT, bool ALIGNED>
+int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
+  if (a.dots) return a.gates ? launch<DT, ALIGNED, true, true>(a, spread, st) : launch<DT, ALIGNED, true, false>(a, spread, st);
+  return a.gates ? launch<DT, ALIGNED, false, true>(a, spread, st) : launch<DT, ALIGNED, false, false>(a, spread, st);
+}
+
+template <int DT>
+int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
+  const int size = DT == TAMD_F32 ? 4 : 2;
+  const auto whole = [&](const void *p, int64_t stride) { return ((uintptr_t)p | (uintptr_t)(stride * size)) % 16 == 0; };
+  const bool aligned = whole(a.src, a.src_stride) && whole(a.dst, a.dst_stride) && (!a.dots || whole(a.other, a.other_stride));
+  return aligned ? launch<DT, true>(a, spread, st) : launch<DT, false>(a, spread, st);
+}
+
+int token_rows(const tamd_token_rows_args *args, size_t args_size, bool spread, void *stream) {
+  if (!args || args_size != sizeof(tamd_token_rows_args)) return TAMD_E_INVALID;
+  const tamd_token_rows_args &a = *args;
+  const auto plain = [](int dt) { return dt == TAMD_F32 || dt == TAMD_BF16 || dt == TAMD_F16; };
+  if (a.T < 0 || a.k < 0 || a.H < 0 || a.n_rows < 0) return TAMD_E_INVALID;
+  if (!plain(a.dtype) || ((a.gates || a.dots) && !plain(a.gates_dtype))) return TAMD_E_UNSUPPORTED;
+  if (a.src_stride < 0 || a.dst_stride < 0 || a.other_stride < 0 || a.row_indx_stride < 0 || a.gates_stride < 0 || a.dots_stride < 0) return TAMD_E_INVALID;
+  if (a.T == 0 || (spread && a.k == 0)) return 0;
+  if (a.k > 0 && !a.row_indx) return TAMD_E_INVALID;
+  // (without expert rows there is nothing behind their pointers)
+  const void *const by_row = spread ? a.dst : a.src, *const by_token = spread ? a.src : a.dst, *const kept_rows = spread ? a.other : nullptr;
+  const void *const kept_tokens = spread ? nullptr : a.other;
+  if (a.H > 0 && (!by_token || (a.n_rows > 0 && !by_row))) return TAMD_E_INVALID;
+  if (a.H > 0 && a.dots && (spread ? a.n_rows > 0 && !kept_rows : !kept_tokens)) return TAMD_E_INVALID;
+  if (a.H == 0 && !a.dots) return 0;
+  const uintptr_t by = a.dtype == TAMD_F32 ? 4 : 2;
+  if (((uintptr_t)a.src | (uintptr_t)a.dst | (uintptr_t)(a.dots ? a.other : nullptr)) % by != 0) return TAMD_E_ALIGNMENT;
+  hipStream_t st = (hipStream_t)stream;
+  return a.dtype == TAMD_F32 ? launch<TAMD_F32>(a, spread, st) : a.dtype == TAMD_BF16 ? launch<TAMD_BF16>(a, spread, st) : launch<TAMD_F16>(a, spread, st);
+}
+
+}  // namespace
+
+extern "C" int tamd_dispatch(const tamd_token_rows_args *args, size_t args_size, void *stream) { return token_rows(args, args_size, true, stream); }
+extern "C" int tamd_combine(const tamd_token_rows_args *args, size_t args_size, void *stream) { return token_rows(args, args_size, false, stream); }
