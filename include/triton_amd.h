@@ -30,7 +30,7 @@ extern "C" {
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
  * 3: tamd_moe_layer, tamd_matvec, tamd_sample
  * 4: tamd_sample_workspace_exact
- * 5: tamd_dispatch, tamd_combine */
+ * 5: tamd_dispatch, tamd_combine, tamd_swiglu_checkpoint, tamd_swiglu_backward */
 #define TAMD_VERSION 5
 
 /* error codes (negative) */
@@ -528,6 +528,22 @@ typedef struct tamd_token_rows_args {
 /* args_size: sizeof(tamd_token_rows_args) as the caller was compiled; other sizes are refused */
 int tamd_dispatch(const tamd_token_rows_args *args, size_t args_size, void *stream);
 int tamd_combine(const tamd_token_rows_args *args, size_t args_size, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Interleaved SwiGLU (tamd_swiglu) whose input is kept in 8 bits, and its gradient from what was kept.  With g = min(a[2n], limit),
+ * l = clamp(a[2n+1], -limit, limit), s = 1 / (1 + exp(-alpha g)):
+ *   out[n] = g s (l + 1);   da[2n] = dout[n] (l + 1) s (1 + alpha g (1 - s)),   da[2n+1] = dout[n] g s,   0 beyond the limit
+ * a, da: [M, 2N]; out, dout: [M, N], all of `dtype` (float32, bfloat16, float16) with unit stride along a row.  values: [M, 2N] e4m3 bytes,
+ * scales: [M, ceil(2N / 32)] e8m0 bytes, what tamd_downcast_mxfp makes of a row (TAMD_ROUND_UP; the last group may be short).  NaN stays NaN, also in a
+ * clamped value; an infinity, and the group of 32 that it is in, is NaN in what is kept.  tamd_swiglu_backward computes at the kept values, and writes out
+ * there again unless it is NULL.  Arithmetic is float32, results are rounded once.  Outputs overlap nothing that is read.
+ */
+int tamd_swiglu_checkpoint(const void *a, int dtype, int64_t M, int64_t N, int64_t a_stride, void *out, int64_t out_stride,
+                           uint8_t *values, int64_t values_stride, uint8_t *scales, int64_t scales_stride, float alpha,
+                           float limit, int has_limit, void *stream);
+int tamd_swiglu_backward(const void *dout, int dtype, int64_t M, int64_t N, int64_t dout_stride, const uint8_t *values,
+                         int64_t values_stride, const uint8_t *scales, int64_t scales_stride, void *da, int64_t da_stride,
+                         void *out, int64_t out_stride, float alpha, float limit, int has_limit, void *stream);
 
 #ifdef __cplusplus
 }

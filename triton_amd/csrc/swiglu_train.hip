@@ -1,0 +1,309 @@
+// SwiGLU for training: the forward pass keeps its input in 8 bits, the backward pass works from that.
+//
+//   g = min(a[2n], limit), l = clamp(a[2n + 1], -limit, limit), s = 1 / (1 + exp(-alpha g))
+//   out[n]  = g s (l + 1)
+//   da[2n]  = dout[n] (l + 1) s (1 + alpha g (1 - s))   where a[2n] <= limit, else 0
+//   da[2n + 1] = dout[n] g s                            where |a[2n + 1]| <= limit, else 0
+//
+// What is kept is the MXFP8 form of a that tamd_downcast_mxfp makes of it (e4m3 values, one e8m0 scale per 32 along a row, rounded up):
+// 1.03 bytes per value in place of the 2 of a itself.  The gradient is that of the function at the kept values.
+//
+// Four lanes share a group of 32, eight values (four pairs) each, U groups per thread.
+#include "mx_values.h"
+#include <type_traits>
+
+using namespace tamd;
+
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_by1_t __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_by1_t __attribute__((ext_vector_type(2), aligned(1)));
+
+template <bool ALIGNED>
+TAMD_DEVICE u32x4_t load16(const void *p) {
+  if constexpr (ALIGNED) return *(const u32x4_t *)p;
+  else return *(const u32x4_by1_t *)p;
+}
+template <bool ALIGNED>
+TAMD_DEVICE u32x2_t load8(const void *p) {
+  if constexpr (ALIGNED) return *(const u32x2_t *)p;
+  else return *(const u32x2_by1_t *)p;
+}
+template <bool ALIGNED>
+TAMD_DEVICE void store16(void *p, u32x4_t q) {
+  if constexpr (ALIGNED) *(u32x4_t *)p = q;
+  else *(u32x4_by1_t *)p = q;
+}
+template <bool ALIGNED>
+TAMD_DEVICE void store8(void *p, u32x2_t q) {
+  if constexpr (ALIGNED) *(u32x2_t *)p = q;
+  else *(u32x2_by1_t *)p = q;
+}
+
+TAMD_DEVICE float widen16(uint32_t bits, int dt) { return dt == TAMD_BF16 ? bf16_bits_to_f32(bits) : f16_bits_to_f32(bits); }
+template <int DT>
+TAMD_DEVICE uint32_t pack2(float a, float b) {
+  if constexpr (DT == TAMD_BF16) return f32_to_bf16_bits(a) | (f32_to_bf16_bits(b) << 16);
+  return f32_to_f16_bits(a) | (f32_to_f16_bits(b) << 16);
+}
+
+// N (4 or 8) elements at p, of which `n` are there
+template <int DT, bool ALIGNED, int N>
+TAMD_DEVICE void load_values(const void *p, int n, float (&v)[N]) {
+  if (n == N) {
+    if constexpr (DT == TAMD_F32) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const u32x4_t q = load16<ALIGNED>((const float *)p + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i + e] = bits_to_f32(q[e]);
+      }
+    } else if constexpr (N == 8) {
+      const u32x4_t q = load16<ALIGNED>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[2 * e] = widen16(q[e] & 0xFFFFu, DT), v[2 * e + 1] = widen16(q[e] >> 16, DT);
+    } else {
+      const u32x2_t q = load8<ALIGNED>(p);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v[2 * e] = widen16(q[e] & 0xFFFFu, DT), v[2 * e + 1] = widen16(q[e] >> 16, DT);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = e < n ? load_as_f32<DT>(p, e) : 0.f;
+  }
+}
+template <int DT, bool ALIGNED, int N>
+TAMD_DEVICE void store_values(void *p, int n, const float (&v)[N]) {
+  if (n == N) {
+    if constexpr (DT == TAMD_F32) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4)
+        store16<ALIGNED>((float *)p + i, u32x4_t{f32_to_bits(v[i]), f32_to_bits(v[i + 1]), f32_to_bits(v[i + 2]), f32_to_bits(v[i + 3])});
+    } else if constexpr (N == 8) {
+      store16<ALIGNED>(p, u32x4_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])});
+    } else {
+      store8<ALIGNED>(p, u32x2_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])});
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < n) store_from_f32<DT>(p, e, v[e]);
+  }
+}
+
+struct GluShape {
+  GroupDiv div;            // rows and groups of a row
+  int64_t L;               // values of a row: 2 N
+  float alpha, limit;
+  int has_limit;
+};
+
+// The clamped pair and the gate's sigmoid, by exp2 and a reciprocal of 1 ulp each.  Comparisons, so that a NaN stays one.
+struct Pair {
+  float g, l, s;
+  bool g_free, l_free;     // not beyond the limit
+};
+TAMD_DEVICE Pair pair_of(float g, float l, const GluShape &sh) {
+  Pair p;
+  p.g_free = !(sh.has_limit && g > sh.limit);
+  p.l_free = !(sh.has_limit && __builtin_fabsf(l) > sh.limit);
+  p.g = p.g_free ? g : sh.limit;
+  p.l = p.l_free ? l : __builtin_copysignf(sh.limit, l);
+  p.s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * sh.alpha * p.g));
+  return p;
+}
+
+template <int DT, bool ALIGNED, int U>
+__global__ __launch_bounds__(256) void checkpoint_kernel(const void *__restrict__ a, int64_t a_stride, void *__restrict__ out, int64_t out_stride,
+                                                         uint8_t *__restrict__ values, int64_t v_stride, uint8_t *__restrict__ scales, int64_t s_stride,
+                                                         GluShape sh) {
+  constexpr int SIZE = DT == TAMD_F32 ? 4 : 2;
+  const int sub = threadIdx.x & 3;
+  const int64_t gid0 = (int64_t)blockIdx.x * (64 * U) + (threadIdx.x >> 2);
+  int64_t r[U], g[U];
+  int n[U];
+  float v[U][8];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t gid = gid0 + u * 64;
+    int64_t b;
+    place_group(sh.div, gid < sh.div.total ? gid : 0, b, r[u], g[u]);
+    const int64_t left = sh.L - g[u] * 32 - sub * 8;
+    n[u] = gid >= sh.div.total || left <= 0 ? 0 : (left < 8 ? (int)left : 8);
+    load_values<DT, ALIGNED, 8>((const char *)a + (r[u] * a_stride + g[u] * 32 + sub * 8) * SIZE, n[u], v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float m = 0.f;
+    bool any_nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m = __builtin_fmaxf(m, __builtin_fabsf(v[u][j]));
+      any_nan |= v[u][j] != v[u][j];
+    }
+    // (the group's four lanes are a quad: swaps inside it are moves in the register file)
+    m = __builtin_fmaxf(m, bits_to_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_to_bits(m), 0xB1, 0xF, 0xF, true)));
+    m = __builtin_fmaxf(m, bits_to_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_to_bits(m), 0x4E, 0xF, 0xF, true)));
+    uint32_t byte, code[2] = {0, 0};
+    const float by = group_scale<QK_E4M3>(m, TAMD_ROUND_UP, byte);
+    if (!any_nan && byte < 0xFEu) {
+      float c[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = __builtin_amdgcn_fmed3f(v[u][j] * by, -448.0f, 448.0f);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        code[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[4 * h + 2], c[4 * h + 3], __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * h], c[4 * h + 1], 0, false), true);
+    } else {   // (an infinite magnitude times a multiplier of zero is a NaN too)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) code[j >> 2] |= fp8_code<QK_E4M3>(v[u][j] * by) << (8 * (j & 3));
+    }
+    float o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Pair p = pair_of(v[u][2 * j], v[u][2 * j + 1], sh);
+      const float gs = p.g * p.s;
+      o[j] = __builtin_fmaf(gs, p.l, gs);
+    }
+    if (n[u] == 0) continue;
+    store_values<DT, ALIGNED, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
+    uint8_t *const vp = values + r[u] * v_stride + g[u] * 32 + sub * 8;
+    if (n[u] == 8) {
+      store8<ALIGNED>(vp, u32x2_t{code[0], code[1]});
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n[u]) vp[j] = (uint8_t)(code[j >> 2] >> (8 * (j & 3)));
+    }
+    if (sub == 0) scales[r[u] * s_stride + g[u]] = (uint8_t)byte;
+  }
+}
+
+template <int DT, bool ALIGNED, bool AGAIN, int U>
+__global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ dout, int64_t d_stride, const uint8_t *__restrict__ values, int64_t v_stride,
+                                                       const uint8_t *__restrict__ scales, int64_t s_stride, void *__restrict__ da, int64_t da_stride,
+                                                       void *__restrict__ out, int64_t out_stride, GluShape sh) {
+  constexpr int SIZE = DT == TAMD_F32 ? 4 : 2;
+  const int sub = threadIdx.x & 3;
+  const int64_t gid0 = (int64_t)blockIdx.x * (64 * U) + (threadIdx.x >> 2);
+  int64_t r[U], g[U];
+  int n[U];
+  uint32_t code[U][2], byte[U];
+  float d[U][4];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t gid = gid0 + u * 64;
+    int64_t b;
+    place_group(sh.div, gid < sh.div.total ? gid : 0, b, r[u], g[u]);
+    const int64_t left = sh.L - g[u] * 32 - sub * 8;
+    n[u] = gid >= sh.div.total || left <= 0 ? 0 : (left < 8 ? (int)left : 8);
+    const uint8_t *const vp = values + r[u] * v_stride + g[u] * 32 + sub * 8;
+    if (n[u] == 8) {
+      const u32x2_t q = load8<ALIGNED>(vp);
+      code[u][0] = q[0], code[u][1] = q[1];
+    } else {
+      code[u][0] = code[u][1] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n[u]) code[u][j >> 2] |= (uint32_t)vp[j] << (8 * (j & 3));
+    }
+    byte[u] = n[u] ? scales[r[u] * s_stride + g[u]] : 0u;
+    load_values<DT, ALIGNED, 4>((const char *)dout + (r[u] * d_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, d[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (n[u] == 0) continue;
+    // 2^(byte - 127); 0 for 0, as tamd_upcast_mxfp has it, NaN for 255
+    const float by = bits_to_f32(byte[u] == 255u ? 0x7FC00000u : byte[u] << 23);
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    float v[8], o[4], dv[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[u][h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[u][h], true);
+      v[4 * h] = lo.x * by, v[4 * h + 1] = lo.y * by, v[4 * h + 2] = hi.x * by, v[4 * h + 3] = hi.y * by;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Pair p = pair_of(v[2 * j], v[2 * j + 1], sh);
+      const float gs = p.g * p.s, ds = d[u][j] * p.s;
+      o[j] = __builtin_fmaf(gs, p.l, gs);
+      const float slope = __builtin_fmaf(sh.alpha * p.g, 1.0f - p.s, 1.0f);
+      dv[2 * j] = p.g_free ? __builtin_fmaf(ds, p.l, ds) * slope : 0.f;
+      dv[2 * j + 1] = p.l_free ? ds * p.g : 0.f;
+    }
+    store_values<DT, ALIGNED, 8>((char *)da + (r[u] * da_stride + g[u] * 32 + sub * 8) * SIZE, n[u], dv);
+    if constexpr (AGAIN) store_values<DT, ALIGNED, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
+  }
+}
+
+constexpr int kU = 2;
+
+bool shape(GluShape &sh, int64_t M, int64_t N, float alpha, float limit, int has_limit, unsigned &blocks) {
+  const int64_t G = (2 * N + 31) / 32;
+  sh.div = group_div(1, M, G);
+  sh.L = 2 * N, sh.alpha = alpha, sh.limit = limit, sh.has_limit = has_limit;
+  const int64_t n = (sh.div.total + 64 * kU - 1) / (64 * kU);
+  blocks = (unsigned)n;
+  return n < ((int64_t)1 << 31);
+}
+bool whole(const void *p, int64_t stride_bytes, int by) { return ((uintptr_t)p | (uintptr_t)stride_bytes) % by == 0; }
+bool plain(int dt) { return dt == TAMD_F32 || dt == TAMD_BF16 || dt == TAMD_F16; }
+
+}  // namespace
+
+extern "C" int tamd_swiglu_checkpoint(const void *a, int dtype, int64_t M, int64_t N, int64_t a_stride, void *out, int64_t out_stride, uint8_t *values,
+                                      int64_t values_stride, uint8_t *scales, int64_t scales_stride, float alpha, float limit, int has_limit, void *stream) {
+  if (M < 0 || N < 0 || a_stride < 0 || out_stride < 0 || values_stride < 0 || scales_stride < 0 || (has_limit && !(limit >= 0.f))) return TAMD_E_INVALID;
+  if (!plain(dtype)) return TAMD_E_UNSUPPORTED;
+  if (M == 0 || N == 0) return 0;
+  if (!a || !out || !values || !scales) return TAMD_E_INVALID;
+  const int size = dtype == TAMD_F32 ? 4 : 2;
+  if (!whole(a, 0, size) || !whole(out, 0, size)) return TAMD_E_ALIGNMENT;
+  if (M >= ((int64_t)1 << 31) || N >= ((int64_t)1 << 30)) return TAMD_E_TOO_LARGE;
+  GluShape sh;
+  unsigned blocks;
+  if (!shape(sh, M, N, alpha, limit, has_limit, blocks)) return TAMD_E_TOO_LARGE;
+  hipStream_t st = (hipStream_t)stream;
+  const bool aligned = whole(a, a_stride * size, 16) && whole(out, out_stride * size, 4 * size) && whole(values, values_stride, 8);
+  const auto go = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (aligned) checkpoint_kernel<DT, true, kU><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
+    else checkpoint_kernel<DT, false, kU><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
+  };
+  if (dtype == TAMD_F32) go(std::integral_constant<int, TAMD_F32>());
+  else if (dtype == TAMD_BF16) go(std::integral_constant<int, TAMD_BF16>());
+  else go(std::integral_constant<int, TAMD_F16>());
+  return launch_status();
+}
+
+extern "C" int tamd_swiglu_backward(const void *dout, int dtype, int64_t M, int64_t N, int64_t dout_stride, const uint8_t *values, int64_t values_stride,
+                                    const uint8_t *scales, int64_t scales_stride, void *da, int64_t da_stride, void *out, int64_t out_stride, float alpha,
+                                    float limit, int has_limit, void *stream) {
+  if (M < 0 || N < 0 || dout_stride < 0 || values_stride < 0 || scales_stride < 0 || da_stride < 0 || out_stride < 0 || (has_limit && !(limit >= 0.f)))
+    return TAMD_E_INVALID;
+  if (!plain(dtype)) return TAMD_E_UNSUPPORTED;
+  if (M == 0 || N == 0) return 0;
+  if (!dout || !values || !scales || !da) return TAMD_E_INVALID;
+  const int size = dtype == TAMD_F32 ? 4 : 2;
+  if (!whole(dout, 0, size) || !whole(da, 0, size) || !whole(out, 0, size)) return TAMD_E_ALIGNMENT;
+  if (M >= ((int64_t)1 << 31) || N >= ((int64_t)1 << 30)) return TAMD_E_TOO_LARGE;
+  GluShape sh;
+  unsigned blocks;
+  if (!shape(sh, M, N, alpha, limit, has_limit, blocks)) return TAMD_E_TOO_LARGE;
+  hipStream_t st = (hipStream_t)stream;
+  const bool aligned = whole(dout, dout_stride * size, 4 * size) && whole(da, da_stride * size, 16) && whole(values, values_stride, 8) &&
+                       (!out || whole(out, out_stride * size, 4 * size));
+  const auto go = [&](auto dt, auto al, auto again) {
+    backward_kernel<decltype(dt)::value, decltype(al)::value, decltype(again)::value, kU>
+        <<<blocks, 256, 0, st>>>(dout, dout_stride, values, values_stride, scales, scales_stride, da, da_stride, out, out_stride, sh);
+  };
+  const auto with = [&](auto dt) {
+    if (aligned) out ? go(dt, std::true_type(), std::true_type()) : go(dt, std::true_type(), std::false_type());
+    else out ? go(dt, std::false_type(), std::true_type()) : go(dt, std::false_type(), std::false_type());
+  };
+  if (dtype == TAMD_F32) with(std::integral_constant<int, TAMD_F32>());
+  else if (dtype == TAMD_BF16) with(std::integral_constant<int, TAMD_BF16>());
+  else with(std::integral_constant<int, TAMD_F16>());
+  return launch_status();
+}
