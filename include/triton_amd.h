@@ -30,7 +30,7 @@ extern "C" {
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
  * 3: tamd_moe_layer, tamd_matvec, tamd_sample
  * 4: tamd_sample_workspace_exact
- * 5: tamd_dispatch, tamd_combine, tamd_swiglu_checkpoint, tamd_swiglu_backward */
+ * 5: tamd_dispatch, tamd_combine, tamd_swiglu_checkpoint, tamd_swiglu_backward, tamd_topk_backward */
 #define TAMD_VERSION 5
 
 /* error codes (negative) */
@@ -544,6 +544,17 @@ int tamd_swiglu_checkpoint(const void *a, int dtype, int64_t M, int64_t N, int64
 int tamd_swiglu_backward(const void *dout, int dtype, int64_t M, int64_t N, int64_t dout_stride, const uint8_t *values,
                          int64_t values_stride, const uint8_t *scales, int64_t scales_stride, void *da, int64_t da_stride,
                          void *out, int64_t out_stride, float alpha, float limit, int has_limit, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Gradient of tamd_topk_forward: dvals [n_rows, k], that of the picks' values, to dx [n_rows, n_cols], that of the logits, in the
+ * logits' type (each float32, bfloat16 or float16).  With p the softmax (float32) of x over the picks of a row, or without it:
+ *   dx[indx[j]] = p_j (dvals_j - sum_m p_m dvals_m)   or   dvals_j,   0 in every other column and in rows from n_live on
+ * An index outside [0, n_cols) is no pick; columns that several picks name get the sum.  x is read at the picks, and with
+ * apply_softmax only.  n_cols < 32768, k <= 64 (TAMD_E_TOO_LARGE).
+ */
+int tamd_topk_backward(const void *x, int dtype, int64_t x_stride, int64_t n_rows, int64_t n_live, int n_cols, int k,
+                       int apply_softmax, const int16_t *indx, int64_t indx_stride, const void *dvals,
+                       int dvals_dtype, int64_t dvals_stride, void *dx, int64_t dx_stride, void *stream);
 
 #ifdef __cplusplus
 }

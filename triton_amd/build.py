@@ -21,7 +21,7 @@ SOURCES = ["api.cpp", "mxfp.hip", "routing.hip", "elementwise.hip", "moe_matmul.
            "moe_matmul_w16_bf16.hip", "moe_matmul_w16_f16.hip",
            "moe_matmul_kk_bf16.hip", "moe_matmul_kk_f16.hip", "moe_matmul_kk_fp8.hip",
            "moe_matmul_kkring_bf16.hip", "moe_matmul_kkring_f16.hip",
-           "moe_layer.hip", "moe_layer_bf16.hip", "moe_layer_f16.hip", "matvec.hip", "matvec_bf16.hip", "matvec_f16.hip", "sampling.hip", "dispatch.hip", "swiglu_train.hip"]
+           "moe_layer.hip", "moe_layer_bf16.hip", "moe_layer_f16.hip", "matvec.hip", "matvec_bf16.hip", "matvec_f16.hip", "sampling.hip", "dispatch.hip", "swiglu_train.hip", "topk_backward.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed fp32 math is switched off on purpose (device code only); the unroll limit is raised because the tile
 # epilogues index their accumulators with loops that must unroll completely (up to 80 element rows per lane):
