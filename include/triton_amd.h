@@ -30,7 +30,7 @@ extern "C" {
 /* 2: tamd_matmul_args ends with y_rows; tamd_matmul_sized, tamd_routing_gates
  * 3: tamd_moe_layer, tamd_matvec, tamd_sample
  * 4: tamd_sample_workspace_exact
- * 5: tamd_dispatch, tamd_combine, tamd_swiglu_checkpoint, tamd_swiglu_backward, tamd_topk_backward */
+ * 5: tamd_dispatch, tamd_combine, tamd_swiglu_checkpoint, tamd_swiglu_backward, tamd_topk_backward, tamd_ragged_k_matmul */
 #define TAMD_VERSION 5
 
 /* error codes (negative) */
@@ -555,6 +555,33 @@ int tamd_swiglu_backward(const void *dout, int dtype, int64_t M, int64_t N, int6
 int tamd_topk_backward(const void *x, int dtype, int64_t x_stride, int64_t n_rows, int64_t n_live, int n_cols, int k,
                        int apply_softmax, const int16_t *indx, int64_t indx_stride, const void *dvals,
                        int dvals_dtype, int64_t dvals_stride, void *dx, int64_t dx_stride, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Products over ragged rows (matmul.py's b_ragged_metadata): y[e, m, n] = sum over the rows r of slice e of x[r, m] d[r, n], with which
+ * the gradients of all experts' weights are one call.  Slice e holds the rows slice_offs[e] .. slice_offs[e + 1] (int32, E + 1 of them, cut to
+ * [0, K]); an empty one gives zeros, and rows of no slice take no part, whatever they hold.
+ * x: [K, M], d: [K, N] of `dtype` (bfloat16, float16), y: [E, M, N] of y_dtype (float32, bfloat16, float16), with unit stride along M, N and N; any
+ * pitch and start, of which whole 16 bytes (and M and N in eights) are the fast form.  Sums are float32, rounded once.
+ * workspace: tamd_ragged_k_matmul_workspace(M, N, E, K) bytes on a 16-byte boundary, NULL if these are 0; calls that may run at the same time
+ * need one each.  y overlaps nothing that is read.
+ */
+typedef struct tamd_ragged_k_args {
+  const void *x;
+  int64_t x_stride;
+  const void *d;
+  int64_t d_stride;
+  const int32_t *slice_offs;
+  void *y;
+  int64_t y_stride_e, y_stride_m;
+  void *workspace;
+  int64_t K;
+  int dtype, y_dtype;
+  int M, N, E;
+} tamd_ragged_k_args;
+
+int64_t tamd_ragged_k_matmul_workspace(int M, int N, int E, int64_t K);
+/* args_size: sizeof(tamd_ragged_k_args) as the caller was compiled; other sizes are refused */
+int tamd_ragged_k_matmul(const tamd_ragged_k_args *args, size_t args_size, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,149 @@
+"""GPU: products over ragged rows (`matmul` with ragged metadata of both operands), the gradients of all experts' weights, against products in 64 bits."""
+import pytest
+import torch
+
+from triton_amd.matmul import PrecisionConfig, matmul
+from triton_amd.tensor import make_ragged_tensor_metadata
+
+pytestmark = pytest.mark.gpu
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+LEAST = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+
+
+def ragged(sizes, rows, device):
+    return make_ragged_tensor_metadata(torch.tensor(sizes, dtype=torch.int32, device=device), rows)
+
+
+def check(got, x, d, sizes, dtype):
+    """Every slice against its product; float32 sums of n products of 16-bit numbers (exact in float32) are off by n half steps of the sum of
+    their sizes at most, the result is rounded once."""
+    at = 0
+    assert got.dtype == dtype and tuple(got.shape) == (len(sizes), x.shape[1], d.shape[1])
+    for e, n in enumerate(sizes):
+        a, b = x[at:at + n].double().t().contiguous(), d[at:at + n].double()
+        want, size = a @ b, a.abs() @ b.abs()
+        bound = HALF_STEP[dtype] * want.abs() * (1 + 2.0 ** -8) + 1.01 * (n + 1) * 2.0 ** -24 * size + LEAST[dtype]
+        err = (got[e].double() - want).abs()
+        assert bool((err <= bound).all()), (e, n, float((err / bound).max()))
+        at += n
+
+
+def laid(t, how):
+    if how == "pitch":
+        return torch.full((t.shape[0], t.shape[1] + 24), float("nan"), dtype=t.dtype, device=t.device)[:, 8:8 + t.shape[1]].copy_(t)
+    if how == "odd":
+        return torch.full((t.numel() + 1,), float("nan"), dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t)
+    return t.t().contiguous().t() if how == "turned" else t
+
+
+SIZES = [[1], [0], [33, 0, 1, 95, 32, 31], [0, 0, 700, 5], [64] * 9, [513, 2, 0, 129]]
+
+
+@pytest.mark.parametrize("M,N", [(1, 1), (8, 16), (7, 130), (128, 128), (264, 136), (300, 96), (129, 257)])
+@pytest.mark.parametrize("sizes", SIZES, ids=str)
+@pytest.mark.parametrize("dtype,out,how", [(torch.bfloat16, None, "dense"), (torch.float16, torch.float32, "pitch"), (torch.float16, None, "odd"),
+                                           (torch.bfloat16, torch.float16, "turned")])
+def test_small(M, N, sizes, dtype, out, how, device):
+    torch.manual_seed(M + N + len(sizes))
+    rows = sum(sizes)
+    x, d = torch.randn(rows, M, device=device).to(dtype), torch.randn(rows, N, device=device).to(dtype)
+    # rows behind the last slice hold NaN, and take no part
+    more = torch.full((5, 1), float("nan"), dtype=dtype, device=device)
+    xs, ds = laid(torch.cat([x, more.expand(5, M)]), how), laid(torch.cat([d, more.expand(5, N)]), how)
+    md = ragged(sizes, rows, device)
+    got = matmul(xs.t(), ds, None, md, md, precision_config=PrecisionConfig(out_dtype=out))
+    check(got, x, d, sizes, out or dtype)
+    assert torch.equal(matmul(xs.t(), ds, None, None, md, precision_config=PrecisionConfig(out_dtype=out)), got)
+
+
+@pytest.mark.parametrize("M,N,sizes", [(2048, 2056, [300, 257, 0, 400]), (520, 8200, [256, 600, 513, 258]), (4097, 1030, [400, 300]), (256, 256, [3000, 9, 0, 4100]),
+                                       (64, 72, [5000, 1]), (1000, 8, [2049, 2048, 2047]), (96, 33, [70000])])
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.float16, torch.float32)])
+def test_larger_tiles_and_splits(M, N, sizes, dtype, out, device):
+    torch.manual_seed(M + N)
+    rows = sum(sizes)
+    x, d = torch.randn(rows, M, device=device).to(dtype), torch.randn(rows, N, device=device).to(dtype)
+    md = ragged(sizes, rows, device)
+    got = matmul(x.t(), d, None, md, md, precision_config=PrecisionConfig(out_dtype=out))
+    check(got, x, d, sizes, out or dtype)
+    for _ in range(2):
+        assert torch.equal(matmul(x.t(), d, None, md, md, precision_config=PrecisionConfig(out_dtype=out)), got)
+
+
+@pytest.mark.parametrize("M,N,sizes", [(136, 72, [40, 0, 50]), (64, 64, [3000, 100])])
+def test_into_given_results(M, N, sizes, device):
+    """c with pitches of its own: only the results are written."""
+    torch.manual_seed(1)
+    rows, E = sum(sizes), len(sizes)
+    x, d = torch.randn(rows, M, device=device).bfloat16(), torch.randn(rows, N, device=device).bfloat16()
+    md = ragged(sizes, rows, device)
+    for skip in (0, 1, 8):
+        room = torch.full((E, M + 3, N + 16), 5.0, device=device)
+        c = room[:, 1:1 + M, skip:skip + N]
+        assert matmul(x.t(), d, None, md, md, c=c) is c
+        check(c, x, d, sizes, torch.float32)
+        c.fill_(5.0)
+        assert bool((room == 5).all())
+
+
+def test_values_of_other_slices_do_not_reach(device):
+    """NaN and infinities in a slice's rows make that slice's results NaN or infinite, and only in their columns."""
+    sizes = [40, 33, 60]
+    x, d = torch.randn(133, 136, device=device).half(), torch.randn(133, 264, device=device).half()
+    md = ragged(sizes, 133, device)
+    clean = matmul(x.t(), d, None, md, md)
+    x[40:73, 5] = float("nan")
+    d[72, 200] = float("inf")
+    got = matmul(x.t(), d, None, md, md)
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+    assert bool(torch.isnan(got[1][5]).all()) and not bool(torch.isfinite(got[1][:, 200]).any())
+    keep = torch.ones(136, 264, dtype=torch.bool, device=device)
+    keep[5], keep[:, 200] = False, False
+    assert torch.equal(got[1][keep], clean[1][keep])
+
+
+@pytest.mark.parametrize("M,N,rows,E", [(0, 8, 10, 2), (8, 0, 10, 2), (8, 8, 0, 2), (16, 24, 0, 1)])
+def test_nothing_there(M, N, rows, E, device):
+    md = ragged([rows] + [0] * (E - 1), rows, device)
+    got = matmul(torch.randn(rows, M, device=device).bfloat16().t(), torch.randn(rows, N, device=device).bfloat16(), None, md, md)
+    assert tuple(got.shape) == (E, M, N) and not bool(got.any() if rows == 0 else False)
+
+
+def test_offsets_past_the_rows_are_cut(device):
+    """Metadata made for more rows than there are: what is there is summed, nothing else is read."""
+    x, d = torch.randn(50, 64, device=device).bfloat16(), torch.randn(50, 64, device=device).bfloat16()
+    md = ragged([30, 40, 50], 120, device)
+    check(matmul(x.t(), d, None, md, md), x, d, [30, 20, 0], torch.bfloat16)
+
+
+def test_rows_past_four_gigabytes(device):
+    """A slice whose rows lie beyond what 32 bits count."""
+    rows, M, N = 2 ** 19 + 100, 4352, 64
+    x, d = torch.zeros(rows, M, dtype=torch.bfloat16, device=device), torch.zeros(rows, N, dtype=torch.bfloat16, device=device)
+    x[-100:], d[-100:] = torch.randn(100, M, device=device), torch.randn(100, N, device=device)
+    sizes = [rows - 100 - 7, 7, 100]
+    md = ragged(sizes, rows, device)
+    got = matmul(x.t(), d, None, md, md)
+    assert not bool(got[:2].any())
+    check(got[2:], x[-100:], d[-100:], [100], torch.bfloat16)
+
+
+def test_another_stream_and_a_graph(device):
+    torch.manual_seed(2)
+    for M, N in ((136, 264), (64, 64)):     # (64 x 64: with partial sums)
+        x, d = torch.randn(2000, M, device=device).bfloat16(), torch.randn(2000, N, device=device).bfloat16()
+        md = ragged([1100, 900], 2000, device)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            mine = matmul(x.t(), d, None, md, md)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(mine, matmul(x.t(), d, None, md, md))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = matmul(x.t(), d, None, md, md)
+        for _ in range(4):
+            x.copy_(torch.randn(2000, M, device=device))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, matmul(x.t(), d, None, md, md))

@@ -156,6 +156,15 @@ class TokenRowsArgs(C.Structure):
     ]
 
 
+class RaggedKArgs(C.Structure):
+    """Mirror of `tamd_ragged_k_args`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("d", C.c_void_p), ("d_stride", C.c_int64), ("slice_offs", C.c_void_p),
+        ("y", C.c_void_p), ("y_stride_e", C.c_int64), ("y_stride_m", C.c_int64), ("workspace", C.c_void_p), ("K", C.c_int64),
+        ("dtype", C.c_int), ("y_dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("E", C.c_int),
+    ]
+
+
 _I64, _INT, _PTR, _F = C.c_int64, C.c_int, C.c_void_p, C.c_float
 _SIGNATURES = {
     "tamd_version": ([], C.c_int),
@@ -196,6 +205,8 @@ _SIGNATURES = {
     "tamd_combine": ([C.POINTER(TokenRowsArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_swiglu_checkpoint": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
     "tamd_topk_backward": ([_PTR, _INT, _I64, _I64, _I64, _INT, _INT, _INT, _PTR, _I64, _PTR, _INT, _I64, _PTR, _I64, _PTR], C.c_int),
+    "tamd_ragged_k_matmul_workspace": ([_INT, _INT, _INT, _I64], C.c_int64),
+    "tamd_ragged_k_matmul": ([C.POINTER(RaggedKArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_swiglu_backward": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
 }
 

@@ -142,6 +142,53 @@ def _k_contiguous_cached(w):
     return turned
 
 
+def _by_rows(t):
+    """[K, C] as the kernels for ragged K read it: unit stride along C."""
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
+    """Y[e] = a[:, slice e] @ b[slice e, :] (matmul.py:376-391 of the reference, ragged_dimension "K")."""
+    a, b = _data(a), _data(b)
+    flex = pc.flex_ctx
+    if (any(getattr(pc, f) is not None for f in ("a_mx_scale", "b_mx_scale", "c_mx_scale", "a_mx_tensor_scale", "b_mx_tensor_scale")) or pc.acc_scale != 1.0
+            or any(d.scale is not None for d in (flex.lhs_data, flex.rhs_data, flex.acc_data)) or flex.lhs_data.dtype is not None
+            or flex.rhs_data.dtype is not None or flex.out_data.expected_scale is not None or flex.out_data.actual_scale is not None):
+        raise NotImplementedError("K-ragged matmul takes unscaled operands")
+    _lib.require_gpu(a, "a")
+    assert a.ndim == 2 and b.ndim == 2 and a.shape[1] == b.shape[0], f"K-ragged operands are [M, K] and [K, N], not {list(a.shape)} and {list(b.shape)}"
+    assert b.device == a.device, "b must live on the device of a"
+    if a.dtype != b.dtype or a.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"K-ragged matmul is built for two bfloat16 or two float16 operands, not {a.dtype} and {b.dtype}")
+    offs = b_ragged.slice_offs
+    E = b_ragged.n_slices
+    assert offs.device == a.device and offs.dtype == torch.int32 and tuple(offs.shape) == (E + 1,) and (offs.stride(0) == 1 or E == 0), \
+        "slice_offs of the ragged metadata are int32 [slices + 1] on the device of a"
+    assert a_ragged is None or a_ragged.n_slices == E, "a and b have different slices"
+    M, K, N = a.shape[0], a.shape[1], b.shape[1]
+    dtype = pc.out_dtype or (c.dtype if c is not None else a.dtype)
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"{dtype} results of a K-ragged matmul are not built")
+    x, d = _by_rows(a.t()), _by_rows(b)
+    if c is None:
+        c = torch.empty((E, M, N), dtype=dtype, device=a.device)
+    else:
+        assert tuple(c.shape) == (E, M, N) and c.dtype == dtype and c.device == a.device and (c.stride(2) == 1 or N <= 1) \
+            and (M < 2 or c.stride(1) >= N) and (E < 2 or c.stride(0) >= (M - 1) * c.stride(1) + N), f"c must be {dtype} [{E}, {M}, {N}] with unit stride along N"
+    L = _lib.lib()
+    n_ws = L.tamd_ragged_k_matmul_workspace(M, N, E, K)
+    if n_ws < 0:
+        _lib.check(n_ws, "matmul (ragged K)")
+    with torch.cuda.device(a.device):
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=a.device) if n_ws else None
+        args = _lib.RaggedKArgs(x=x.data_ptr(), x_stride=x.stride(0) if K > 1 else M, d=d.data_ptr(), d_stride=d.stride(0) if K > 1 else N,
+                                slice_offs=offs.data_ptr(), y=c.data_ptr(), y_stride_e=c.stride(0), y_stride_m=c.stride(1),
+                                workspace=None if ws is None else ws.data_ptr(), K=K, dtype=_lib.dtype_code(a.dtype), y_dtype=_lib.dtype_code(dtype),
+                                M=M, N=N, E=E)
+        _lib.check(L.tamd_ragged_k_matmul(ctypes.byref(args), ctypes.sizeof(args), _lib.stream_ptr(a.device)), "matmul (ragged K)")
+    return c
+
+
 def matmul(a, b, bias, a_ragged_metadata: Optional[RaggedTensorMetadata] = None,
            b_ragged_metadata: Optional[RaggedTensorMetadata] = None, gather_indx: Optional[torch.Tensor] = None,
            scatter_indx: Optional[torch.Tensor] = None, precision_config: Optional[PrecisionConfig] = None,
@@ -158,6 +205,11 @@ def matmul(a, b, bias, a_ragged_metadata: Optional[RaggedTensorMetadata] = None,
        holds their e8m0 scales [E, K/32, N].
     a_ragged_metadata: rows of `a` (after gather) are grouped by slice.
     gather_indx / scatter_indx: int32 row maps (scatter -1 drops the row).
+
+    b_ragged_metadata: the axis K that is summed over is ragged.  Y[e] = a[:, rows of slice e] @ b[rows of slice e, :] for the slices of both
+    (a_ragged_metadata the same, or None): a [M, K], b [K, N] of bf16 / fp16 give Y [slices, M, N].  With a = x.t() of sorted rows x and b the
+    gradients of what they were multiplied to, this is the gradient of every expert's weights; empty slices give zeros, rows of no slice take no
+    part.  out_dtype (or c [slices, M, N]) float32, bfloat16 or float16; nothing else is built for it.
     """
     if type(a) is torch.Tensor and a.is_cuda and b_ragged_metadata is None and fused_comm is None and c_acc_in is None:
         done = _native.matmul(a, b, bias, a_ragged_metadata, gather_indx, scatter_indx, precision_config, betas, gammas,
@@ -181,7 +233,13 @@ def matmul(a, b, bias, a_ragged_metadata: Optional[RaggedTensorMetadata] = None,
         assert fused_comm is None, "fused comm is not supported in batched mode"
         assert b.ndim == 3 and b.shape[0] == a.shape[0]
     if b_ragged_metadata is not None:
-        raise NotImplementedError("K-ragged matmul is not built for gfx950")
+        for value, name in ((bias, "bias"), (gather_indx, "gather_indx"), (scatter_indx, "scatter_indx"), (betas, "betas"), (gammas, "gammas"),
+                            (out_alpha, "out_alpha"), (fused_comm, "fused_comm"), (c_acc_in, "c_acc_in")):
+            if value is not None:
+                raise NotImplementedError(f"{name} of a K-ragged matmul is not built")
+        if fused_activation.specs.name != "dflt" or epilogue.specs.name != "dflt":
+            raise NotImplementedError("K-ragged matmul is built without activation and epilogue")
+        return _matmul_ragged_k(a, b, a_ragged_metadata, b_ragged_metadata, precision_config, c)
     if fused_comm is not None:
         raise NotImplementedError("fused communication needs more than one GPU")
     if c_acc_in is not None:
