@@ -43,15 +43,23 @@ struct Abi {
   int (*matvec)(const tamd_matvec_args *, size_t, void *);
   int (*sample)(const tamd_sample_args *, size_t, void *);
   int64_t (*sample_workspace)(int, int);
+  int (*dispatch)(const tamd_token_rows_args *, size_t, void *);
+  int (*combine)(const tamd_token_rows_args *, size_t, void *);
+  int (*swiglu_checkpoint)(const void *, int, int64_t, int64_t, int64_t, void *, int64_t, uint8_t *, int64_t, uint8_t *, int64_t, float, float, int, void *);
+  int (*swiglu_backward)(const void *, int, int64_t, int64_t, int64_t, const uint8_t *, int64_t, const uint8_t *, int64_t, void *, int64_t, void *, int64_t, float,
+                         float, int, void *);
+  int (*topk_backward)(const void *, int, int64_t, int64_t, int64_t, int, int, int, const int16_t *, int64_t, const void *, int, int64_t, void *, int64_t, void *);
+  int64_t (*ragged_k_workspace)(int, int, int, int64_t);
+  int (*ragged_k)(const tamd_ragged_k_args *, size_t, void *);
 } abi;
-PyObject *cls_tensor, *cls_value_layout, *cls_scale_layout, *obj_fp4, *ctx_constraints, *ctx_flags, *cls_int4, *obj_plain_flex;
+PyObject *cls_tensor, *cls_value_layout, *cls_scale_layout, *obj_fp4, *ctx_constraints, *ctx_flags, *cls_int4, *obj_plain_flex, *obj_plain_glu_flex;
 
 struct Names {
   PyObject *storage, *data, *layout, *dtype, *shape, *c_mx_scale, *c_microblock_size, *c_value_pack_factor, *a_mx_tensor_scale,
       *b_mx_tensor_scale, *acc_scale, *a_mx_scale, *a_microblock_size, *b_mx_scale, *b_microblock_size, *flex_ctx, *lhs_data,
       *rhs_data, *out_data, *acc_data, *scale, *expected_scale, *actual_scale, *checksum_scale, *out_dtype,
       *flexpoint_saturate_inf, *specs, *name, *fn_arg_names, *fn_args, *reduction_n, *slice_sizes, *slice_offs,
-      *block_offs_data, *block_schedule_data, *expected_slice_size, *native, *scales, *zeros, *group_size;
+      *block_offs_data, *block_schedule_data, *expected_slice_size, *native, *scales, *zeros, *group_size, *limit;
 } nm;
 
 // ------------------------------------------------------------------ small helpers
@@ -908,6 +916,196 @@ PyObject *py_sample(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
   });
 }
 
+// ------------------------------------------------------------------ training: rows to experts and back
+// a matrix of one or more rows, of a plain floating type, whose rows have unit stride
+inline const at::Tensor &matrix(const at::Tensor &t) {
+  need(t.dim() == 2 && t.size(0) >= 1 && t.size(1) >= 1 && (t.stride(1) == 1 || t.size(1) == 1) && plain_code(type_code(t.scalar_type())));
+  return t;
+}
+inline int64_t pitch_of(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+// (first, second or None); the second may be undefined
+PyObject *pair_or_none(const at::Tensor &a, const at::Tensor &b) {
+  if (b.defined()) return pair(a, b);
+  Ref x(THPVariable_Wrap(a));
+  return x.p ? PyTuple_Pack(2, x.p, Py_None) : nullptr;
+}
+
+// One call of the library, `src` to `dst` (made here where none is given); `other` with the gates gives the products that are their gradient.
+int token_rows(bool spread, int dev, const at::Tensor &src, PyObject *indx_o, PyObject *gates_o, PyObject *other_o, PyObject *out_o, at::Tensor &dst, at::Tensor &dots) {
+  const at::Tensor &indx = gpu_tensor(indx_o, dev);
+  need(indx.dim() == 2 && indx.scalar_type() == at::kInt);
+  const int64_t T = indx.size(0), k = indx.size(1), H = src.size(1);
+  need(T >= 1 && k >= 1 && T * k < 1ll << 31 && H < 1ll << 31 && (k == 1 || indx.stride(1) == 1) && (!spread || src.size(0) == T) && src.size(0) < 1ll << 31);
+  tamd_token_rows_args g;
+  std::memset(&g, 0, sizeof g);
+  if (out_o != Py_None) {
+    dst = matrix(gpu_tensor(out_o, dev));
+    need(dst.size(1) == H && dst.scalar_type() == src.scalar_type() && (dst.size(0) < 2 || dst.stride(0) >= H) && (spread || dst.size(0) == T));
+  } else {
+    dst = new_empty({spread ? T * k : T, H}, src.scalar_type(), dev);
+  }
+  const int64_t n_rows = spread ? dst.size(0) : src.size(0);
+  need(n_rows < 1ll << 31);
+  if (gates_o != Py_None) {
+    const at::Tensor &gates = gpu_tensor(gates_o, dev);
+    need(gates.dim() == 2 && gates.size(0) == T && gates.size(1) == k && (k == 1 || gates.stride(1) == 1));
+    g.gates = gates.data_ptr(), g.gates_stride = pitch_of(gates), g.gates_dtype = type_code(gates.scalar_type());
+    need(plain_code(g.gates_dtype));
+    if (other_o != Py_None) {
+      const at::Tensor &other = matrix(gpu_tensor(other_o, dev));
+      need(other.size(0) == (spread ? n_rows : T) && other.size(1) == H && other.scalar_type() == src.scalar_type());
+      dots = new_empty({T, k}, gates.scalar_type(), dev);
+      g.other = other.data_ptr(), g.other_stride = pitch_of(other), g.dots = dots.data_ptr(), g.dots_stride = k;
+    }
+  }
+  g.src = src.data_ptr(), g.src_stride = pitch_of(src), g.dst = dst.data_ptr(), g.dst_stride = pitch_of(dst);
+  g.row_indx = (const int32_t *)indx.data_ptr(), g.row_indx_stride = pitch_of(indx), g.dtype = type_code(src.scalar_type());
+  g.T = (int)T, g.k = (int)k, g.H = (int)H, g.n_rows = (int)n_rows;
+  void *st = stream_of(dev);
+  return without_gil([&] { return (spread ? abi.dispatch : abi.combine)(&g, sizeof g, st); });
+}
+
+// (rows, row_indx, gates, out)
+template <bool SPREAD>
+PyObject *token_rows_forward(PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 4);
+    int dev = -1;
+    at::Tensor dst, dots;
+    const int rc = token_rows(SPREAD, dev, matrix(current_gpu_tensor(v[0], dev)), v[1], v[2], Py_None, v[3], dst, dots);
+    return rc != 0 ? PyLong_FromLong(rc) : THPVariable_Wrap(dst);
+  });
+}
+PyObject *py_dispatch(PyObject *, PyObject *const *v, Py_ssize_t nargs) { return token_rows_forward<true>(v, nargs); }
+PyObject *py_combine(PyObject *, PyObject *const *v, Py_ssize_t nargs) { return token_rows_forward<false>(v, nargs); }
+// (gradient, row_indx, what the forward pass had, gates, out)
+template <bool SPREAD>
+PyObject *token_rows_backward(PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 5);
+    int dev = -1;
+    at::Tensor dst, dots;
+    const int rc = token_rows(SPREAD, dev, matrix(current_gpu_tensor(v[0], dev)), v[1], v[3], v[2], v[4], dst, dots);
+    return rc != 0 ? PyLong_FromLong(rc) : pair_or_none(dst, dots);
+  });
+}
+PyObject *py_combine_backward(PyObject *, PyObject *const *v, Py_ssize_t nargs) { return token_rows_backward<true>(v, nargs); }
+PyObject *py_dispatch_backward(PyObject *, PyObject *const *v, Py_ssize_t nargs) { return token_rows_backward<false>(v, nargs); }
+
+// ------------------------------------------------------------------ training: SwiGLU kept in 8 bits
+// the limit of a PrecisionConfig without flexpoint scales
+void glu_limit(PyObject *pc, float &limit, int &has_limit) {
+  Ref flex(attr(pc, nm.flex_ctx)), l(attr(pc, nm.limit));
+  need(flex.p == obj_plain_glu_flex);
+  has_limit = !l.none();
+  const double v = l.none() ? 0.0 : as_double(l.p);
+  need(v >= 0);
+  limit = (float)v;
+}
+
+// (a, alpha, precision_config): (out, values, scales)
+PyObject *py_swiglu_checkpoint(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 3);
+    int dev = -1;
+    const at::Tensor &a = matrix(current_gpu_tensor(v[0], dev));
+    const int64_t M = a.size(0), L = a.size(1), G = (L + 31) / 32;
+    need(L % 2 == 0);
+    const double alpha = as_double(v[1]);
+    float limit;
+    int has_limit;
+    glu_limit(v[2], limit, has_limit);
+    at::Tensor out = new_empty({M, L / 2}, a.scalar_type(), dev), values = new_empty({M, L}, at::ScalarType::Float8_e4m3fn, dev), scales = new_empty({M, G}, at::kByte, dev);
+    const int code = type_code(a.scalar_type());
+    void *st = stream_of(dev);
+    const int rc = without_gil([&] {
+      return abi.swiglu_checkpoint(a.data_ptr(), code, M, L / 2, a.stride(0), out.data_ptr(), L / 2, (uint8_t *)values.data_ptr(), L, (uint8_t *)scales.data_ptr(), G,
+                                   (float)alpha, limit, has_limit, st);
+    });
+    if (rc != 0) return PyLong_FromLong(rc);
+    Ref x(THPVariable_Wrap(out)), y(THPVariable_Wrap(values)), z(THPVariable_Wrap(scales));
+    return x.p && y.p && z.p ? PyTuple_Pack(3, x.p, y.p, z.p) : nullptr;
+  });
+}
+
+// (dout, values, scales, alpha, precision_config, return_out): (da, out or None)
+PyObject *py_swiglu_backward(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 6 && PyBool_Check(v[5]));
+    int dev = -1;
+    const at::Tensor &d = matrix(current_gpu_tensor(v[0], dev)), &values = gpu_tensor(v[1], dev), &scales = gpu_tensor(v[2], dev);
+    const int64_t M = d.size(0), N = d.size(1), G = (2 * N + 31) / 32;
+    need(values.dim() == 2 && values.size(0) == M && values.size(1) == 2 * N && values.stride(1) == 1 && values.scalar_type() == at::ScalarType::Float8_e4m3fn);
+    need(scales.dim() == 2 && scales.size(0) == M && scales.size(1) == G && (scales.stride(1) == 1 || G == 1) && scales.scalar_type() == at::kByte);
+    const double alpha = as_double(v[3]);
+    float limit;
+    int has_limit;
+    glu_limit(v[4], limit, has_limit);
+    at::Tensor da = new_empty({M, 2 * N}, d.scalar_type(), dev), out;
+    if (v[5] == Py_True) out = new_empty({M, N}, d.scalar_type(), dev);
+    const int code = type_code(d.scalar_type());
+    void *st = stream_of(dev), *again = out.defined() ? out.data_ptr() : nullptr;
+    const int rc = without_gil([&] {
+      return abi.swiglu_backward(d.data_ptr(), code, M, N, d.stride(0), (const uint8_t *)values.data_ptr(), values.stride(0), (const uint8_t *)scales.data_ptr(),
+                                 scales.stride(0), da.data_ptr(), 2 * N, again, N, (float)alpha, limit, has_limit, st);
+    });
+    if (rc != 0) return PyLong_FromLong(rc);
+    return pair_or_none(da, out);
+  });
+}
+
+// ------------------------------------------------------------------ training: the gate and the weights
+// (x, indx, dvals, apply_softmax): the gradient of the logits, all of whose rows were routed.
+PyObject *py_topk_backward(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 4 && PyBool_Check(v[3]));
+    int dev = -1;
+    const at::Tensor &x = matrix(current_gpu_tensor(v[0], dev)), &indx = gpu_tensor(v[1], dev), &d = matrix(gpu_tensor(v[2], dev));
+    const int64_t T = x.size(0), E = x.size(1), k = indx.dim() == 2 ? indx.size(1) : 0;
+    need(E < 32768 && T < 1ll << 32 && k >= 1 && k <= 64 && indx.size(0) == T && indx.scalar_type() == at::kShort && (k == 1 || indx.stride(1) == 1));
+    need(d.size(0) == T && d.size(1) == k);
+    at::Tensor dx = new_empty({T, E}, x.scalar_type(), dev);
+    const int code = type_code(x.scalar_type()), d_code = type_code(d.scalar_type()), softmax = v[3] == Py_True;
+    void *st = stream_of(dev);
+    const int rc = without_gil([&] {
+      return abi.topk_backward(x.data_ptr(), code, x.stride(0), T, T, (int)E, (int)k, softmax, (const int16_t *)indx.data_ptr(), indx.stride(0), d.data_ptr(), d_code,
+                               d.stride(0), dx.data_ptr(), E, st);
+    });
+    if (rc != 0) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(dx);
+  });
+}
+
+// (a [M, K], b [K, N], slice_offs, slices, the output's type or None): the product over every slice's rows, [slices, M, N].
+PyObject *py_matmul_ragged_k(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
+  return covered([&]() -> PyObject * {
+    need(nargs == 5);
+    int dev = -1;
+    const at::Tensor &a = current_gpu_tensor(v[0], dev), &b = gpu_tensor(v[1], dev), &offs = gpu_tensor(v[2], dev);
+    const int64_t E = as_int(v[3]);
+    need(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0) && a.scalar_type() == b.scalar_type());
+    const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
+    need(M >= 1 && N >= 1 && K >= 1 && E >= 1 && M < 1ll << 30 && N < 1ll << 30 && E < 1ll << 30 && K < 1ll << 31);
+    need((a.stride(0) == 1 || M == 1) && (b.stride(1) == 1 || N == 1) && offs.scalar_type() == at::kInt && offs.dim() == 1 && offs.size(0) == E + 1 && offs.stride(0) == 1);
+    tamd_ragged_k_args g;
+    std::memset(&g, 0, sizeof g);
+    const at::ScalarType t = v[4] == Py_None ? a.scalar_type() : dtype_of(v[4]);
+    g.dtype = type_code(a.scalar_type()), g.y_dtype = type_code(t);
+    need((g.dtype == TAMD_BF16 || g.dtype == TAMD_F16) && plain_code(g.y_dtype));
+    const int64_t n_ws = abi.ragged_k_workspace((int)M, (int)N, (int)E, K);
+    if (n_ws < 0) return PyLong_FromLong((long)n_ws);
+    at::Tensor y = new_empty({E, M, N}, t, dev), ws;
+    if (n_ws) ws = new_empty({n_ws}, at::kByte, dev), g.workspace = ws.data_ptr();
+    g.x = a.data_ptr(), g.x_stride = K > 1 ? a.stride(1) : M, g.d = b.data_ptr(), g.d_stride = K > 1 ? b.stride(0) : N;
+    g.slice_offs = (const int32_t *)offs.data_ptr(), g.y = y.data_ptr(), g.y_stride_e = M * N, g.y_stride_m = N;
+    g.K = K, g.M = (int)M, g.N = (int)N, g.E = (int)E;
+    void *st = stream_of(dev);
+    const int rc = without_gil([&] { return abi.ragged_k(&g, sizeof g, st); });
+    if (rc != 0) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(y);
+  });
+}
+
 // ------------------------------------------------------------------ module
 PyObject *py_choose_block_m(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
   return covered([&]() -> PyObject * {
@@ -961,13 +1159,14 @@ PyObject *py_routing_block_rows(PyObject *, PyObject *const *v, Py_ssize_t nargs
 }
 
 // (addresses of the C ABI functions by name, Tensor, CDNA4MXValueLayout, CDNA4MXScaleLayout, FP4, constraints ContextVar,
-//  flags ContextVar, Int4Weights, the FlexCtx of a PrecisionConfig without one)
+//  flags ContextVar, Int4Weights, the FlexCtx of a PrecisionConfig without one, that of swiglu's)
 PyObject *py_init(PyObject *, PyObject *args) {
   PyObject *addr;
-  if (!PyArg_ParseTuple(args, "O!OOOOOOOO", &PyDict_Type, &addr, &cls_tensor, &cls_value_layout, &cls_scale_layout, &obj_fp4,
-                        &ctx_constraints, &ctx_flags, &cls_int4, &obj_plain_flex))
+  if (!PyArg_ParseTuple(args, "O!OOOOOOOOO", &PyDict_Type, &addr, &cls_tensor, &cls_value_layout, &cls_scale_layout, &obj_fp4,
+                        &ctx_constraints, &ctx_flags, &cls_int4, &obj_plain_flex, &obj_plain_glu_flex))
     return nullptr;
-  for (PyObject *o : {cls_tensor, cls_value_layout, cls_scale_layout, obj_fp4, ctx_constraints, ctx_flags, cls_int4, obj_plain_flex}) Py_INCREF(o);
+  for (PyObject *o : {cls_tensor, cls_value_layout, cls_scale_layout, obj_fp4, ctx_constraints, ctx_flags, cls_int4, obj_plain_flex, obj_plain_glu_flex})
+    Py_INCREF(o);
   auto take = [&](const char *name, void *slot) {
     PyObject *o = PyDict_GetItemString(addr, name);
     void *p = o ? PyLong_AsVoidPtr(o) : nullptr;
@@ -977,7 +1176,10 @@ PyObject *py_init(PyObject *, PyObject *args) {
   if (!take("tamd_matmul_sized", &abi.matmul) || !take("tamd_routing_gates", &abi.routing) || !take("tamd_reduce", &abi.reduce) ||
       !take("tamd_downcast_mxfp", &abi.downcast) || !take("tamd_upcast_mxfp", &abi.upcast) || !take("tamd_moe_layer", &abi.moe_layer) ||
       !take("tamd_moe_layer_workspace", &abi.moe_layer_workspace) || !take("tamd_matvec", &abi.matvec) || !take("tamd_sample", &abi.sample) ||
-      !take("tamd_sample_workspace_exact", &abi.sample_workspace)) {
+      !take("tamd_sample_workspace_exact", &abi.sample_workspace) || !take("tamd_dispatch", &abi.dispatch) || !take("tamd_combine", &abi.combine) ||
+      !take("tamd_swiglu_checkpoint", &abi.swiglu_checkpoint) || !take("tamd_swiglu_backward", &abi.swiglu_backward) ||
+      !take("tamd_topk_backward", &abi.topk_backward) || !take("tamd_ragged_k_matmul_workspace", &abi.ragged_k_workspace) ||
+      !take("tamd_ragged_k_matmul", &abi.ragged_k)) {
     PyErr_SetString(PyExc_RuntimeError, "an entry point of the library is missing");
     return nullptr;
   }
@@ -990,7 +1192,7 @@ PyObject *py_init(PyObject *, PyObject *args) {
       TAMD_NAME(out_dtype), TAMD_NAME(flexpoint_saturate_inf), TAMD_NAME(specs), TAMD_NAME(name), TAMD_NAME(fn_arg_names),
       TAMD_NAME(fn_args), TAMD_NAME(reduction_n), TAMD_NAME(slice_sizes), TAMD_NAME(slice_offs), TAMD_NAME(block_offs_data),
       TAMD_NAME(block_schedule_data), TAMD_NAME(expected_slice_size), TAMD_NAME(native), TAMD_NAME(scales), TAMD_NAME(zeros),
-      TAMD_NAME(group_size);
+      TAMD_NAME(group_size), TAMD_NAME(limit);
 #undef TAMD_NAME
   Py_RETURN_NONE;
 }
@@ -1008,6 +1210,14 @@ PyMethodDef methods[] = {{"init", py_init, METH_VARARGS, nullptr},
                          {"moe_layer", TAMD_FAST(py_moe_layer)},
                          {"matvec", TAMD_FAST(py_matvec)},
                          {"sample", TAMD_FAST(py_sample)},
+                         {"dispatch", TAMD_FAST(py_dispatch)},
+                         {"combine", TAMD_FAST(py_combine)},
+                         {"dispatch_backward", TAMD_FAST(py_dispatch_backward)},
+                         {"combine_backward", TAMD_FAST(py_combine_backward)},
+                         {"swiglu_checkpoint", TAMD_FAST(py_swiglu_checkpoint)},
+                         {"swiglu_backward", TAMD_FAST(py_swiglu_backward)},
+                         {"topk_backward", TAMD_FAST(py_topk_backward)},
+                         {"matmul_ragged_k", TAMD_FAST(py_matmul_ragged_k)},
                          {"choose_block_m", TAMD_FAST(py_choose_block_m)},
                          {"blocks_of_16_stream", TAMD_FAST(py_blocks_of_16_stream)},
                          {"dense_block_m", TAMD_FAST(py_dense_block_m)},

@@ -17,7 +17,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, _native
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -84,6 +84,11 @@ def dispatch(x: torch.Tensor, row_indx: torch.Tensor, gates: Optional[torch.Tens
 
     Returns [T * k, H] in x's type, or writes to `out` (any number of rows; it must not overlap an input).  Rows that no pick
     names are left as they are -- in a new tensor: undefined.  Without gates rows are copied bit for bit."""
+    done = _native.dispatch(x, row_indx, gates, out)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "dispatch")
+        return done
     x = _by_row(x, "x")
     out = _rows_out(x, row_indx, out)
     _run(True, x, out, row_indx, gates, None, out.shape[0], "dispatch")
@@ -96,6 +101,11 @@ def combine(rows: torch.Tensor, row_indx: torch.Tensor, gates: Optional[torch.Te
 
     Returns [T, H] in the rows' type (`out`, if given, which must not overlap an input); the sum is float32, in the order of j,
     and rounded once.  A token none of whose picks has a row gets zeros."""
+    done = _native.combine(rows, row_indx, gates, out)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "combine")
+        return done
     rows = _by_row(rows, "rows")
     T, H = row_indx.shape[0], rows.shape[1]
     if out is None:
@@ -116,6 +126,11 @@ def dispatch_backward(drows: torch.Tensor, row_indx: torch.Tensor, x: Optional[t
 
     Returns (dx [T, H] in drows' type, dgates [T, k] in the gates' type).  dgates is None without gates, and without x, which
     nothing else needs."""
+    done = _native.dispatch_backward(drows, row_indx, x, gates, None)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "dispatch_backward")
+        return done
     drows = _by_row(drows, "drows")
     T, H = row_indx.shape[0], drows.shape[1]
     x = None if x is None or gates is None else _kept(x, T, H, drows, "x")
@@ -132,6 +147,11 @@ def combine_backward(dy: torch.Tensor, row_indx: torch.Tensor, rows: Optional[to
 
     Returns (drows, dgates [T, k] in the gates' type).  drows is [T * k, H] in dy's type, or `out`, as in `dispatch`: rows that no pick names
     are left as they are.  dgates is None without gates, and without rows, which nothing else needs and which are as many as drows."""
+    done = _native.combine_backward(dy, row_indx, rows, gates, out)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "combine_backward")
+        return done
     dy = _by_row(dy, "dy")
     drows = _rows_out(dy, row_indx, out)
     rows = None if rows is None or gates is None else _kept(rows, drows.shape[0], dy.shape[1], dy, "rows")

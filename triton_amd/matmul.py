@@ -155,6 +155,12 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
             or any(d.scale is not None for d in (flex.lhs_data, flex.rhs_data, flex.acc_data)) or flex.lhs_data.dtype is not None
             or flex.rhs_data.dtype is not None or flex.out_data.expected_scale is not None or flex.out_data.actual_scale is not None):
         raise NotImplementedError("K-ragged matmul takes unscaled operands")
+    if c is None and (a_ragged is None or a_ragged.n_slices == b_ragged.n_slices):
+        done = _native.matmul_ragged_k(a, b, b_ragged.slice_offs, b_ragged.n_slices, pc.out_dtype)
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done, "matmul (ragged K)")
+            return done
     _lib.require_gpu(a, "a")
     assert a.ndim == 2 and b.ndim == 2 and a.shape[1] == b.shape[0], f"K-ragged operands are [M, K] and [K, N], not {list(a.shape)} and {list(b.shape)}"
     assert b.device == a.device, "b must live on the device of a"

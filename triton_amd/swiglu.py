@@ -5,7 +5,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
+from . import _lib, _native
 from .numerics import InFlexData, OutFlexData
 
 
@@ -85,6 +85,11 @@ def swiglu_checkpoint(a: torch.Tensor, alpha: float, precision_config: Precision
     scales are those of `downcast_to_mxfp(a, torch.float8_e4m3fn, -1)`, which `upcast_from_mxfp` reads, with a short last group
     where 32 does not divide 2 N.  out is computed from a itself, in float32, and rounded once.  Unlike in `swiglu`, a NaN stays one beside a
     limit; the group of an infinity is NaN in what is kept."""
+    done = _native.swiglu_checkpoint(a, alpha, precision_config)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "swiglu_checkpoint")
+        return done
     _check_type(a, "a")
     limit, has_limit = _limits(precision_config)
     assert a.shape[-1] % 2 == 0, "a has a gate and a linear column per value"
@@ -109,6 +114,11 @@ def swiglu_backward(dout: torch.Tensor, values: torch.Tensor, scales: torch.Tens
     With a = values * 2^(scales - 127), g = min(a[2n], limit), l = clamp(a[2n+1], -limit, limit), s = sigmoid(alpha g):
       da[2n] = dout[n] * (l + 1) * s * (1 + alpha g (1 - s)),   da[2n+1] = dout[n] * g * s,   0 where the limit cut a off.
     return_out: also the activation at the kept values, for the gradient of the weights that it was multiplied with."""
+    done = _native.swiglu_backward(dout, values, scales, alpha, precision_config, return_out)
+    if done is not None:
+        if type(done) is int:
+            _lib.check(done, "swiglu_backward")
+        return done
     _check_type(dout, "dout")
     limit, has_limit = _limits(precision_config)
     N = dout.shape[-1]

@@ -3,7 +3,7 @@ from typing import Optional, Union
 
 import torch
 
-from . import _lib
+from . import _lib, _native
 from .tensor import BIT, SparseMatrix, Tensor, wrap_torch_tensor
 
 
@@ -62,6 +62,12 @@ def topk_backward(x: Union[Tensor, torch.Tensor], indx: torch.Tensor, dvals: tor
     and 0 elsewhere and in rows from n_rows on, which were not routed.  x: the logits [T, E] (float32 / bf16 / fp16, E < 32768), of which the
     picked ones are read; indx: int16 [T, k] as `topk` and `routing` return it, k <= 64 (an index outside [0, E) is no pick); dvals
     may be of another floating type than x.  Returns [T, E] in x's type; arithmetic is float32, rounded once."""
+    if n_rows is None and type(x) is torch.Tensor:
+        done = _native.topk_backward(x, indx, dvals, apply_softmax)
+        if done is not None:
+            if type(done) is int:
+                _lib.check(done, "topk_backward")
+            return done
     if isinstance(x, Tensor):
         n_rows = x.shape[0] if n_rows is None else n_rows
         x = x.storage.data
