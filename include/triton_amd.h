@@ -561,9 +561,9 @@ int tamd_topk_backward(const void *x, int dtype, int64_t x_stride, int64_t n_row
  * the gradients of all experts' weights are one call.  Slice e holds the rows slice_offs[e] .. slice_offs[e + 1] (int32, E + 1 of them, cut to
  * [0, K]); an empty one gives zeros, and rows of no slice take no part, whatever they hold.
  * x: [K, M], d: [K, N] of `dtype` (bfloat16, float16), y: [E, M, N] of y_dtype (float32, bfloat16, float16), with unit stride along M, N and N; any
- * pitch and start, of which whole 16 bytes (and M and N in eights) are the fast form.  Sums are float32, rounded once.
- * workspace: tamd_ragged_k_matmul_workspace(M, N, E, K) bytes on a 16-byte boundary, NULL if these are 0; calls that may run at the same time
- * need one each.  y overlaps nothing that is read.
+ * pitch and start, of which whole 16 bytes (and M and N in eights) are taken as they are, others laid out so first.  Sums are float32, rounded once.
+ * workspace: tamd_ragged_k_matmul_workspace(args, size) bytes for the same arguments but this one (negative: what the call would
+ * answer), on a 16-byte boundary, NULL if these are 0; calls that may run at the same time need one each.  y overlaps nothing that is read.
  */
 typedef struct tamd_ragged_k_args {
   const void *x;
@@ -579,7 +579,7 @@ typedef struct tamd_ragged_k_args {
   int M, N, E;
 } tamd_ragged_k_args;
 
-int64_t tamd_ragged_k_matmul_workspace(int M, int N, int E, int64_t K);
+int64_t tamd_ragged_k_matmul_workspace(const tamd_ragged_k_args *args, size_t args_size);
 /* args_size: sizeof(tamd_ragged_k_args) as the caller was compiled; other sizes are refused */
 int tamd_ragged_k_matmul(const tamd_ragged_k_args *args, size_t args_size, void *stream);
 

@@ -57,7 +57,7 @@ def test_small(M, N, sizes, dtype, out, how, device):
 
 
 @pytest.mark.parametrize("M,N,sizes", [(2048, 2056, [300, 257, 0, 400]), (520, 8200, [256, 600, 513, 258]), (4097, 1030, [400, 300]), (256, 256, [3000, 9, 0, 4100]),
-                                       (64, 72, [5000, 1]), (1000, 8, [2049, 2048, 2047]), (96, 33, [70000])])
+                                       (64, 72, [5000, 1]), (1000, 8, [2049, 2048, 2047]), (96, 33, [70000]), (4100, 2600, [320, 350, 0, 700, 400]), (2600, 4104, [333, 650, 0, 700])])
 @pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.float16, torch.float32)])
 def test_larger_tiles_and_splits(M, N, sizes, dtype, out, device):
     torch.manual_seed(M + N)

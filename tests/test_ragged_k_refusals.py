@@ -32,11 +32,14 @@ def test_c_entry_point():
             assert code(good(M=64, **{field: 0x1001})) == _lib.E_ALIGNMENT, field
     assert code(good(M=64, y_dtype=_lib.F32, y=0x4002)) == _lib.E_ALIGNMENT
     assert code(good(M=64, K=1 << 31)) == _lib.E_TOO_LARGE and code(good(M=2 ** 31 - 1, N=2 ** 31 - 1)) == _lib.E_TOO_LARGE
-    # long slices of few tiles are cut: their partial sums need room
-    n = L.tamd_ragged_k_matmul_workspace(64, 64, 2, 10000)
-    assert n > 0 and n % (2 * 64 * 64 * 4) == 0 and L.tamd_ragged_k_matmul_workspace(64, 64, 2, 100) == 0
+    # long slices of few tiles are cut: their partial sums need room; so do rows that are not whole pieces of 16 bytes
+    room = lambda a, size=C.sizeof(_lib.RaggedKArgs): L.tamd_ragged_k_matmul_workspace(C.byref(a), size)  # noqa: E731
+    n = room(good(M=64, K=10000))
+    assert n > 0 and n % (2 * 64 * 64 * 4) == 0 and room(good(M=64)) == room(good()) == 0
     assert code(good(M=64, K=10000)) == _lib.E_INVALID and code(good(M=64, K=10000, workspace=0x5004)) == _lib.E_ALIGNMENT
-    assert L.tamd_ragged_k_matmul_workspace(-1, 64, 2, 100) == _lib.E_INVALID and L.tamd_ragged_k_matmul_workspace(64, 64, 2, 1 << 31) == _lib.E_TOO_LARGE
+    assert room(good(M=64, x=0x1002)) == 100 * 64 * 2 and room(good(M=63, d_stride=65)) == 100 * 64 * 2 * 2 and code(good(M=63)) == _lib.E_INVALID
+    assert room(good(M=-1)) == room(good(), 8) == L.tamd_ragged_k_matmul_workspace(None, C.sizeof(_lib.RaggedKArgs)) == _lib.E_INVALID
+    assert room(good(M=64, K=1 << 31)) == room(good(M=1 << 24)) == _lib.E_TOO_LARGE
 
 
 def test_structure_matches_the_header(tmp_path):

@@ -205,7 +205,7 @@ _SIGNATURES = {
     "tamd_combine": ([C.POINTER(TokenRowsArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_swiglu_checkpoint": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
     "tamd_topk_backward": ([_PTR, _INT, _I64, _I64, _I64, _INT, _INT, _INT, _PTR, _I64, _PTR, _INT, _I64, _PTR, _I64, _PTR], C.c_int),
-    "tamd_ragged_k_matmul_workspace": ([_INT, _INT, _INT, _I64], C.c_int64),
+    "tamd_ragged_k_matmul_workspace": ([C.POINTER(RaggedKArgs), C.c_size_t], C.c_int64),
     "tamd_ragged_k_matmul": ([C.POINTER(RaggedKArgs), C.c_size_t, _PTR], C.c_int),
     "tamd_swiglu_backward": ([_PTR, _INT, _I64, _I64, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _PTR, _I64, _F, _F, _INT, _PTR], C.c_int),
 }

@@ -49,7 +49,7 @@ struct Abi {
   int (*swiglu_backward)(const void *, int, int64_t, int64_t, int64_t, const uint8_t *, int64_t, const uint8_t *, int64_t, void *, int64_t, void *, int64_t, float,
                          float, int, void *);
   int (*topk_backward)(const void *, int, int64_t, int64_t, int64_t, int, int, int, const int16_t *, int64_t, const void *, int, int64_t, void *, int64_t, void *);
-  int64_t (*ragged_k_workspace)(int, int, int, int64_t);
+  int64_t (*ragged_k_workspace)(const tamd_ragged_k_args *, size_t);
   int (*ragged_k)(const tamd_ragged_k_args *, size_t, void *);
 } abi;
 PyObject *cls_tensor, *cls_value_layout, *cls_scale_layout, *obj_fp4, *ctx_constraints, *ctx_flags, *cls_int4, *obj_plain_flex, *obj_plain_glu_flex;
@@ -1092,13 +1092,13 @@ PyObject *py_matmul_ragged_k(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     const at::ScalarType t = v[4] == Py_None ? a.scalar_type() : dtype_of(v[4]);
     g.dtype = type_code(a.scalar_type()), g.y_dtype = type_code(t);
     need((g.dtype == TAMD_BF16 || g.dtype == TAMD_F16) && plain_code(g.y_dtype));
-    const int64_t n_ws = abi.ragged_k_workspace((int)M, (int)N, (int)E, K);
-    if (n_ws < 0) return PyLong_FromLong((long)n_ws);
     at::Tensor y = new_empty({E, M, N}, t, dev), ws;
-    if (n_ws) ws = new_empty({n_ws}, at::kByte, dev), g.workspace = ws.data_ptr();
     g.x = a.data_ptr(), g.x_stride = K > 1 ? a.stride(1) : M, g.d = b.data_ptr(), g.d_stride = K > 1 ? b.stride(0) : N;
     g.slice_offs = (const int32_t *)offs.data_ptr(), g.y = y.data_ptr(), g.y_stride_e = M * N, g.y_stride_m = N;
     g.K = K, g.M = (int)M, g.N = (int)N, g.E = (int)E;
+    const int64_t n_ws = abi.ragged_k_workspace(&g, sizeof g);
+    if (n_ws < 0) return PyLong_FromLong((long)n_ws);
+    if (n_ws) ws = new_empty({n_ws}, at::kByte, dev), g.workspace = ws.data_ptr();
     void *st = stream_of(dev);
     const int rc = without_gil([&] { return abi.ragged_k(&g, sizeof g, st); });
     if (rc != 0) return PyLong_FromLong(rc);

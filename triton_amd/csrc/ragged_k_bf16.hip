@@ -2,5 +2,5 @@
 #include "ragged_k.h"
 
 namespace tamd {
-int ragged_k_bf16(const RaggedK &a, int tile, bool dma, void *stream) { return ragged_k_typed<TAMD_BF16>(a, tile, dma, (hipStream_t)stream); }
+int ragged_k_bf16(const RaggedK &a, int tile, void *stream) { return ragged_k_typed<TAMD_BF16>(a, tile, (hipStream_t)stream); }
 }  // namespace tamd

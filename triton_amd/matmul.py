@@ -181,16 +181,16 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
     else:
         assert tuple(c.shape) == (E, M, N) and c.dtype == dtype and c.device == a.device and (c.stride(2) == 1 or N <= 1) \
             and (M < 2 or c.stride(1) >= N) and (E < 2 or c.stride(0) >= (M - 1) * c.stride(1) + N), f"c must be {dtype} [{E}, {M}, {N}] with unit stride along N"
+    args = _lib.RaggedKArgs(x=x.data_ptr(), x_stride=x.stride(0) if K > 1 else M, d=d.data_ptr(), d_stride=d.stride(0) if K > 1 else N,
+                            slice_offs=offs.data_ptr(), y=c.data_ptr(), y_stride_e=c.stride(0), y_stride_m=c.stride(1), K=K,
+                            dtype=_lib.dtype_code(a.dtype), y_dtype=_lib.dtype_code(dtype), M=M, N=N, E=E)
     L = _lib.lib()
-    n_ws = L.tamd_ragged_k_matmul_workspace(M, N, E, K)
+    n_ws = L.tamd_ragged_k_matmul_workspace(ctypes.byref(args), ctypes.sizeof(args))
     if n_ws < 0:
         _lib.check(n_ws, "matmul (ragged K)")
     with torch.cuda.device(a.device):
         ws = torch.empty(n_ws, dtype=torch.uint8, device=a.device) if n_ws else None
-        args = _lib.RaggedKArgs(x=x.data_ptr(), x_stride=x.stride(0) if K > 1 else M, d=d.data_ptr(), d_stride=d.stride(0) if K > 1 else N,
-                                slice_offs=offs.data_ptr(), y=c.data_ptr(), y_stride_e=c.stride(0), y_stride_m=c.stride(1),
-                                workspace=None if ws is None else ws.data_ptr(), K=K, dtype=_lib.dtype_code(a.dtype), y_dtype=_lib.dtype_code(dtype),
-                                M=M, N=N, E=E)
+        args.workspace = None if ws is None else ws.data_ptr()
         _lib.check(L.tamd_ragged_k_matmul(ctypes.byref(args), ctypes.sizeof(args), _lib.stream_ptr(a.device)), "matmul (ragged K)")
     return c
 
