@@ -51,7 +51,8 @@ def scattered(p, values, into):
 
 
 CASES = [(1, 1, 1, 1, 0.0), (1, 4, 2880, 4, 0.0), (3, 2, 7, 6, 0.3), (5, 8, 64, 50, 0.2), (17, 3, 1063, 60, 0.0), (65, 4, 520, 260, 0.1), (9, 9, 96, 81, 0.2),
-         (6, 17, 264, 110, 0.1), (4100, 2, 136, 8300, 0.1), (4099, 1, 33, 4099, 0.0), (4101, 11, 40, 45111, 0.1), (33, 6, 3000, 198, 1.0)]
+         (6, 17, 264, 110, 0.1), (4100, 2, 136, 8300, 0.1), (4099, 1, 33, 4099, 0.0), (4101, 11, 40, 45111, 0.1), (33, 6, 3000, 198, 1.0),
+         (8200, 2, 264, 16400, 0.1), (4200, 9, 1100, 37800, 0.1), (2600, 3, 1064, 7900, 0.2), (2501, 2, 2600, 5002, 0.1), (700, 12, 256, 8400, 0.0)]
 
 
 @pytest.mark.parametrize("T,k,H,n,drop", CASES)

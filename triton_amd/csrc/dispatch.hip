@@ -7,6 +7,7 @@
 // the dispatch.  Both go by token, so that a token's row is read (or written) once whatever k is, and its k expert rows are whole,
 // contiguous pieces of memory.  Sums are float32 in the order of j, a dot's partial sums are joined in a fixed order: no atomics.
 #include "common.h"
+#include <type_traits>
 
 using namespace tamd;
 
@@ -63,35 +64,47 @@ TAMD_DEVICE void store_gate(void *p, int dt, int64_t i, float v) {
   else store_from_f32<TAMD_F16>(p, i, v);
 }
 
-TAMD_DEVICE float wave_sum(float v) {
-  return bits_to_f32(group_reduce<64>(f32_to_bits(v), [](uint32_t a, uint32_t b) { return f32_to_bits(bits_to_f32(a) + bits_to_f32(b)); }));
+template <int LANES>
+TAMD_DEVICE float sum_over(float v) {
+  return bits_to_f32(group_reduce<LANES>(f32_to_bits(v), [](uint32_t a, uint32_t b) { return f32_to_bits(bits_to_f32(a) + bits_to_f32(b)); }));
 }
 
-// What a wave (or the workgroup, WAVES of them) knows of its token: up to kPicks of its expert rows and their weights.
+// What the LANES lanes of a token (16, a wave, or the workgroup's 256) know of it: up to kPicks of its expert rows and their weights, from 64 lanes on
+// in scalar registers.
 struct Picks {
   int32_t row[kPicks];
   float gate[kPicks];
 };
+template <int LANES>
 TAMD_DEVICE void load_picks(const tamd_token_rows_args &a, int64_t t, int j0, Picks &p) {
 #pragma unroll
   for (int j = 0; j < kPicks; ++j) {
     p.row[j] = -1;
     p.gate[j] = 1.0f;
     if (j0 + j < a.k) {
-      const int32_t r = __builtin_amdgcn_readfirstlane(a.row_indx[t * a.row_indx_stride + j0 + j]);
+      int32_t r = a.row_indx[t * a.row_indx_stride + j0 + j];
+      if constexpr (LANES >= 64) r = __builtin_amdgcn_readfirstlane(r);
       p.row[j] = (uint32_t)r < (uint32_t)a.n_rows ? r : -1;
       if (a.gates) p.gate[j] = load_gate(a.gates, a.gates_dtype, t * a.gates_stride + j0 + j);
     }
   }
 }
 
+template <int LANES>
+TAMD_DEVICE int64_t token_of() {
+  if constexpr (LANES == 256) return (int64_t)blockIdx.x;
+  else if constexpr (LANES == 64) return (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  else return (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+}
+
 // dots of the picks j0 ..: the lanes' sums joined, and the waves' in their order
-template <int WAVES>
+template <int LANES>
 TAMD_DEVICE void store_dots(const tamd_token_rows_args &a, int64_t t, int j0, const float (&dot)[kPicks], float *lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int WAVES = LANES / 64, OF_WAVE = LANES < 64 ? LANES : 64;
+  const int lane = threadIdx.x & (OF_WAVE - 1), wave = threadIdx.x >> 6;
   float all[kPicks];
 #pragma unroll
-  for (int j = 0; j < kPicks; ++j) all[j] = j0 + j < a.k ? wave_sum(dot[j]) : 0.f;
+  for (int j = 0; j < kPicks; ++j) all[j] = j0 + j < a.k ? sum_over<OF_WAVE>(dot[j]) : 0.f;
   if constexpr (WAVES > 1) {
     sync_threads();
     if (lane == 0) {
@@ -112,19 +125,19 @@ TAMD_DEVICE void store_dots(const tamd_token_rows_args &a, int64_t t, int j0, co
     if (lane == j && j0 + j < a.k) store_gate(a.dots, a.gates_dtype, t * a.dots_stride + j0 + j, all[j]);
 }
 
-// WAVES waves to a token: 4 make a workgroup, or 1 of the 4 that a workgroup has.  Without gates rows are copied as bits.
-template <int DT, bool ALIGNED, int WAVES, bool DOTS, bool GATES>
+// Without gates rows are copied as bits.
+template <int DT, bool ALIGNED, int LANES, bool DOTS, bool GATES>
 __global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
-  constexpr int V = kPiece<DT>, SIZE = 16 / V, LANES = 64 * WAVES;
+  constexpr int V = kPiece<DT>, SIZE = 16 / V;
   __shared__ float lds[4 * kPicks];
-  const int64_t t = WAVES == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  const int64_t t = token_of<LANES>();
   if (t >= a.T) return;
   const int at = threadIdx.x & (LANES - 1);
   const char *const src = (const char *)a.src + t * a.src_stride * SIZE;
   const int pieces = a.H / V, rest = a.H % V;
   for (int j0 = 0; j0 < a.k; j0 += kPicks) {
     Picks p;
-    load_picks(a, t, j0, p);
+    load_picks<LANES>(a, t, j0, p);
     float dot[kPicks] = {};
     for (int c = at; c < pieces; c += LANES) {
       const u32x4_t q = load_raw<ALIGNED>(src, c);
@@ -163,15 +176,15 @@ __global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
         else ((uint16_t *)row)[i] = ((const uint16_t *)src)[i];
       }
     }
-    if constexpr (DOTS) store_dots<WAVES>(a, t, j0, dot, lds);
+    if constexpr (DOTS) store_dots<LANES>(a, t, j0, dot, lds);
   }
 }
 
-template <int DT, bool ALIGNED, int WAVES, bool DOTS>
+template <int DT, bool ALIGNED, int LANES, bool DOTS>
 __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
-  constexpr int V = kPiece<DT>, SIZE = 16 / V, LANES = 64 * WAVES;
+  constexpr int V = kPiece<DT>, SIZE = 16 / V;
   __shared__ float lds[4 * kPicks];
-  const int64_t t = WAVES == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  const int64_t t = token_of<LANES>();
   if (t >= a.T) return;
   const int at = threadIdx.x & (LANES - 1);
   char *const dst = (char *)a.dst + t * a.dst_stride * SIZE;
@@ -179,13 +192,13 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
   const int pieces = a.H / V, rest = a.H % V;
   const bool few = a.k <= kPicks;    // all picks at once: their dots come with the sum
   Picks p;
-  load_picks(a, t, 0, p);
+  load_picks<LANES>(a, t, 0, p);
   float dot[kPicks] = {};
   for (int c = at; c < pieces; c += LANES) {
     float sum[V] = {}, x[V];
     if constexpr (DOTS) widen<DT>(load_raw<ALIGNED>(other, c), x);
     for (int j0 = 0; j0 < a.k; j0 += kPicks) {
-      if (j0) load_picks(a, t, j0, p);
+      if (j0) load_picks<LANES>(a, t, j0, p);
 #pragma unroll
       for (int j = 0; j < kPicks; ++j) {
         if (p.row[j] < 0) continue;
@@ -201,7 +214,7 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
         }
       }
     }
-    if (!few) load_picks(a, t, 0, p);
+    if (!few) load_picks<LANES>(a, t, 0, p);
     store_raw<ALIGNED>(dst, c, narrow<DT>(sum));
   }
   if (at < rest) {
@@ -218,7 +231,7 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
   if constexpr (DOTS) {
     for (int j0 = 0; j0 < a.k; j0 += kPicks) {
       if (!few) {
-        load_picks(a, t, j0, p);
+        load_picks<LANES>(a, t, j0, p);
 #pragma unroll
         for (int j = 0; j < kPicks; ++j) dot[j] = 0.f;
         for (int c = at; c < pieces; c += LANES) {
@@ -241,23 +254,35 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
         for (int j = 0; j < kPicks; ++j)
           if (p.row[j] >= 0) dot[j] = __builtin_fmaf(x, load_as_f32<DT>((const char *)a.src + p.row[j] * a.src_stride * SIZE, i), dot[j]);
       }
-      store_dots<WAVES>(a, t, j0, dot, lds);
+      store_dots<LANES>(a, t, j0, dot, lds);
     }
   }
 }
 
-// Four waves to a token where one each would leave CUs idle or a wave with a long row.
+// The lanes of a token: 16 for short rows, the workgroup where a wave to a token would leave the chip's 8192 places for waves empty, or the row is long, else
+// a wave (us, four picks unless said otherwise):
+//   dispatch of 20000 rows of 64 bf16, eight picks, 6.7 by 16 lanes and 15.1 by a wave; 7816 of 176, six picks, 6.4 and 7.3; 2386 of 352 4.9 and 3.9
+//   dispatch of 64 rows of 2880 bf16 5.4 by a wave and 3.1 by 256 lanes; 1000 of 1440, eight picks, 8.3 and 6.8; 16384 of 2880 102 and 96
+//   combine of 4099 rows of 1063 float32, two picks, 15.4 by a wave and 18.5 by 256 lanes; 1021 of 2016 bf16, six picks, 14.6 and 7.8
+//   combine_backward of 4096 rows of 2880 bf16 47 by a wave and 53 by 256 lanes; 1021 of 2016, six picks, 25.7 and 16.3
+inline int lanes_of(int T, int pieces, bool dots) {
+  if (pieces <= 32 || (pieces <= 64 && T >= 8192)) return 16;
+  if (pieces >= 128 && (T < (dots ? 2500 : 4096) || (!dots && pieces >= 320))) return 256;
+  return 64;
+}
+
 template <int DT, bool ALIGNED, bool DOTS, bool GATES>
 int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
-  const bool wide = a.T <= 4096;
-  const dim3 grid(wide ? (unsigned)a.T : (unsigned)(((int64_t)a.T + 3) / 4));
-  if (spread) {
-    if (wide) spread_kernel<DT, ALIGNED, 4, DOTS, GATES><<<grid, 256, 0, st>>>(a);
-    else spread_kernel<DT, ALIGNED, 1, DOTS, GATES><<<grid, 256, 0, st>>>(a);
-  } else {
-    if (wide) collect_kernel<DT, ALIGNED, 4, DOTS><<<grid, 256, 0, st>>>(a);
-    else collect_kernel<DT, ALIGNED, 1, DOTS><<<grid, 256, 0, st>>>(a);
-  }
+  const int lanes = lanes_of(a.T, a.H / kPiece<DT>, DOTS);
+  const auto go = [&](auto of) {
+    constexpr int LANES = decltype(of)::value;
+    const unsigned grid = (unsigned)(((int64_t)a.T * LANES + 255) / 256);
+    if (spread) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES><<<grid, 256, 0, st>>>(a);
+    else collect_kernel<DT, ALIGNED, LANES, DOTS><<<grid, 256, 0, st>>>(a);
+  };
+  if (lanes == 16) go(std::integral_constant<int, 16>());
+  else if (lanes == 64) go(std::integral_constant<int, 64>());
+  else go(std::integral_constant<int, 256>());
   return launch_status();
 }
 template <int DT, bool ALIGNED>
