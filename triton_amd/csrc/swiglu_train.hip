@@ -8,7 +8,11 @@
 // What is kept is the MXFP8 form of a that tamd_downcast_mxfp makes of it (e4m3 values, one e8m0 scale per 32 along a row, rounded up):
 // 1.03 bytes per value in place of the 2 of a itself.  The gradient is that of the function at the kept values.
 //
-// Four lanes share a group of 32, eight values (four pairs) each, U groups per thread.
+// Four lanes share a group of 32, eight values (four pairs) each.  What bounds it is memory: 65536 x 2880 bf16 takes 252 us forward (6.0 TB/s) and 305
+// backward with the activation again (6.2).  BIG, from 64 MB on: two groups per thread, everything past the caches, which do not keep that much until
+// it is used (16384 x 2880: 66 us, 71 through them).  Below: one group per thread (1024 x 1056: 4.0 us, 5.1 with two), a and the results through the
+// caches.  float32 takes the second form always: 16-byte pieces of its results are every other one of a line, which past the caches costs
+// 6 % in place of gaining 4.  The kept values go past the caches in both: nothing reads them before the backward pass.
 #include "mx_values.h"
 #include <type_traits>
 
@@ -21,24 +25,28 @@ typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_by1_t __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t u32x2_by1_t __attribute__((ext_vector_type(2), aligned(1)));
 
-template <bool ALIGNED>
+template <bool ALIGNED, bool ONCE>
 TAMD_DEVICE u32x4_t load16(const void *p) {
-  if constexpr (ALIGNED) return *(const u32x4_t *)p;
+  if constexpr (ALIGNED && ONCE) return __builtin_nontemporal_load((const u32x4_t *)p);
+  else if constexpr (ALIGNED) return *(const u32x4_t *)p;
   else return *(const u32x4_by1_t *)p;
 }
-template <bool ALIGNED>
+template <bool ALIGNED, bool ONCE>
 TAMD_DEVICE u32x2_t load8(const void *p) {
-  if constexpr (ALIGNED) return *(const u32x2_t *)p;
+  if constexpr (ALIGNED && ONCE) return __builtin_nontemporal_load((const u32x2_t *)p);
+  else if constexpr (ALIGNED) return *(const u32x2_t *)p;
   else return *(const u32x2_by1_t *)p;
 }
-template <bool ALIGNED>
+template <bool ALIGNED, bool ONCE>
 TAMD_DEVICE void store16(void *p, u32x4_t q) {
-  if constexpr (ALIGNED) *(u32x4_t *)p = q;
+  if constexpr (ALIGNED && ONCE) __builtin_nontemporal_store(q, (u32x4_t *)p);
+  else if constexpr (ALIGNED) *(u32x4_t *)p = q;
   else *(u32x4_by1_t *)p = q;
 }
-template <bool ALIGNED>
+template <bool ALIGNED, bool ONCE>
 TAMD_DEVICE void store8(void *p, u32x2_t q) {
-  if constexpr (ALIGNED) *(u32x2_t *)p = q;
+  if constexpr (ALIGNED && ONCE) __builtin_nontemporal_store(q, (u32x2_t *)p);
+  else if constexpr (ALIGNED) *(u32x2_t *)p = q;
   else *(u32x2_by1_t *)p = q;
 }
 
@@ -50,22 +58,22 @@ TAMD_DEVICE uint32_t pack2(float a, float b) {
 }
 
 // N (4 or 8) elements at p, of which `n` are there
-template <int DT, bool ALIGNED, int N>
+template <int DT, bool ALIGNED, bool ONCE, int N>
 TAMD_DEVICE void load_values(const void *p, int n, float (&v)[N]) {
   if (n == N) {
     if constexpr (DT == TAMD_F32) {
 #pragma unroll
       for (int i = 0; i < N; i += 4) {
-        const u32x4_t q = load16<ALIGNED>((const float *)p + i);
+        const u32x4_t q = load16<ALIGNED, ONCE>((const float *)p + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[i + e] = bits_to_f32(q[e]);
       }
     } else if constexpr (N == 8) {
-      const u32x4_t q = load16<ALIGNED>(p);
+      const u32x4_t q = load16<ALIGNED, ONCE>(p);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[2 * e] = widen16(q[e] & 0xFFFFu, DT), v[2 * e + 1] = widen16(q[e] >> 16, DT);
     } else {
-      const u32x2_t q = load8<ALIGNED>(p);
+      const u32x2_t q = load8<ALIGNED, ONCE>(p);
 #pragma unroll
       for (int e = 0; e < 2; ++e) v[2 * e] = widen16(q[e] & 0xFFFFu, DT), v[2 * e + 1] = widen16(q[e] >> 16, DT);
     }
@@ -74,17 +82,17 @@ TAMD_DEVICE void load_values(const void *p, int n, float (&v)[N]) {
     for (int e = 0; e < N; ++e) v[e] = e < n ? load_as_f32<DT>(p, e) : 0.f;
   }
 }
-template <int DT, bool ALIGNED, int N>
+template <int DT, bool ALIGNED, bool ONCE, int N>
 TAMD_DEVICE void store_values(void *p, int n, const float (&v)[N]) {
   if (n == N) {
     if constexpr (DT == TAMD_F32) {
 #pragma unroll
       for (int i = 0; i < N; i += 4)
-        store16<ALIGNED>((float *)p + i, u32x4_t{f32_to_bits(v[i]), f32_to_bits(v[i + 1]), f32_to_bits(v[i + 2]), f32_to_bits(v[i + 3])});
+        store16<ALIGNED, ONCE>((float *)p + i, u32x4_t{f32_to_bits(v[i]), f32_to_bits(v[i + 1]), f32_to_bits(v[i + 2]), f32_to_bits(v[i + 3])});
     } else if constexpr (N == 8) {
-      store16<ALIGNED>(p, u32x4_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])});
+      store16<ALIGNED, ONCE>(p, u32x4_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])});
     } else {
-      store8<ALIGNED>(p, u32x2_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])});
+      store8<ALIGNED, ONCE>(p, u32x2_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])});
     }
   } else {
 #pragma unroll
@@ -115,11 +123,11 @@ TAMD_DEVICE Pair pair_of(float g, float l, const GluShape &sh) {
   return p;
 }
 
-template <int DT, bool ALIGNED, int U>
+template <int DT, bool ALIGNED, bool BIG>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const void *__restrict__ a, int64_t a_stride, void *__restrict__ out, int64_t out_stride,
                                                          uint8_t *__restrict__ values, int64_t v_stride, uint8_t *__restrict__ scales, int64_t s_stride,
                                                          GluShape sh) {
-  constexpr int SIZE = DT == TAMD_F32 ? 4 : 2;
+  constexpr int SIZE = DT == TAMD_F32 ? 4 : 2, U = BIG ? 2 : 1;
   const int sub = threadIdx.x & 3;
   const int64_t gid0 = (int64_t)blockIdx.x * (64 * U) + (threadIdx.x >> 2);
   int64_t r[U], g[U];
@@ -132,7 +140,7 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const void *__restrict_
     place_group(sh.div, gid < sh.div.total ? gid : 0, b, r[u], g[u]);
     const int64_t left = sh.L - g[u] * 32 - sub * 8;
     n[u] = gid >= sh.div.total || left <= 0 ? 0 : (left < 8 ? (int)left : 8);
-    load_values<DT, ALIGNED, 8>((const char *)a + (r[u] * a_stride + g[u] * 32 + sub * 8) * SIZE, n[u], v[u]);
+    load_values<DT, ALIGNED, BIG, 8>((const char *)a + (r[u] * a_stride + g[u] * 32 + sub * 8) * SIZE, n[u], v[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -167,10 +175,10 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const void *__restrict_
       o[j] = __builtin_fmaf(gs, p.l, gs);
     }
     if (n[u] == 0) continue;
-    store_values<DT, ALIGNED, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
+    store_values<DT, ALIGNED, BIG, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
     uint8_t *const vp = values + r[u] * v_stride + g[u] * 32 + sub * 8;
     if (n[u] == 8) {
-      store8<ALIGNED>(vp, u32x2_t{code[0], code[1]});
+      store8<ALIGNED, true>(vp, u32x2_t{code[0], code[1]});
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -180,11 +188,11 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const void *__restrict_
   }
 }
 
-template <int DT, bool ALIGNED, bool AGAIN, int U>
+template <int DT, bool ALIGNED, bool AGAIN, bool BIG>
 __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ dout, int64_t d_stride, const uint8_t *__restrict__ values, int64_t v_stride,
                                                        const uint8_t *__restrict__ scales, int64_t s_stride, void *__restrict__ da, int64_t da_stride,
                                                        void *__restrict__ out, int64_t out_stride, GluShape sh) {
-  constexpr int SIZE = DT == TAMD_F32 ? 4 : 2;
+  constexpr int SIZE = DT == TAMD_F32 ? 4 : 2, U = BIG ? 2 : 1;
   const int sub = threadIdx.x & 3;
   const int64_t gid0 = (int64_t)blockIdx.x * (64 * U) + (threadIdx.x >> 2);
   int64_t r[U], g[U];
@@ -200,7 +208,7 @@ __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ 
     n[u] = gid >= sh.div.total || left <= 0 ? 0 : (left < 8 ? (int)left : 8);
     const uint8_t *const vp = values + r[u] * v_stride + g[u] * 32 + sub * 8;
     if (n[u] == 8) {
-      const u32x2_t q = load8<ALIGNED>(vp);
+      const u32x2_t q = load8<ALIGNED, BIG>(vp);
       code[u][0] = q[0], code[u][1] = q[1];
     } else {
       code[u][0] = code[u][1] = 0;
@@ -209,7 +217,7 @@ __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ 
         if (j < n[u]) code[u][j >> 2] |= (uint32_t)vp[j] << (8 * (j & 3));
     }
     byte[u] = n[u] ? scales[r[u] * s_stride + g[u]] : 0u;
-    load_values<DT, ALIGNED, 4>((const char *)dout + (r[u] * d_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, d[u]);
+    load_values<DT, ALIGNED, BIG, 4>((const char *)dout + (r[u] * d_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, d[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -232,21 +240,20 @@ __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ 
       dv[2 * j] = p.g_free ? __builtin_fmaf(ds, p.l, ds) * slope : 0.f;
       dv[2 * j + 1] = p.l_free ? ds * p.g : 0.f;
     }
-    store_values<DT, ALIGNED, 8>((char *)da + (r[u] * da_stride + g[u] * 32 + sub * 8) * SIZE, n[u], dv);
-    if constexpr (AGAIN) store_values<DT, ALIGNED, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
+    store_values<DT, ALIGNED, BIG, 8>((char *)da + (r[u] * da_stride + g[u] * 32 + sub * 8) * SIZE, n[u], dv);
+    if constexpr (AGAIN) store_values<DT, ALIGNED, BIG, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
   }
 }
 
-constexpr int kU = 2;
-
-bool shape(GluShape &sh, int64_t M, int64_t N, float alpha, float limit, int has_limit, unsigned &blocks) {
-  const int64_t G = (2 * N + 31) / 32;
+bool shape(GluShape &sh, int64_t M, int64_t N, float alpha, float limit, int has_limit, bool big, unsigned &blocks) {
+  const int64_t G = (2 * N + 31) / 32, per = big ? 128 : 64;
   sh.div = group_div(1, M, G);
   sh.L = 2 * N, sh.alpha = alpha, sh.limit = limit, sh.has_limit = has_limit;
-  const int64_t n = (sh.div.total + 64 * kU - 1) / (64 * kU);
+  const int64_t n = (sh.div.total + per - 1) / per;
   blocks = (unsigned)n;
   return n < ((int64_t)1 << 31);
 }
+bool is_big(int dtype, bool aligned, int64_t M, int64_t N, int bytes) { return dtype != TAMD_F32 && aligned && (double)M * N * bytes >= 64e6; }
 bool whole(const void *p, int64_t stride_bytes, int by) { return ((uintptr_t)p | (uintptr_t)stride_bytes) % by == 0; }
 bool plain(int dt) { return dt == TAMD_F32 || dt == TAMD_BF16 || dt == TAMD_F16; }
 
@@ -261,15 +268,17 @@ extern "C" int tamd_swiglu_checkpoint(const void *a, int dtype, int64_t M, int64
   const int size = dtype == TAMD_F32 ? 4 : 2;
   if (!whole(a, 0, size) || !whole(out, 0, size)) return TAMD_E_ALIGNMENT;
   if (M >= ((int64_t)1 << 31) || N >= ((int64_t)1 << 30)) return TAMD_E_TOO_LARGE;
+  const bool aligned = whole(a, a_stride * size, 16) && whole(out, out_stride * size, 4 * size) && whole(values, values_stride, 8);
+  const bool big = is_big(dtype, aligned, M, N, 8);
   GluShape sh;
   unsigned blocks;
-  if (!shape(sh, M, N, alpha, limit, has_limit, blocks)) return TAMD_E_TOO_LARGE;
+  if (!shape(sh, M, N, alpha, limit, has_limit, big, blocks)) return TAMD_E_TOO_LARGE;
   hipStream_t st = (hipStream_t)stream;
-  const bool aligned = whole(a, a_stride * size, 16) && whole(out, out_stride * size, 4 * size) && whole(values, values_stride, 8);
   const auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (aligned) checkpoint_kernel<DT, true, kU><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
-    else checkpoint_kernel<DT, false, kU><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
+    if (big) checkpoint_kernel<DT, true, DT != TAMD_F32><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
+    else if (aligned) checkpoint_kernel<DT, true, false><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
+    else checkpoint_kernel<DT, false, false><<<blocks, 256, 0, st>>>(a, a_stride, out, out_stride, values, values_stride, scales, scales_stride, sh);
   };
   if (dtype == TAMD_F32) go(std::integral_constant<int, TAMD_F32>());
   else if (dtype == TAMD_BF16) go(std::integral_constant<int, TAMD_BF16>());
@@ -288,19 +297,24 @@ extern "C" int tamd_swiglu_backward(const void *dout, int dtype, int64_t M, int6
   const int size = dtype == TAMD_F32 ? 4 : 2;
   if (!whole(dout, 0, size) || !whole(da, 0, size) || !whole(out, 0, size)) return TAMD_E_ALIGNMENT;
   if (M >= ((int64_t)1 << 31) || N >= ((int64_t)1 << 30)) return TAMD_E_TOO_LARGE;
-  GluShape sh;
-  unsigned blocks;
-  if (!shape(sh, M, N, alpha, limit, has_limit, blocks)) return TAMD_E_TOO_LARGE;
-  hipStream_t st = (hipStream_t)stream;
   const bool aligned = whole(dout, dout_stride * size, 4 * size) && whole(da, da_stride * size, 16) && whole(values, values_stride, 8) &&
                        (!out || whole(out, out_stride * size, 4 * size));
-  const auto go = [&](auto dt, auto al, auto again) {
-    backward_kernel<decltype(dt)::value, decltype(al)::value, decltype(again)::value, kU>
+  const bool big = is_big(dtype, aligned, M, N, 8);
+  GluShape sh;
+  unsigned blocks;
+  if (!shape(sh, M, N, alpha, limit, has_limit, big, blocks)) return TAMD_E_TOO_LARGE;
+  hipStream_t st = (hipStream_t)stream;
+  const auto go = [&](auto dt, auto al, auto again, auto large) {
+    constexpr int DT = decltype(dt)::value;
+    backward_kernel<DT, decltype(al)::value, decltype(again)::value, DT != TAMD_F32 && decltype(large)::value>
         <<<blocks, 256, 0, st>>>(dout, dout_stride, values, values_stride, scales, scales_stride, da, da_stride, out, out_stride, sh);
   };
   const auto with = [&](auto dt) {
-    if (aligned) out ? go(dt, std::true_type(), std::true_type()) : go(dt, std::true_type(), std::false_type());
-    else out ? go(dt, std::false_type(), std::true_type()) : go(dt, std::false_type(), std::false_type());
+    const std::true_type yes;
+    const std::false_type no;
+    if (big) out ? go(dt, yes, yes, yes) : go(dt, yes, no, yes);
+    else if (aligned) out ? go(dt, yes, yes, no) : go(dt, yes, no, no);
+    else out ? go(dt, no, yes, no) : go(dt, no, no, no);
   };
   if (dtype == TAMD_F32) with(std::integral_constant<int, TAMD_F32>());
   else if (dtype == TAMD_BF16) with(std::integral_constant<int, TAMD_BF16>());
