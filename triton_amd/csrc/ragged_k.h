@@ -163,7 +163,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
     for (int f = 0; f < NF; ++f) df[into][f] = fragment(d_at[f] + slot + k * 16 * 2 * BN, 2 * BN);
 #pragma unroll
     for (int f = 0; f < MF; ++f) xf[into][f] = fragment(x_at[f] + slot + k * 16 * 2 * BM, 2 * BM);
-    __builtin_amdgcn_sched_barrier(0);
   };
   // between(f) is called behind the f-th part of the instructions
   const auto multiply = [&](int from, auto between) {
@@ -171,8 +170,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
     for (int f = 0; f < MF; ++f) {
 #pragma unroll
       for (int h = 0; h < NF; ++h) acc[f][h] = mma<DT>(df[from][h], xf[from][f], acc[f][h]);
-      __builtin_amdgcn_sched_barrier(0);
       between(f);
+    }
+    // two reads of the next step's fragments, one product: 1.97 ms in place of 2.06 with all reads in front (65536 rows over 32 slices, 2880 x 5760)
+#pragma unroll
+    for (int g = 0; g < MF * NF; ++g) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
   };
   struct Stage {
@@ -206,7 +210,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
       multiply(0, [&](int f) {   // the rest of the stage that the slot before takes
 #pragma unroll
         for (int c = FIRST + f * (COPIES - FIRST) / MF; c < FIRST + (f + 1) * (COPIES - FIRST) / MF; ++c) copy(b, c, before);
-        __builtin_amdgcn_sched_barrier(0);
       });
       wait_copies<(RING - 2) * COPIES>();
       sync_threads();   // stage s + 1 is visible; every wave has read stage s
@@ -215,7 +218,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
       multiply(1, [&](int f) {
 #pragma unroll
         for (int c = f * FIRST / MF; c < (f + 1) * FIRST / MF; ++c) copy(b, c, slot);
-        __builtin_amdgcn_sched_barrier(0);
       });
       before = slot;
       slot = next;
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
 }
 
 // The tiles that there are (BM x BN, stages in flight).  One of 128 x 256 or 256 x 128, two to a CU, for long slices of many tiles: 65536 rows over 32 slices,
-// 2880 x 5760, 2.05 ms, and 2.24 with 128 x 128; 4096 over 8, 2048 x 4096, 80 and 80 us, 2048 over 8 56 and 52.  (256 x 256, one to a CU: 2.03 ms, 81 and 58.)
+// 2880 x 5760, 1.97 ms, and 2.24 with 128 x 128; 4096 over 8, 2048 x 4096, 80 and 80 us, 2048 over 8 56 and 52.  (256 x 256, one to a CU: 1.99 ms, 81 and 58.)
 // 128 x 128 with two stages, four to a CU, where a slice has few of them: 1332 rows over 32 slices, 2016 x 2112, 53 us, 62 with three, which
 // cost a CU its fourth workgroup; with 2500 rows of 64 x 64 each the third stage gives 47 in place of 72.
 enum RaggedTile { kTile128x256, kTile256x128, kTile128Short, kTile128 };
