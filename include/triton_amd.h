@@ -506,7 +506,8 @@ int tamd_sample(const tamd_sample_args *args, size_t args_size, void *stream);
  * Without a row a pick adds nothing, and its dot is 0; tamd_dispatch leaves rows of dst that no pick names as they are, and rows that
  * several picks name hold one of them, or a mixture.  Sums are float32, in the order of j; results are rounded once.
  * dots (and with it other): NULL, or [T, k] in gates_dtype.  src, dst and other are of `dtype` (float32, bfloat16, float16), with unit stride along
- * H and any row pitch; rows that all start on 16-byte boundaries are the fast form.  dst overlaps nothing that is read.
+ * H and any row pitch; rows that all start on 16-byte boundaries are the fast form.  dst overlaps nothing that is read, but
+ * for tamd_dispatch's may be `other` itself.
  */
 typedef struct tamd_token_rows_args {
   const void *src;

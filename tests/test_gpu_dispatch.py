@@ -227,3 +227,15 @@ def test_another_stream_and_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+@pytest.mark.parametrize("T,k,H", [(40, 4, 264), (3000, 2, 1032), (9, 11, 77), (9000, 3, 64)])
+def test_gradient_in_the_place_of_the_rows(T, k, H, device):
+    """combine_backward into the rows that it reads: what it gives elsewhere."""
+    torch.manual_seed(T)
+    for dtype in (torch.bfloat16, torch.float32):
+        p, gates = places(T, k, T * k, 0.1).to(device), torch.rand(T, k, device=device)
+        dy, rows = torch.randn(T, H, device=device).to(dtype), torch.randn(T * k, H, device=device).to(dtype)
+        want, dgates = combine_backward(dy, p, rows=rows, gates=gates, out=rows.clone())
+        got, same = combine_backward(dy, p, rows=rows, gates=gates, out=rows)
+        assert got is rows and torch.equal(got, want) and torch.equal(same, dgates)

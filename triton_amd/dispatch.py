@@ -146,7 +146,7 @@ def combine_backward(dy: torch.Tensor, row_indx: torch.Tensor, rows: Optional[to
       drows[row_indx[t, j]] = gates[t, j] * dy[t]        dgates[t, j] = <dy[t], rows[row_indx[t, j]]>
 
     Returns (drows, dgates [T, k] in the gates' type).  drows is [T * k, H] in dy's type, or `out`, as in `dispatch`: rows that no pick names
-    are left as they are.  dgates is None without gates, and without rows, which nothing else needs and which are as many as drows."""
+    are left as they are.  out may be `rows` itself, which the gradient then takes the place of.  dgates is None without gates, and without rows, which nothing else needs and which are as many as drows."""
     done = _native.combine_backward(dy, row_indx, rows, gates, out)
     if done is not None:
         if type(done) is int:

@@ -83,7 +83,7 @@ def swiglu_checkpoint(a: torch.Tensor, alpha: float, precision_config: Precision
 
     a: [..., 2 N].  Returns (out [..., N] in a's type, values float8_e4m3fn [..., 2 N], scales uint8 [..., ceil(2 N / 32)]): values and
     scales are those of `downcast_to_mxfp(a, torch.float8_e4m3fn, -1)`, which `upcast_from_mxfp` reads, with a short last group
-    where 32 does not divide 2 N.  out is computed from a itself, in float32, and rounded once.  Unlike in `swiglu`, a NaN stays one beside a
+    where 32 does not divide 2 N (they may share one storage).  out is computed from a itself, in float32, and rounded once.  Unlike in `swiglu`, a NaN stays one beside a
     limit; the group of an infinity is NaN in what is kept."""
     done = _native.swiglu_checkpoint(a, alpha, precision_config)
     if done is not None:
