@@ -148,7 +148,7 @@ def _by_rows(t):
 
 
 def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
-    """Y[e] = a[:, slice e] @ b[slice e, :] (matmul.py:376-391 of the reference, ragged_dimension "K")."""
+    """Y[e] = a[:, slice e] @ b[slice e, :] (matmul.py:376 of the reference, ragged_dimension "K")."""
     a, b = _data(a), _data(b)
     flex = pc.flex_ctx
     if (any(getattr(pc, f) is not None for f in ("a_mx_scale", "b_mx_scale", "c_mx_scale", "a_mx_tensor_scale", "b_mx_tensor_scale")) or pc.acc_scale != 1.0
