@@ -559,8 +559,8 @@ int tamd_topk_backward(const void *x, int dtype, int64_t x_stride, int64_t n_row
 
 /* ---------------------------------------------------------------------------
  * Products over ragged rows (matmul.py's b_ragged_metadata): y[e, m, n] = sum over the rows r of slice e of x[r, m] d[r, n], with which
- * the gradients of all experts' weights are one call.  Slice e holds the rows slice_offs[e] .. slice_offs[e + 1] (int32, E + 1 of them, cut to
- * [0, K]); an empty one gives zeros, and rows of no slice take no part, whatever they hold.
+ * the gradients of all experts' weights are one call.  Slice e holds the slice_sizes[e] rows from slice_offs[e] on (int32, E of each, cut to
+ * [0, K]); an empty one gives zeros, and rows of no slice, as between padded ones, take no part, whatever they hold.
  * x: [K, M], d: [K, N] of `dtype` (bfloat16, float16), y: [E, M, N] of y_dtype (float32, bfloat16, float16), with unit stride along M, N and N; any
  * pitch and start, of which whole 16 bytes (and M and N in eights) are taken as they are, others laid out so first.  Sums are float32, rounded once.
  * workspace: tamd_ragged_k_matmul_workspace(args, size) bytes for the same arguments but this one (negative: what the call would
@@ -571,7 +571,7 @@ typedef struct tamd_ragged_k_args {
   int64_t x_stride;
   const void *d;
   int64_t d_stride;
-  const int32_t *slice_offs;
+  const int32_t *slice_offs, *slice_sizes;
   void *y;
   int64_t y_stride_e, y_stride_m;
   void *workspace;

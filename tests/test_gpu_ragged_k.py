@@ -116,6 +116,18 @@ def test_offsets_past_the_rows_are_cut(device):
     check(matmul(x.t(), d, None, md, md), x, d, [30, 20, 0], torch.bfloat16)
 
 
+def test_padded_slices(device):
+    """Slices that begin on multiples of 64, with NaN in the rows between them: only a slice's own rows are summed."""
+    sizes, starts = [40, 0, 64, 3], [0, 64, 64, 128]
+    x, d = torch.full((200, 72), float("nan"), device=device).bfloat16(), torch.full((200, 136), float("nan"), device=device).bfloat16()
+    for n, at in zip(sizes, starts):
+        x[at:at + n], d[at:at + n] = torch.randn(n, 72, device=device), torch.randn(n, 136, device=device)
+    md = ragged(sizes, 200, device)
+    md.slice_offs = torch.tensor([*starts, 192], dtype=torch.int32, device=device)
+    rows = torch.cat([torch.arange(at, at + n) for n, at in zip(sizes, starts)]).to(device)
+    check(matmul(x.t(), d, None, md, md), x[rows], d[rows], sizes, torch.bfloat16)
+
+
 def test_rows_past_four_gigabytes(device):
     """A slice whose rows lie beyond what 32 bits count."""
     rows, M, N = 2 ** 19 + 100, 4352, 64

@@ -12,7 +12,7 @@ from triton_amd.tensor import RaggedTensorMetadata
 
 
 def good(**more):
-    return _lib.RaggedKArgs(**{**dict(x=0x1000, x_stride=64, d=0x2000, d_stride=64, slice_offs=0x3000, y=0x4000, y_stride_e=4096, y_stride_m=64, K=100, dtype=_lib.BF16,
+    return _lib.RaggedKArgs(**{**dict(x=0x1000, x_stride=64, d=0x2000, d_stride=64, slice_offs=0x3000, slice_sizes=0x3800, y=0x4000, y_stride_e=4096, y_stride_m=64, K=100, dtype=_lib.BF16,
                                       y_dtype=_lib.BF16, M=0, N=64, E=2), **more})
 
 
@@ -26,9 +26,9 @@ def test_c_entry_point():
     for dtype in (_lib.F32, _lib.FP8_E4M3):
         assert code(good(dtype=dtype)) == _lib.E_UNSUPPORTED
     assert code(good(y_dtype=_lib.FP8_E4M3)) == _lib.E_UNSUPPORTED
-    for field in ("x", "d", "y", "slice_offs"):
+    for field in ("x", "d", "y", "slice_offs", "slice_sizes"):
         assert code(good(M=64, **{field: None})) == _lib.E_INVALID, field
-        if field != "slice_offs":
+        if not field.startswith("slice"):
             assert code(good(M=64, **{field: 0x1001})) == _lib.E_ALIGNMENT, field
     assert code(good(M=64, y_dtype=_lib.F32, y=0x4002)) == _lib.E_ALIGNMENT
     assert code(good(M=64, K=1 << 31)) == _lib.E_TOO_LARGE and code(good(M=2 ** 31 - 1, N=2 ** 31 - 1)) == _lib.E_TOO_LARGE

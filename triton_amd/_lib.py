@@ -159,7 +159,7 @@ class TokenRowsArgs(C.Structure):
 class RaggedKArgs(C.Structure):
     """Mirror of `tamd_ragged_k_args`."""
     _fields_ = [
-        ("x", C.c_void_p), ("x_stride", C.c_int64), ("d", C.c_void_p), ("d_stride", C.c_int64), ("slice_offs", C.c_void_p),
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("d", C.c_void_p), ("d_stride", C.c_int64), ("slice_offs", C.c_void_p), ("slice_sizes", C.c_void_p),
         ("y", C.c_void_p), ("y_stride_e", C.c_int64), ("y_stride_m", C.c_int64), ("workspace", C.c_void_p), ("K", C.c_int64),
         ("dtype", C.c_int), ("y_dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("E", C.c_int),
     ]

@@ -1079,17 +1079,18 @@ PyObject *py_topk_backward(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
   });
 }
 
-// (a [M, K], b [K, N], slice_offs, slices, the output's type or None): the product over every slice's rows, [slices, M, N].
+// (a [M, K], b [K, N], slice_offs, slice_sizes, the output's type or None): the product over every slice's rows, [slices, M, N].
 PyObject *py_matmul_ragged_k(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
   return covered([&]() -> PyObject * {
     need(nargs == 5);
     int dev = -1;
-    const at::Tensor &a = current_gpu_tensor(v[0], dev), &b = gpu_tensor(v[1], dev), &offs = gpu_tensor(v[2], dev);
-    const int64_t E = as_int(v[3]);
+    const at::Tensor &a = current_gpu_tensor(v[0], dev), &b = gpu_tensor(v[1], dev), &offs = gpu_tensor(v[2], dev), &sizes = gpu_tensor(v[3], dev);
+    const int64_t E = sizes.dim() == 1 ? sizes.size(0) : 0;
     need(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(0) && a.scalar_type() == b.scalar_type());
     const int64_t M = a.size(0), K = a.size(1), N = b.size(1);
     need(M >= 1 && N >= 1 && K >= 1 && E >= 1 && M < 1ll << 30 && N < 1ll << 30 && E < 1ll << 30 && K < 1ll << 31);
     need((a.stride(0) == 1 || M == 1) && (b.stride(1) == 1 || N == 1) && offs.scalar_type() == at::kInt && offs.dim() == 1 && offs.size(0) == E + 1 && offs.stride(0) == 1);
+    need(sizes.scalar_type() == at::kInt && sizes.stride(0) == 1);
     tamd_ragged_k_args g;
     std::memset(&g, 0, sizeof g);
     const at::ScalarType t = v[4] == Py_None ? a.scalar_type() : dtype_of(v[4]);
@@ -1097,7 +1098,7 @@ PyObject *py_matmul_ragged_k(PyObject *, PyObject *const *v, Py_ssize_t nargs) {
     need((g.dtype == TAMD_BF16 || g.dtype == TAMD_F16) && plain_code(g.y_dtype));
     at::Tensor y = new_empty({E, M, N}, t, dev), ws;
     g.x = a.data_ptr(), g.x_stride = K > 1 ? a.stride(1) : M, g.d = b.data_ptr(), g.d_stride = K > 1 ? b.stride(0) : N;
-    g.slice_offs = (const int32_t *)offs.data_ptr(), g.y = y.data_ptr(), g.y_stride_e = M * N, g.y_stride_m = N;
+    g.slice_offs = (const int32_t *)offs.data_ptr(), g.slice_sizes = (const int32_t *)sizes.data_ptr(), g.y = y.data_ptr(), g.y_stride_e = M * N, g.y_stride_m = N;
     g.K = K, g.M = (int)M, g.N = (int)N, g.E = (int)E;
     const int64_t n_ws = abi.ragged_k_workspace(&g, sizeof g);
     if (n_ws < 0) return PyLong_FromLong((long)n_ws);

@@ -20,7 +20,7 @@ struct RaggedK {
   const void *x, *d;
   int64_t x_pitch, d_pitch;           // elements, a multiple of 8
   int x_cols, d_cols;                 // columns that can be read: M and N, filled up to a multiple of 8
-  const int32_t *offs;                // [E + 1]
+  const int32_t *offs, *sizes;        // [E]
   void *y;
   int64_t y_stride_e, y_stride_m, y_stride_split;
   int64_t K;                          // rows of x and d
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
   const uint32_t w = a.tiles_n - 4u * g < 4u ? a.tiles_n - 4u * g : 4u;
   const int m0 = (int)(tg / w) * BM, n0 = (int)(4u * g + tg % w) * BN;
 
-  int64_t begin = a.offs[e], end = a.offs[e + 1];
+  int64_t begin = a.offs[e], end = begin + a.sizes[e];
   begin = begin < 0 ? 0 : begin;
   end = end > a.K ? a.K : end;
   const int64_t stages = end > begin ? (end - begin + kRaggedBK - 1) / kRaggedBK : 0;

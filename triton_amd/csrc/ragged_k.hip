@@ -117,7 +117,7 @@ int check(const tamd_ragged_k_args *args, size_t args_size, bool &ok) {
   if (a.x_stride < 0 || a.d_stride < 0 || a.y_stride_e < 0 || a.y_stride_m < 0) return TAMD_E_INVALID;
   if (a.M == 0 || a.N == 0 || a.E == 0) return 0;
   if (too_large(a.M, a.N, a.E, a.K)) return TAMD_E_TOO_LARGE;
-  if (!a.y || !a.slice_offs || (a.K > 0 && (!a.x || !a.d))) return TAMD_E_INVALID;
+  if (!a.y || !a.slice_offs || !a.slice_sizes || (a.K > 0 && (!a.x || !a.d))) return TAMD_E_INVALID;
   if ((uintptr_t)a.x % 2 || (uintptr_t)a.d % 2 || (uintptr_t)a.y % (a.y_dtype == TAMD_F32 ? 4 : 2)) return TAMD_E_ALIGNMENT;
   ok = true;
   return 0;
@@ -142,7 +142,7 @@ extern "C" int tamd_ragged_k_matmul(const tamd_ragged_k_args *args, size_t args_
   hipStream_t st = (hipStream_t)stream;
   uint8_t *const room = (uint8_t *)a.workspace;
   const int size = a.y_dtype == TAMD_F32 ? 4 : 2;
-  RaggedK k{a.x, a.d, a.x_stride, a.d_stride, a.M, a.N, a.slice_offs, a.y, a.y_stride_e, a.y_stride_m, 0, a.K, a.M, a.N, a.E, a.y_dtype, 0, 0, p.tiles_m, p.tiles_n, p.splits};
+  RaggedK k{a.x, a.d, a.x_stride, a.d_stride, a.M, a.N, a.slice_offs, a.slice_sizes, a.y, a.y_stride_e, a.y_stride_m, 0, a.K, a.M, a.N, a.E, a.y_dtype, 0, 0, p.tiles_m, p.tiles_n, p.splits};
   LaidBoth both;
   int n = 0;
   if (p.lay_x) {

@@ -156,7 +156,7 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
             or flex.rhs_data.dtype is not None or flex.out_data.expected_scale is not None or flex.out_data.actual_scale is not None):
         raise NotImplementedError("K-ragged matmul takes unscaled operands")
     if c is None and (a_ragged is None or a_ragged.n_slices == b_ragged.n_slices):
-        done = _native.matmul_ragged_k(a, b, b_ragged.slice_offs, b_ragged.n_slices, pc.out_dtype)
+        done = _native.matmul_ragged_k(a, b, b_ragged.slice_offs, b_ragged.slice_sizes, pc.out_dtype)
         if done is not None:
             if type(done) is int:
                 _lib.check(done, "matmul (ragged K)")
@@ -166,10 +166,11 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
     assert b.device == a.device, "b must live on the device of a"
     if a.dtype != b.dtype or a.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"K-ragged matmul is built for two bfloat16 or two float16 operands, not {a.dtype} and {b.dtype}")
-    offs = b_ragged.slice_offs
+    offs, sizes = b_ragged.slice_offs, b_ragged.slice_sizes
     E = b_ragged.n_slices
     assert offs.device == a.device and offs.dtype == torch.int32 and tuple(offs.shape) == (E + 1,) and (offs.stride(0) == 1 or E == 0), \
         "slice_offs of the ragged metadata are int32 [slices + 1] on the device of a"
+    assert sizes.device == a.device and sizes.dtype == torch.int32 and (E <= 1 or sizes.stride(0) == 1), "slice_sizes are int32 [slices] on the device of a"
     assert a_ragged is None or a_ragged.n_slices == E, "a and b have different slices"
     M, K, N = a.shape[0], a.shape[1], b.shape[1]
     dtype = pc.out_dtype or (c.dtype if c is not None else a.dtype)
@@ -182,7 +183,7 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
         assert tuple(c.shape) == (E, M, N) and c.dtype == dtype and c.device == a.device and (c.stride(2) == 1 or N <= 1) \
             and (M < 2 or c.stride(1) >= N) and (E < 2 or c.stride(0) >= (M - 1) * c.stride(1) + N), f"c must be {dtype} [{E}, {M}, {N}] with unit stride along N"
     args = _lib.RaggedKArgs(x=x.data_ptr(), x_stride=x.stride(0) if K > 1 else M, d=d.data_ptr(), d_stride=d.stride(0) if K > 1 else N,
-                            slice_offs=offs.data_ptr(), y=c.data_ptr(), y_stride_e=c.stride(0), y_stride_m=c.stride(1), K=K,
+                            slice_offs=offs.data_ptr(), slice_sizes=sizes.data_ptr(), y=c.data_ptr(), y_stride_e=c.stride(0), y_stride_m=c.stride(1), K=K,
                             dtype=_lib.dtype_code(a.dtype), y_dtype=_lib.dtype_code(dtype), M=M, N=N, E=E)
     L = _lib.lib()
     n_ws = L.tamd_ragged_k_matmul_workspace(ctypes.byref(args), ctypes.sizeof(args))
@@ -212,8 +213,8 @@ def matmul(a, b, bias, a_ragged_metadata: Optional[RaggedTensorMetadata] = None,
     a_ragged_metadata: rows of `a` (after gather) are grouped by slice.
     gather_indx / scatter_indx: int32 row maps (scatter -1 drops the row).
 
-    b_ragged_metadata: the axis K that is summed over is ragged.  Y[e] = a[:, rows of slice e] @ b[rows of slice e, :] for the slices of both
-    (a_ragged_metadata the same, or None): a [M, K], b [K, N] of bf16 / fp16 give Y [slices, M, N].  With a = x.t() of sorted rows x and b the
+    b_ragged_metadata: the axis K that is summed over is ragged.  Y[e] = a[:, rows of slice e] @ b[rows of slice e, :] for the slices of both,
+    slice_sizes[e] rows from slice_offs[e] on (a_ragged_metadata the same, or None): a [M, K], b [K, N] of bf16 / fp16 give Y [slices, M, N].  With a = x.t() of sorted rows x and b the
     gradients of what they were multiplied to, this is the gradient of every expert's weights; empty slices give zeros, rows of no slice take no
     part.  out_dtype (or c [slices, M, N]) float32, bfloat16 or float16; nothing else is built for it.
     """
