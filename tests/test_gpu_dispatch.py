@@ -229,7 +229,7 @@ def test_another_stream_and_a_graph(device):
         assert all(torch.equal(a, b) for a, b in zip(kept, step()))
 
 
-@pytest.mark.parametrize("T,k,H", [(40, 4, 264), (3000, 2, 1032), (9, 11, 77), (9000, 3, 64)])
+@pytest.mark.parametrize("T,k,H", [(40, 4, 264), (3000, 2, 1032), (9, 11, 77), (9000, 3, 64), (9001, 3, 1037), (700, 2, 2050), (50, 3, 5)])
 def test_gradient_in_the_place_of_the_rows(T, k, H, device):
     """combine_backward into the rows that it reads: what it gives elsewhere."""
     torch.manual_seed(T)
@@ -239,3 +239,22 @@ def test_gradient_in_the_place_of_the_rows(T, k, H, device):
         want, dgates = combine_backward(dy, p, rows=rows, gates=gates, out=rows.clone())
         got, same = combine_backward(dy, p, rows=rows, gates=gates, out=rows)
         assert got is rows and torch.equal(got, want) and torch.equal(same, dgates)
+
+
+@pytest.mark.parametrize("T,k,H", [(9001, 4, 1037), (2000, 3, 1037), (700, 2, 2050), (9000, 3, 60), (30, 5, 9)])
+def test_ragged_rows_as_whole_ones(T, k, H, device):
+    """Rows that are no whole 16-byte pieces: bit for bit what the same rows give with zeros behind them."""
+    torch.manual_seed(H)
+    n = T * k
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        p, gates = places(T, k, n, 0.1).to(device), torch.rand(T, k, device=device)
+        x, rows = torch.randn(T, H, device=device).to(dtype), torch.randn(n, H, device=device).to(dtype)
+        filled = lambda t: torch.nn.functional.pad(t, (0, -H % 8))
+        rest = filled(torch.zeros(n, H, device=device).to(dtype))
+        assert torch.equal(dispatch(x, p, gates=gates, out=torch.zeros_like(rows)), dispatch(filled(x), p, gates=gates, out=rest)[:, :H])
+        assert torch.equal(combine(rows, p, gates=gates), combine(filled(rows), p, gates=gates)[:, :H])
+        for got, want in zip(dispatch_backward(rows, p, x=x, gates=gates), dispatch_backward(filled(rows), p, x=filled(x), gates=gates)):
+            assert torch.equal(got, want[:, :got.shape[1]])
+        for got, want in zip(combine_backward(x, p, rows=rows, gates=gates, out=torch.zeros_like(rows)),
+                             combine_backward(filled(x), p, rows=filled(rows), gates=gates, out=rest)):
+            assert torch.equal(got, want[:, :got.shape[1]])

@@ -16,23 +16,44 @@ namespace {
 
 constexpr int kPicks = 8;   // expert rows of a token that are handled together
 
-// 16 bytes of a row: V elements, aligned to 16 bytes or to an element only
+// 16 bytes of a row: V elements.  ALIGNED: rows are made of such pieces on 16-byte boundaries; else pieces begin anywhere
 template <int DT>
 constexpr int kPiece = DT == TAMD_F32 ? 4 : 8;
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
 
+template <bool ALIGNED>
+using Piece = std::conditional_t<ALIGNED, u32x4_t, u32x4_by2_t>;
 template <bool ALIGNED, bool ONCE = false>
-TAMD_DEVICE u32x4_t load_raw(const void *row, int64_t i) {
-  if constexpr (ALIGNED && ONCE) return __builtin_nontemporal_load((const u32x4_t *)((const char *)row + i * 16));
-  else if constexpr (ALIGNED) return *(const u32x4_t *)((const char *)row + i * 16);
-  else return *(const u32x4_by2_t *)((const char *)row + i * 16);
+TAMD_DEVICE u32x4_t load_raw(const void *row, int64_t byte) {
+  const auto *const p = (const Piece<ALIGNED> *)((const char *)row + byte);
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  else return *p;
 }
 template <bool ALIGNED, bool ONCE>
-TAMD_DEVICE void store_raw(void *row, int64_t i, u32x4_t q) {
-  if constexpr (ALIGNED && ONCE) __builtin_nontemporal_store(q, (u32x4_t *)((char *)row + i * 16));
-  else if constexpr (ALIGNED) *(u32x4_t *)((char *)row + i * 16) = q;
-  else *(u32x4_by2_t *)((char *)row + i * 16) = q;
+TAMD_DEVICE void store_raw(void *row, int64_t byte, u32x4_t q) {
+  auto *const p = (Piece<ALIGNED> *)((char *)row + byte);
+  if constexpr (ONCE) __builtin_nontemporal_store((Piece<ALIGNED>)q, p);
+  else *p = q;
+}
+// How a row of H elements is cut: into pieces of V, the last of which ends with the row and so may begin inside the one before (`again` of its elements
+// are that one's too: both store the same, and the dots leave them out).  A tail by elements was one more wait for memory: 37125 tokens of 730 bf16, four
+// picks, took 83 us for the dispatch, 85 for the sum, 150 and 110 for their gradients, and take 80, 71, 136 and 88 so.  Rows of less than a piece go by elements.
+template <int DT, bool ALIGNED>
+struct Cut {
+  static constexpr int V = kPiece<DT>;
+  int H, pieces, few;
+  TAMD_DEVICE Cut(int H_) : H(H_), pieces(H_ < V ? 0 : H_ / V + (!ALIGNED && H_ % V != 0)), few(H_ < V ? H_ : 0) {}
+  TAMD_DEVICE int first(int c) const { return ALIGNED || c * V <= H - V ? c * V : H - V; }
+  TAMD_DEVICE int64_t byte(int c) const { return (int64_t)first(c) * (16 / V); }
+  TAMD_DEVICE int again(int c) const { return ALIGNED ? 0 : c * V - first(c); }
+};
+// <x, y> of a piece, without its first `again` elements
+template <int V>
+TAMD_DEVICE float add_dot(const float (&x)[V], const float (&y)[V], int again, float dot) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) dot = e >= again ? __builtin_fmaf(x[e], y[e], dot) : dot;
+  return dot;
 }
 template <int DT>
 TAMD_DEVICE void widen(u32x4_t q, float (&v)[kPiece<DT>]) {
@@ -137,13 +158,14 @@ __global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
   if (t >= a.T) return;
   const int at = threadIdx.x & (LANES - 1);
   const char *const src = (const char *)a.src + t * a.src_stride * SIZE;
-  const int pieces = a.H / V, rest = a.H % V;
+  const Cut<DT, ALIGNED> cut(a.H);
   for (int j0 = 0; j0 < a.k; j0 += kPicks) {
     Picks p;
     load_picks<LANES>(a, t, j0, p);
     float dot[kPicks] = {};
-    for (int c = at; c < pieces; c += LANES) {
-      const u32x4_t q = load_raw<ALIGNED, ONCE>(src, c);
+    for (int c = at; c < cut.pieces; c += LANES) {
+      const int64_t byte = cut.byte(c);
+      const u32x4_t q = load_raw<ALIGNED, ONCE>(src, byte);
       float x[V];
       widen<DT>(q, x);
 #pragma unroll
@@ -151,32 +173,30 @@ __global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
         if (p.row[j] < 0) continue;
         if constexpr (DOTS) {
           float y[V];
-          widen<DT>(load_raw<ALIGNED, ONCE>((const char *)a.other + p.row[j] * a.other_stride * SIZE, c), y);
-#pragma unroll
-          for (int e = 0; e < V; ++e) dot[j] = __builtin_fmaf(x[e], y[e], dot[j]);
+          widen<DT>(load_raw<ALIGNED, ONCE>((const char *)a.other + p.row[j] * a.other_stride * SIZE, byte), y);
+          dot[j] = add_dot<V>(x, y, cut.again(c), dot[j]);
         }
         char *const row = (char *)a.dst + p.row[j] * a.dst_stride * SIZE;
         if constexpr (GATES) {
           float out[V];
 #pragma unroll
           for (int e = 0; e < V; ++e) out[e] = x[e] * p.gate[j];
-          store_raw<ALIGNED, ONCE>(row, c, narrow<DT>(out));
+          store_raw<ALIGNED, ONCE>(row, byte, narrow<DT>(out));
         } else {
-          store_raw<ALIGNED, ONCE>(row, c, q);
+          store_raw<ALIGNED, ONCE>(row, byte, q);
         }
       }
     }
-    if (at < rest) {
-      const int64_t i = (int64_t)pieces * V + at;
-      const float x = load_as_f32<DT>(src, i);
+    if (!ALIGNED && at < cut.few) {
+      const float x = load_as_f32<DT>(src, at);
 #pragma unroll
       for (int j = 0; j < kPicks; ++j) {
         if (p.row[j] < 0) continue;
-        if constexpr (DOTS) dot[j] = __builtin_fmaf(x, load_as_f32<DT>((const char *)a.other + p.row[j] * a.other_stride * SIZE, i), dot[j]);
+        if constexpr (DOTS) dot[j] = x * load_as_f32<DT>((const char *)a.other + p.row[j] * a.other_stride * SIZE, at);
         char *const row = (char *)a.dst + p.row[j] * a.dst_stride * SIZE;
-        if constexpr (GATES) store_from_f32<DT>(row, i, x * p.gate[j]);
-        else if constexpr (DT == TAMD_F32) ((uint32_t *)row)[i] = ((const uint32_t *)src)[i];
-        else ((uint16_t *)row)[i] = ((const uint16_t *)src)[i];
+        if constexpr (GATES) store_from_f32<DT>(row, at, x * p.gate[j]);
+        else if constexpr (DT == TAMD_F32) ((uint32_t *)row)[at] = ((const uint32_t *)src)[at];
+        else ((uint16_t *)row)[at] = ((const uint16_t *)src)[at];
       }
     }
     if constexpr (DOTS) store_dots<LANES>(a, t, j0, dot, lds);
@@ -192,44 +212,41 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
   const int at = threadIdx.x & (LANES - 1);
   char *const dst = (char *)a.dst + t * a.dst_stride * SIZE;
   const char *const other = DOTS ? (const char *)a.other + t * a.other_stride * SIZE : nullptr;
-  const int pieces = a.H / V, rest = a.H % V;
+  const Cut<DT, ALIGNED> cut(a.H);
   const bool few = a.k <= kPicks;    // all picks at once: their dots come with the sum
   Picks p;
   load_picks<LANES>(a, t, 0, p);
   float dot[kPicks] = {};
-  for (int c = at; c < pieces; c += LANES) {
+  for (int c = at; c < cut.pieces; c += LANES) {
+    const int64_t byte = cut.byte(c);
     float sum[V] = {}, x[V];
-    if constexpr (DOTS) widen<DT>(load_raw<ALIGNED, ONCE>(other, c), x);
+    if constexpr (DOTS) widen<DT>(load_raw<ALIGNED, ONCE>(other, byte), x);
     for (int j0 = 0; j0 < a.k; j0 += kPicks) {
       if (j0) load_picks<LANES>(a, t, j0, p);
 #pragma unroll
       for (int j = 0; j < kPicks; ++j) {
         if (p.row[j] < 0) continue;
         float y[V];
-        widen<DT>(load_raw<ALIGNED, ONCE>((const char *)a.src + p.row[j] * a.src_stride * SIZE, c), y);
+        widen<DT>(load_raw<ALIGNED, ONCE>((const char *)a.src + p.row[j] * a.src_stride * SIZE, byte), y);
 #pragma unroll
         for (int e = 0; e < V; ++e) sum[e] = __builtin_fmaf(y[e], p.gate[j], sum[e]);
         if constexpr (DOTS) {
-          if (few) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) dot[j] = __builtin_fmaf(x[e], y[e], dot[j]);
-          }
+          if (few) dot[j] = add_dot<V>(x, y, cut.again(c), dot[j]);
         }
       }
     }
     if (!few) load_picks<LANES>(a, t, 0, p);
-    store_raw<ALIGNED, ONCE>(dst, c, narrow<DT>(sum));
+    store_raw<ALIGNED, ONCE>(dst, byte, narrow<DT>(sum));
   }
-  if (at < rest) {
-    const int64_t i = (int64_t)pieces * V + at;
+  if (!ALIGNED && at < cut.few) {
     float sum = 0.f;
     for (int j = 0; j < a.k; ++j) {
       const int32_t r = a.row_indx[t * a.row_indx_stride + j];
       if ((uint32_t)r >= (uint32_t)a.n_rows) continue;
       const float g = a.gates ? load_gate(a.gates, a.gates_dtype, t * a.gates_stride + j) : 1.0f;
-      sum = __builtin_fmaf(load_as_f32<DT>((const char *)a.src + r * a.src_stride * SIZE, i), g, sum);
+      sum = __builtin_fmaf(load_as_f32<DT>((const char *)a.src + r * a.src_stride * SIZE, at), g, sum);
     }
-    store_from_f32<DT>(dst, i, sum);
+    store_from_f32<DT>(dst, at, sum);
   }
   if constexpr (DOTS) {
     for (int j0 = 0; j0 < a.k; j0 += kPicks) {
@@ -237,25 +254,24 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
         load_picks<LANES>(a, t, j0, p);
 #pragma unroll
         for (int j = 0; j < kPicks; ++j) dot[j] = 0.f;
-        for (int c = at; c < pieces; c += LANES) {
+        for (int c = at; c < cut.pieces; c += LANES) {
+          const int64_t byte = cut.byte(c);
           float x[V];
-          widen<DT>(load_raw<ALIGNED>(other, c), x);
+          widen<DT>(load_raw<ALIGNED>(other, byte), x);
 #pragma unroll
           for (int j = 0; j < kPicks; ++j) {
             if (p.row[j] < 0) continue;
             float y[V];
-            widen<DT>(load_raw<ALIGNED>((const char *)a.src + p.row[j] * a.src_stride * SIZE, c), y);
-#pragma unroll
-            for (int e = 0; e < V; ++e) dot[j] = __builtin_fmaf(x[e], y[e], dot[j]);
+            widen<DT>(load_raw<ALIGNED>((const char *)a.src + p.row[j] * a.src_stride * SIZE, byte), y);
+            dot[j] = add_dot<V>(x, y, cut.again(c), dot[j]);
           }
         }
       }
-      if (at < rest) {
-        const int64_t i = (int64_t)pieces * V + at;
-        const float x = load_as_f32<DT>(other, i);
+      if (!ALIGNED && at < cut.few) {
+        const float x = load_as_f32<DT>(other, at);
 #pragma unroll
         for (int j = 0; j < kPicks; ++j)
-          if (p.row[j] >= 0) dot[j] = __builtin_fmaf(x, load_as_f32<DT>((const char *)a.src + p.row[j] * a.src_stride * SIZE, i), dot[j]);
+          if (p.row[j] >= 0) dot[j] = x * load_as_f32<DT>((const char *)a.src + p.row[j] * a.src_stride * SIZE, at);
       }
       store_dots<LANES>(a, t, j0, dot, lds);
     }
@@ -279,15 +295,16 @@ int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
   const int lanes = lanes_of(a.T, a.H / kPiece<DT>, DOTS);
   // Rows of more than the caches keep until they are used again go past them, read and written (us, four picks of 2880 bf16, 16384 tokens: dispatch 93 in place
   // of 96, sum 88 and 99, gradients 179 and 184, 113 and 124).  Below, what an operator leaves or finds in the caches is worth more: 1021 tokens of 2016,
-  // six picks, whose rows the caches hold, sum 7.6 in place of 8.9.  Unaligned rows share lines with their neighbours, whose parts the caches put together.
+  // six picks, whose rows the caches hold, sum 7.6 in place of 8.9.  Unaligned rows too: 37125 tokens of 730 81 for 80, 64 for 71, 135 for 136, 81 for 88;
+  // 10000 of 2038 58 for 67, 44 for 48, 94 for 97, 54 for 57 (loads alone past the caches: 68, 46, 105, 56).
   const double bytes = (double)a.T * ((double)a.k * (spread && DOTS ? 2 : 1) + 1) * a.H * (16 / kPiece<DT>);
-  const bool once = ALIGNED && bytes >= 64e6;
+  const bool once = bytes >= 64e6;
   const auto go = [&](auto of) {
     constexpr int LANES = decltype(of)::value;
     const unsigned grid = (unsigned)(((int64_t)a.T * LANES + 255) / 256);
-    if (spread && once) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, ALIGNED><<<grid, 256, 0, st>>>(a);
+    if (spread && once) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, true><<<grid, 256, 0, st>>>(a);
     else if (spread) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, false><<<grid, 256, 0, st>>>(a);
-    else if (once) collect_kernel<DT, ALIGNED, LANES, DOTS, ALIGNED><<<grid, 256, 0, st>>>(a);
+    else if (once) collect_kernel<DT, ALIGNED, LANES, DOTS, true><<<grid, 256, 0, st>>>(a);
     else collect_kernel<DT, ALIGNED, LANES, DOTS, false><<<grid, 256, 0, st>>>(a);
   };
   if (lanes == 16) go(std::integral_constant<int, 16>());
@@ -305,7 +322,7 @@ template <int DT>
 int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
   const int size = DT == TAMD_F32 ? 4 : 2;
   const auto whole = [&](const void *p, int64_t stride) { return ((uintptr_t)p | (uintptr_t)(stride * size)) % 16 == 0; };
-  const bool aligned = whole(a.src, a.src_stride) && whole(a.dst, a.dst_stride) && (!a.dots || whole(a.other, a.other_stride));
+  const bool aligned = a.H % kPiece<DT> == 0 && whole(a.src, a.src_stride) && whole(a.dst, a.dst_stride) && (!a.dots || whole(a.other, a.other_stride));
   return aligned ? launch<DT, true>(a, spread, st) : launch<DT, false>(a, spread, st);
 }
 
