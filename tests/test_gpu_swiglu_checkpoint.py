@@ -83,7 +83,8 @@ def test_forward_and_backward(M, N, dtype, how, limit, device):
     within(again, want, (slack_of_s(g) + 3 * 2.0 ** -24) * want.abs() + tiny, dtype)
     d, ag = d.double(), (ALPHA * g).abs()
     slope = 1 + ALPHA * g * (1 - s)
-    # the slope: alpha g is rounded twice, 1 - s is off by s and a half step, the sum by a half step
+    # the slope times s, as s + alpha (g s - (g s) s): s is off as above, g s, the difference and alpha are rounded, the sum by a half step (of these
+    # three, which count alpha g (1 - s), two are written so and one as alpha g)
     slack = 2.0 ** -24 * (2 * ag * (1 - s) + slope.abs() + ag) + ag * s * slack_of_s(g)
     factor = (d * (l + 1) * s).abs()
     dgate = torch.where(free[0], d * (l + 1) * s * slope, 0.0)
@@ -134,6 +135,30 @@ def test_extremes_are_kept_as_downcast_keeps_them(dtype, device):
     lost = torch.isnan(kept[:, 0::2]) | torch.isnan(kept[:, 1::2])
     assert torch.equal(torch.isnan(again), lost) and bool(lost[5, 16:].all() and not lost[5, :16].any() and lost[7, 20] and int(lost[7].sum()) == 1)
     assert bool(torch.isnan(da[:, 0::2])[lost].all()) and not bool(torch.isnan(da[:, 0::2])[~lost].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("limit", [None, 7.0])
+def test_the_lowest_and_the_greatest_values(dtype, limit, device):
+    """A gate at the type's lowest value (kept as -2^128) gives zeros, one at the greatest its linear value, where they are kept alone in their groups."""
+    most = torch.finfo(dtype).max
+    a = torch.zeros(6, 32, dtype=dtype, device=device)
+    for row, g in enumerate((-most, most, -most / 2, most / 2, -most * 0.6, 2.0 ** 120)):
+        a[row, 6] = g
+    a[5, 7] = a[0, 7] = a[2, 7] = -most
+    d = torch.full((6, 16), 2.0, dtype=dtype, device=device)
+    pc = PrecisionConfig(limit=limit)
+    out, values, scales = swiglu_checkpoint(a, ALPHA, pc)
+    da, again = swiglu_backward(d, values, scales, ALPHA, pc, return_out=True)
+    power = torch.ldexp(torch.ones(6, 1, dtype=torch.float64, device=device), scales.double() - 127)
+    want, s, g, l, free = glu64(values.double() * torch.where(scales == 0, 0.0, power), limit)
+    slope = 1 + ALPHA * g * (1 - s)
+    for got, right in ((da[:, 0::2], torch.where(free[0], 2 * (l + 1) * s * slope, 0.0)), (da[:, 1::2], torch.where(free[1], 2 * g * s, 0.0)), (again, want)):
+        near = right.clamp(-2.0 ** 128, 2.0 ** 128)   # (beyond the type's range both are infinite, or its greatest value stands for 2^128)
+        got = got.double().clamp(-2.0 ** 128, 2.0 ** 128)
+        slack = 1.01 * HALF_STEP[dtype] + slack_of_s(g.clamp(-100, 100)) + 4 * 2.0 ** -24
+        assert bool(((got - near).abs() <= slack * near.abs() + LEAST[dtype]).all())
+    assert bool((da[0, 6:8] == 0).all() and again[0, 3] == 0 and out[0, 3] == 0)
 
 
 def test_at_the_limit_the_gradient_passes(device):

@@ -50,6 +50,8 @@ TAMD_DEVICE void store8(void *p, u32x2_t q) {
   else *(u32x2_by1_t *)p = q;
 }
 
+constexpr float kMost = 3.40282346638528859812e38f;   // the greatest of float32
+
 TAMD_DEVICE float widen16(uint32_t bits, int dt) { return dt == TAMD_BF16 ? bf16_bits_to_f32(bits) : f16_bits_to_f32(bits); }
 template <int DT>
 TAMD_DEVICE uint32_t pack2(float a, float b) {
@@ -104,7 +106,7 @@ TAMD_DEVICE void store_values(void *p, int n, const float (&v)[N]) {
 struct GluShape {
   GroupDiv div;            // rows and groups of a row
   int64_t L;               // values of a row: 2 N
-  float alpha, limit;
+  float alpha, limit;      // (limit: the greatest number without one)
   int has_limit;
 };
 
@@ -113,13 +115,18 @@ struct Pair {
   float g, l, s;
   bool g_free, l_free;     // not beyond the limit
 };
+// KEPT: a type's lowest value may have been kept as -2^128.  It counts as the lowest of float32, so that the zero of its sigmoid makes zeros; the sigmoid of
+// a NaN is one, and is in all that follows.
+template <bool KEPT>
 TAMD_DEVICE Pair pair_of(float g, float l, const GluShape &sh) {
   Pair p;
-  p.g_free = !(sh.has_limit && g > sh.limit);
-  p.l_free = !(sh.has_limit && __builtin_fabsf(l) > sh.limit);
-  p.g = p.g_free ? g : sh.limit;
-  p.l = p.l_free ? l : __builtin_copysignf(sh.limit, l);
+  const bool g_in = !(g > sh.limit), l_in = !(__builtin_fabsf(l) > sh.limit);
+  p.g_free = g_in || !sh.has_limit;
+  p.l_free = l_in || !sh.has_limit;
+  p.g = (KEPT ? g_in : p.g_free) ? g : sh.limit;
+  p.l = (KEPT ? l_in : p.l_free) ? l : __builtin_copysignf(sh.limit, l);
   p.s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * sh.alpha * p.g));
+  if constexpr (KEPT) p.g = __builtin_fmaxf(p.g, -kMost);
   return p;
 }
 
@@ -170,7 +177,7 @@ __global__ __launch_bounds__(256) void checkpoint_kernel(const void *__restrict_
     float o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const Pair p = pair_of(v[u][2 * j], v[u][2 * j + 1], sh);
+      const Pair p = pair_of<false>(v[u][2 * j], v[u][2 * j + 1], sh);
       const float gs = p.g * p.s;
       o[j] = __builtin_fmaf(gs, p.l, gs);
     }
@@ -233,12 +240,13 @@ __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ 
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const Pair p = pair_of(v[2 * j], v[2 * j + 1], sh);
-      const float gs = p.g * p.s, ds = d[u][j] * p.s;
+      const Pair p = pair_of<true>(v[2 * j], v[2 * j + 1], sh);
+      const float gs = p.g * p.s;
       o[j] = __builtin_fmaf(gs, p.l, gs);
-      const float slope = __builtin_fmaf(sh.alpha * p.g, 1.0f - p.s, 1.0f);
-      dv[2 * j] = p.g_free ? __builtin_fmaf(ds, p.l, ds) * slope : 0.f;
-      dv[2 * j + 1] = p.l_free ? ds * p.g : 0.f;
+      // s (1 + alpha g (1 - s)) as s + alpha (g s - (g s) s), of which nothing overflows where s is 0 or 1
+      const float slope = d[u][j] * __builtin_fmaf(sh.alpha, __builtin_fmaf(-gs, p.s, gs), p.s);
+      dv[2 * j] = p.g_free ? __builtin_fmaf(slope, p.l, slope) : 0.f;
+      dv[2 * j + 1] = p.l_free ? d[u][j] * gs : 0.f;
     }
     store_values<DT, ALIGNED, BIG, 8>((char *)da + (r[u] * da_stride + g[u] * 32 + sub * 8) * SIZE, n[u], dv);
     if constexpr (AGAIN) store_values<DT, ALIGNED, BIG, 4>((char *)out + (r[u] * out_stride + g[u] * 16 + sub * 4) * SIZE, n[u] / 2, o);
@@ -248,7 +256,7 @@ __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ 
 bool shape(GluShape &sh, int64_t M, int64_t N, float alpha, float limit, int has_limit, bool big, unsigned &blocks) {
   const int64_t G = (2 * N + 31) / 32, per = big ? 128 : 64;
   sh.div = group_div(1, M, G);
-  sh.L = 2 * N, sh.alpha = alpha, sh.limit = limit, sh.has_limit = has_limit;
+  sh.L = 2 * N, sh.alpha = alpha, sh.limit = has_limit ? limit : kMost, sh.has_limit = has_limit;
   const int64_t n = (sh.div.total + per - 1) / per;
   blocks = (unsigned)n;
   return n < ((int64_t)1 << 31);
