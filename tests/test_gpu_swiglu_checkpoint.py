@@ -137,6 +137,22 @@ def test_extremes_are_kept_as_downcast_keeps_them(dtype, device):
     assert bool(torch.isnan(da[:, 0::2])[lost].all()) and not bool(torch.isnan(da[:, 0::2])[~lost].any())
 
 
+@pytest.mark.parametrize("M,N", [(8100, 1001), (8100, 1002), (8100, 1003), (700, 98), (3, 1), (5, 2), (5, 3), (9, 5), (300, 33)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ragged_rows_as_whole_ones(M, N, dtype, device):
+    """Rows that end inside a piece: bit for bit what the same rows give with zeros behind them."""
+    torch.manual_seed(N)
+    a, d = torch.randn(M, 2 * N, device=device).to(dtype), torch.randn(M, N, device=device).to(dtype)
+    filled = lambda t, to: torch.nn.functional.pad(t, (0, -t.shape[1] % to))
+    pc = PrecisionConfig(limit=1.5)
+    out, values, scales = swiglu_checkpoint(a, ALPHA, pc)
+    want = swiglu_checkpoint(filled(a, 32), ALPHA, pc)
+    assert torch.equal(out, want[0][:, :N]) and torch.equal(values.view(torch.uint8), want[1].view(torch.uint8)[:, :2 * N]) and torch.equal(scales, want[2])
+    da, again = swiglu_backward(d, values, scales, ALPHA, pc, return_out=True)
+    want_da, want_again = swiglu_backward(filled(d, 16), want[1], scales, ALPHA, pc, return_out=True)
+    assert torch.equal(da, want_da[:, :2 * N]) and torch.equal(again, want_again[:, :N])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("limit", [None, 7.0])
 def test_the_lowest_and_the_greatest_values(dtype, limit, device):
