@@ -151,9 +151,10 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
     """Y[e] = a[:, slice e] @ b[slice e, :] (matmul.py:376 of the reference, ragged_dimension "K")."""
     a, b = _data(a), _data(b)
     flex = pc.flex_ctx
-    if (any(getattr(pc, f) is not None for f in ("a_mx_scale", "b_mx_scale", "c_mx_scale", "a_mx_tensor_scale", "b_mx_tensor_scale")) or pc.acc_scale != 1.0
-            or any(d.scale is not None for d in (flex.lhs_data, flex.rhs_data, flex.acc_data)) or flex.lhs_data.dtype is not None
-            or flex.rhs_data.dtype is not None or flex.out_data.expected_scale is not None or flex.out_data.actual_scale is not None):
+    lhs, rhs, out = flex.lhs_data, flex.rhs_data, flex.out_data
+    if (pc.a_mx_scale is not None or pc.b_mx_scale is not None or pc.c_mx_scale is not None or pc.a_mx_tensor_scale is not None
+            or pc.b_mx_tensor_scale is not None or pc.acc_scale != 1.0 or lhs.scale is not None or rhs.scale is not None or flex.acc_data.scale is not None
+            or lhs.dtype is not None or rhs.dtype is not None or out.expected_scale is not None or out.actual_scale is not None):
         raise NotImplementedError("K-ragged matmul takes unscaled operands")
     if c is None and (a_ragged is None or a_ragged.n_slices == b_ragged.n_slices):
         done = _native.matmul_ragged_k(a, b, b_ragged.slice_offs, b_ragged.slice_sizes, pc.out_dtype)
@@ -240,10 +241,10 @@ def matmul(a, b, bias, a_ragged_metadata: Optional[RaggedTensorMetadata] = None,
         assert fused_comm is None, "fused comm is not supported in batched mode"
         assert b.ndim == 3 and b.shape[0] == a.shape[0]
     if b_ragged_metadata is not None:
-        for value, name in ((bias, "bias"), (gather_indx, "gather_indx"), (scatter_indx, "scatter_indx"), (betas, "betas"), (gammas, "gammas"),
-                            (out_alpha, "out_alpha"), (fused_comm, "fused_comm"), (c_acc_in, "c_acc_in")):
-            if value is not None:
-                raise NotImplementedError(f"{name} of a K-ragged matmul is not built")
+        if not (bias is gather_indx is scatter_indx is betas is gammas is out_alpha is fused_comm is c_acc_in is None):
+            names = {"bias": bias, "gather_indx": gather_indx, "scatter_indx": scatter_indx, "betas": betas, "gammas": gammas, "out_alpha": out_alpha,
+                     "fused_comm": fused_comm, "c_acc_in": c_acc_in}
+            raise NotImplementedError(f"{next(name for name, value in names.items() if value is not None)} of a K-ragged matmul is not built")
         if fused_activation.specs.name != "dflt" or epilogue.specs.name != "dflt":
             raise NotImplementedError("K-ragged matmul is built without activation and epilogue")
         return _matmul_ragged_k(a, b, a_ragged_metadata, b_ragged_metadata, precision_config, c)
