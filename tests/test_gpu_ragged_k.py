@@ -70,6 +70,20 @@ def test_larger_tiles_and_splits(M, N, sizes, dtype, out, device):
         assert torch.equal(matmul(x.t(), d, None, md, md, precision_config=PrecisionConfig(out_dtype=out)), got)
 
 
+@pytest.mark.parametrize("E", [2, 7, 40, 64, 65])
+@pytest.mark.parametrize("M,N", [(136, 264), (40, 33)])
+def test_long_slices_of_all_lengths(E, M, N, device):
+    """Slices whose longest ones go first: every one has its turn, whatever the order of their lengths, those of equal and of no length among them."""
+    torch.manual_seed(E)
+    share = torch.rand(E) * (torch.rand(E) < 0.8)
+    share[-1] = share[0] = share.max()
+    for sizes in ([1100] * E, (share * 2 * 1100).int().tolist() if E > 2 else [0, 1500], list(range(1000, 1000 + E)), [1030 + E - e for e in range(E)]):
+        rows = sum(sizes)
+        x, d = torch.randn(rows, M, device=device).bfloat16(), torch.randn(rows, N, device=device).bfloat16()
+        md = ragged(sizes, rows, device)
+        check(matmul(x.t(), d, None, md, md), x, d, sizes, torch.bfloat16)
+
+
 @pytest.mark.parametrize("M,N,sizes", [(136, 72, [40, 0, 50]), (64, 64, [3000, 100])])
 def test_into_given_results(M, N, sizes, device):
     """c with pitches of its own: only the results are written."""

@@ -27,6 +27,7 @@ struct RaggedK {
   int M, N, E, y_dtype;
   int whole_lines, past_caches;       // y's rows begin on lines of 128 bytes, and are results; others are stored past the caches
   int tiles_m, tiles_n, splits;
+  int longest_first;                  // slices in the order of their rows (at most 64)
 };
 
 constexpr int kRaggedBK = 32;
@@ -116,12 +117,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
   const uint32_t id = run * 256u + (in % 8u) * 32u + in / 8u;
   if (id >= total) return;
   const uint32_t es = id / per, t = id - es * per;
-  const int e = (int)(es / a.splits), split = (int)(es - (uint32_t)e * a.splits);
+  const int turn = (int)(es / a.splits), split = (int)(es - (uint32_t)turn * a.splits);
+  int e = turn;
+  int64_t begin, end;
+  if (a.longest_first) {
+    // a lane per slice, which counts the slices that go before its own: keys are distinct, so that every slice has its turn
+    const int off = lane < a.E ? a.offs[lane] : 0, size = lane < a.E ? a.sizes[lane] : 0;
+    const uint32_t key = lane < a.E ? (uint32_t)(size < 0 ? 0 : size < 1 << 25 ? size : (1 << 25) - 1) << 6 | (uint32_t)(63 - lane) : 0u;
+    int before = 0;
+    for (int f0 = 0; f0 < a.E; f0 += 8)   // (a lane without a slice has a key of 0)
+#pragma unroll
+      for (int f = 0; f < 8; ++f) before += (uint32_t)__builtin_amdgcn_readlane((int)key, f0 + f) > key;
+    e = __builtin_ctzll(__ballot(lane < a.E && before == turn));
+    begin = __builtin_amdgcn_readlane(off, e), end = begin + __builtin_amdgcn_readlane(size, e);
+  } else {
+    begin = a.offs[e], end = begin + a.sizes[e];
+  }
   const uint32_t g = t / (4u * a.tiles_m), tg = t - g * 4u * a.tiles_m;
   const uint32_t w = a.tiles_n - 4u * g < 4u ? a.tiles_n - 4u * g : 4u;
   const int m0 = (int)(tg / w) * BM, n0 = (int)(4u * g + tg % w) * BN;
 
-  int64_t begin = a.offs[e], end = begin + a.sizes[e];
   begin = begin < 0 ? 0 : begin;
   end = end > a.K ? a.K : end;
   const int64_t stages = end > begin ? (end - begin + kRaggedBK - 1) / kRaggedBK : 0;

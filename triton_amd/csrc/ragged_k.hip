@@ -10,6 +10,7 @@ namespace {
 struct Plan {
   int tile, tiles_m, tiles_n, splits;   // tile: a RaggedTile
   int64_t pitch;                        // elements of a row of partial sums
+  bool longest_first;
   bool lay_x, lay_d;                    // operands that the copies cannot take as they are
   int64_t x_at, d_at, part_at, bytes;   // where these and the partial sums lie in the workspace
 };
@@ -35,6 +36,10 @@ Plan make_plan(const tamd_ragged_k_args &a) {
     const double t = 0.57 * up((int64_t)stages, s) + 5.0 + (double)s * E * M * N * 8 / 4e6;
     if (t < best) best = t, p.splits = s;
   }
+  // The longest slices first, so that the last round of workgroups is of short ones, where a slice has rows enough to pay for the order (8 comparisons to
+  // eight slices in every workgroup): 30966 rows over 8 slices of 1200 to 7800, 2152 x 424, 123 us in place of 154; 6448 over 8, 1152 x 4736, 86 and 95; 43728
+  // over 32, 640 x 4608, 287 and 295; 17056 over 60, 936 x 4040, 254 and 252 (not so, with 284 rows).  Slices of one length lose up to 1 %.
+  p.longest_first = E > 1 && E <= 64 && rows > 128 && rows >= 16 * E;
   p.pitch = ((int64_t)N + 3) / 4 * 4;
   // rows that copies of 16 bytes take whole, and a stage's of which 31 bits count
   const auto whole = [](const void *q, int64_t pitch, int cols) { return (uintptr_t)q % 16 == 0 && pitch % 8 == 0 && cols % 8 == 0 && pitch < 1 << 24; };
@@ -142,7 +147,7 @@ extern "C" int tamd_ragged_k_matmul(const tamd_ragged_k_args *args, size_t args_
   hipStream_t st = (hipStream_t)stream;
   uint8_t *const room = (uint8_t *)a.workspace;
   const int size = a.y_dtype == TAMD_F32 ? 4 : 2;
-  RaggedK k{a.x, a.d, a.x_stride, a.d_stride, a.M, a.N, a.slice_offs, a.slice_sizes, a.y, a.y_stride_e, a.y_stride_m, 0, a.K, a.M, a.N, a.E, a.y_dtype, 0, 0, p.tiles_m, p.tiles_n, p.splits};
+  RaggedK k{a.x, a.d, a.x_stride, a.d_stride, a.M, a.N, a.slice_offs, a.slice_sizes, a.y, a.y_stride_e, a.y_stride_m, 0, a.K, a.M, a.N, a.E, a.y_dtype, 0, 0, p.tiles_m, p.tiles_n, p.splits, p.longest_first};
   LaidBoth both;
   int n = 0;
   if (p.lay_x) {
