@@ -33,6 +33,9 @@ def test_c_entry_points(entry):
         assert code(good(T=3, **{field: None})) == _lib.E_INVALID, field
         if field != "row_indx":
             assert code(good(T=3, **{field: 0x1001})) == _lib.E_ALIGNMENT, field
+    assert code(good(T=3, row_indx=0x3002)) == _lib.E_ALIGNMENT
+    assert code(good(T=3, gates=0x4002, gates_dtype=_lib.F32)) == code(good(T=3, gates=0x4001, gates_dtype=_lib.BF16)) == _lib.E_ALIGNMENT
+    assert code(good(T=1 << 28)) == code(good(T=1 << 26, H=1000)) == _lib.E_TOO_LARGE     # more threads than a launch has
     assert code(good(T=3, dots=0x5000, dots_stride=4)) == _lib.E_INVALID        # (without the other operand)
     assert code(good(T=3, dots=0x5000, dots_stride=4, other=0x6001)) == _lib.E_ALIGNMENT
 

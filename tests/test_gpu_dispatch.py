@@ -258,3 +258,13 @@ def test_ragged_rows_as_whole_ones(T, k, H, device):
         for got, want in zip(combine_backward(x, p, rows=rows, gates=gates, out=torch.zeros_like(rows)),
                              combine_backward(filled(x), p, rows=filled(rows), gates=gates, out=rest)):
             assert torch.equal(got, want[:, :got.shape[1]])
+
+
+def test_rows_that_are_too_long(device):
+    """2^31 elements and more to a row are refused, before anything is made of them."""
+    p = torch.zeros(1, 1, dtype=torch.int32, device=device)
+    for H in (2 ** 31, 2 ** 32 + 8):
+        long = torch.zeros(1, 1, dtype=torch.bfloat16, device=device).expand(1, H)
+        for call in (dispatch, combine, combine_backward, dispatch_backward):
+            with pytest.raises(NotImplementedError):
+                call(long, p)

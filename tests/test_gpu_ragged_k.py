@@ -173,3 +173,13 @@ def test_another_stream_and_a_graph(device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, matmul(x.t(), d, None, md, md))
+
+
+def test_results_that_are_too_large(device):
+    """2^24 rows or columns and more are refused, before anything is made of them."""
+    md = ragged([2], 2, device)
+    for n in (2 ** 24, 2 ** 32 + 8):
+        wide, d = torch.zeros(1, 1, dtype=torch.bfloat16, device=device).expand(2, n), torch.zeros(2, 8, dtype=torch.bfloat16, device=device)
+        for a, b in ((wide.t(), d), (d.t(), wide)):
+            with pytest.raises(NotImplementedError):
+                matmul(a, b, None, md, md)

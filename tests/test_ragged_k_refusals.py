@@ -19,6 +19,7 @@ def good(**more):
 def test_c_entry_point():
     L = _lib.lib()
     code = lambda a, size=C.sizeof(_lib.RaggedKArgs): L.tamd_ragged_k_matmul(C.byref(a), size, None)  # noqa: E731
+    room_of = lambda a: L.tamd_ragged_k_matmul_workspace(C.byref(a), C.sizeof(_lib.RaggedKArgs))  # noqa: E731
     assert L.tamd_ragged_k_matmul(None, C.sizeof(_lib.RaggedKArgs), None) == _lib.E_INVALID
     assert code(good()) == 0 and code(good(), C.sizeof(_lib.RaggedKArgs) - 8) == _lib.E_INVALID
     for field in ("M", "N", "E", "K", "x_stride", "d_stride", "y_stride_e", "y_stride_m"):
@@ -28,10 +29,12 @@ def test_c_entry_point():
     assert code(good(y_dtype=_lib.FP8_E4M3)) == _lib.E_UNSUPPORTED
     for field in ("x", "d", "y", "slice_offs", "slice_sizes"):
         assert code(good(M=64, **{field: None})) == _lib.E_INVALID, field
-        if not field.startswith("slice"):
-            assert code(good(M=64, **{field: 0x1001})) == _lib.E_ALIGNMENT, field
+        assert code(good(M=64, **{field: 0x1001})) == _lib.E_ALIGNMENT, field
     assert code(good(M=64, y_dtype=_lib.F32, y=0x4002)) == _lib.E_ALIGNMENT
     assert code(good(M=64, K=1 << 31)) == _lib.E_TOO_LARGE and code(good(M=2 ** 31 - 1, N=2 ** 31 - 1)) == _lib.E_TOO_LARGE
+    # rows that would have to be laid out first, by more threads than a launch has
+    assert code(good(M=2047, K=1 << 28, x_stride=2047)) == room_of(good(M=2047, K=1 << 28, x_stride=2047)) == _lib.E_TOO_LARGE
+    assert room_of(good(M=2048, K=1 << 28, x_stride=2048)) >= 0
     # long slices of few tiles are cut: their partial sums need room; so do rows that are not whole pieces of 16 bytes
     room = lambda a, size=C.sizeof(_lib.RaggedKArgs): L.tamd_ragged_k_matmul_workspace(C.byref(a), size)  # noqa: E731
     n = room(good(M=64, K=10000))

@@ -28,6 +28,7 @@ def test_c_entry_points(call, strides, pointers):
     for name in pointers:
         if name not in "vs":
             assert call(M=3, **{name: 0x1001}) == _lib.E_ALIGNMENT, name
+    assert call(M=1 << 29, N=64) == _lib.E_TOO_LARGE      # more threads than a launch has
     assert call(M=1 << 31) == _lib.E_TOO_LARGE and call(M=1, N=1 << 30) == _lib.E_TOO_LARGE and call(M=(1 << 31) - 1, N=(1 << 30) - 1) == _lib.E_TOO_LARGE
 
 

@@ -15,7 +15,7 @@ def test_c_entry_point():
     for name in ("sx", "rows", "live", "cols", "k", "si", "sd", "sdx"):
         assert call(**{name: -1}) == _lib.E_INVALID, name
     assert call(dtype=_lib.FP8_E4M3) == call(dd=_lib.FP8_E5M2) == _lib.E_UNSUPPORTED
-    assert call(cols=32768) == call(k=65) == call(rows=1 << 32) == _lib.E_TOO_LARGE
+    assert call(cols=32768) == call(k=65) == call(rows=1 << 32) == call(rows=1 << 28, live=0) == call(rows=1 << 26, live=0, k=17) == _lib.E_TOO_LARGE
     for name in ("x", "indx", "d", "dx"):
         assert call(rows=3, live=3, **{name: None}) == _lib.E_INVALID, name
         assert call(rows=3, live=3, **{name: 0x1001}) == _lib.E_ALIGNMENT, name

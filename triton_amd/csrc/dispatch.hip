@@ -14,6 +14,7 @@ using namespace tamd;
 
 namespace {
 
+constexpr int64_t kMostThreads = 0xFFFFFF00ll;   // of a launch: whole workgroups, counted in 32 bits
 constexpr int kPicks = 8;   // expert rows of a token that are handled together
 
 // 16 bytes of a row: V elements.  ALIGNED: rows are made of such pieces on 16-byte boundaries; else pieces begin anywhere
@@ -293,6 +294,7 @@ inline int lanes_of(int T, int pieces, bool dots) {
 template <int DT, bool ALIGNED, bool DOTS, bool GATES>
 int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
   const int lanes = lanes_of(a.T, a.H / kPiece<DT>, DOTS);
+  if ((int64_t)a.T * lanes > kMostThreads) return TAMD_E_TOO_LARGE;
   // Rows of more than the caches keep until they are used again go past them, read and written (us, four picks of 2880 bf16, 16384 tokens: dispatch 93 in place
   // of 96, sum 88 and 99, gradients 179 and 184, 113 and 124).  Below, what an operator leaves or finds in the caches is worth more: 1021 tokens of 2016,
   // six picks, whose rows the caches hold, sum 7.6 in place of 8.9.  Unaligned rows too: 37125 tokens of 730 81 for 80, 64 for 71, 135 for 136, 81 for 88;
@@ -342,7 +344,8 @@ int token_rows(const tamd_token_rows_args *args, size_t args_size, bool spread, 
   if (a.H > 0 && a.dots && (spread ? a.n_rows > 0 && !kept_rows : !kept_tokens)) return TAMD_E_INVALID;
   if (a.H == 0 && !a.dots) return 0;
   const uintptr_t by = a.dtype == TAMD_F32 ? 4 : 2;
-  if (((uintptr_t)a.src | (uintptr_t)a.dst | (uintptr_t)(a.dots ? a.other : nullptr)) % by != 0) return TAMD_E_ALIGNMENT;
+  if (((uintptr_t)a.src | (uintptr_t)a.dst | (uintptr_t)(a.dots ? a.other : nullptr)) % by != 0 || (uintptr_t)a.row_indx % 4 != 0) return TAMD_E_ALIGNMENT;
+  if (((uintptr_t)a.gates | (uintptr_t)a.dots) % (a.gates_dtype == TAMD_F32 && (a.gates || a.dots) ? 4 : 2) != 0) return TAMD_E_ALIGNMENT;
   hipStream_t st = (hipStream_t)stream;
   return a.dtype == TAMD_F32 ? launch<TAMD_F32>(a, spread, st) : a.dtype == TAMD_BF16 ? launch<TAMD_BF16>(a, spread, st) : launch<TAMD_F16>(a, spread, st);
 }

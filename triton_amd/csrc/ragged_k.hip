@@ -17,6 +17,11 @@ struct Plan {
 
 int filled_up(int cols) { return (cols + 7) / 8 * 8; }
 
+// Rows that copies of 16 bytes take whole, and a stage's of which 31 bits count
+bool whole(const void *q, int64_t pitch, int cols) { return (uintptr_t)q % 16 == 0 && pitch % 8 == 0 && cols % 8 == 0 && pitch < 1 << 24; }
+// Rows that can be laid out by one launch, whose threads are counted in 32 bits
+bool few_enough(int64_t K, int cols) { return K * (filled_up(cols) / 8) <= 0xFFFFFF00ll; }
+
 // The tile by the rows of a slice in the mean and the tiles that there are (figures beside RaggedTile), and the splits of long slices of few
 // tiles: a stage of 32 rows takes 0.57 us in a workgroup of its own; the partial sums cost a launch of 5 us, and 8 bytes each at the caches' rate.
 Plan make_plan(const tamd_ragged_k_args &a) {
@@ -41,8 +46,6 @@ Plan make_plan(const tamd_ragged_k_args &a) {
   // over 32, 640 x 4608, 287 and 295; 17056 over 60, 936 x 4040, 254 and 252 (not so, with 284 rows).  Slices of one length lose up to 1 %.
   p.longest_first = E > 1 && E <= 64 && rows > 128 && rows >= 16 * E;
   p.pitch = ((int64_t)N + 3) / 4 * 4;
-  // rows that copies of 16 bytes take whole, and a stage's of which 31 bits count
-  const auto whole = [](const void *q, int64_t pitch, int cols) { return (uintptr_t)q % 16 == 0 && pitch % 8 == 0 && cols % 8 == 0 && pitch < 1 << 24; };
   p.lay_x = K > 0 && !whole(a.x, a.x_stride, M), p.lay_d = K > 0 && !whole(a.d, a.d_stride, N);
   p.x_at = 0;
   p.d_at = p.x_at + (p.lay_x ? K * filled_up(M) * 2 : 0);
@@ -122,8 +125,9 @@ int check(const tamd_ragged_k_args *args, size_t args_size, bool &ok) {
   if (a.x_stride < 0 || a.d_stride < 0 || a.y_stride_e < 0 || a.y_stride_m < 0) return TAMD_E_INVALID;
   if (a.M == 0 || a.N == 0 || a.E == 0) return 0;
   if (too_large(a.M, a.N, a.E, a.K)) return TAMD_E_TOO_LARGE;
+  if ((!whole(a.x, a.x_stride, a.M) && !few_enough(a.K, a.M)) || (!whole(a.d, a.d_stride, a.N) && !few_enough(a.K, a.N))) return TAMD_E_TOO_LARGE;
   if (!a.y || !a.slice_offs || !a.slice_sizes || (a.K > 0 && (!a.x || !a.d))) return TAMD_E_INVALID;
-  if ((uintptr_t)a.x % 2 || (uintptr_t)a.d % 2 || (uintptr_t)a.y % (a.y_dtype == TAMD_F32 ? 4 : 2)) return TAMD_E_ALIGNMENT;
+  if ((uintptr_t)a.slice_offs % 4 || (uintptr_t)a.slice_sizes % 4 || (uintptr_t)a.x % 2 || (uintptr_t)a.d % 2 || (uintptr_t)a.y % (a.y_dtype == TAMD_F32 ? 4 : 2)) return TAMD_E_ALIGNMENT;
   ok = true;
   return 0;
 }

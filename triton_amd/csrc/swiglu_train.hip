@@ -306,7 +306,7 @@ bool shape(GluShape &sh, int64_t M, int64_t N, float alpha, float limit, int has
   sh.L = 2 * N, sh.alpha = alpha, sh.limit = has_limit ? limit : kMost, sh.has_limit = has_limit;
   const int64_t n = (sh.div.total + per - 1) / per;
   blocks = (unsigned)n;
-  return n < ((int64_t)1 << 31);
+  return n < 1 << 24;    // (a launch counts its threads in 32 bits)
 }
 bool is_big(int dtype, int64_t M, int64_t N) { return dtype != TAMD_F32 && (double)M * N * 8 >= 64e6; }
 bool whole(const void *p, int64_t stride_bytes, int by) { return ((uintptr_t)p | (uintptr_t)stride_bytes) % by == 0; }

@@ -102,6 +102,7 @@ extern "C" int tamd_topk_backward(const void *x, int dtype, int64_t x_stride, in
   const bool aligned = ((uintptr_t)dx | (uintptr_t)(dx_stride * size)) % 16 == 0;
   // 16 lanes to a row where they hold its picks and write it in few turns, else a wave
   const bool narrow = k <= 16 && n_cols <= 512;
+  if (n_rows * (narrow ? 16 : 64) > 0xFFFFFF00ll) return TAMD_E_TOO_LARGE;   // (a launch counts its threads in 32 bits)
   const auto go = [&](auto dt, auto lanes) {
     constexpr int DT = decltype(dt)::value, L = decltype(lanes)::value;
     const unsigned blocks = (unsigned)((n_rows + 256 / L - 1) / (256 / L));

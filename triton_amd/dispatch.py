@@ -28,6 +28,8 @@ def _by_row(t: torch.Tensor, name: str) -> torch.Tensor:
     assert t.ndim == 2, f"{name} is a matrix of rows"
     if t.dtype not in _TYPES:
         raise NotImplementedError(f"{name} of {t.dtype} is not built (float32, bfloat16 and float16 are)")
+    if t.shape[1] >= 1 << 31:
+        raise NotImplementedError(f"{name}: rows of 2^31 elements and more are not built")
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 

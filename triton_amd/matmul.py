@@ -177,6 +177,8 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
     dtype = pc.out_dtype or (c.dtype if c is not None else a.dtype)
     if dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise NotImplementedError(f"{dtype} results of a K-ragged matmul are not built")
+    if M >= 1 << 24 or N >= 1 << 24:
+        raise NotImplementedError(f"K-ragged matmul is built for fewer than 2^24 rows and columns of results, not {M} and {N}")
     x, d = _by_rows(a.t()), _by_rows(b)
     if c is None:
         c = torch.empty((E, M, N), dtype=dtype, device=a.device)
