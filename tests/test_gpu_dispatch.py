@@ -241,7 +241,7 @@ def test_gradient_in_the_place_of_the_rows(T, k, H, device):
         assert got is rows and torch.equal(got, want) and torch.equal(same, dgates)
 
 
-@pytest.mark.parametrize("T,k,H", [(9001, 4, 1037), (2000, 3, 1037), (700, 2, 2050), (9000, 3, 60), (30, 5, 9)])
+@pytest.mark.parametrize("T,k,H", [(9001, 4, 1037), (2000, 3, 1037), (700, 2, 2050), (9000, 3, 60), (30, 5, 9), (30001, 4, 301)])
 def test_ragged_rows_as_whole_ones(T, k, H, device):
     """Rows that are no whole 16-byte pieces: bit for bit what the same rows give with zeros behind them."""
     torch.manual_seed(H)

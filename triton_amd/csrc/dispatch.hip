@@ -293,14 +293,18 @@ inline int lanes_of(int T, int pieces, bool dots) {
 
 template <int DT, bool ALIGNED, bool DOTS, bool GATES>
 int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
+  constexpr int SIZE = 16 / kPiece<DT>;
+  const auto on_lines = [&](const void *p, int64_t stride) { return ((uintptr_t)p | (uintptr_t)(stride * SIZE)) % 128 == 0; };
+  const bool whole_lines = ALIGNED && (int64_t)a.H * SIZE % 128 == 0 && on_lines(a.src, a.src_stride) && on_lines(a.dst, a.dst_stride) && (!DOTS || on_lines(a.other, a.other_stride));
   const int lanes = lanes_of(a.T, a.H / kPiece<DT>, DOTS);
   if ((int64_t)a.T * lanes > kMostThreads) return TAMD_E_TOO_LARGE;
   // Rows of more than the caches keep until they are used again go past them, read and written (us, four picks of 2880 bf16, 16384 tokens: dispatch 93 in place
   // of 96, sum 88 and 99, gradients 179 and 184, 113 and 124).  Below, what an operator leaves or finds in the caches is worth more: 1021 tokens of 2016,
-  // six picks, whose rows the caches hold, sum 7.6 in place of 8.9.  Unaligned rows too: 37125 tokens of 730 81 for 80, 64 for 71, 135 for 136, 81 for 88;
-  // 10000 of 2038 58 for 67, 44 for 48, 94 for 97, 54 for 57 (loads alone past the caches: 68, 46, 105, 56).
+  // six picks, whose rows the caches hold, sum 7.6 in place of 8.9.  Short rows whose ends share lines with others go through the caches, which put these
+  // together (60000 tokens of 304, dispatch and gradients 66, 105, 67 in place of 75, 119, 71; 256, past the caches, 33, 59, 46 for 35, 62, 50); of long ones the
+  // shared lines are few (12000 of 1500: 51, 82, 47 past them, 57, 85, 51 through them; 36058 of 736: 61, 111, 71 and 71, 119, 80).
   const double bytes = (double)a.T * ((double)a.k * (spread && DOTS ? 2 : 1) + 1) * a.H * (16 / kPiece<DT>);
-  const bool once = bytes >= 64e6;
+  const bool once = bytes >= 64e6 && (whole_lines || a.H > 64 * kPiece<DT>);
   const auto go = [&](auto of) {
     constexpr int LANES = decltype(of)::value;
     const unsigned grid = (unsigned)(((int64_t)a.T * LANES + 255) / 256);
