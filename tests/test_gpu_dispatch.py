@@ -229,9 +229,10 @@ def test_another_stream_and_a_graph(device):
         assert all(torch.equal(a, b) for a, b in zip(kept, step()))
 
 
-@pytest.mark.parametrize("T,k,H", [(40, 4, 264), (3000, 2, 1032), (9, 11, 77), (9000, 3, 64), (9001, 3, 1037), (700, 2, 2050), (50, 3, 5)])
+@pytest.mark.parametrize("T,k,H", [(40, 4, 264), (3000, 2, 1032), (9, 11, 77), (9000, 3, 64), (9001, 3, 1037), (700, 2, 2050), (50, 3, 5), (300, 4, 2060), (64, 2, 4108), (2400, 3, 1026)])
 def test_gradient_in_the_place_of_the_rows(T, k, H, device):
-    """combine_backward into the rows that it reads: what it gives elsewhere."""
+    """combine_backward into the rows that it reads: what it gives elsewhere.  (Rows whose last piece is another wave's than the one before it are among them: what
+    one wave stores, the other must have read, or store itself.)"""
     torch.manual_seed(T)
     for dtype in (torch.bfloat16, torch.float32):
         p, gates = places(T, k, T * k, 0.1).to(device), torch.rand(T, k, device=device)

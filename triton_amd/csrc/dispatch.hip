@@ -37,8 +37,19 @@ TAMD_DEVICE void store_raw(void *row, int64_t byte, u32x4_t q) {
   if constexpr (ONCE) __builtin_nontemporal_store((Piece<ALIGNED>)q, p);
   else *p = q;
 }
+// The last elements of a piece, without its first `again`
+template <int DT>
+TAMD_DEVICE void store_rest(void *row, int64_t byte, u32x4_t q, int again) {
+#pragma unroll
+  for (int e = 0; e < kPiece<DT>; ++e) {
+    if (e < again) continue;
+    if constexpr (DT == TAMD_F32) *(uint32_t *)((char *)row + byte + 4 * e) = q[e];
+    else *(uint16_t *)((char *)row + byte + 2 * e) = (uint16_t)(q[e / 2] >> (16 * (e & 1)));
+  }
+}
 // How a row of H elements is cut: into pieces of V, the last of which ends with the row and so may begin inside the one before (`again` of its elements
-// are that one's too: both store the same, and the dots leave them out).  A tail by elements was one more wait for memory: 37125 tokens of 730 bf16, four
+// are that one's too: both store the same, and the dots leave them out; where the result lies in the place of what the dots read, the last piece
+// stores its own elements only, since another wave may still have to read the others: 36058 rows of 730 bf16 136 us, 130 elsewhere).  A tail by elements was one more wait for memory: 37125 tokens of 730 bf16, four
 // picks, took 83 us for the dispatch, 85 for the sum, 150 and 110 for their gradients, and take 80, 71, 136 and 88 so.  Rows of less than a piece go by elements.
 template <int DT, bool ALIGNED>
 struct Cut {
@@ -152,7 +163,7 @@ TAMD_DEVICE void store_dots(const tamd_token_rows_args &a, int64_t t, int j0, co
 
 // Without gates rows are copied as bits.
 template <int DT, bool ALIGNED, int LANES, bool DOTS, bool GATES, bool ONCE>
-__global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
+__global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a, bool in_place) {
   constexpr int V = kPiece<DT>, SIZE = 16 / V;
   __shared__ float lds[4 * kPicks];
   const int64_t t = token_of<LANES>();
@@ -178,14 +189,15 @@ __global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a) {
           dot[j] = add_dot<V>(x, y, cut.again(c), dot[j]);
         }
         char *const row = (char *)a.dst + p.row[j] * a.dst_stride * SIZE;
+        u32x4_t to = q;
         if constexpr (GATES) {
           float out[V];
 #pragma unroll
           for (int e = 0; e < V; ++e) out[e] = x[e] * p.gate[j];
-          store_raw<ALIGNED, ONCE>(row, byte, narrow<DT>(out));
-        } else {
-          store_raw<ALIGNED, ONCE>(row, byte, q);
+          to = narrow<DT>(out);
         }
+        if (DOTS && !ALIGNED && in_place && cut.again(c) > 0) store_rest<DT>(row, byte, to, cut.again(c));
+        else store_raw<ALIGNED, ONCE>(row, byte, to);
       }
     }
     if (!ALIGNED && at < cut.few) {
@@ -305,11 +317,13 @@ int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
   // shared lines are few (12000 of 1500: 51, 82, 47 past them, 57, 85, 51 through them; 36058 of 736: 61, 111, 71 and 71, 119, 80).
   const double bytes = (double)a.T * ((double)a.k * (spread && DOTS ? 2 : 1) + 1) * a.H * (16 / kPiece<DT>);
   const bool once = bytes >= 64e6 && (whole_lines || a.H > 64 * kPiece<DT>);
+  const auto end = [&](const void *p, int64_t stride) { return (uintptr_t)p + (uintptr_t)((int64_t)(a.n_rows - 1) * stride + a.H) * SIZE; };
+  const bool in_place = spread && DOTS && a.n_rows > 0 && (uintptr_t)a.dst < end(a.other, a.other_stride) && (uintptr_t)a.other < end(a.dst, a.dst_stride);
   const auto go = [&](auto of) {
     constexpr int LANES = decltype(of)::value;
     const unsigned grid = (unsigned)(((int64_t)a.T * LANES + 255) / 256);
-    if (spread && once) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, true><<<grid, 256, 0, st>>>(a);
-    else if (spread) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, false><<<grid, 256, 0, st>>>(a);
+    if (spread && once) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, true><<<grid, 256, 0, st>>>(a, in_place);
+    else if (spread) spread_kernel<DT, ALIGNED, LANES, DOTS, GATES, false><<<grid, 256, 0, st>>>(a, in_place);
     else if (once) collect_kernel<DT, ALIGNED, LANES, DOTS, true><<<grid, 256, 0, st>>>(a);
     else collect_kernel<DT, ALIGNED, LANES, DOTS, false><<<grid, 256, 0, st>>>(a);
   };
