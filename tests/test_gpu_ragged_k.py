@@ -183,3 +183,45 @@ def test_results_that_are_too_large(device):
         for a, b in ((wide.t(), d), (d.t(), wide)):
             with pytest.raises(NotImplementedError):
                 matmul(a, b, None, md, md)
+
+
+def overlapping(rows, C, dtype, device, step):
+    """[rows, C] whose rows begin `step` elements after each other: one row again and again, or a window that slides."""
+    return torch.randn((rows - 1) * step + C if rows else 0, device=device).to(dtype).as_strided((rows, C), (step, 1))
+
+
+@pytest.mark.parametrize("sizes", [[1], [5, 1, 0, 40], [40, 3], [64, 31, 33], [3000, 9, 700]], ids=str)
+@pytest.mark.parametrize("M,N", [(8, 16), (64, 136), (33, 72)])
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.float32), (torch.float16, None)])
+def test_rows_that_overlap(M, N, sizes, dtype, out, device):
+    """Expanded operands and sliding windows, one of them or both: a slice sums its own rows, not those that its last stage reaches."""
+    torch.manual_seed(M + len(sizes))
+    rows = sum(sizes)
+    dense = lambda C: torch.randn(rows, C, device=device).to(dtype)  # noqa: E731
+    md = ragged(sizes, rows, device)
+    for step in (0, 8):
+        for x, d in ((overlapping(rows, M, dtype, device, step), dense(N)), (dense(M), overlapping(rows, N, dtype, device, step)),
+                     (overlapping(rows, M, dtype, device, step), overlapping(rows, N, dtype, device, step))):
+            check(matmul(x.t(), d, None, md, md, precision_config=PrecisionConfig(out_dtype=out)), x, d, sizes, out or dtype)
+
+
+def test_gradient_of_a_bias(device):
+    """Ones times the gradient of a sum over tokens, both expanded: whole numbers, exactly."""
+    for sizes in ([40, 3], [40, 0, 1, 300]):
+        K, md = sum(sizes), ragged(sizes, sum(sizes), device)
+        one, dy = torch.ones(1, 8, dtype=torch.bfloat16, device=device).expand(K, 8), torch.ones(1, 16, dtype=torch.bfloat16, device=device).expand(K, 16)
+        got = matmul(one.t(), dy, None, md, md, precision_config=PrecisionConfig(out_dtype=torch.float32))
+        assert torch.equal(got, torch.tensor(sizes, device=device).float()[:, None, None].expand(-1, 8, 16))
+
+
+def test_overlapping_rows_behind_a_slice_do_not_reach(device):
+    """A window that slides over NaN behind the first slice's rows, times whole rows: the first slice is clean."""
+    sizes = [40, 25]
+    flat = torch.randn(64 * 8 + 64, device=device).bfloat16()
+    flat[39 * 8 + 64:] = float("nan")                       # (what the first forty windows do not reach)
+    windows, whole = flat.as_strided((65, 64), (8, 1)), torch.randn(65, 72, device=device).bfloat16()
+    md = ragged(sizes, 65, device)
+    for x, d in ((windows, whole), (whole, windows)):
+        got = matmul(x.t(), d, None, md, md)
+        check(got[:1], x[:40], d[:40], [40], torch.bfloat16)
+        assert bool(torch.isnan(got[1]).any())

@@ -45,6 +45,15 @@ def test_c_entry_point():
     assert room(good(M=64, K=1 << 31)) == room(good(M=1 << 24)) == _lib.E_TOO_LARGE
 
 
+@pytest.mark.parametrize("pitch", [0, 8, 56])
+@pytest.mark.parametrize("K", [1, 5, 100])
+def test_rows_that_overlap_are_laid_out_first(pitch, K):
+    """A pitch below the columns: the copies' bounds would let rows behind a slice in, so there has to be room for rows of their own."""
+    room = lambda **more: _lib.lib().tamd_ragged_k_matmul_workspace(C.byref(good(M=64, K=K, **more)), C.sizeof(_lib.RaggedKArgs))  # noqa: E731
+    assert room(x_stride=pitch) == room(d_stride=pitch) == K * 64 * 2 and room(x_stride=pitch, d_stride=pitch) == 2 * K * 64 * 2
+    assert room() == room(x_stride=72, d_stride=80) == 0
+
+
 def test_structure_matches_the_header(tmp_path):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     names = [n for n, _ in _lib.RaggedKArgs._fields_]

@@ -18,7 +18,7 @@ namespace tamd {
 
 struct RaggedK {
   const void *x, *d;
-  int64_t x_pitch, d_pitch;           // elements, a multiple of 8
+  int64_t x_pitch, d_pitch;           // elements, a multiple of 8, no less than the columns that can be read
   int x_cols, d_cols;                 // columns that can be read: M and N, filled up to a multiple of 8
   const int32_t *offs, *sizes;        // [E]
   void *y;

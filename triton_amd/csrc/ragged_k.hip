@@ -17,8 +17,9 @@ struct Plan {
 
 int filled_up(int cols) { return (cols + 7) / 8 * 8; }
 
-// Rows that copies of 16 bytes take whole, and a stage's of which 31 bits count
-bool whole(const void *q, int64_t pitch, int cols) { return (uintptr_t)q % 16 == 0 && pitch % 8 == 0 && cols % 8 == 0 && pitch < 1 << 24; }
+// Rows that copies of 16 bytes take whole, and a stage's of which 31 bits count.  Rows that overlap (an expanded operand's have a pitch of 0) are
+// none: the copies' bounds end a slice by the bytes up to its last row's end, which keep the next row out only if that begins behind them.
+bool whole(const void *q, int64_t pitch, int cols) { return (uintptr_t)q % 16 == 0 && pitch % 8 == 0 && cols % 8 == 0 && pitch >= cols && pitch < 1 << 24; }
 // Rows that can be laid out by one launch, whose threads are counted in 32 bits
 bool few_enough(int64_t K, int cols) { return K * (filled_up(cols) / 8) <= 0xFFFFFF00ll; }
 
