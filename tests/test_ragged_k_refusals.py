@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from triton_amd import _lib
-from triton_amd.matmul import FnSpecs, FusedActivation, PrecisionConfig, matmul
+from triton_amd.matmul import FlexCtx, FnSpecs, FusedActivation, PrecisionConfig, matmul
+from triton_amd.numerics import InFlexData, OutFlexData
 from triton_amd.tensor import RaggedTensorMetadata
 
 
@@ -93,3 +94,18 @@ def test_python_calls(monkeypatch):
                  lambda: matmul(x.t()[None], d[None], None, md, md)):
         with pytest.raises(AssertionError):
             call()
+
+
+@pytest.mark.parametrize("settings", [dict(c_value_pack_factor=2), *(dict(flex_ctx=FlexCtx(out_data=OutFlexData(**{name: torch.ones(1)}))) for name in ("checksum_scale", "expected_scale", "actual_scale")),
+                                      dict(flex_ctx=FlexCtx(acc_data=InFlexData(scale=torch.ones(1)))), dict(a_mx_tensor_scale=torch.ones(1)), dict(c_mx_scale=torch.zeros(1, dtype=torch.uint8))],
+                         ids=["packed", "checksum", "expected", "actual", "accumulator", "per tensor", "results' scales"])
+@pytest.mark.parametrize("given", [False, True])
+def test_settings_that_change_the_result_are_not_dropped(settings, given, monkeypatch):
+    """What has no kernel here is refused before the native call as behind it, whether the caller has results of their own or not."""
+    from triton_amd import _native
+    x, d, md = torch.zeros(10, 16).bfloat16(), torch.zeros(10, 24).bfloat16(), metadata(3)
+    monkeypatch.setattr(_lib, "require_gpu", lambda t, name: None)
+    for holder, name in ((_native, "matmul_ragged_k"), (_lib.lib(), "tamd_ragged_k_matmul")):
+        monkeypatch.setattr(holder, name, lambda *a: pytest.fail("called"))
+    with pytest.raises(NotImplementedError):
+        matmul(x.t(), d, None, md, md, c=torch.zeros(3, 16, 24).bfloat16() if given else None, precision_config=PrecisionConfig(**settings))

@@ -154,8 +154,11 @@ def _matmul_ragged_k(a, b, a_ragged, b_ragged, pc: PrecisionConfig, c):
     lhs, rhs, out = flex.lhs_data, flex.rhs_data, flex.out_data
     if (pc.a_mx_scale is not None or pc.b_mx_scale is not None or pc.c_mx_scale is not None or pc.a_mx_tensor_scale is not None
             or pc.b_mx_tensor_scale is not None or pc.acc_scale != 1.0 or lhs.scale is not None or rhs.scale is not None or flex.acc_data.scale is not None
-            or lhs.dtype is not None or rhs.dtype is not None or out.expected_scale is not None or out.actual_scale is not None):
-        raise NotImplementedError("K-ragged matmul takes unscaled operands")
+            or lhs.dtype is not None or rhs.dtype is not None or out.expected_scale is not None or out.actual_scale is not None
+            or out.checksum_scale is not None):
+        raise NotImplementedError("K-ragged matmul takes unscaled operands and gives unscaled results")
+    if pc.c_value_pack_factor != 1:
+        raise NotImplementedError("packed output values (c_value_pack_factor != 1) are not built")
     if c is None and (a_ragged is None or a_ragged.n_slices == b_ragged.n_slices):
         done = _native.matmul_ragged_k(a, b, b_ragged.slice_offs, b_ragged.slice_sizes, pc.out_dtype)
         if done is not None:
