@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from triton_amd import _lib
-from triton_amd.numerics import InFlexData
+from triton_amd.numerics import InFlexData, OutFlexData
 from triton_amd.swiglu import FlexCtx, PrecisionConfig, swiglu_backward, swiglu_checkpoint
 
 
@@ -61,3 +61,15 @@ def test_shapes_types_and_options(monkeypatch):
             swiglu_checkpoint(a, 1.0, PrecisionConfig(limit=limit))
         with pytest.raises(ValueError):
             swiglu_backward(d, v, s, 1.0, PrecisionConfig(limit=limit))
+
+
+@pytest.mark.parametrize("name", ["expected_scale", "actual_scale", "checksum_scale"])
+def test_scales_of_the_result_are_not_dropped(name, monkeypatch):
+    monkeypatch.setattr(_lib, "require_gpu", lambda t, name: None)
+    for entry in ("tamd_swiglu_checkpoint", "tamd_swiglu_backward"):
+        monkeypatch.setattr(_lib.lib(), entry, lambda *a: pytest.fail("launched"))
+    pc = PrecisionConfig(limit=7.0, flex_ctx=FlexCtx(out_data=OutFlexData(**{name: torch.ones(1)})))
+    with pytest.raises(NotImplementedError):
+        swiglu_checkpoint(torch.zeros(2, 32), 1.0, pc)
+    with pytest.raises(NotImplementedError):
+        swiglu_backward(torch.zeros(2, 16), torch.zeros(2, 32).to(torch.float8_e4m3fn), torch.zeros(2, 1, dtype=torch.uint8), 1.0, pc)

@@ -53,7 +53,8 @@ _MX_GROUP = 32
 def _limits(precision_config):
     """(limit, whether there is one) of a call without flexpoint scales."""
     fc = precision_config.flex_ctx
-    if fc.inp_data.scale is not None or fc.out_data.expected_scale is not None or fc.out_data.actual_scale is not None:
+    out = fc.out_data
+    if fc.inp_data.scale is not None or out.expected_scale is not None or out.actual_scale is not None or out.checksum_scale is not None:
         raise NotImplementedError("flexpoint scaling in the standalone swiglu is not built")
     limit = precision_config.limit
     if limit is not None and not limit >= 0:
