@@ -177,6 +177,27 @@ def test_the_lowest_and_the_greatest_values(dtype, limit, device):
     assert bool((da[0, 6:8] == 0).all() and again[0, 3] == 0 and out[0, 3] == 0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("limit", [float("inf"), 1e300])
+def test_a_limit_beyond_the_numbers_is_none(dtype, limit, device):
+    """An infinite limit, or one that float32 has no number for, cuts nothing off: bit for bit what no limit gives, also at values that are kept as 2^128."""
+    torch.manual_seed(4)
+    most = torch.finfo(dtype).max
+    a = torch.randn(9, 96, device=device).to(dtype)
+    for row, (at, v) in enumerate(((6, most), (7, most), (6, -most), (7, -most), (6, float("inf")), (7, float("-inf")), (6, most / 2), (6, float("nan")))):
+        a[row, at] = v
+    d = torch.randn(9, 48, device=device).to(dtype)
+    kept, free = swiglu_checkpoint(a, ALPHA, PrecisionConfig(limit=limit)), swiglu_checkpoint(a, ALPHA, PrecisionConfig(limit=None))
+    bits = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+    assert all(torch.equal(bits(x), bits(y)) for x, y in zip(kept, free))
+    got = swiglu_backward(d, *kept[1:], ALPHA, PrecisionConfig(limit=limit), return_out=True)
+    want = swiglu_backward(d, *kept[1:], ALPHA, PrecisionConfig(limit=None), return_out=True)
+    lost = torch.isnan(read(*kept[1:]))
+    for x, y in zip(got, want):
+        assert torch.equal(torch.isnan(x), torch.isnan(y)) and torch.equal(x.nan_to_num(nan=0.0), y.nan_to_num(nan=0.0))
+    assert not bool(torch.isnan(got[0][:4])[~lost[:4]].any())
+
+
 def test_at_the_limit_the_gradient_passes(device):
     """7 and -7 are kept exactly and are not beyond a limit of 7; the next values are."""
     a = torch.tensor([[7.0, 7.0, 7.0, -7.0, 7.5, 0.5, 0.5, 7.5, -9.0, -7.5, 0.0, 0.0]], device=device)

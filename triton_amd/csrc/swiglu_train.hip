@@ -303,7 +303,9 @@ __global__ __launch_bounds__(256) void backward_kernel(const void *__restrict__ 
 bool shape(GluShape &sh, int64_t M, int64_t N, float alpha, float limit, int has_limit, bool big, unsigned &blocks) {
   const int64_t G = (2 * N + 31) / 32, per = big ? 128 : 64;
   sh.div = group_div(1, M, G);
-  sh.L = 2 * N, sh.alpha = alpha, sh.limit = has_limit ? limit : kMost, sh.has_limit = has_limit;
+  // (an infinite limit cuts nothing off: it is none, so that a value that is kept as 2^128 counts as the greatest here too)
+  const bool cuts = has_limit && limit <= kMost;
+  sh.L = 2 * N, sh.alpha = alpha, sh.limit = cuts ? limit : kMost, sh.has_limit = cuts;
   const int64_t n = (sh.div.total + per - 1) / per;
   blocks = (unsigned)n;
   return n < 1 << 24;    // (a launch counts its threads in 32 bits)
