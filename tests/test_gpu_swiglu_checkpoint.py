@@ -198,6 +198,25 @@ def test_a_limit_beyond_the_numbers_is_none(dtype, limit, device):
     assert not bool(torch.isnan(got[0][:4])[~lost[:4]].any())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("alpha", [0.0, 2.0 ** -126, -2.0 ** -126, -1.0])
+def test_the_lowest_value_with_a_flat_sigmoid(dtype, alpha, device):
+    """A gate kept as -2^128 whose sigmoid is no zero, as alpha is (nearly) 0 or negative: it counts as the lowest of float32 there too."""
+    most = torch.finfo(dtype).max
+    a = torch.zeros(2, 32, dtype=dtype, device=device)
+    a[0, 6], a[1, 6] = -most, most
+    pc, d = PrecisionConfig(limit=None), torch.full((2, 16), 0.25, dtype=dtype, device=device)
+    _, values, scales = swiglu_checkpoint(a, alpha, pc)
+    da, again = swiglu_backward(d, values, scales, alpha, pc, return_out=True)
+    g = torch.tensor([-2.0 ** 128, 2.0 ** 128], dtype=torch.float64, device=device)
+    s = torch.sigmoid(alpha * g)
+    # (no more than |alpha g| = 4 where the sigmoid is neither 0 nor 1: a float32 exponential and reciprocal, and the steps behind them, are off by 2^-18 at most)
+    for got, want in ((again[:, 3], g * s), (da[:, 6], 0.25 * (s + alpha * g * s * (1 - s))), (da[:, 7], 0.25 * g * s)):
+        want = want.clamp(-float(most), float(most))
+        got = got.double().clamp(-float(most), float(most))
+        assert bool(((got - want).abs() <= (HALF_STEP[dtype] + 2.0 ** -18) * want.abs() + LEAST[dtype]).all()), (got, want)
+
+
 def test_at_the_limit_the_gradient_passes(device):
     """7 and -7 are kept exactly and are not beyond a limit of 7; the next values are."""
     a = torch.tensor([[7.0, 7.0, 7.0, -7.0, 7.5, 0.5, 0.5, 7.5, -9.0, -7.5, 0.0, 0.0]], device=device)

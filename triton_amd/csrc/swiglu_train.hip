@@ -147,8 +147,8 @@ struct Pair {
   float g, l, s;
   bool g_free, l_free;     // not beyond the limit
 };
-// KEPT: a type's lowest value may have been kept as -2^128.  It counts as the lowest of float32, so that the zero of its sigmoid makes zeros; the sigmoid of
-// a NaN is one, and is in all that follows.
+// KEPT: a type's lowest value may have been kept as -2^128.  It counts as the lowest of float32, so that the zero of its sigmoid makes zeros, and so that it
+// has a sigmoid where alpha is 0.
 template <bool KEPT>
 TAMD_DEVICE Pair pair_of(float g, float l, const GluShape &sh) {
   Pair p;
@@ -157,8 +157,8 @@ TAMD_DEVICE Pair pair_of(float g, float l, const GluShape &sh) {
   p.l_free = l_in || !sh.has_limit;
   p.g = (KEPT ? g_in : p.g_free) ? g : sh.limit;
   p.l = (KEPT ? l_in : p.l_free) ? l : __builtin_copysignf(sh.limit, l);
+  if constexpr (KEPT) p.g = p.g < -kMost ? -kMost : p.g;
   p.s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * sh.alpha * p.g));
-  if constexpr (KEPT) p.g = __builtin_fmaxf(p.g, -kMost);
   return p;
 }
 
