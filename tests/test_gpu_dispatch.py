@@ -1,8 +1,11 @@
 """GPU: rows of tokens to the rows of their experts and back (`dispatch`, `combine`) and their gradients, against the formulas in 64 bits: every type,
 tokens and picks without a row, rows that nothing names, odd sizes, pitches and starts, more picks than one turn of the kernels takes."""
+import ctypes
+
 import pytest
 import torch
 
+from triton_amd import _lib
 from triton_amd.dispatch import combine, combine_backward, dispatch, dispatch_backward
 from triton_amd.routing import routing
 
@@ -269,3 +272,29 @@ def test_rows_that_are_too_long(device):
         for call in (dispatch, combine, combine_backward, dispatch_backward):
             with pytest.raises(NotImplementedError):
                 call(long, p)
+
+
+@pytest.mark.parametrize("T,k,H", [(5, 3, 40), (300, 2, 1037), (50, 4, 2880), (64, 9, 2061)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_products_without_gates(T, k, H, dtype, device):
+    """The C entry points give the rows' products without gate weights too (each counts as 1)."""
+    torch.manual_seed(H)
+    n = T * k
+    p = places(T, k, n, 0.1)
+    tokens, rows = torch.randn(T, H).to(dtype), torch.randn(n, H).to(dtype)
+    pd, td, rd = p.to(device), tokens.to(device), rows.to(device)
+    products = (of(p, rows) * tokens.double()[:, None])
+    slack = (H / 16 + 18) * 2.0 ** -24 * products.abs().sum(-1)      # (16 lanes or more add up a row, and are joined)
+    for spread, out in ((True, torch.full((n, H), 3.0, dtype=dtype, device=device)), (False, torch.empty(T, H, dtype=dtype, device=device))):
+        src, other = (td, rd) if spread else (rd, td)
+        dots = torch.empty(T, k, device=device)
+        a = _lib.TokenRowsArgs(src=src.data_ptr(), src_stride=H, dst=out.data_ptr(), dst_stride=H, row_indx=pd.data_ptr(), row_indx_stride=k, gates_dtype=_lib.F32,
+                               other=other.data_ptr(), other_stride=H, dots=dots.data_ptr(), dots_stride=k, dtype=_lib.dtype_code(dtype), T=T, k=k, H=H, n_rows=n)
+        entry = _lib.lib().tamd_dispatch if spread else _lib.lib().tamd_combine
+        assert entry(ctypes.byref(a), ctypes.sizeof(a), _lib.stream_ptr(device)) == 0
+        rounded(dots, products.sum(-1), torch.float32, slack)
+        if spread:
+            assert torch.equal(out.cpu(), scattered(p, tokens.double()[:, None].expand(T, k, H), torch.full((n, H), 3.0)).to(dtype))
+        else:
+            terms = of(p, rows)
+            rounded(out, terms.sum(1), dtype, (k + 1) * 2.0 ** -24 * terms.abs().sum(1))

@@ -161,7 +161,7 @@ TAMD_DEVICE void store_dots(const tamd_token_rows_args &a, int64_t t, int j0, co
     if (lane == j && j0 + j < a.k) store_gate(a.dots, a.gates_dtype, t * a.dots_stride + j0 + j, all[j]);
 }
 
-// Without gates rows are copied as bits.
+// Without gates (and without dots) rows are copied as bits.
 template <int DT, bool ALIGNED, int LANES, bool DOTS, bool GATES, bool ONCE>
 __global__ __launch_bounds__(256) void spread_kernel(tamd_token_rows_args a, bool in_place) {
   constexpr int V = kPiece<DT>, SIZE = 16 / V;
@@ -334,7 +334,7 @@ int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
 }
 template <int DT, bool ALIGNED>
 int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
-  if (a.dots) return a.gates ? launch<DT, ALIGNED, true, true>(a, spread, st) : launch<DT, ALIGNED, true, false>(a, spread, st);
+  if (a.dots) return launch<DT, ALIGNED, true, true>(a, spread, st);   // (without gates by weights of 1, which load_picks gives)
   return a.gates ? launch<DT, ALIGNED, false, true>(a, spread, st) : launch<DT, ALIGNED, false, false>(a, spread, st);
 }
 
