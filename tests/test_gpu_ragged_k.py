@@ -225,3 +225,24 @@ def test_overlapping_rows_behind_a_slice_do_not_reach(device):
         got = matmul(x.t(), d, None, md, md)
         check(got[:1], x[:40], d[:40], [40], torch.bfloat16)
         assert bool(torch.isnan(got[1]).any())
+
+
+@pytest.mark.parametrize("M,N,sizes", [(4100, 2624, [320, 350, 0, 700, 400]), (2600, 4160, [333, 650, 0, 700]), (136, 128, [40, 0, 50]), (300, 192, [500, 9])])
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float16, torch.float16)])
+def test_results_on_whole_lines(M, N, sizes, dtype, out, device):
+    """Rows of results that begin on lines of 128 bytes, with M no whole tiles: the large tiles of both shapes, and small ones; and rows that end inside a line, or a
+    piece, with nothing written behind them."""
+    torch.manual_seed(M + N)
+    rows, E = sum(sizes), len(sizes)
+    x, d = torch.randn(rows, M, device=device).to(dtype), torch.randn(rows, N, device=device).to(dtype)
+    md = ragged(sizes, rows, device)
+    assert N * out.itemsize % 128 == 0
+    got = matmul(x.t(), d, None, md, md, precision_config=PrecisionConfig(out_dtype=out))
+    check(got, x, d, sizes, out)
+    for less in (1, 13, 40):
+        room = torch.full((E, M, N), 5.0, dtype=out, device=device)
+        c, fewer = room[:, :, :N - less], d[:, :N - less]
+        assert c.data_ptr() % 128 == 0
+        matmul(x.t(), fewer, None, md, md, c=c)
+        check(c, x, fewer, sizes, out)
+        assert bool((room[:, :, N - less:] == 5).all())
