@@ -85,3 +85,20 @@ def test_in_the_place_of_the_rows_and_again(T, k, H, lanes16, lanes32, dtype, de
         assert torch.equal(combine_backward(x, p, rows=rows, gates=gates)[1], dgates)
     got, same = combine_backward(x, p, rows=rows, gates=gates, out=rows)
     assert got is rows and torch.equal(got, want) and torch.equal(same, dgates)
+
+
+@pytest.mark.parametrize("T,H,lanes", [(2600, 5760, 64), (9000, 256, 16), (40, 5760, 256)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_small_products_beside_large_ones(T, H, lanes, dtype, device):
+    """A row whose products are one of 1 per lane and 2^-25 else, each of which a sum of 1 and more would lose: a piece's products are added up by themselves, so
+    that a sum has as many steps as a lane has pieces, a piece elements, and the joins."""
+    V = 4 if dtype == torch.float32 else 8
+    pieces = H // V
+    y = torch.full((1, H), 2.0 ** -25, dtype=dtype, device=device)
+    y[0, :min(pieces, lanes) * V:V] = 1.0
+    rows, x, gates = y.expand(T, H).contiguous(), torch.ones(T, H, dtype=dtype, device=device), torch.ones(T, 1, device=device)
+    p = torch.arange(T, dtype=torch.int32, device=device)[:, None]
+    want = y.double().sum()
+    steps = -(-pieces // lanes) + V + min(lanes, 64).bit_length() - 1 + (3 if lanes == 256 else 0)
+    for dg in (combine_backward(x, p, rows=rows, gates=gates)[1], dispatch_backward(rows, p, x=x, gates=gates)[1]):
+        assert bool(((dg.double() - want).abs() <= 1.01 * steps * 2.0 ** -24 * want).all()), (float(dg[0, 0]) / float(want) - 1) * 2 ** 24

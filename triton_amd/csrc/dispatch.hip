@@ -60,12 +60,14 @@ struct Cut {
   TAMD_DEVICE int64_t byte(int c) const { return (int64_t)first(c) * (16 / V); }
   TAMD_DEVICE int again(int c) const { return ALIGNED ? 0 : c * V - first(c); }
 };
-// <x, y> of a piece, without its first `again` elements
+// <x, y> of a piece, without its first `again` elements, added to a lane's sum.  A piece has a sum of its own, so that the lane's has a step per piece and not one
+// per element: 5760 float32 by a wave are off by 33 half steps at most, in place of 96, in the same time.
 template <int V>
 TAMD_DEVICE float add_dot(const float (&x)[V], const float (&y)[V], int again, float dot) {
+  float of_piece = 0.f;
 #pragma unroll
-  for (int e = 0; e < V; ++e) dot = e >= again ? __builtin_fmaf(x[e], y[e], dot) : dot;
-  return dot;
+  for (int e = 0; e < V; ++e) of_piece = e >= again ? __builtin_fmaf(x[e], y[e], of_piece) : of_piece;
+  return dot + of_piece;
 }
 template <int DT>
 TAMD_DEVICE void widen(u32x4_t q, float (&v)[kPiece<DT>]) {
