@@ -32,10 +32,9 @@ def near(got, want, dtype, slack=0.0):
 
 
 def additions(H, lanes, dtype):
-    """Of one lane: its pieces of the row, of whose elements each is a step of the sum; those that join a wave's lanes, and the waves."""
+    """The steps of a sum over a row: a piece's elements, a lane's pieces, those that join a wave's lanes, and the waves."""
     V = 4 if dtype == torch.float32 else 8
-    pieces = -(-H // V)
-    return -(-pieces // lanes) * V + min(lanes, 64).bit_length() - 1 + (3 if lanes == 256 else 0)
+    return V + -(-H // V // lanes) + min(lanes, 64).bit_length() - 1 + (3 if lanes == 256 else 0)
 
 
 @pytest.mark.parametrize("T,k,H,lanes16,lanes32", PAST_THE_CACHES + MANY_PICKS)
@@ -99,6 +98,6 @@ def test_small_products_beside_large_ones(T, H, lanes, dtype, device):
     rows, x, gates = y.expand(T, H).contiguous(), torch.ones(T, H, dtype=dtype, device=device), torch.ones(T, 1, device=device)
     p = torch.arange(T, dtype=torch.int32, device=device)[:, None]
     want = y.double().sum()
-    steps = -(-pieces // lanes) + V + min(lanes, 64).bit_length() - 1 + (3 if lanes == 256 else 0)
+    steps = additions(H, lanes, dtype)
     for dg in (combine_backward(x, p, rows=rows, gates=gates)[1], dispatch_backward(rows, p, x=x, gates=gates)[1]):
         assert bool(((dg.double() - want).abs() <= 1.01 * steps * 2.0 ** -24 * want).all()), (float(dg[0, 0]) / float(want) - 1) * 2 ** 24

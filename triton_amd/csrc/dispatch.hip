@@ -5,8 +5,8 @@
 //   collect   dst[t, :] = sum_j g[t,j] src[p[t,j], :]     dots[t,j] = <other[t, :], src[p[t,j], :]>
 // `spread` is the dispatch and, with dots, the gradient of the sum; `collect` the sum over the picks and, with dots, the gradient of
 // the dispatch.  Both go by token, so that a token's row is read (or written) once whatever k is, and its k expert rows are whole,
-// contiguous pieces of memory.  What bounds it is memory: 16384 tokens of 2880 bf16, four picks, take 93 us for the dispatch (5.1 TB/s), 88 for the sum with gate
-// weights (5.3), 179 and 113 for their gradients (4.8 and 5.0).  Sums are float32 in the order of j, a dot's partial sums are joined in a fixed order: no atomics.
+// contiguous pieces of memory.  What bounds it is memory: 16384 tokens of 2880 bf16, four picks, take 92 us for the dispatch (5.1 TB/s), 82 for the sum with gate
+// weights (5.8), 173 and 108 for their gradients (4.9 and 5.2).  Sums are float32 in the order of j, a dot's partial sums are joined in a fixed order: no atomics.
 #include "common.h"
 #include <type_traits>
 
@@ -49,8 +49,8 @@ TAMD_DEVICE void store_rest(void *row, int64_t byte, u32x4_t q, int again) {
 }
 // How a row of H elements is cut: into pieces of V, the last of which ends with the row and so may begin inside the one before (`again` of its elements
 // are that one's too: both store the same, and the dots leave them out; where the result lies in the place of what the dots read, the last piece
-// stores its own elements only, since another wave may still have to read the others: 36058 rows of 730 bf16 136 us, 130 elsewhere).  A tail by elements was one more wait for memory: 37125 tokens of 730 bf16, four
-// picks, took 83 us for the dispatch, 85 for the sum, 150 and 110 for their gradients, and take 80, 71, 136 and 88 so.  Rows of less than a piece go by elements.
+// stores its own elements only, since another wave may still have to read the others: 36058 tokens of 730 bf16, four picks, 134 us, 131 elsewhere).  A tail by elements was one more wait for memory: 37125 tokens of 730 bf16, four
+// picks, took 83 us for the dispatch, 85 for the sum, 150 and 110 for their gradients, and take 80, 64, 136 and 81 so.  Rows of less than a piece go by elements.
 template <int DT, bool ALIGNED>
 struct Cut {
   static constexpr int V = kPiece<DT>;
@@ -294,11 +294,11 @@ __global__ __launch_bounds__(256) void collect_kernel(tamd_token_rows_args a) {
 }
 
 // The lanes of a token: 16 for short rows, the workgroup where a wave to a token would leave the chip's 8192 places for waves empty, or the row is long, else
-// a wave (us, four picks unless said otherwise):
-//   dispatch of 20000 rows of 64 bf16, eight picks, 6.7 by 16 lanes and 15.1 by a wave; 7816 of 176, six picks, 6.4 and 7.3; 2386 of 352 4.9 and 3.9
-//   dispatch of 64 rows of 2880 bf16 5.4 by a wave and 3.1 by 256 lanes; 1000 of 1440, eight picks, 8.3 and 6.8; 16384 of 2880 102 and 96
-//   combine of 4099 rows of 1063 float32, two picks, 15.4 by a wave and 18.5 by 256 lanes; 1021 of 2016 bf16, six picks, 14.6 and 7.8
-//   combine_backward of 4096 rows of 2880 bf16 47 by a wave and 53 by 256 lanes; 1021 of 2016, six picks, 25.7 and 16.3
+// a wave (us, four picks unless said otherwise, rows that the caches do not hold):
+//   dispatch of 20000 rows of 64 bf16, eight picks, 7.9 by 16 lanes and 17.8 by a wave; 7816 of 176, six picks, 8.8 and 10.6; 2386 of 352 6.0 and 4.4
+//   dispatch of 64 rows of 2880 bf16 5.4 by a wave and 3.1 by 256 lanes; 1000 of 1440, eight picks, 10.7 and 7.7; 16384 of 2880 99 and 93
+//   combine of 4099 rows of 1063 float32, two picks, 15.0 by a wave and 17.0 by 256 lanes; 1021 of 2016 bf16, six picks, 17.9 and 10.0
+//   combine_backward of 4096 rows of 2880 bf16 45 by a wave and 50 by 256 lanes; 1021 of 2016, six picks, 25.7 and 16.3
 inline int lanes_of(int T, int pieces, bool dots) {
   if (pieces <= 32 || (pieces <= 64 && T >= 8192)) return 16;
   if (pieces >= 128 && (T < (dots ? 2500 : 4096) || (!dots && pieces >= 320))) return 256;
@@ -313,10 +313,10 @@ int launch(const tamd_token_rows_args &a, bool spread, hipStream_t st) {
   const int lanes = lanes_of(a.T, a.H / kPiece<DT>, DOTS);
   if ((int64_t)a.T * lanes > kMostThreads) return TAMD_E_TOO_LARGE;
   // Rows of more than the caches keep until they are used again go past them, read and written (us, four picks of 2880 bf16, 16384 tokens: dispatch 93 in place
-  // of 96, sum 88 and 99, gradients 179 and 184, 113 and 124).  Below, what an operator leaves or finds in the caches is worth more: 1021 tokens of 2016,
+  // of 96, sum 82 and 95, gradients 175 and 181, 108 and 121).  Below, what an operator leaves or finds in the caches is worth more: 1021 tokens of 2016,
   // six picks, whose rows the caches hold, sum 7.6 in place of 8.9.  Short rows whose ends share lines with others go through the caches, which put these
-  // together (60000 tokens of 304, dispatch and gradients 66, 105, 67 in place of 75, 119, 71; 256, past the caches, 33, 59, 46 for 35, 62, 50); of long ones the
-  // shared lines are few (12000 of 1500: 51, 82, 47 past them, 57, 85, 51 through them; 36058 of 736: 61, 111, 71 and 71, 119, 80).
+  // together (60000 tokens of 304, dispatch and gradients 66, 105, 66 in place of 75, 119, 70; 256, past the caches, 33, 59, 46 for 35, 62, 50); of long ones the
+  // shared lines are few (12000 of 1500: 50, 83, 48 past them, 58, 85, 51 through them; 36058 of 736: 60, 111, 71 and 71, 119, 80).
   const double bytes = (double)a.T * ((double)a.k * (spread && DOTS ? 2 : 1) + 1) * a.H * (16 / kPiece<DT>);
   const bool once = bytes >= 64e6 && (whole_lines || a.H > 64 * kPiece<DT>);
   const auto end = [&](const void *p, int64_t stride) { return (uintptr_t)p + (uintptr_t)((int64_t)(a.n_rows - 1) * stride + a.H) * SIZE; };

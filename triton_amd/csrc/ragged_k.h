@@ -41,7 +41,8 @@ typedef uint32_t u32x4_by2_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef int s32x4_t __attribute__((ext_vector_type(4)));
 
 // (The copies take 16-byte pieces at 16-byte addresses; operands that are not made of these are laid out so first, by a launch of its own, which
-// also fills their rows up with zeros: 66000 rows over 16 slices, 1000 x 1001, 272 us so and 558 with unaligned loads through registers.)
+// also fills their rows up with zeros: 66000 rows over 16 slices, 1000 x 1001, 244 us so, of which the pass takes
+// 43; with unaligned loads through registers 558, where the pass gave 272.)
 
 // 16 bytes per lane from memory to LDS, lane l's to lds_at + 16 l; offsets past the descriptor's end deliver zeros.  (The wait states cover the
 // scalar registers that the compiler may have written just before, and M0.)
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
     uint8_t *const y = (uint8_t *)a.y + ((int64_t)e * a.y_stride_e + split * a.y_stride_split) * SIZE;
     if (a.whole_lines) {
       // Rows that begin on lines of 128 bytes: a wave's strip is whole lines of them, 32 rows at a time through LDS of its own, stored past
-      // the caches (1332 rows over 32 slices, 2016 x 2112: 53 us, 76 with ordinary stores).
+      // the caches (1332 rows over 32 slices, 2016 x 2112: 58 us, 76 with ordinary stores).
       constexpr int CHUNKS = NF * 32 / PIECE, PITCH = NF * 32 * SIZE + 16;
       uint8_t *const strip_lds = lds + wave * (32 * PITCH);
       const uint32_t from = wave_lds_offset((uint32_t)((lane / CHUNKS) * PITCH + (lane % CHUNKS) * 16));
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
     }
     // Others: the tile's rows (half of them at a time in float32) through all of LDS, so that a wave stores whole rows of the tile, of which it leaves
     // the fewest lines to others.  With few rows to a slice, where the stores are what takes the time, into the caches, which put these lines
-    // together (760 rows over 60 slices, 237 x 2261: 21 us, 25 past them), else past them (20000 over 60, 700 x 720: 73, 86 into them).
+    // together (760 rows over 60 slices, 237 x 2261: 26 us, 29 past them), else past them (20000 over 60, 700 x 720: 66, 70 into them).
     constexpr int TURNS = SIZE / 2, CHUNKS = BN / PIECE, PITCH = BN * SIZE + 16, FRAGMENTS = MF / TURNS, ROWS = BM / TURNS;
     static_assert(ROWS * PITCH <= S::LDS && ROWS * CHUNKS % (64 * WAVES) == 0, "a turn fits");
 #pragma unroll
@@ -328,9 +329,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ragged_k_kernel(RaggedK a) {
 }
 
 // The tiles that there are (BM x BN, stages in flight).  One of 128 x 256 or 256 x 128, two to a CU, for long slices of many tiles: 65536 rows over 32 slices,
-// 2880 x 5760, 1.97 ms, and 2.24 with 128 x 128; 4096 over 8, 2048 x 4096, 80 and 80 us, 2048 over 8 56 and 52.  (256 x 256, one to a CU: 1.99 ms, 81 and 58.)
-// 128 x 128 with two stages, four to a CU, where a slice has few of them: 1332 rows over 32 slices, 2016 x 2112, 53 us, 62 with three, which
-// cost a CU its fourth workgroup; with 2500 rows of 64 x 64 each the third stage gives 47 in place of 72.
+// 2880 x 5760, 1.97 ms, and 2.27 with 128 x 128; 4096 over 8 of unequal lengths, 2048 x 4096, 91 and 104 us, 2048 over 8 55 and 57.  (256 x 256, one to a CU, gave 1.99
+// ms, and with equal lengths 81 us where 128 x 256 gives 80.)
+// 128 x 128 with two stages, four to a CU, where a slice has few of them: 1332 rows over 32 slices, 2016 x 2112, 58 us, 64 with three, which
+// cost a CU its fourth workgroup; with 2500 rows to each of 64 slices, 64 x 64, the third stage gives 28 in place of 40.
 enum RaggedTile { kTile128x256, kTile256x128, kTile128Short, kTile128 };
 
 int ragged_k_bf16(const RaggedK &a, int tile, void *stream);

@@ -8,10 +8,10 @@
 // What is kept is the MXFP8 form of a that tamd_downcast_mxfp makes of it (e4m3 values, one e8m0 scale per 32 along a row, rounded up):
 // 1.03 bytes per value in place of the 2 of a itself.  The gradient is that of the function at the kept values.
 //
-// Four lanes share a group of 32, eight values (four pairs) each.  What bounds it is memory: 65536 x 2880 bf16 takes 254 us forward (6.0 TB/s) and 300
-// backward with the activation again (6.3).  BIG, from 64 MB on: two groups per thread, everything past the caches, which do not keep that much until
-// it is used (16384 x 2880: 66 us, 71 through them; ragged rows 40000 x 1002: 63 and 73, backward 61 and 69).  Below: one group per thread (1024 x 1056:
-// 4.0 us, 5.1 with two), a and the results through the caches.  float32 takes the second form always: 16-byte pieces of its results are every other one
+// Four lanes share a group of 32, eight values (four pairs) each.  What bounds it is memory: 65536 x 2880 bf16 takes 242 us forward (6.3 TB/s) and 297
+// backward with the activation again (6.4).  BIG, from 64 MB on: two groups per thread, everything past the caches, which do not keep that much until
+// it is used (16384 x 2880: 62 us, 69 through them; ragged rows 40000 x 1002: 60 and 67, backward 57 and 64).  Below: one group per thread (1024 x 1056:
+// 4.0 us, 4.4 with two), a and the results through the caches.  float32 takes the second form always: 16-byte pieces of its results are every other one
 // of a line, which past the caches costs 6 % in place of gaining 4.  The kept values go past the caches in both: nothing reads them before the backward pass.
 #include "mx_values.h"
 #include <type_traits>
