@@ -246,3 +246,21 @@ def test_results_on_whole_lines(M, N, sizes, dtype, out, device):
         matmul(x.t(), fewer, None, md, md, c=c)
         check(c, x, fewer, sizes, out)
         assert bool((room[:, :, N - less:] == 5).all())
+
+
+@pytest.mark.parametrize("sizes", [[1], [2, 3, 0, 40], [700]], ids=str)
+@pytest.mark.parametrize("scale", [1e-4, 1e-5, 1e-6])
+def test_subnormal_float16(sizes, scale, device):
+    """Products that are added at the place of the largest, for which a number below 2^-14 counts as 2^-14: every one of n products, the running sum and the last
+    rounding are off by a step of float32 at most at that place.  One row alone is exact."""
+    torch.manual_seed(len(sizes))
+    rows = sum(sizes)
+    md = ragged(sizes, rows, device)
+    x, d = (scale * torch.randn(rows, 136, device=device)).half(), torch.randn(rows, 264, device=device).half()
+    for a, b in ((x, d), (d, x), (x, x)):
+        got, at = matmul(a.t(), b, None, md, md, precision_config=PrecisionConfig(out_dtype=torch.float32)), 0
+        for e, n in enumerate(sizes):
+            p, q = a[at:at + n].double().t().contiguous(), b[at:at + n].double()
+            bound = 2 * (n + 2) * 2.0 ** -24 * (p.abs().clamp(min=2.0 ** -14) @ q.abs().clamp(min=2.0 ** -14)) if n > 1 else 0.0
+            assert bool(((got[e].double() - p @ q).abs() <= bound).all()), (e, n)
+            at += n
